@@ -471,6 +471,121 @@ int32_t rnsmx_decode_garner(const int8_t *residues_dev, int64_t count,
                             const rnsmx_moduli_t *mods, int64_t *out_dev,
                             void *stream);
 
+/*
+ * Key/value cache in 8 bits: pages of `page` tokens, shared by any number of
+ * sequences.  k_dev and v_dev hold [blocks][heads][page][row_bytes] bytes, a
+ * value's code plus 128 each (zero in the columns past head_dim); scales_dev
+ * holds [blocks][heads][2] float32, a page's scale for the keys of a head and
+ * for its values: value = code * scale, code in [-127, 127].  No counterpart in
+ * the reference, whose path ends with the projections.
+ */
+typedef struct rnsmx_kv_cache {
+  uint8_t *k_dev, *v_dev;
+  float *scales_dev;
+  int32_t blocks;    /* pages                                              */
+  int32_t page;      /* tokens a page: 16, 32, 64 or 128                    */
+  int32_t heads;     /* key/value heads                                    */
+  int32_t head_dim;  /* 1 to RNSMX_KV_MAX_DIM                               */
+  int32_t row_bytes; /* rnsmx_kv_row_bytes(head_dim)                        */
+} rnsmx_kv_cache_t;
+
+/*
+ * The sequences of one call.  Sequence s holds lengths_dev[s] tokens (those of
+ * this call among them), token t in page table_dev[s * table_stride + t / page].
+ * Its rows of the call, starts_dev[s] to starts_dev[s + 1] - 1 (starts_dev null:
+ * row s alone), are its last tokens; a row before its first token (a sequence
+ * with fewer tokens than rows: the empty slot of a batch of fixed size) has no
+ * token.  A page number outside [0, blocks) is a page that is not there: not
+ * written, read as zeros, not attended to.  Lengths past max_length and rows
+ * past max_rows or `rows` are cut off; nothing out of range is accessed.
+ */
+typedef struct rnsmx_kv_batch {
+  const int32_t *table_dev;
+  int64_t table_stride;
+  const int32_t *lengths_dev;
+  const int32_t *starts_dev;
+  int32_t seqs;
+  int32_t table_width; /* pages a sequence may have                        */
+  int32_t rows;        /* rows of the call                                 */
+  int32_t max_rows;    /* most rows of one sequence                        */
+  int32_t max_length;  /* most tokens of one sequence, <= table_width * page */
+} rnsmx_kv_batch_t;
+
+#define RNSMX_KV_MAX_DIM 256
+
+/* Host only.  Bytes of one token's codes of one head in a page (the head
+ * dimension rounded up to one the kernels are built for); -1 if head_dim is
+ * out of range. */
+int32_t rnsmx_kv_row_bytes(int32_t head_dim);
+
+/*
+ * Quantises the batch's rows into the cache: k and v [rows][heads][head_dim]
+ * (FLOAT32, FLOAT16 or BFLOAT16), rows and heads at the given strides in
+ * elements.  For every page and head written,
+ *   scale = max(max|x| * fl32(1/127), 2^-23), code = clamp(rint(x / scale), +-127)
+ * over its new tokens, in float32.  A page that held tokens of the sequence
+ * before keeps the larger of its scale and the new tokens'; where that is
+ * larger than its own its older codes are quantised again, from code * scale.
+ * A value that is not finite makes the scale of its page and head so: every
+ * value there reads as NaN.  Rows of one call must not share a page with
+ * another sequence's.
+ */
+int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                        const void *k_dev, const void *v_dev, int32_t dtype,
+                        int64_t k_row_stride, int64_t k_head_stride,
+                        int64_t v_row_stride, int64_t v_head_stride, void *stream);
+
+/* The values of the batch's rows, code * scale rounded to dtype, ->
+ * k_dev and v_dev [rows][heads][head_dim] contiguous (zeros in rows that have
+ * no token or whose page is not there). */
+int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                      void *k_dev, void *v_dev, int32_t dtype, void *stream);
+
+/*
+ * The queries of rnsmx_kv_attention.  q_dev [rows][q_heads][head_dim] at the
+ * given strides in elements, q_heads a multiple of the cache's heads (head h
+ * reads key/value head h / (q_heads / heads)).  A row sees the tokens up to its
+ * own (causal 1; with window > 0 the last `window` of them) or all of its
+ * sequence (causal 0), but for those that the mask hides.  mask_dev (null: none)
+ * [rows][q_heads][mask_len] at its strides (0 where it is broadcast):
+ * mask_dtype INT8: bytes, zero hides; FLOAT32, FLOAT16, BFLOAT16: added to the
+ * scaled product, minus infinity hides.  Tokens at mask_len and past it are
+ * hidden.  A hidden token contributes nothing, whatever the cache or the mask
+ * holds there, and a row that sees no token is zero.
+ */
+typedef struct rnsmx_kv_query {
+  const void *q_dev;
+  int64_t row_stride, head_stride;
+  const void *mask_dev;
+  int64_t mask_row_stride, mask_head_stride, mask_token_stride;
+  int32_t dtype; /* of q and of the output */
+  int32_t q_heads;
+  int32_t mask_dtype;
+  int32_t mask_len;
+  int32_t causal;
+  int32_t window; /* 0: none */
+  float scale;    /* of the products, > 0 */
+} rnsmx_kv_query_t;
+
+/* Bytes of workspace the call needs (0 where no sequence's tokens are split
+ * over workgroups); -1 for arguments that rnsmx_kv_attention refuses.  Its
+ * first RNSMX_KV_TICKETS 32-bit counters must be zero when it is first used;
+ * every call leaves them zero, whatever its shape. */
+#define RNSMX_KV_TICKETS 16384
+int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                                           const rnsmx_kv_query_t *query);
+
+/*
+ * out[row][head] = sum_t softmax_t(scale * q . k_t + mask) v_t over the tokens
+ * the row sees -> out_dev [rows][q_heads][head_dim] contiguous.  Products of
+ * the queries and codes and of the softmax weights and codes run on the matrix
+ * cores in float16 (FLOAT32 queries: two halves each, 22 bits), with float32
+ * sums, maxima and exponentials.
+ */
+int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                           const rnsmx_kv_query_t *query, void *workspace_dev,
+                           int64_t workspace_bytes, void *out_dev, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,447 @@
+// The 8-bit key/value cache: quantising tokens into pages, reading them back,
+// and the host side of its C ABI.
+#include <algorithm>
+#include <cmath>
+
+#include "rnsmx_kv.hpp"
+
+namespace rnsmx {
+
+struct KvAppendArgs {
+  KvBatchArgs b;
+  const void *src[2];
+  int64_t row_stride[2], head_stride[2];
+  int32_t dtype, pages, vec;  // pages: most pages of one sequence that the rows touch
+};
+
+struct KvReadArgs {
+  KvBatchArgs b;
+  void *dst[2];
+  int32_t dtype, pages, vec;
+};
+
+constexpr float kKvMax = 127.0f;
+constexpr int kKvHeld = 4;  // groups of 8 values a thread of kv_append_kernel holds
+
+template <typename T>
+__device__ __forceinline__ void kv_load8(float (&x)[8], const T *p, int32_t left, bool vec) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+      kv_for<4>([&](auto I_) { constexpr int I = decltype(I_)::value; x[I] = a[I], x[I + 4] = b[I]; });
+    } else {
+      const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
+      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
+        const uint16_t bits = static_cast<uint16_t>(a[I / 2] >> (16 * (I % 2)));
+        if constexpr (std::is_same<T, _Float16>::value)
+          x[I] = static_cast<float>(__builtin_bit_cast(_Float16, bits));
+        else
+          x[I] = kv_bf16(bits);
+      });
+    }
+    return;
+  }
+  kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
+    float v = 0.0f;
+    if (I < left) {
+      if constexpr (std::is_same<T, uint16_t>::value)
+        v = kv_bf16(p[I]);
+      else
+        v = static_cast<float>(p[I]);
+    }
+    x[I] = v;
+  });
+}
+
+// clamp(rint(x / s), +-127) + 128; a quotient that is not a number gives 128
+// (the scale then says that nothing of the page can be read).
+__device__ __forceinline__ uint32_t kv_code(float x, float s) {
+  const float r = rintf(x / s);
+  return r != r ? 128u : static_cast<uint32_t>(static_cast<int32_t>(fminf(fmaxf(r, -kKvMax), kKvMax)) + 128);
+}
+
+__device__ __forceinline__ u32x2 kv_codes(const float (&x)[8], float s) {
+  u32x2 c = {0u, 0u};
+  kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; c[I / 4] |= kv_code(x[I], s) << (8 * (I % 4)); });
+  return c;
+}
+
+// code * scale in float32.  The product is kept apart from a conversion to
+// float16 after it: the compiler would join them into one operation, which
+// rounds once, where the definition has float32 values.
+__device__ __forceinline__ float kv_value(u32x2 c, int i, float s) {
+  float v = static_cast<float>(static_cast<int32_t>((c[i / 4] >> (8 * (i % 4))) & 0xFFu) - 128) * s;
+  asm("" : "+v"(v));
+  return v;
+}
+
+// One workgroup for the new tokens of one page and head, keys or values.
+template <int DT, typename T>
+__global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
+  constexpr int CPT = DT / 8;
+  __shared__ uint32_t tops[16];
+  const KvBatchArgs &b = a.b;
+  int32_t id = blockIdx.x;
+  const int32_t part = id & 1;
+  id >>= 1;
+  const int32_t head = id % b.heads;
+  id /= b.heads;
+  const int32_t seq = id / a.pages, index = id - seq * a.pages;
+  const KvSeq q = kv_seq(b, seq);
+  const int32_t page_size = 1 << b.log_page, from = max(q.len - q.n, 0);
+  const int32_t pg = (from >> b.log_page) + index, start = pg << b.log_page;
+  if (start >= q.len) return;
+  const int32_t id_page = b.table[seq * b.table_stride + pg];
+  if (static_cast<uint32_t>(id_page) >= static_cast<uint32_t>(b.blocks)) return;
+  const int32_t old = max(from - start, 0), end = min(q.len - start, page_size);  // tokens old..end-1 are new
+  const int64_t slot = static_cast<int64_t>(id_page) * b.heads + head;
+  uint8_t *page = (part ? b.v : b.k) + (slot << b.log_page) * DT;
+  const T *src = static_cast<const T *>(part ? a.src[1] : a.src[0]);
+  const int64_t rs = part ? a.row_stride[1] : a.row_stride[0], hs = part ? a.head_stride[1] : a.head_stride[0];
+  const int32_t groups = (end - old) * CPT;
+  src += (q.row + (start + old) - (q.len - q.n)) * rs + head * hs;
+
+  float x[kKvHeld][8];
+  uint32_t top = 0;  // of |x| as bits: ordered as the values are, a NaN above all
+  kv_for<kKvHeld>([&](auto J_) { constexpr int J = decltype(J_)::value;
+    const int32_t c = threadIdx.x + J * blockDim.x;
+    const int32_t t = c / CPT, d = (c - t * CPT) * 8;
+    if (c < groups && d < b.dim) {
+      kv_load8<T>(x[J], src + t * rs + d, b.dim - d, a.vec);
+    } else {
+      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; x[J][I] = 0.0f; });
+    }
+    kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; top = max(top, __float_as_uint(x[J][I]) & 0x7FFFFFFFu); });
+  });
+  float *scale = b.scales + slot * 2 + part;
+  const float held = old > 0 ? *scale : 0.0f;
+  kv_for<6>([&](auto I_) { constexpr int I = decltype(I_)::value; top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1 << I))); });
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (uint32_t w = 0; w < (blockDim.x + 63) / 64; ++w) top = max(top, tops[w]);
+  const float amax = __uint_as_float(top);
+  float s = amax != amax ? amax : fmaxf(amax * (1.0f / kKvMax), 1.1920928955078125e-07f);
+  if (old > 0) s = (s != s || held != held) ? __builtin_nanf("") : fmaxf(s, held);
+  if (threadIdx.x == 0) *scale = s;
+  kv_for<kKvHeld>([&](auto J_) { constexpr int J = decltype(J_)::value;
+    const int32_t c = threadIdx.x + J * blockDim.x;
+    if (c < groups) *reinterpret_cast<u32x2 *>(page + old * DT + c * 8) = kv_codes(x[J], s);
+  });
+  if (old > 0 && s != held)  // the older tokens' codes, to the larger scale
+    for (int32_t c = threadIdx.x; c < old * CPT; c += blockDim.x) {
+      u32x2 *p = reinterpret_cast<u32x2 *>(page + c * 8);
+      float v[8];
+      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; v[I] = kv_value(*p, I, held); });
+      *p = kv_codes(v, s);
+    }
+}
+
+// One workgroup for the rows of one page and head, keys or values.
+template <int DT, typename T>
+__global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
+  constexpr int CPT = DT / 8;
+  const KvBatchArgs &b = a.b;
+  int32_t id = blockIdx.x;
+  const int32_t part = id & 1;
+  id >>= 1;
+  const int32_t head = id % b.heads;
+  id /= b.heads;
+  const int32_t seq = id / a.pages, index = id - seq * a.pages;
+  const KvSeq q = kv_seq(b, seq);
+  const int32_t page_size = 1 << b.log_page, from = max(q.len - q.n, 0);
+  T *dst = static_cast<T *>(part ? a.dst[1] : a.dst[0]) + head * b.dim;
+  const int64_t rs = static_cast<int64_t>(b.heads) * b.dim;
+  if (index == 0)  // rows that have no token
+    for (int32_t i = threadIdx.x; i < max(q.n - q.len, 0) * b.dim; i += 256) {
+      const int32_t r = i / b.dim;
+      dst[(q.row + r) * rs + (i - r * b.dim)] = static_cast<T>(0);
+    }
+  const int32_t pg = (from >> b.log_page) + index, start = pg << b.log_page;
+  if (start >= q.len || q.n == 0) return;
+  const int32_t id_page = b.table[seq * b.table_stride + pg];
+  const bool there = static_cast<uint32_t>(id_page) < static_cast<uint32_t>(b.blocks);
+  const int32_t old = max(from - start, 0), end = min(q.len - start, page_size);
+  const int64_t slot = static_cast<int64_t>(there ? id_page : 0) * b.heads + head;
+  const uint8_t *page = (part ? b.v : b.k) + (slot << b.log_page) * DT;
+  const float s = there ? b.scales[slot * 2 + part] : 0.0f;
+  dst += (q.row + (start + old) - (q.len - q.n)) * rs;
+  for (int32_t c = threadIdx.x; c < (end - old) * CPT; c += 256) {
+    const int32_t t = c / CPT, d = (c - t * CPT) * 8;
+    if (d >= b.dim) continue;
+    const u32x2 code = *reinterpret_cast<const u32x2 *>(page + old * DT + c * 8);
+    float x[8];
+    kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; x[I] = there ? kv_value(code, I, s) : 0.0f; });
+    T *to = dst + t * rs + d;
+    T y[8];
+    kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
+      if constexpr (std::is_same<T, uint16_t>::value)
+        y[I] = kv_to_bf16(x[I]);
+      else
+        y[I] = static_cast<T>(x[I]);
+    });
+    if (a.vec) {
+      kv_for<sizeof(T) / 2>([&](auto I_) { constexpr int I = decltype(I_)::value; reinterpret_cast<u32x4 *>(to)[I] = reinterpret_cast<u32x4 *>(y)[I]; });
+    } else {
+      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
+        if (d + I < b.dim) to[I] = y[I];
+      });
+    }
+  }
+}
+
+static int32_t kv_row_bytes(int32_t dim) {
+  for (int d : kKvDims)
+    if (dim >= 1 && dim <= d) return d;
+  return -1;
+}
+
+static int32_t kv_check(const char *what) {
+  const hipError_t err = hipGetLastError();
+  if (err == hipSuccess) return RNSMX_OK;
+  set_error("%s: %s", what, hipGetErrorString(err));
+  return RNSMX_ELAUNCH;
+}
+
+static bool aligned(const void *p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+static int64_t dtype_bytes(int32_t dtype) { return dtype == RNSMX_FLOAT32 ? 4 : dtype == RNSMX_INT8 ? 1 : 2; }
+static bool is_float(int32_t dtype) {
+  return dtype == RNSMX_FLOAT32 || dtype == RNSMX_FLOAT16 || dtype == RNSMX_BFLOAT16;
+}
+
+static int32_t kv_batch_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, KvBatchArgs &a) {
+  if (!cache || !batch) return fail(RNSMX_EINVAL, "null cache or batch");
+  if (cache->page != 16 && cache->page != 32 && cache->page != 64 && cache->page != 128)
+    return fail(RNSMX_EINVAL, "a page holds 16, 32, 64 or 128 tokens");
+  if (cache->blocks < 1 || cache->heads < 1) return fail(RNSMX_EINVAL, "a cache has at least one page and one head");
+  if (kv_row_bytes(cache->head_dim) < 0) return fail(RNSMX_EINVAL, "head dimensions are 1 to 256");
+  if (cache->row_bytes != kv_row_bytes(cache->head_dim)) return fail(RNSMX_EINVAL, "row_bytes is not the head dimension's");
+  if (!cache->k_dev || !cache->v_dev || !cache->scales_dev) return fail(RNSMX_EINVAL, "null cache pointer");
+  if (!aligned(cache->k_dev, 16) || !aligned(cache->v_dev, 16) || !aligned(cache->scales_dev, 8))
+    return fail(RNSMX_EINVAL, "codes start on 16-byte boundaries, scales on 8-byte ones");
+  if (batch->seqs < 0 || batch->rows < 0 || batch->max_rows < 0 || batch->max_length < 0 || batch->table_width < 1 ||
+      batch->table_stride < 0)
+    return fail(RNSMX_EINVAL, "bad batch sizes");
+  if (batch->max_length > 1 << 30) return fail(RNSMX_EINVAL, "sequences hold at most 2^30 tokens");
+  if (batch->max_length > static_cast<int64_t>(batch->table_width) * cache->page)
+    return fail(RNSMX_EINVAL, "max_length is past the block table");
+  if (batch->seqs > 0 && (!batch->table_dev || !batch->lengths_dev)) return fail(RNSMX_EINVAL, "null batch pointer");
+  if (!batch->starts_dev && batch->rows != batch->seqs) return fail(RNSMX_EINVAL, "one row a sequence without row starts");
+  a.k = cache->k_dev;
+  a.v = cache->v_dev;
+  a.scales = cache->scales_dev;
+  a.table = batch->table_dev;
+  a.lengths = batch->lengths_dev;
+  a.starts = batch->starts_dev;
+  a.table_stride = batch->table_stride;
+  a.blocks = cache->blocks;
+  a.log_page = cache->page == 16 ? 4 : cache->page == 32 ? 5 : cache->page == 64 ? 6 : 7;
+  a.heads = cache->heads;
+  a.dim = cache->head_dim;
+  a.row_bytes = cache->row_bytes;
+  a.seqs = batch->seqs;
+  a.table_width = batch->table_width;
+  a.rows = batch->rows;
+  a.max_rows = batch->starts_dev ? std::min(batch->max_rows, batch->rows) : 1;
+  a.max_length = batch->max_length;
+  return RNSMX_OK;
+}
+
+// Most pages that max_rows tokens in a row can lie in.
+static int64_t pages_touched(const KvBatchArgs &a) {
+  const int64_t page = 1 << a.log_page, n = std::min(a.max_rows, a.max_length);
+  return n < 1 ? 1 : (n + page - 2) / page + 1;
+}
+
+static int32_t grid_of(int64_t groups, unsigned &grid) {
+  if (groups > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many sequences, pages and heads for one launch");
+  grid = static_cast<unsigned>(groups);
+  return RNSMX_OK;
+}
+
+#define RNSMX_KV_DIM_CASE(D, ...) \
+  case D: {                       \
+    constexpr int DT = D;         \
+    __VA_ARGS__;                  \
+    break;                        \
+  }
+// the statement with DT the row size
+#define RNSMX_KV_DIMS(dim, ...)          \
+  switch (dim) {                         \
+    RNSMX_KV_DIM_CASE(64, __VA_ARGS__)   \
+    RNSMX_KV_DIM_CASE(96, __VA_ARGS__)   \
+    RNSMX_KV_DIM_CASE(128, __VA_ARGS__)  \
+    RNSMX_KV_DIM_CASE(160, __VA_ARGS__)  \
+    RNSMX_KV_DIM_CASE(192, __VA_ARGS__)  \
+    RNSMX_KV_DIM_CASE(256, __VA_ARGS__)  \
+  }
+
+// The split of a call's tokens over workgroups.
+static void kv_split(KvAttnArgs &a) {
+  const int64_t span = a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32)
+                                    : a.b.max_length;
+  const int64_t tasks = static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles;
+  const int64_t steps = std::max<int64_t>(1, (span + kKvChunkUnit - 1) / kKvChunkUnit);
+  int64_t splits = 1;
+  if (tasks > 0 && tasks <= RNSMX_KV_TICKETS) splits = std::max<int64_t>(1, std::min<int64_t>(steps, 768 / tasks));
+  const int64_t each = (steps + splits - 1) / splits;
+  a.chunk = static_cast<int32_t>(std::min<int64_t>(each * kKvChunkUnit, 1 << 30));
+  a.splits = static_cast<int32_t>((steps + each - 1) / each);
+}
+
+static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const rnsmx_kv_query_t *query,
+                            KvAttnArgs &a) {
+  if (int32_t rc = kv_batch_args(cache, batch, a.b)) return rc;
+  if (!query) return fail(RNSMX_EINVAL, "null query");
+  if (!is_float(query->dtype)) return fail(RNSMX_EINVAL, "queries are float32, float16 or bfloat16");
+  if (query->q_heads < 1 || query->q_heads % cache->heads != 0)
+    return fail(RNSMX_EINVAL, "query heads are a multiple of the cache's heads");
+  if (!(query->scale > 0.0f) || !std::isfinite(query->scale)) return fail(RNSMX_EINVAL, "the scale is positive and finite");
+  if (query->window < 0 || (query->window > 0 && !query->causal)) return fail(RNSMX_EINVAL, "a window needs causal rows");
+  if (query->mask_dev) {
+    if (query->mask_dtype != RNSMX_INT8 && !is_float(query->mask_dtype))
+      return fail(RNSMX_EINVAL, "masks are bytes, float32, float16 or bfloat16");
+    if (query->mask_len < 0) return fail(RNSMX_EINVAL, "bad mask length");
+    if (!aligned(query->mask_dev, dtype_bytes(query->mask_dtype))) return fail(RNSMX_EINVAL, "the mask is not aligned to its type");
+  }
+  const int64_t size = dtype_bytes(query->dtype);
+  if (a.b.rows > 0 && (!query->q_dev || !aligned(query->q_dev, size))) return fail(RNSMX_EINVAL, "queries null or not aligned to their type");
+  a.q = query->q_dev;
+  a.q_rs = query->row_stride;
+  a.q_hs = query->head_stride;
+  a.mask = query->mask_dev;
+  a.mask_rs = query->mask_row_stride;
+  a.mask_hs = query->mask_head_stride;
+  a.mask_ts = query->mask_token_stride;
+  a.mask_dtype = query->mask_dtype;
+  a.mask_len = query->mask_len;
+  a.q_heads = query->q_heads;
+  a.group = query->q_heads / cache->heads;
+  a.dtype = query->dtype;
+  a.causal = query->causal != 0;
+  a.window = query->window;
+  a.scale = query->scale;
+  a.vec = cache->head_dim % 8 == 0 && aligned(query->q_dev, 16) && query->row_stride * size % 16 == 0 &&
+          query->head_stride * size % 16 == 0;
+  const int64_t tiles = (static_cast<int64_t>(a.b.max_rows) * a.group + kKvRowTile - 1) / kKvRowTile;
+  if (tiles > 0x7FFFFFFF) return fail(RNSMX_EINVAL, "too many rows");
+  a.row_tiles = static_cast<int32_t>(tiles);
+  kv_split(a);
+  return RNSMX_OK;
+}
+
+static int64_t kv_tasks(const KvAttnArgs &a) { return static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles; }
+
+static int64_t kv_workspace(const KvAttnArgs &a) {
+  if (a.splits < 2) return 0;
+  return RNSMX_KV_TICKETS * 4 + kv_tasks(a) * a.splits * kv_partial_floats(a.b.row_bytes) * 4;
+}
+
+}  // namespace rnsmx
+
+using namespace rnsmx;
+
+extern "C" {
+
+int32_t rnsmx_kv_row_bytes(int32_t head_dim) { return kv_row_bytes(head_dim); }
+
+int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const void *k_dev,
+                        const void *v_dev, int32_t dtype, int64_t k_row_stride, int64_t k_head_stride,
+                        int64_t v_row_stride, int64_t v_head_stride, void *stream) {
+  clear_error();
+  KvAppendArgs a{};
+  if (int32_t rc = kv_batch_args(cache, batch, a.b)) return rc;
+  if (!is_float(dtype)) return fail(RNSMX_EINVAL, "keys and values are float32, float16 or bfloat16");
+  if (a.b.rows == 0 || a.b.seqs == 0) return RNSMX_OK;
+  const int64_t size = dtype_bytes(dtype);
+  if (!k_dev || !v_dev || !aligned(k_dev, size) || !aligned(v_dev, size))
+    return fail(RNSMX_EINVAL, "keys or values null or not aligned to their type");
+  a.src[0] = k_dev;
+  a.src[1] = v_dev;
+  a.row_stride[0] = k_row_stride;
+  a.row_stride[1] = v_row_stride;
+  a.head_stride[0] = k_head_stride;
+  a.head_stride[1] = v_head_stride;
+  a.dtype = dtype;
+  a.vec = a.b.dim % 8 == 0 && aligned(k_dev, 16) && aligned(v_dev, 16) && k_row_stride * size % 16 == 0 &&
+          v_row_stride * size % 16 == 0 && k_head_stride * size % 16 == 0 && v_head_stride * size % 16 == 0;
+  const int64_t pages = pages_touched(a.b);
+  a.pages = static_cast<int32_t>(pages);
+  unsigned grid;
+  if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads * 2, grid)) return rc;
+  // every thread holds kKvHeld groups of 8 values of the tokens that a page can get
+  const int64_t tokens = std::min<int64_t>(cache->page, a.b.max_rows);
+  const int64_t groups = (tokens * (a.b.row_bytes / 8) + kKvHeld - 1) / kKvHeld;
+  const unsigned threads = static_cast<unsigned>(std::max<int64_t>(64, (groups + 63) / 64 * 64));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == RNSMX_FLOAT32) {
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, float>), dim3(grid), dim3(threads), 0, st, a))
+  } else if (dtype == RNSMX_FLOAT16) {
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, _Float16>), dim3(grid), dim3(threads), 0, st, a))
+  } else {
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, uint16_t>), dim3(grid), dim3(threads), 0, st, a))
+  }
+  return kv_check("kv_append");
+}
+
+int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, void *k_dev, void *v_dev,
+                      int32_t dtype, void *stream) {
+  clear_error();
+  KvReadArgs a{};
+  if (int32_t rc = kv_batch_args(cache, batch, a.b)) return rc;
+  if (!is_float(dtype)) return fail(RNSMX_EINVAL, "values are read as float32, float16 or bfloat16");
+  if (a.b.rows == 0 || a.b.seqs == 0) return RNSMX_OK;
+  const int64_t size = dtype_bytes(dtype);
+  if (!k_dev || !v_dev || !aligned(k_dev, size) || !aligned(v_dev, size))
+    return fail(RNSMX_EINVAL, "keys or values null or not aligned to their type");
+  a.dst[0] = k_dev;
+  a.dst[1] = v_dev;
+  a.dtype = dtype;
+  a.vec = a.b.dim % 8 == 0 && aligned(k_dev, 16) && aligned(v_dev, 16);
+  const int64_t pages = pages_touched(a.b);
+  a.pages = static_cast<int32_t>(pages);
+  unsigned grid;
+  if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads * 2, grid)) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == RNSMX_FLOAT32) {
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, float>), dim3(grid), dim3(256), 0, st, a))
+  } else if (dtype == RNSMX_FLOAT16) {
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, _Float16>), dim3(grid), dim3(256), 0, st, a))
+  } else {
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, uint16_t>), dim3(grid), dim3(256), 0, st, a))
+  }
+  return kv_check("kv_read");
+}
+
+int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                                           const rnsmx_kv_query_t *query) {
+  clear_error();
+  KvAttnArgs a{};
+  if (kv_attn_args(cache, batch, query, a)) return -1;
+  return kv_workspace(a);
+}
+
+int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const rnsmx_kv_query_t *query,
+                           void *workspace_dev, int64_t workspace_bytes, void *out_dev, void *stream) {
+  clear_error();
+  KvAttnArgs a{};
+  if (int32_t rc = kv_attn_args(cache, batch, query, a)) return rc;
+  if (a.b.rows == 0 || a.b.seqs == 0) return RNSMX_OK;
+  if (!out_dev || !aligned(out_dev, dtype_bytes(a.dtype))) return fail(RNSMX_EINVAL, "output null or not aligned to its type");
+  const int64_t need = kv_workspace(a);
+  if (need > 0) {
+    if (!workspace_dev || !aligned(workspace_dev, 16)) return fail(RNSMX_EINVAL, "workspace null or not on a 16-byte boundary");
+    if (workspace_bytes < need) return fail(RNSMX_ESPACE, "workspace too small");
+    a.tickets = static_cast<uint32_t *>(workspace_dev);
+    a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace_dev) + RNSMX_KV_TICKETS * 4);
+  }
+  a.out = out_dev;
+  unsigned grid;
+  if (int32_t rc = grid_of(kv_tasks(a) * a.splits, grid)) return rc;
+  if (grid == 0) return RNSMX_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_rows<DT>(a, st))
+  return kv_check("kv_attention");
+}
+
+}  // extern "C"

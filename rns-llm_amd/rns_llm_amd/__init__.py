@@ -4,6 +4,8 @@ Nek1tt/rns-llm.  Public names mirror ``rns_llm`` (``src/rns_llm/__init__.py``,
 from .backends import (
     AdaptiveMetadata,
     HipRNSBackend,
+    KVBatch,
+    KVCache,
     PreparedAdaptiveRNSWeight,
     PreparedRNSWeight,
     RNSRequestBatchWorkspace,
@@ -30,7 +32,7 @@ from .moduli import (
 )
 
 __all__ = [
-    "AdaptiveMetadata", "HipRNSBackend", "PreparedAdaptiveRNSWeight", "PreparedRNSWeight",
+    "AdaptiveMetadata", "HipRNSBackend", "KVBatch", "KVCache", "PreparedAdaptiveRNSWeight", "PreparedRNSWeight",
     "RNSRequestBatchWorkspace", "RNSWorkspace", "hip_extension_available", "CachedRNSQKV",
     "InstalledQKVFusion", "RNSLinear", "RNSQKVProjection", "install_opt_qkv_fusion",
     "replace_opt_attention_blocks",

@@ -49,9 +49,16 @@ EXPORTED_SYMBOLS = (
     "rnsmx_linear_workspace_bytes",
     "rnsmx_linear_forward",
     "rnsmx_decode_garner",
+    "rnsmx_kv_row_bytes",
+    "rnsmx_kv_append",
+    "rnsmx_kv_read",
+    "rnsmx_kv_attention_workspace_bytes",
+    "rnsmx_kv_attention",
 )
 
 QUANT_SCRATCH = 1025  # RNSMX_QUANT_SCRATCH
+KV_MAX_DIM = 256  # RNSMX_KV_MAX_DIM
+KV_TICKETS = 16384  # RNSMX_KV_TICKETS
 
 
 class Moduli(ctypes.Structure):
@@ -121,6 +128,58 @@ class Adaptive(ctypes.Structure):
     ]
 
 
+class KVCacheStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_kv_cache_t``."""
+
+    _fields_ = [
+        ("k_dev", ctypes.c_void_p),
+        ("v_dev", ctypes.c_void_p),
+        ("scales_dev", ctypes.c_void_p),
+        ("blocks", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("row_bytes", ctypes.c_int32),
+    ]
+
+
+class KVBatchStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_kv_batch_t``."""
+
+    _fields_ = [
+        ("table_dev", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("lengths_dev", ctypes.c_void_p),
+        ("starts_dev", ctypes.c_void_p),
+        ("seqs", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+        ("max_length", ctypes.c_int32),
+    ]
+
+
+class KVQueryStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_kv_query_t``."""
+
+    _fields_ = [
+        ("q_dev", ctypes.c_void_p),
+        ("row_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("mask_dev", ctypes.c_void_p),
+        ("mask_row_stride", ctypes.c_int64),
+        ("mask_head_stride", ctypes.c_int64),
+        ("mask_token_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("mask_dtype", ctypes.c_int32),
+        ("mask_len", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -166,9 +225,15 @@ _SIGNATURES = {
         _I32, [_P, _I32, _I32, _I32, _I32, _I32, _P, ctypes.POINTER(Moduli), _P, _P,
                ctypes.POINTER(Adaptive), _P, _I64, _P, _P]),
     "rnsmx_decode_garner": (_I32, [_P, _I64, ctypes.POINTER(Moduli), _P, _P]),
+    "rnsmx_kv_row_bytes": (_I32, [_I32]),
+    # structures by address, so that a bound one costs no conversion per call
+    "rnsmx_kv_append": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _P]),
+    "rnsmx_kv_read": (_I32, [_P, _P, _P, _P, _I32, _P]),
+    "rnsmx_kv_attention_workspace_bytes": (_I64, [_P, _P, _P]),
+    "rnsmx_kv_attention": (_I32, [_P, _P, _P, _P, _I64, _P, _P]),
 }
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 
 class NativeError(RuntimeError):

@@ -7,10 +7,13 @@ from .hip_backend import (
     RNSWorkspace,
     hip_extension_available,
 )
+from .kv_cache import KVBatch, KVCache
 
 __all__ = [
     "AdaptiveMetadata",
     "HipRNSBackend",
+    "KVBatch",
+    "KVCache",
     "PreparedAdaptiveRNSWeight",
     "PreparedRNSWeight",
     "RNSRequestBatchWorkspace",

@@ -42,6 +42,7 @@ from ..moduli import (
     safe_l1_dot_bound,
     validate_moduli,
 )
+from .kv_cache import KVCacheOps
 
 KERNEL_NAME = "mfma"
 
@@ -301,10 +302,10 @@ class LinearCall:
         return AdaptiveMetadata(meta, self._full_moduli, stats)
 
 
-class HipRNSBackend:
+class HipRNSBackend(KVCacheOps):
     """RNS backend on MI355X: one MFMA GEMM launch for all residue channels
     with the modular reduction, Garner reconstruction and signed correction
-    in its epilogue."""
+    in its epilogue; and the 8-bit key/value cache (``kv_cache.py``)."""
 
     name = "hip-rns-mfma"
 
@@ -315,7 +316,10 @@ class HipRNSBackend:
         self._device_cache: dict[tuple[int, tuple[int, ...]], _DeviceConstants] = {}
         self._quant_scratch: dict[tuple[int, int], torch.Tensor] = {}
         self._ws_bytes: dict[tuple[int, int, int], int] = {}
+        self._kv_scratch: dict[tuple[int, int], list[torch.Tensor]] = {}
         self._stats: Counter[str] = Counter()
+
+    _stream_of = staticmethod(_stream_handle)
 
     # ------------------------------------------------------------------
     # Stats (cuda_backend.py:129-135)

@@ -17,6 +17,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+typedef __attribute__((address_space(4))) int32_t kv_const_i32;
+
 template <typename F, int... I>
 __device__ __forceinline__ void kv_for_impl(F &&f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
@@ -24,6 +26,27 @@ __device__ __forceinline__ void kv_for_impl(F &&f, std::integer_sequence<int, I.
 template <int N, typename F>
 __device__ __forceinline__ void kv_for(F &&f) {
   kv_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// Quotients by a divisor known on the host, for n below 2^31: with s = ceil(log2
+// d) and mul = floor(2^32 (2^s - d) / d) + 1 (Granlund and Montgomery's method),
+// n / d = (mulhi(mul, n) + n) >> s.  A division in scalar code takes some 250
+// cycles, and a workgroup finds its place with half a dozen.
+struct KvDiv {
+  uint32_t mul, shift, d;
+};
+inline KvDiv kv_div(uint32_t d) {
+  KvDiv r{0, 0, d};
+  while ((1ull << r.shift) < d) ++r.shift;
+  r.mul = static_cast<uint32_t>((((1ull << r.shift) - d) << 32) / d + 1);
+  return r;
+}
+__device__ __forceinline__ uint32_t kv_quot(const KvDiv &v, uint32_t n) { return (__umulhi(v.mul, n) + n) >> v.shift; }
+// n becomes the quotient; the remainder
+__device__ __forceinline__ uint32_t kv_rem(const KvDiv &v, uint32_t &n) {
+  const uint32_t q = kv_quot(v, n), r = n - q * v.d;
+  n = q;
+  return r;
 }
 
 // Row sizes the attention kernels are built for; a head dimension takes the
@@ -46,10 +69,12 @@ struct KvSeq {
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvBatchArgs &a, int32_t s) {
   KvSeq r;
-  r.len = min(max(a.lengths[s], 0), a.max_length);
+  // through the scalar cache: s is one for the workgroup
+  const kv_const_i32 *lengths = (const kv_const_i32 *)a.lengths, *starts = (const kv_const_i32 *)a.starts;
+  r.len = min(max(lengths[s], 0), a.max_length);
   if (a.starts) {
-    r.row = min(max(a.starts[s], 0), a.rows);
-    r.n = min(max(a.starts[s + 1] - r.row, 0), min(a.max_rows, a.rows - r.row));
+    r.row = min(max(starts[s], 0), a.rows);
+    r.n = min(max(starts[s + 1] - r.row, 0), min(a.max_rows, a.rows - r.row));
   } else {
     r.row = s;
     r.n = 1;
@@ -87,21 +112,38 @@ struct KvAttnArgs {
   float *partial;     // [tasks][splits] partial results, tasks = seqs * heads * row tiles
   uint32_t *tickets;  // one arrival counter per task
   int64_t q_rs, q_hs, mask_rs, mask_hs, mask_ts;
-  int32_t q_heads, group, dtype, mask_dtype, mask_len;
-  int32_t causal, window, vec;  // vec: q rows are read 16 bytes at a time
-  int32_t chunk, splits, row_tiles;
+  int32_t q_heads, dtype, mask_dtype, mask_len;
+  int32_t causal, window, vec, out_vec;  // vec: q rows are read 16 bytes at a time; out_vec: out starts on 16 bytes
+  int32_t chunk, splits, waves;  // waves of a workgroup of kv_rows_kernel
+  int32_t tile_rows, row_tiles;  // rows of a workgroup (which says the kernel), workgroups over a sequence's rows
+  KvDiv by_group, by_splits, by_tiles, by_heads;
   float scale;
 };
 
-constexpr int kKvRowTile = 16;   // query rows of a workgroup of kv_rows_kernel
-constexpr int kKvChunkUnit = 128;  // tokens four waves take per step
+constexpr int kKvRows = 16;          // query rows of a workgroup of kv_rows_kernel
+// Whether it is built with eight waves: row sizes whose waves are two to a SIMD.
+constexpr bool kv_wide(int row_bytes) { return row_bytes <= 160; }
 
-// Floats of one split's partial result: 16 rows of row_bytes values, then each
+// Floats of one split's partial result: rows of row_bytes values, then each
 // row's reference and sum.
-inline int64_t kv_partial_floats(int32_t row_bytes) { return kKvRowTile * (static_cast<int64_t>(row_bytes) + 2); }
+inline int64_t kv_partial_floats(int32_t rows, int32_t row_bytes) {
+  return static_cast<int64_t>(rows) * (static_cast<int64_t>(row_bytes) + 2);
+}
+
+// Workgroups go to the 8 XCDs in turn: the n-th of an XCD takes the n-th of a
+// contiguous part of the work, so that what shares keys shares an L2.
+__device__ __forceinline__ int32_t kv_xcd_order(uint32_t id, uint32_t count) {
+  const uint32_t xcd = id & 7, per = count >> 3, more = count & 7;
+  return static_cast<int32_t>(xcd * per + min(xcd, more) + (id >> 3));
+}
 
 // rnsmx_kv_rows.hip, one object per row size
 template <int DT>
 void launch_kv_rows(const KvAttnArgs &a, hipStream_t st);
+
+// rnsmx_kv_tiles.hip, one object per row size
+constexpr int kKvTileRows = 128;  // query rows of a workgroup of kv_tiles_kernel
+template <int DT>
+void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st);
 
 }  // namespace rnsmx

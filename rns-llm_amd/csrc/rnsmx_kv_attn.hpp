@@ -1,0 +1,116 @@
+// Attention over the 8-bit key/value cache: what its two kernels share
+// (rnsmx_kv_rows.hip for few rows, rnsmx_kv_tiles.hip for prompts).
+#pragma once
+
+#include "rnsmx_kv.hpp"
+
+namespace rnsmx {
+
+// Two stored bytes (code + 128) as halves code / 512: a byte alone in a half's
+// low bits is that many 2^-24, so one multiply by 2^15 and one subtraction of
+// 128 / 512 give it, both exact.
+template <int LO, int HI>
+__device__ __forceinline__ h16x2 kv_halves(uint32_t lo, uint32_t hi) {
+  constexpr uint32_t sel = LO | 0x0C00u | (static_cast<uint32_t>(4 + HI) << 16) | 0x0C000000u;
+  const h16x2 u = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(hi, lo, sel));
+  const h16x2 up = {static_cast<_Float16>(32768.0f), static_cast<_Float16>(32768.0f)};
+  const h16x2 off = {static_cast<_Float16>(-0.25f), static_cast<_Float16>(-0.25f)};
+  return __builtin_elementwise_fma(u, up, off);
+}
+constexpr float kKvUnit = 512.0f;
+
+__device__ __forceinline__ h16x8 kv_join(h16x2 a, h16x2 b, h16x2 c, h16x2 d) {
+  return h16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Eight consecutive codes of a row.
+__device__ __forceinline__ h16x8 kv_row8(uint32_t w0, uint32_t w1) {
+  return kv_join(kv_halves<0, 1>(w0, w0), kv_halves<2, 3>(w0, w0), kv_halves<0, 1>(w1, w1), kv_halves<2, 3>(w1, w1));
+}
+
+constexpr float kKvLog2e = 1.44269504088896340736f;
+// A row's reference is put 4 below its largest weight's exponent and follows
+// when one passes 12: weights stay below 2^12 (float16 ends at 2^16), and those
+// 2^-18 of the largest keep all their bits.
+constexpr float kKvBelow = 4.0f, kKvAbove = 12.0f;
+
+struct F32x2 {
+  float x, y;
+};
+
+// One row's element d of a query, 8 of them from d on, as float32.
+template <int N>
+__device__ __forceinline__ void kv_query8(float (&x)[N], const KvAttnArgs &a, int64_t at, int32_t d) {
+  static_assert(N == 8, "eight values");
+  if (a.vec && d < a.b.dim) {
+    if (a.dtype == RNSMX_FLOAT32) {
+      const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + at + d);
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        x[j] = p[j / 4][j % 4];
+      });
+    } else {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q) + at + d);
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        const uint16_t bits = static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2)));
+        x[j] = a.dtype == RNSMX_FLOAT16 ? static_cast<float>(__builtin_bit_cast(_Float16, bits)) : kv_bf16(bits);
+      });
+    }
+  } else {
+    kv_for<8>([&](auto J) {
+      constexpr int j = J;
+      x[j] = d + j < a.b.dim ? kv_load(a.q, at + d + j, a.dtype) : 0.0f;
+    });
+  }
+}
+
+// The power of two that brings a row's largest query below 2^15 (as its
+// exponent); a row of zeros or with an infinity stays as it is.
+__device__ __forceinline__ int32_t kv_query_exponent(float top) {
+  return max(top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0, -120);
+}
+
+// Eight tokens of a mask's row from t on, as they are stored (0 from mask_len
+// on): loads that do not depend on each other or on what is seen.
+__device__ __forceinline__ void kv_mask_load(uint32_t (&m)[8], const KvAttnArgs &a, int64_t row, int32_t q_head, int32_t t) {
+  const int64_t at = row * a.mask_rs + static_cast<int64_t>(q_head) * a.mask_hs;
+  kv_for<8>([&](auto J) {
+    const int64_t i = at + static_cast<int64_t>(min(t + J, a.mask_len - 1)) * a.mask_ts;
+    if (a.mask_len <= 0)
+      m[J] = 0;
+    else if (a.mask_dtype == RNSMX_INT8)
+      m[J] = static_cast<const uint8_t *>(a.mask)[i];
+    else if (a.mask_dtype == RNSMX_FLOAT32)
+      m[J] = static_cast<const uint32_t *>(a.mask)[i];
+    else
+      m[J] = static_cast<const uint16_t *>(a.mask)[i];
+  });
+}
+// Whether it hides token t; an additive mask's value goes onto the score.
+__device__ __forceinline__ bool kv_mask_hides(const KvAttnArgs &a, uint32_t m, int32_t t, float &x) {
+  if (t >= a.mask_len) return true;
+  if (a.mask_dtype == RNSMX_INT8) return m == 0;
+  const float v = a.mask_dtype == RNSMX_FLOAT32   ? __uint_as_float(m)
+                  : a.mask_dtype == RNSMX_FLOAT16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m)))
+                                                  : kv_bf16(static_cast<uint16_t>(m));
+  x += v;
+  return v == -INFINITY;
+}
+
+// One candidate (x, lv) for a row's reference against another, e and e2 being
+// how far each lies above the present one: of those that pass kKvAbove the one
+// with the larger sum, of equals the larger x, then the larger lv, so that lanes
+// that exchange theirs take the same one.
+template <bool MASK>
+__device__ __forceinline__ void kv_higher(float &e, float &x, float &lv, float e2, float x2, float lv2) {
+  constexpr float kNat = MASK ? kKvLog2e : 1.0f;
+  const float s1 = x * kNat + lv, s2 = x2 * kNat + lv2;
+  const bool take = !(e > kKvAbove) ? e2 > kKvAbove
+                                    : (e2 > kKvAbove && (s2 > s1 || (s2 == s1 && (x2 > x || (x2 == x && lv2 > lv)))));
+  e = take ? e2 : e;
+  x = take ? x2 : x;
+  lv = take ? lv2 : lv;
+}
+
+}  // namespace rnsmx

@@ -276,18 +276,33 @@ static int32_t grid_of(int64_t groups, unsigned &grid) {
     RNSMX_KV_DIM_CASE(256, __VA_ARGS__)  \
   }
 
-// The split of a call's tokens over workgroups.
+// How a call's tokens are split over waves and workgroups (device time, 32-wide
+// pages and up).  Eight waves take a step of 256 tokens where the workgroups
+// leave room for them on the chip (24 x 8 heads of 80, window 1023: 13.6 us, 15.3
+// with four) or sequences are long (62 x 32 heads of 128, up to 4096 tokens: 222,
+// 230); many short ones take four (256 x 12 heads of 64, 512 tokens: 34.7, 44.2
+// with eight).  Splitting costs the parts' way through memory and the ticket's,
+// some 5 us: not past a workgroup a CU (one token against 131071, 8 heads: 61 us,
+// 69 with twice as many), and not below 1024 tokens each (32 heads, 1024 tokens:
+// 12.0 whole, 13.7 in two).
+constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWideTokens = 4096;
 static void kv_split(KvAttnArgs &a) {
   const int64_t span = a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32)
                                     : a.b.max_length;
   const int64_t tasks = static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles;
-  const int64_t steps = std::max<int64_t>(1, (span + kKvChunkUnit - 1) / kKvChunkUnit);
+  a.waves = kv_wide(a.b.row_bytes) && span > 128 && (tasks < kWideTasks || span >= kWideTokens) ? 8 : 4;
+  const int64_t unit = 32 * a.waves;
+  const int64_t steps = std::max<int64_t>(1, (span + unit - 1) / unit);
   int64_t splits = 1;
-  if (tasks > 0 && tasks <= RNSMX_KV_TICKETS) splits = std::max<int64_t>(1, std::min<int64_t>(steps, 768 / tasks));
+  if (a.tile_rows == kKvRows && tasks > 0 && tasks <= RNSMX_KV_TICKETS)
+    splits = std::max<int64_t>(1, std::min(span / kSplitTokens, kSplitGroups / tasks));
   const int64_t each = (steps + splits - 1) / splits;
-  a.chunk = static_cast<int32_t>(std::min<int64_t>(each * kKvChunkUnit, 1 << 30));
+  a.chunk = static_cast<int32_t>(std::min<int64_t>(each * unit, 1 << 30));
   a.splits = static_cast<int32_t>((steps + each - 1) / each);
 }
+
+// Up to so many rows of a sequence and key/value head run 16 to a workgroup.
+constexpr int64_t kFewRows = 64;
 
 static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const rnsmx_kv_query_t *query,
                             KvAttnArgs &a) {
@@ -316,17 +331,22 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   a.mask_dtype = query->mask_dtype;
   a.mask_len = query->mask_len;
   a.q_heads = query->q_heads;
-  a.group = query->q_heads / cache->heads;
   a.dtype = query->dtype;
   a.causal = query->causal != 0;
   a.window = query->window;
   a.scale = query->scale;
   a.vec = cache->head_dim % 8 == 0 && aligned(query->q_dev, 16) && query->row_stride * size % 16 == 0 &&
           query->head_stride * size % 16 == 0;
-  const int64_t tiles = (static_cast<int64_t>(a.b.max_rows) * a.group + kKvRowTile - 1) / kKvRowTile;
+  const int64_t rows = static_cast<int64_t>(a.b.max_rows) * (query->q_heads / cache->heads);
+  a.tile_rows = rows <= kFewRows ? kKvRows : kKvTileRows;
+  const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows;
   if (tiles > 0x7FFFFFFF) return fail(RNSMX_EINVAL, "too many rows");
   a.row_tiles = static_cast<int32_t>(tiles);
   kv_split(a);
+  a.by_group = kv_div(query->q_heads / cache->heads);
+  a.by_splits = kv_div(a.splits);
+  a.by_tiles = kv_div(std::max(a.row_tiles, 1));
+  a.by_heads = kv_div(cache->heads);
   return RNSMX_OK;
 }
 
@@ -334,7 +354,7 @@ static int64_t kv_tasks(const KvAttnArgs &a) { return static_cast<int64_t>(a.b.s
 
 static int64_t kv_workspace(const KvAttnArgs &a) {
   if (a.splits < 2) return 0;
-  return RNSMX_KV_TICKETS * 4 + kv_tasks(a) * a.splits * kv_partial_floats(a.b.row_bytes) * 4;
+  return RNSMX_KV_TICKETS * 4 + kv_tasks(a) * a.splits * kv_partial_floats(a.tile_rows, a.b.row_bytes) * 4;
 }
 
 }  // namespace rnsmx
@@ -440,7 +460,12 @@ int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t
   if (int32_t rc = grid_of(kv_tasks(a) * a.splits, grid)) return rc;
   if (grid == 0) return RNSMX_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_rows<DT>(a, st))
+  a.out_vec = aligned(out_dev, 16);
+  if (a.tile_rows == kKvTileRows) {
+    RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_tiles<DT>(a, st))
+  } else {
+    RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_rows<DT>(a, st))
+  }
   return kv_check("kv_attention");
 }
 

@@ -1,0 +1,362 @@
+// Attention of many query rows (prompts) over the 8-bit key/value cache (built
+// once per row size, RNSMX_KV_DIM).
+#include "rnsmx_kv_attn.hpp"
+
+namespace rnsmx {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// v_mfma_f32_32x32x16_f16: lane l feeds row (l & 31) of A and column (l & 31)
+// of B, both at k = 8 * (l >> 5) + 0..7, and gets rows 8 (i / 4) + 4 (l >> 5) +
+// i % 4, i = 0..15, of column (l & 31).
+__device__ __forceinline__ f32x16 kv_mfma32(h16x8 a, h16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kStep = 64;  // tokens of a step
+
+// The token of A's row r that leaves lane half h tokens 8 h .. 8 h + 7 and 16 +
+// 8 h .. of 32 in its 16 results, in order: what P^T's operand wants.
+__device__ __forceinline__ int32_t tile_token(int32_t r) {
+  const int32_t i = 4 * (r >> 3) + (r & 3);
+  return 16 * (i >> 3) + 8 * ((r >> 2) & 1) + (i & 7);
+}
+// 16-byte columns of the staged tiles are exchanged by these, so that the eight
+// lanes that the shared memory serves at a time meet eight of its columns: keys
+// are read by tile_token's rows and written along a row, values read down eight
+// rows and written four rows apart.
+__device__ __forceinline__ int32_t key_swap(int32_t t) { return (t & 3) | ((t >> 3 & 1) << 2); }
+__device__ __forceinline__ int32_t value_swap(int32_t d) { return (d & 7) ^ (d >> 2 & 7); }
+
+// A workgroup of four waves for 128 query rows (32 a wave, token-major over the
+// heads of a group) of one sequence and key/value head.  Steps of 64 tokens are
+// staged for all four as halves, keys by token and values by column, each code
+// converted once; wave w loads and converts tokens 16 w .. 16 w + 15, which lie
+// in one page.  The products and the weights are as kv_rows_kernel's, with
+// 32 x 32 products: a row is one lane pair's.
+template <int DT, bool SPLIT, bool MASK>
+__global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(const KvAttnArgs a) {
+  constexpr int KS = DT / 16, DB = DT / 32, QN = SPLIT ? 2 : 1;
+  constexpr int KROW = (DT + 63) / 64 * 64;  // halves of a staged key
+  constexpr int KR = DT / 32;                // loads of 8 codes a lane and step, keys
+  constexpr int VD = DT == 64 ? 2 : DT == 256 ? 8 : 4;  // columns of 8 tokens that a lane converts
+  constexpr int VG = DT / VD, VR = (2 * VG + 63) / 64;  // of a token group, and rounds
+  __shared__ __attribute__((aligned(128))) _Float16 keys[2][kStep * KROW];
+  __shared__ __attribute__((aligned(128))) _Float16 values[2][DT * kStep];
+  __shared__ float pages_of_step[2][4][4];  // key scale, log2 and reciprocal of the value scale, whether it is there
+
+  const KvBatchArgs &b = a.b;
+  uint32_t id = kv_xcd_order(blockIdx.x, gridDim.x);
+  const int32_t tile = a.row_tiles - 1 - static_cast<int32_t>(kv_rem(a.by_tiles, id));  // the longest first
+  const int32_t head = kv_rem(a.by_heads, id), seq = id, group = a.by_group.d;
+  const KvSeq q = kv_seq(b, seq);
+  const int32_t rows = q.n * group, row0 = tile * kKvTileRows;
+  if (row0 >= rows) return;
+  const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t col = lane & 31, h = lane >> 5;
+  const int32_t base = q.len - q.n;
+  auto kv_of = [&](int32_t r) { return static_cast<int32_t>(kv_quot(a.by_group, r)); };  // the token of a row
+  // what the workgroup's rows see, and this wave's
+  const int32_t last_row = min(row0 + kKvTileRows, rows) - 1;
+  const int32_t hi = max(a.causal ? base + kv_of(last_row) + 1 : q.len, 0);
+  const int32_t lo = a.window > 0 ? max(base + kv_of(row0) + 1 - a.window, 0) & ~(kStep - 1) : 0;
+  const int32_t w_first = row0 + 32 * wave, w_last = min(w_first + 31, rows - 1);
+  const bool w_any = w_first < rows;
+  const int32_t t_first = kv_of(w_first), t_last = kv_of(w_last);
+  const int32_t w_hi = !w_any ? 0 : a.causal ? base + t_last + 1 : q.len;
+  const int32_t w_lo = a.window > 0 ? base + t_first + 1 - a.window : 0;
+  const int32_t full_hi = a.causal ? base + t_first + 1 : q.len;
+  const int32_t full_lo = a.window > 0 ? max(base + t_last + 1 - a.window, 0) : 0;
+
+  const int32_t row = min(w_first + col, rows - 1);
+  const int32_t t_row = kv_of(row), q_head = head * group + (row - t_row * group);
+  const int32_t end_row = a.causal ? base + t_row + 1 : q.len;
+  const int32_t begin_row = a.window > 0 ? max(base + t_row + 1 - a.window, 0) : 0;
+
+  // loads of a step: this wave's 16 tokens
+  u32x2 kr[KR];
+  uint32_t vr[VR][8][VD / 4 + 1];
+  F32x2 sr;
+  bool there = false;
+  // read through the scalar cache: one number a wave, whose wait leaves the
+  // codes' loads in flight
+  const kv_const_i32 *table = (const kv_const_i32 *)(b.table + seq * b.table_stride);
+  const int32_t in_page = (1 << b.log_page) - 1;
+  auto page_of = [&](int32_t t0) {
+    return table[min((t0 + 16 * wave) >> b.log_page, b.table_width - 1)];
+  };
+  auto load_step = [&](int32_t t0, int32_t page) {
+    there = static_cast<uint32_t>(page) < static_cast<uint32_t>(b.blocks);
+    const int64_t slot = static_cast<int64_t>(there ? page : 0) * b.heads + head;
+    const int64_t at = ((slot << b.log_page) + ((t0 + 16 * wave) & in_page)) * DT;
+    kv_for<KR>([&](auto R) {
+      constexpr int r = R;
+      kr[r] = *reinterpret_cast<const u32x2 *>(b.k + at + lane * 8 + r * 512);
+    });
+    kv_for<VR>([&](auto R) {
+      constexpr int r = R;
+      const int32_t item = lane + 64 * r;
+      if (2 * VG % 64 == 0 || item < 2 * VG) {
+        const uint8_t *p = b.v + at + (item / VG) * 8 * DT + (item % VG) * VD;
+        kv_for<8>([&](auto J) {
+          constexpr int j = J;
+          if constexpr (VD == 8) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(p + j * DT);
+            vr[r][j][0] = w[0];
+            vr[r][j][1] = w[1];
+          } else if constexpr (VD == 4) {
+            vr[r][j][0] = *reinterpret_cast<const uint32_t *>(p + j * DT);
+          } else {
+            vr[r][j][0] = *reinterpret_cast<const uint16_t *>(p + j * DT);
+          }
+        });
+      }
+    });
+    sr = *reinterpret_cast<const F32x2 *>(b.scales + slot * 2);
+  };
+  auto stage = [&](int32_t buf) {
+    kv_for<KR>([&](auto R) {
+      constexpr int r = R;
+      const int32_t item = lane + 64 * r, t = 16 * wave + item / (DT / 8), c = item % (DT / 8);
+      *reinterpret_cast<h16x8 *>(&keys[buf][t * KROW + (c ^ key_swap(t)) * 8]) = kv_row8(kr[r][0], kr[r][1]);
+    });
+    kv_for<VR>([&](auto R) {
+      constexpr int r = R;
+      const int32_t item = lane + 64 * r;
+      if (2 * VG % 64 == 0 || item < 2 * VG) {
+        const int32_t group = 2 * wave + item / VG, d0 = (item % VG) * VD;
+        kv_for<VD>([&](auto I) {
+          constexpr int i = I, w = i / 4, byte = i % 4;
+          const auto &v = vr[r];
+          const h16x8 x = kv_join(kv_halves<byte, byte>(v[0][w], v[1][w]), kv_halves<byte, byte>(v[2][w], v[3][w]),
+                                  kv_halves<byte, byte>(v[4][w], v[5][w]), kv_halves<byte, byte>(v[6][w], v[7][w]));
+          *reinterpret_cast<h16x8 *>(&values[buf][(d0 + i) * kStep + (group ^ value_swap(d0 + i)) * 8]) = x;
+        });
+      }
+    });
+    if (lane == 0) {
+      pages_of_step[buf][wave][0] = sr.x;
+      pages_of_step[buf][wave][1] = __builtin_amdgcn_logf(sr.y);
+      pages_of_step[buf][wave][2] = __builtin_amdgcn_rcpf(sr.y);
+      pages_of_step[buf][wave][3] = there ? 1.0f : 0.0f;
+    }
+  };
+
+  int32_t page = 0;
+  if (lo < hi) {
+    load_step(lo, page_of(lo));
+    page = page_of(lo + kStep);
+  }
+
+  h16x8 qf[QN][KS];
+  float q_scale;
+  {
+    float x[KS][8];
+    const int64_t at = static_cast<int64_t>(q.row + t_row) * a.q_rs + static_cast<int64_t>(q_head) * a.q_hs;
+    float top = 0.0f;
+    kv_for<KS>([&](auto S) {
+      constexpr int s = S;
+      kv_query8(x[s], a, at, 16 * s + 8 * h);
+      kv_for<8>([&](auto J) { top = fmaxf(top, fabsf(x[s][J])); });
+    });
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const int32_t e = kv_query_exponent(top);
+    kv_for<KS>([&](auto S) {
+      constexpr int s = S;
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        const float v = ldexpf(x[s][j], -e);
+        const _Float16 half = static_cast<_Float16>(v);
+        qf[0][s][j] = half;
+        if constexpr (SPLIT) qf[1][s][j] = static_cast<_Float16>(v - static_cast<float>(half));
+      });
+    });
+    q_scale = ldexpf(a.scale * kKvUnit, e);
+    if constexpr (!MASK) q_scale *= kKvLog2e;
+  }
+
+  f32x16 o[DB];
+  kv_for<DB>([&](auto I) { kv_for<16>([&](auto J) { o[I][static_cast<int>(J)] = 0.0f; }); });
+  // the row's reference and its weights' sum over the value scale, in units of 2^ml
+  float mx = -INFINITY, ml = 0.0f, sum = 0.0f;
+  constexpr float kNat = MASK ? kKvLog2e : 1.0f;
+
+  auto compute = [&](int32_t buf, int32_t t0) {
+    f32x16 acc[2];
+    kv_for<2>([&](auto B) { kv_for<16>([&](auto J) { acc[B][static_cast<int>(J)] = 0.0f; }); });
+    const int32_t kt = tile_token(col), swap = key_swap(kt);
+    kv_for<KS>([&](auto S) {
+      constexpr int s = S;
+      kv_for<2>([&](auto B) {
+        constexpr int sub = B;
+        const h16x8 k = *reinterpret_cast<const h16x8 *>(&keys[buf][(32 * sub + kt) * KROW + (((2 * s + h)) ^ swap) * 8]);
+        kv_for<QN>([&](auto P) { acc[sub] = kv_mfma32(k, qf[P][s], acc[sub]); });
+      });
+    });
+    float c[4], lv[4], rv[4], w[4][8], xm[4];
+    bool there[4], all_there = true;
+    kv_for<4>([&](auto G) {
+      constexpr int g = G;
+      const f32x4 sc = *reinterpret_cast<const f32x4 *>(pages_of_step[buf][g]);
+      c[g] = q_scale * sc[0];
+      lv[g] = sc[1];
+      rv[g] = sc[2];
+      there[g] = sc[3] != 0.0f;
+      all_there = all_there && there[g];
+      // results i of a product are tokens 16 (i / 8) + 8 h + i % 8: four groups of eight
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        const float x = acc[g / 2][8 * (g % 2) + j];
+        w[g][j] = MASK ? x * c[g] : x;
+      });
+    });
+    // what every row of the wave sees needs no look at single tokens
+    if (MASK || t0 < full_lo || t0 + kStep > full_hi || !__all(all_there))
+      // scores of what is not seen are minus infinity; a lane that sees none of
+      // a group does without its page's scales, which may be anything
+      kv_for<4>([&](auto G) {
+        constexpr int g = G;
+        const int32_t t8 = t0 + 16 * g + 8 * h;
+        uint32_t m[8];
+        if constexpr (MASK) kv_mask_load(m, a, q.row + t_row, q_head, t8);
+        bool any = false;
+        kv_for<8>([&](auto J) {
+          constexpr int j = J;
+          bool see = there[g] && t8 + j < end_row && t8 + j >= begin_row;
+          if constexpr (MASK) see = !kv_mask_hides(a, m[j], t8 + j, w[g][j]) && see;
+          w[g][j] = see ? w[g][j] : -INFINITY;
+          any |= see;
+        });
+        c[g] = any ? c[g] : 1.0f;
+        lv[g] = any ? lv[g] : 0.0f;
+        rv[g] = any ? rv[g] : 0.0f;
+      });
+    kv_for<4>([&](auto G) {
+      constexpr int g = G;
+      xm[g] = w[g][0];
+      kv_for<7>([&](auto J) { xm[g] = fmaxf(xm[g], w[g][J + 1]); });
+      if constexpr (!MASK) xm[g] *= c[g];
+    });
+    float em[4];
+    bool above = false;
+    kv_for<4>([&](auto G) {
+      constexpr int g = G;
+      em[g] = (xm[g] - mx) * kNat + (lv[g] - ml);
+      above |= em[g] > kKvAbove;
+    });
+    if (__any(above)) {
+      float best = em[0], bx = xm[0], bl = lv[0];
+      kv_for<3>([&](auto G) { kv_higher<MASK>(best, bx, bl, em[G + 1], xm[G + 1], lv[G + 1]); });
+      kv_higher<MASK>(best, bx, bl, __shfl_xor(best, 32), __shfl_xor(bx, 32), __shfl_xor(bl, 32));
+      if (best > kKvAbove) {
+        const float nl = bl - kKvBelow;
+        const float fo = __builtin_amdgcn_exp2f((mx - bx) * kNat + (ml - nl));
+        sum *= fo;
+        kv_for<DB>([&](auto I) { o[I] *= fo; });
+        mx = bx;
+        ml = nl;
+      }
+    }
+    h16x8 p[QN][4];
+    // a row without a reference has nothing but minus infinities (and not-a-numbers) so far
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    kv_for<4>([&](auto G) {
+      constexpr int g = G;
+      const float off = MASK ? lv[g] - ml : lv[g] - ml - ref;
+      float part = 0.0f;
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        w[g][j] = __builtin_amdgcn_exp2f(MASK ? fmaf(w[g][j] - ref, kNat, off) : fmaf(w[g][j], c[g], off));
+        part += w[g][j];
+      });
+      sum = fmaf(part, rv[g], sum);
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        const _Float16 half = static_cast<_Float16>(w[g][j]);
+        p[0][g][j] = half;
+        if constexpr (SPLIT) p[1][g][j] = static_cast<_Float16>(w[g][j] - static_cast<float>(half));
+      });
+    });
+    kv_for<DB>([&](auto I) {
+      constexpr int i = I;
+      const int32_t d = 32 * i + col, vswap = value_swap(d);
+      kv_for<4>([&](auto G) {
+        constexpr int g = G;
+        const h16x8 v = *reinterpret_cast<const h16x8 *>(&values[buf][d * kStep + ((2 * g + h) ^ vswap) * 8]);
+        kv_for<QN>([&](auto P) { o[i] = kv_mfma32(v, p[P][g], o[i]); });
+      });
+    });
+  };
+
+  if (lo < hi) {
+    stage(0);
+    int32_t buf = 0;
+    for (int32_t t0 = lo; t0 < hi; t0 += kStep, buf ^= 1) {
+      __syncthreads();  // this step is staged, and the other buffer's readers are done
+      const bool more = t0 + kStep < hi;
+      if (more) {
+        load_step(t0 + kStep, page);
+        page = page_of(t0 + 2 * kStep);
+      }
+      if (t0 < w_hi && t0 + kStep > w_lo) compute(buf, t0);
+      if (more) stage(buf ^ 1);
+    }
+  }
+  if (!w_any) return;
+
+  sum += __shfl_xor(sum, 32);
+  if (w_first + col >= rows) return;
+  // l = sum 2^ml, and the codes' unit
+  const float f = sum == 0.0f ? 0.0f : kKvUnit / sum;
+  const int64_t out = (static_cast<int64_t>(q.row + t_row) * a.q_heads + q_head) * b.dim;
+  kv_for<DB>([&](auto I) {
+    kv_for<4>([&](auto R) {
+      constexpr int i = I, r = R;
+      const int32_t d = 32 * i + 8 * r + 4 * h;
+      float y[4];
+      kv_for<4>([&](auto J) {
+        constexpr int j = J;
+        y[j] = sum == 0.0f ? 0.0f : o[i][4 * r + j] * f;
+      });
+      if (a.out_vec && b.dim % 4 == 0) {
+        if (d >= b.dim) return;
+        if (a.dtype == RNSMX_FLOAT32) {
+          *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + out + d) = f32x4{y[0], y[1], y[2], y[3]};
+        } else {
+          uint16_t bits[4];
+          kv_for<4>([&](auto J) {
+            constexpr int j = J;
+            bits[j] = a.dtype == RNSMX_FLOAT16 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(y[j])) : kv_to_bf16(y[j]);
+          });
+          *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + out + d) =
+              u32x2{bits[0] | static_cast<uint32_t>(bits[1]) << 16, bits[2] | static_cast<uint32_t>(bits[3]) << 16};
+        }
+      } else {
+        kv_for<4>([&](auto J) {
+          constexpr int j = J;
+          if (d + j < b.dim) kv_store(a.out, out + d + j, a.dtype, y[j]);
+        });
+      }
+    });
+  });
+}
+
+template <int DT>
+void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles)), block(256);
+  const bool split = a.dtype == RNSMX_FLOAT32;
+  if (a.mask) {
+    if (split)
+      hipLaunchKernelGGL((kv_tiles_kernel<DT, true, true>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((kv_tiles_kernel<DT, false, true>), grid, block, 0, st, a);
+  } else if (split) {
+    hipLaunchKernelGGL((kv_tiles_kernel<DT, true, false>), grid, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((kv_tiles_kernel<DT, false, false>), grid, block, 0, st, a);
+  }
+}
+
+template void launch_kv_tiles<RNSMX_KV_DIM>(const KvAttnArgs &a, hipStream_t st);
+
+}  // namespace rnsmx

@@ -24,7 +24,8 @@ KV_DIMS = (64, 96, 128, 160, 192, 256)  # row sizes of the key/value cache
 UNITS = [("rnsmx_kernels.hip", "rnsmx_kernels", []), ("rnsmx_bytes.hip", "rnsmx_bytes", []),
          ("rnsmx_linear.hip", "rnsmx_linear", []), ("rnsmx_units.hip", "rnsmx_units", []),
          ("rnsmx_kv_cache.hip", "rnsmx_kv_cache", []), ("rnsmx_host.cpp", "rnsmx_host", [])] + [
-    ("rnsmx_kv_rows.hip", f"rnsmx_kv_rows_{d}", [f"-DRNSMX_KV_DIM={d}"]) for d in KV_DIMS] + [
+    (f"rnsmx_kv_{part}.hip", f"rnsmx_kv_{part}_{d}", [f"-DRNSMX_KV_DIM={d}"])
+    for part in ("rows", "tiles") for d in KV_DIMS] + [
     ("rnsmx_gemm_part.hip", f"rnsmx_gemm_r{r}_p{p}", [f"-DRNSMX_RCAP={r}", f"-DRNSMX_PART={p}"])
     for r in GEMM_CAPACITIES for p in range(GEMM_PARTS)]
 ARCH = os.environ.get("RNSMX_OFFLOAD_ARCH", "gfx950")

@@ -542,8 +542,8 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
                       void *k_dev, void *v_dev, int32_t dtype, void *stream);
 
 /*
- * The queries of rnsmx_kv_attention.  q_dev [rows][q_heads][head_dim] at the
- * given strides in elements, q_heads a multiple of the cache's heads (head h
+ * How rnsmx_kv_attention reads its queries and masks.  q_dev [rows][q_heads]
+ * [head_dim] at the given strides in elements, q_heads a multiple of the cache's heads (head h
  * reads key/value head h / (q_heads / heads)).  A row sees the tokens up to its
  * own (causal 1; with window > 0 the last `window` of them) or all of its
  * sequence (causal 0), but for those that the mask hides.  mask_dev (null: none)
@@ -554,13 +554,11 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
  * holds there, and a row that sees no token is zero.
  */
 typedef struct rnsmx_kv_query {
-  const void *q_dev;
   int64_t row_stride, head_stride;
-  const void *mask_dev;
   int64_t mask_row_stride, mask_head_stride, mask_token_stride;
   int32_t dtype; /* of q and of the output */
   int32_t q_heads;
-  int32_t mask_dtype;
+  int32_t mask_dtype; /* mask fields are ignored without a mask */
   int32_t mask_len;
   int32_t causal;
   int32_t window; /* 0: none */
@@ -583,7 +581,8 @@ int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const 
  * sums, maxima and exponentials.
  */
 int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
-                           const rnsmx_kv_query_t *query, void *workspace_dev,
+                           const rnsmx_kv_query_t *query, const void *q_dev,
+                           const void *mask_dev, void *workspace_dev,
                            int64_t workspace_bytes, void *out_dev, void *stream);
 
 #ifdef __cplusplus

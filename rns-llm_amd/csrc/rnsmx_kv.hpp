@@ -124,17 +124,21 @@ constexpr int kKvRows = 16;          // query rows of a workgroup of kv_rows_ker
 // Whether it is built with eight waves: row sizes whose waves are two to a SIMD.
 constexpr bool kv_wide(int row_bytes) { return row_bytes <= 160; }
 
-// Floats of one split's partial result: rows of row_bytes values, then each
-// row's reference and sum.
-inline int64_t kv_partial_floats(int32_t rows, int32_t row_bytes) {
-  return static_cast<int64_t>(rows) * (static_cast<int64_t>(row_bytes) + 2);
-}
+// Floats of one split's partial result.  Of kv_rows_kernel: rows of row_bytes
+// values, then each row's reference and sum; of kv_tiles_kernel: what the 256
+// lanes hold, row_bytes / 2 values, a reference of two and a sum each.
+constexpr int64_t kv_row_floats(int row_bytes) { return kKvRows * (static_cast<int64_t>(row_bytes) + 2); }
+constexpr int64_t kv_tile_floats(int row_bytes) { return 256 * (static_cast<int64_t>(row_bytes) / 2 + 4); }
 
 // Workgroups go to the 8 XCDs in turn: the n-th of an XCD takes the n-th of a
-// contiguous part of the work, so that what shares keys shares an L2.
-__device__ __forceinline__ int32_t kv_xcd_order(uint32_t id, uint32_t count) {
-  const uint32_t xcd = id & 7, per = count >> 3, more = count & 7;
-  return static_cast<int32_t>(xcd * per + min(xcd, more) + (id >> 3));
+// contiguous part of the work, so that what shares keys shares an L2.  turn: of
+// work ordered from long to short and two workgroups to a CU, every other 32 (an
+// XCD's CUs) in reverse, so that the long ones share theirs with the short.
+__device__ __forceinline__ int32_t kv_xcd_order(uint32_t id, uint32_t count, bool turn = false) {
+  const uint32_t xcd = id & 7, per = count >> 3, more = count & 7, size = per + (xcd < more ? 1 : 0);
+  uint32_t n = id >> 3;
+  if (turn && (n & 32) && (n | 31) < size) n ^= 31;
+  return static_cast<int32_t>(xcd * per + min(xcd, more) + n);
 }
 
 // rnsmx_kv_rows.hip, one object per row size

@@ -38,31 +38,70 @@ struct F32x2 {
   float x, y;
 };
 
-// One row's element d of a query, 8 of them from d on, as float32.
-template <int N>
-__device__ __forceinline__ void kv_query8(float (&x)[N], const KvAttnArgs &a, int64_t at, int32_t d) {
-  static_assert(N == 8, "eight values");
-  if (a.vec && d < a.b.dim) {
-    if (a.dtype == RNSMX_FLOAT32) {
-      const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + at + d);
-      kv_for<8>([&](auto J) {
-        constexpr int j = J;
-        x[j] = p[j / 4][j % 4];
-      });
-    } else {
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q) + at + d);
-      kv_for<8>([&](auto J) {
-        constexpr int j = J;
-        const uint16_t bits = static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2)));
-        x[j] = a.dtype == RNSMX_FLOAT16 ? static_cast<float>(__builtin_bit_cast(_Float16, bits)) : kv_bf16(bits);
-      });
-    }
+// A row's queries as float32, S groups of 8 from column first(s) on, zeros past
+// the head dimension.  Every load is issued before the first is waited for: no
+// branch but on what is one for the call, columns past the end read the last.
+template <int S, bool SPLIT, typename F>
+__device__ __forceinline__ void kv_query(float (&x)[S][8], const KvAttnArgs &a, int64_t at, F &&first) {
+  const int32_t dim = a.b.dim;
+  if (a.vec) {
+    kv_for<S>([&](auto G) {
+      constexpr int g = G;
+      const int32_t d = min(first(G), dim - 8);
+      if constexpr (SPLIT) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(a.q) + at + d);
+        const f32x4 lo = p[0], hi = p[1];
+        kv_for<4>([&](auto J) {
+          constexpr int j = J;
+          x[g][j] = lo[j];
+          x[g][j + 4] = hi[j];
+        });
+      } else {
+        // two halves to a word until all are here
+        const f32x4 w = *reinterpret_cast<const f32x4 *>(static_cast<const uint16_t *>(a.q) + at + d);
+        kv_for<4>([&](auto J) {
+          constexpr int j = J;
+          x[g][j] = w[j];
+        });
+      }
+    });
   } else {
-    kv_for<8>([&](auto J) {
-      constexpr int j = J;
-      x[j] = d + j < a.b.dim ? kv_load(a.q, at + d + j, a.dtype) : 0.0f;
+    kv_for<S>([&](auto G) {
+      constexpr int g = G;
+      kv_for<8>([&](auto J) {
+        constexpr int j = J;
+        const int64_t i = at + min(first(G) + j, dim - 1);
+        if constexpr (SPLIT) {
+          x[g][j] = static_cast<const float *>(a.q)[i];
+        } else {
+          const uint32_t bits = static_cast<const uint16_t *>(a.q)[i];
+          x[g][j / 2] = __uint_as_float(j % 2 ? __float_as_uint(x[g][j / 2]) | bits << 16 : bits);
+        }
+      });
     });
   }
+  kv_for<S>([&](auto G) {
+    constexpr int g = G;
+    if constexpr (!SPLIT) {
+      uint32_t w[4];
+      kv_for<4>([&](auto J) { w[J] = __float_as_uint(x[g][J]); });
+      if (a.dtype == RNSMX_FLOAT16) {
+        kv_for<8>([&](auto J) {
+          constexpr int j = J;
+          x[g][j] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2)))));
+        });
+      } else {
+        kv_for<8>([&](auto J) {
+          constexpr int j = J;
+          x[g][j] = __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+        });
+      }
+    }
+    kv_for<8>([&](auto J) {
+      constexpr int j = J;
+      x[g][j] = first(G) + j < dim ? x[g][j] : 0.0f;
+    });
+  });
 }
 
 // The power of two that brings a row's largest query below 2^15 (as its

@@ -286,16 +286,19 @@ static int32_t grid_of(int64_t groups, unsigned &grid) {
 // 69 with twice as many), and not below 1024 tokens each (32 heads, 1024 tokens:
 // 12.0 whole, 13.7 in two).
 constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWideTokens = 4096;
+constexpr int64_t kTileGroups = 768, kTileTokens = 512;
 static void kv_split(KvAttnArgs &a) {
   const int64_t span = a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32)
                                     : a.b.max_length;
   const int64_t tasks = static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles;
-  a.waves = kv_wide(a.b.row_bytes) && span > 128 && (tasks < kWideTasks || span >= kWideTokens) ? 8 : 4;
-  const int64_t unit = 32 * a.waves;
+  const bool few = a.tile_rows == kKvRows;
+  a.waves = few && kv_wide(a.b.row_bytes) && span > 128 && (tasks < kWideTasks || span >= kWideTokens) ? 8 : 4;
+  const int64_t unit = few ? 32 * a.waves : 64;
   const int64_t steps = std::max<int64_t>(1, (span + unit - 1) / unit);
   int64_t splits = 1;
-  if (a.tile_rows == kKvRows && tasks > 0 && tasks <= RNSMX_KV_TICKETS)
-    splits = std::max<int64_t>(1, std::min(span / kSplitTokens, kSplitGroups / tasks));
+  if (tasks > 0 && tasks <= RNSMX_KV_TICKETS)
+    splits = few ? std::min(span / kSplitTokens, kSplitGroups / tasks) : std::min(span / kTileTokens, kTileGroups / tasks);
+  splits = std::max<int64_t>(splits, 1);
   const int64_t each = (steps + splits - 1) / splits;
   a.chunk = static_cast<int32_t>(std::min<int64_t>(each * unit, 1 << 30));
   a.splits = static_cast<int32_t>((steps + each - 1) / each);
@@ -313,18 +316,8 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
     return fail(RNSMX_EINVAL, "query heads are a multiple of the cache's heads");
   if (!(query->scale > 0.0f) || !std::isfinite(query->scale)) return fail(RNSMX_EINVAL, "the scale is positive and finite");
   if (query->window < 0 || (query->window > 0 && !query->causal)) return fail(RNSMX_EINVAL, "a window needs causal rows");
-  if (query->mask_dev) {
-    if (query->mask_dtype != RNSMX_INT8 && !is_float(query->mask_dtype))
-      return fail(RNSMX_EINVAL, "masks are bytes, float32, float16 or bfloat16");
-    if (query->mask_len < 0) return fail(RNSMX_EINVAL, "bad mask length");
-    if (!aligned(query->mask_dev, dtype_bytes(query->mask_dtype))) return fail(RNSMX_EINVAL, "the mask is not aligned to its type");
-  }
-  const int64_t size = dtype_bytes(query->dtype);
-  if (a.b.rows > 0 && (!query->q_dev || !aligned(query->q_dev, size))) return fail(RNSMX_EINVAL, "queries null or not aligned to their type");
-  a.q = query->q_dev;
   a.q_rs = query->row_stride;
   a.q_hs = query->head_stride;
-  a.mask = query->mask_dev;
   a.mask_rs = query->mask_row_stride;
   a.mask_hs = query->mask_head_stride;
   a.mask_ts = query->mask_token_stride;
@@ -335,8 +328,6 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   a.causal = query->causal != 0;
   a.window = query->window;
   a.scale = query->scale;
-  a.vec = cache->head_dim % 8 == 0 && aligned(query->q_dev, 16) && query->row_stride * size % 16 == 0 &&
-          query->head_stride * size % 16 == 0;
   const int64_t rows = static_cast<int64_t>(a.b.max_rows) * (query->q_heads / cache->heads);
   a.tile_rows = rows <= kFewRows ? kKvRows : kKvTileRows;
   const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows;
@@ -354,7 +345,8 @@ static int64_t kv_tasks(const KvAttnArgs &a) { return static_cast<int64_t>(a.b.s
 
 static int64_t kv_workspace(const KvAttnArgs &a) {
   if (a.splits < 2) return 0;
-  return RNSMX_KV_TICKETS * 4 + kv_tasks(a) * a.splits * kv_partial_floats(a.tile_rows, a.b.row_bytes) * 4;
+  return RNSMX_KV_TICKETS * 4 +
+         kv_tasks(a) * a.splits * (a.tile_rows == kKvRows ? kv_row_floats(a.b.row_bytes) : kv_tile_floats(a.b.row_bytes)) * 4;
 }
 
 }  // namespace rnsmx
@@ -442,12 +434,25 @@ int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const 
 }
 
 int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const rnsmx_kv_query_t *query,
-                           void *workspace_dev, int64_t workspace_bytes, void *out_dev, void *stream) {
+                           const void *q_dev, const void *mask_dev, void *workspace_dev, int64_t workspace_bytes,
+                           void *out_dev, void *stream) {
   clear_error();
   KvAttnArgs a{};
   if (int32_t rc = kv_attn_args(cache, batch, query, a)) return rc;
   if (a.b.rows == 0 || a.b.seqs == 0) return RNSMX_OK;
-  if (!out_dev || !aligned(out_dev, dtype_bytes(a.dtype))) return fail(RNSMX_EINVAL, "output null or not aligned to its type");
+  const int64_t size = dtype_bytes(a.dtype);
+  if (!q_dev || !aligned(q_dev, size)) return fail(RNSMX_EINVAL, "queries null or not aligned to their type");
+  if (mask_dev) {
+    if (query->mask_dtype != RNSMX_INT8 && !is_float(query->mask_dtype))
+      return fail(RNSMX_EINVAL, "masks are bytes, float32, float16 or bfloat16");
+    if (query->mask_len < 0) return fail(RNSMX_EINVAL, "bad mask length");
+    if (!aligned(mask_dev, dtype_bytes(query->mask_dtype))) return fail(RNSMX_EINVAL, "the mask is not aligned to its type");
+  }
+  a.q = q_dev;
+  a.mask = mask_dev;
+  a.vec = cache->head_dim % 8 == 0 && aligned(q_dev, 16) && query->row_stride * size % 16 == 0 &&
+          query->head_stride * size % 16 == 0;
+  if (!out_dev || !aligned(out_dev, size)) return fail(RNSMX_EINVAL, "output null or not aligned to its type");
   const int64_t need = kv_workspace(a);
   if (need > 0) {
     if (!workspace_dev || !aligned(workspace_dev, 16)) return fail(RNSMX_EINVAL, "workspace null or not on a 16-byte boundary");

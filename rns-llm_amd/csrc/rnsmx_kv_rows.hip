@@ -134,13 +134,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
     float x[KS][8];
     const int64_t at = static_cast<int64_t>(q.row + t_row) * a.q_rs + static_cast<int64_t>(q_head) * a.q_hs;
     float top = 0.0f;
-    kv_for<KS>([&](auto S) {
+    // lane group g takes bytes 16 g .. of a 64-value chunk, the first eight in its first step
+    kv_query<KS, SPLIT>(x, a, at, [&](auto S) {
       constexpr int s = S;
-      // lane group g takes bytes 16 g .. of a 64-value chunk, the first eight in its first step
-      const int32_t d = s < 2 * C64 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 64 * C64 + 8 * g;
-      kv_query8(x[s], a, at, d);
-      kv_for<8>([&](auto J) { top = fmaxf(top, fabsf(x[s][J])); });
+      return s < 2 * C64 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 64 * C64 + 8 * g;
     });
+    kv_for<KS>([&](auto S) { kv_for<8>([&](auto J) { top = fmaxf(top, fabsf(x[S][J])); }); });
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const int32_t e = kv_query_exponent(top);

@@ -43,10 +43,12 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   constexpr int VG = DT / VD, VR = (2 * VG + 63) / 64;  // of a token group, and rounds
   __shared__ __attribute__((aligned(128))) _Float16 keys[2][kStep * KROW];
   __shared__ __attribute__((aligned(128))) _Float16 values[2][DT * kStep];
-  __shared__ float pages_of_step[2][4][4];  // key scale, log2 and reciprocal of the value scale, whether it is there
+  __shared__ int32_t last;
+  __shared__ __attribute__((aligned(16))) float pages_of_step[2][4][4];  // key scale, log2 and reciprocal of the value scale, whether it is there
 
   const KvBatchArgs &b = a.b;
-  uint32_t id = kv_xcd_order(blockIdx.x, gridDim.x);
+  uint32_t id = kv_xcd_order(blockIdx.x, gridDim.x, true);
+  const int32_t split = kv_rem(a.by_splits, id), task = id;
   const int32_t tile = a.row_tiles - 1 - static_cast<int32_t>(kv_rem(a.by_tiles, id));  // the longest first
   const int32_t head = kv_rem(a.by_heads, id), seq = id, group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
@@ -60,6 +62,9 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   const int32_t last_row = min(row0 + kKvTileRows, rows) - 1;
   const int32_t hi = max(a.causal ? base + kv_of(last_row) + 1 : q.len, 0);
   const int32_t lo = a.window > 0 ? max(base + kv_of(row0) + 1 - a.window, 0) & ~(kStep - 1) : 0;
+  const int32_t c0 = lo + split * a.chunk;
+  if (split > 0 && c0 >= hi) return;
+  const int32_t c1 = min(hi, c0 + a.chunk);
   const int32_t w_first = row0 + 32 * wave, w_last = min(w_first + 31, rows - 1);
   const bool w_any = w_first < rows;
   const int32_t t_first = kv_of(w_first), t_last = kv_of(w_last);
@@ -143,9 +148,9 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   };
 
   int32_t page = 0;
-  if (lo < hi) {
-    load_step(lo, page_of(lo));
-    page = page_of(lo + kStep);
+  if (c0 < c1) {
+    load_step(c0, page_of(c0));
+    page = page_of(c0 + kStep);
   }
 
   h16x8 qf[QN][KS];
@@ -154,11 +159,8 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     float x[KS][8];
     const int64_t at = static_cast<int64_t>(q.row + t_row) * a.q_rs + static_cast<int64_t>(q_head) * a.q_hs;
     float top = 0.0f;
-    kv_for<KS>([&](auto S) {
-      constexpr int s = S;
-      kv_query8(x[s], a, at, 16 * s + 8 * h);
-      kv_for<8>([&](auto J) { top = fmaxf(top, fabsf(x[s][J])); });
-    });
+    kv_query<KS, SPLIT>(x, a, at, [&](auto S) { return 16 * S + 8 * h; });
+    kv_for<KS>([&](auto S) { kv_for<8>([&](auto J) { top = fmaxf(top, fabsf(x[S][J])); }); });
     top = fmaxf(top, __shfl_xor(top, 32));
     const int32_t e = kv_query_exponent(top);
     kv_for<KS>([&](auto S) {
@@ -288,12 +290,12 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     });
   };
 
-  if (lo < hi) {
+  if (c0 < c1) {
     stage(0);
     int32_t buf = 0;
-    for (int32_t t0 = lo; t0 < hi; t0 += kStep, buf ^= 1) {
+    for (int32_t t0 = c0; t0 < c1; t0 += kStep, buf ^= 1) {
       __syncthreads();  // this step is staged, and the other buffer's readers are done
-      const bool more = t0 + kStep < hi;
+      const bool more = t0 + kStep < c1;
       if (more) {
         load_step(t0 + kStep, page);
         page = page_of(t0 + 2 * kStep);
@@ -302,10 +304,70 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
       if (more) stage(buf ^ 1);
     }
   }
-  if (!w_any) return;
-
   sum += __shfl_xor(sum, 32);
-  if (w_first + col >= rows) return;
+
+  // Split over its tokens, a workgroup leaves its sums in the workspace as the
+  // lanes hold them, two at a time; the one that draws the task's last ticket
+  // joins them, in the order of the splits (kv_rows_kernel has the protocol).
+  const int32_t active = a.splits == 1 ? 1 : max((hi - lo + a.chunk - 1) / a.chunk, 1);
+  if (active > 1) {
+    constexpr int64_t kPart = kv_tile_floats(DT);
+    float *at = a.partial + static_cast<int64_t>(task) * a.splits * kPart + tid * 2;
+    auto put = [&](int64_t i, float x, float y) {
+      __hip_atomic_store(reinterpret_cast<uint64_t *>(at + split * kPart + i),
+                         static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+    };
+    if (w_any) {
+      kv_for<DB>([&](auto I) {
+        kv_for<8>([&](auto J) {
+          constexpr int i = I, j = J;
+          put((8 * i + j) * 512, o[i][2 * j], o[i][2 * j + 1]);
+        });
+      });
+      put(8 * DB * 512, mx, ml);
+      put((8 * DB + 1) * 512, sum, 0.0f);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      const uint32_t old = __hip_atomic_fetch_add(a.tickets + task, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = old == static_cast<uint32_t>(active - 1);
+      if (last) __hip_atomic_store(a.tickets + task, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last || !w_any) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    auto get = [&](int32_t s, int64_t i) { return *reinterpret_cast<const F32x2 *>(at + s * kPart + i); };
+    // the highest reference of all, as kv_higher orders them
+    mx = -INFINITY;
+    ml = 0.0f;
+    for (int32_t s = 0; s < active; ++s) {
+      const F32x2 r = get(s, 8 * DB * 512);
+      const float s1 = mx * kNat + ml, s2 = r.x * kNat + r.y;
+      const bool take = r.x > -INFINITY && (!(mx > -INFINITY) || s2 > s1 || (s2 == s1 && (r.x > mx || (r.x == mx && r.y > ml))));
+      mx = take ? r.x : mx;
+      ml = take ? r.y : ml;
+    }
+    sum = 0.0f;
+    kv_for<DB>([&](auto I) { kv_for<16>([&](auto J) { o[I][static_cast<int>(J)] = 0.0f; }); });
+    for (int32_t s = 0; s < active; ++s) {
+      const F32x2 r = get(s, 8 * DB * 512), t = get(s, (8 * DB + 1) * 512);
+      // not-a-numbers of a part without a reference go through
+      const float f = r.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((r.x - mx) * kNat + (r.y - ml));
+      sum = fmaf(t.x, f, sum);
+      kv_for<DB>([&](auto I) {
+        kv_for<8>([&](auto J) {
+          constexpr int i = I, j = J;
+          const F32x2 v = get(s, (8 * i + j) * 512);
+          o[i][2 * j] = fmaf(v.x, f, o[i][2 * j]);
+          o[i][2 * j + 1] = fmaf(v.y, f, o[i][2 * j + 1]);
+        });
+      });
+    }
+  }
+
+  if (!w_any || w_first + col >= rows) return;
   // l = sum 2^ml, and the codes' unit
   const float f = sum == 0.0f ? 0.0f : kKvUnit / sum;
   const int64_t out = (static_cast<int64_t>(q.row + t_row) * a.q_heads + q_head) * b.dim;
@@ -343,7 +405,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
 
 template <int DT>
 void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles)), block(256);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles * a.splits)), block(256);
   const bool split = a.dtype == RNSMX_FLOAT32;
   if (a.mask) {
     if (split)

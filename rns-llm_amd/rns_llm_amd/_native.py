@@ -163,10 +163,8 @@ class KVQueryStruct(ctypes.Structure):
     """Mirror of ``rnsmx_kv_query_t``."""
 
     _fields_ = [
-        ("q_dev", ctypes.c_void_p),
         ("row_stride", ctypes.c_int64),
         ("head_stride", ctypes.c_int64),
-        ("mask_dev", ctypes.c_void_p),
         ("mask_row_stride", ctypes.c_int64),
         ("mask_head_stride", ctypes.c_int64),
         ("mask_token_stride", ctypes.c_int64),
@@ -230,7 +228,7 @@ _SIGNATURES = {
     "rnsmx_kv_append": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _P]),
     "rnsmx_kv_read": (_I32, [_P, _P, _P, _P, _I32, _P]),
     "rnsmx_kv_attention_workspace_bytes": (_I64, [_P, _P, _P]),
-    "rnsmx_kv_attention": (_I32, [_P, _P, _P, _P, _I64, _P, _P]),
+    "rnsmx_kv_attention": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _P, _P]),
 }
 
 ABI_VERSION = 6

@@ -42,12 +42,10 @@ class KVCache:
     block_size: int
     kv_heads: int
     head_dim: int
+    device: torch.device
     _struct: object = field(repr=False, compare=False, default=None)
     _ref: int = field(repr=False, compare=False, default=0)
-
-    @property
-    def device(self) -> torch.device:
-        return self.scales.device
+    _shape: tuple = field(repr=False, compare=False, default=())  # what checks of arguments depend on
 
     @property
     def nbytes(self) -> int:
@@ -76,7 +74,8 @@ class KVBatch:
     longest: int | None = None  # of the lengths given as numbers
     _struct: object = field(repr=False, compare=False, default=None)
     _ref: int = field(repr=False, compare=False, default=0)
-    _need: dict = field(repr=False, compare=False, default_factory=dict)
+    # arguments that were checked: their types, shapes and strides -> what a call passes on
+    _checked: dict = field(repr=False, compare=False, default_factory=dict)
 
     @property
     def sequences(self) -> int:
@@ -117,7 +116,8 @@ class KVCacheOps:
         scales = torch.full(shape[:2] + (2,), torch.finfo(torch.float32).eps, dtype=torch.float32, device=device)
         struct = _native.KVCacheStruct(k.data_ptr(), v.data_ptr(), scales.data_ptr(), shape[0], shape[2], shape[1],
                                        int(head_dim), row_bytes)
-        return KVCache(k, v, scales, shape[0], shape[2], shape[1], int(head_dim), struct, ctypes.addressof(struct))
+        return KVCache(k, v, scales, shape[0], shape[2], shape[1], int(head_dim), scales.device, struct,
+                       ctypes.addressof(struct), (shape[1], shape[2], int(head_dim), scales.device))
 
     def kv_batch(self, cache: KVCache, block_table: torch.Tensor, lengths, *,
                  query_lengths: Sequence[int] | None = None, query_starts: torch.Tensor | None = None,
@@ -200,12 +200,18 @@ class KVCacheOps:
         own, its older codes are quantised again from the values they stood for.
         A value that is not finite makes every value of its page and head read
         as NaN.  Sequences of one call must not share pages that it writes to."""
-        k = self._check_rows(k, "k", batch, cache.kv_heads, cache)
-        v = self._check_rows(v, "v", batch, cache.kv_heads, cache)
-        if k.dtype != v.dtype:
-            raise ValueError("k and v must have one dtype")
-        rc = self._lib.rnsmx_kv_append(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), _FLOAT_CODES[k.dtype],
-                                       k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+        key = (k.dtype, k.shape, k.stride(), k.device, v.dtype, v.shape, v.stride(), v.device, cache._shape)
+        args = batch._checked.get(key)
+        if args is None:
+            plain_k = self._check_rows(k, "k", batch, cache.kv_heads, cache)
+            plain_v = self._check_rows(v, "v", batch, cache.kv_heads, cache)
+            if k.dtype != v.dtype:
+                raise ValueError("k and v must have one dtype")
+            if plain_k is not k or plain_v is not v:
+                return self.kv_append(cache, batch, plain_k, plain_v)
+            args = (_FLOAT_CODES[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+            batch._checked[key] = args
+        rc = self._lib.rnsmx_kv_append(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), *args,
                                        self._stream_of(cache.device))
         if rc:
             _native.check(rc)
@@ -242,7 +248,40 @@ class KVCacheOps:
         numbers.  What is hidden contributes nothing whatever it holds, and a row
         that sees no token is zero.  ``workspace``: zero-initialised uint8 of
         ``kv_attention_workspace_bytes``, by default one kept per stream."""
-        q = self._check_rows(q, "q", batch, None, cache)
+        key = (q.dtype, q.shape, q.stride(), q.device, cache._shape, scale, causal, window,
+               None if mask is None else (mask.dtype, mask.shape, mask.stride(), mask.device))
+        checked = batch._checked.get(key)
+        if checked is None:
+            plain = self._check_rows(q, "q", batch, None, cache)
+            if plain is not q:
+                return self.kv_attention(plain, cache, batch, scale=scale, causal=causal, window=window, mask=mask,
+                                         out=out, workspace=workspace)
+            query = self._query_of(q, cache, batch, scale, causal, window, mask)
+            need = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ctypes.addressof(query)))
+            checked = batch._checked[key] = (query, ctypes.addressof(query), need)
+        _, ref, need = checked
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+            raise ValueError("out must be contiguous and like q")
+        stream = self._stream_of(cache.device)
+        space, size = None, 0
+        if workspace is not None:
+            if workspace.dtype != torch.uint8 or workspace.device != cache.device or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be contiguous uint8 on {cache.device}")
+            space, size = workspace.data_ptr(), workspace.numel()
+        elif need > 0:
+            scratch = self._kv_scratch_for(need, cache.device, stream)
+            space, size = scratch.data_ptr(), scratch.numel()
+        rc = self._lib.rnsmx_kv_attention(cache._ref, batch._ref, ref, q.data_ptr(),
+                                          None if mask is None else mask.data_ptr(), space, size, out.data_ptr(), stream)
+        if rc:
+            _native.check(rc)
+        self._stats["kv_attention_calls"] += 1
+        return out
+
+    def _query_of(self, q: torch.Tensor, cache: KVCache, batch: KVBatch, scale, causal, window, mask):
+        """The checked arguments of ``kv_attention`` as the library takes them."""
         heads = int(q.shape[1])
         if heads < 1 or heads % cache.kv_heads:
             raise ValueError(f"q has {heads} heads, not a multiple of the cache's {cache.kv_heads}")
@@ -254,57 +293,34 @@ class KVCacheOps:
             window = 0
         elif window < 1 or not causal:
             raise ValueError("window must be at least 1, of causal rows")
-        dtype = _FLOAT_CODES[q.dtype]
-        mask_args = (None, 0, 0, 0)
-        mask_dtype = mask_len = 0
+        mask_args, mask_code, mask_len = (0, 0, 0), _native.INT8, 0
         if mask is not None:
-            mask = self._check_mask(mask, batch, heads, cache)
-            mask_args = (mask.data_ptr(), *mask.stride())
-            mask_dtype, mask_len = _MASK_CODES[mask.dtype], int(mask.shape[2])
-        query = _native.KVQueryStruct(q.data_ptr(), q.stride(0), q.stride(1), *mask_args, dtype, heads, mask_dtype,
-                                      mask_len, causal, min(int(window), MAX_LENGTH), scale)
-        ref = ctypes.addressof(query)
-        if out is None:
-            out = torch.empty((batch.rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-            raise ValueError("out must be contiguous and like q")
-        stream = self._stream_of(cache.device)
-        if workspace is None:
-            key = (cache.kv_heads, cache.head_dim, cache.block_size, heads, window, q.dtype, mask is None)
-            need = batch._need.get(key)
-            if need is None:
-                need = batch._need[key] = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ref))
-            workspace = self._kv_scratch_for(need, cache.device, stream) if need > 0 else None
-        elif workspace.dtype != torch.uint8 or workspace.device != cache.device or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be contiguous uint8 on {cache.device}")
-        rc = self._lib.rnsmx_kv_attention(cache._ref, batch._ref, ref, None if workspace is None else workspace.data_ptr(),
-                                          0 if workspace is None else workspace.numel(), out.data_ptr(), stream)
-        if rc:
-            _native.check(rc)
-        self._stats["kv_attention_calls"] += 1
-        return out
+            self._check_mask(mask, batch, heads, cache)
+            mask_len, mask_code = int(mask.shape[2]), _MASK_CODES[mask.dtype]
+            mask_args = mask.expand(batch.rows, heads, mask_len).stride()
+        return _native.KVQueryStruct(q.stride(0), q.stride(1), *mask_args, _FLOAT_CODES[q.dtype], heads, mask_code,
+                                     mask_len, bool(causal), min(int(window), MAX_LENGTH), scale)
 
     def kv_attention_workspace_bytes(self, cache: KVCache, batch: KVBatch, *, q_heads: int, dtype: torch.dtype,
                                      window: int | None = None) -> int:
         """Bytes of ``workspace`` that ``kv_attention`` needs for such a call."""
         if dtype not in _FLOAT_CODES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        query = _native.KVQueryStruct(cache.scales.data_ptr(), 0, 0, None, 0, 0, 0, _FLOAT_CODES[dtype], int(q_heads),
-                                      0, 0, 1, min(int(window or 0), MAX_LENGTH), 1.0)
+        query = _native.KVQueryStruct(0, 0, 0, 0, 0, _FLOAT_CODES[dtype], int(q_heads), 0, 0, 1,
+                                      min(int(window or 0), MAX_LENGTH), 1.0)
         need = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ctypes.addressof(query)))
         if need < 0:
             _native.check(_native.EINVAL)
         return need
 
     @staticmethod
-    def _check_mask(mask: torch.Tensor, batch: KVBatch, heads: int, cache: KVCache) -> torch.Tensor:
+    def _check_mask(mask: torch.Tensor, batch: KVBatch, heads: int, cache: KVCache) -> None:
         if mask.dtype not in _MASK_CODES or mask.device != cache.device:
             raise ValueError(f"mask must be bool, float32, float16 or bfloat16 on {cache.device}")
         if mask.ndim != 3 or mask.shape[0] not in (1, batch.rows) or mask.shape[1] not in (1, heads):
             raise ValueError(f"mask must be [{batch.rows} or 1, {heads} or 1, tokens], got {tuple(mask.shape)}")
         if batch.longest is not None and mask.shape[2] < batch.longest:
             raise ValueError(f"mask covers {mask.shape[2]} tokens of sequences of up to {batch.longest}")
-        return mask.expand(batch.rows, heads, mask.shape[2])
 
     def _kv_scratch_for(self, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
         """The stream's scratch, replaced by a larger one where a call needs it

@@ -124,20 +124,24 @@ def test_queries_that_do_not_fit(q):
         backend().kv_attention(q, c, batch(c))
 
 
-def call(cache_changes=(), batch_changes=(), query_changes=()):
+def call(cache_changes=(), batch_changes=(), query_changes=(), q_dev=4096, mask_dev=None, out_dev=4096):
     """rnsmx_kv_attention with valid sizes but for the changes, on zero
     sequences, so that nothing is launched."""
     c = _native.KVCacheStruct(4096, 8192, 4096, 4, 16, 2, 40, 64)
     b = _native.KVBatchStruct(4096, 2, 4096, 4096, 0, 2, 0, 1, 32)
-    q = _native.KVQueryStruct(4096, 80, 40, None, 0, 0, 0, _native.FLOAT16, 4, 0, 0, 1, 0, 0.5)
+    q = _native.KVQueryStruct(80, 40, 0, 0, 0, _native.FLOAT16, 4, 0, 0, 1, 0, 0.5)
     for struct, changes in ((c, cache_changes), (b, batch_changes), (q, query_changes)):
         for name, value in dict(changes).items():
             setattr(struct, name, value)
-    return _native.lib().rnsmx_kv_attention(ctypes.addressof(c), ctypes.addressof(b), ctypes.addressof(q), None, 0, 4096, None)
+    return _native.lib().rnsmx_kv_attention(ctypes.addressof(c), ctypes.addressof(b), ctypes.addressof(q), q_dev, mask_dev,
+                                             None, 0, out_dev, None)
 
 
 def test_c_abi_accepts_no_sequences():
     assert call() == _native.OK
+
+
+WITH_ROWS = {"seqs": 1, "rows": 1}  # past the call of zero sequences; refused before a launch
 
 
 @pytest.mark.parametrize("changes", [
@@ -148,9 +152,12 @@ def test_c_abi_accepts_no_sequences():
     {"batch_changes": {"seqs": 2, "lengths_dev": None}}, {"batch_changes": {"seqs": 2, "starts_dev": None, "rows": 3}},
     {"query_changes": {"dtype": _native.INT8}}, {"query_changes": {"q_heads": 3}}, {"query_changes": {"q_heads": 0}},
     {"query_changes": {"scale": 0.0}}, {"query_changes": {"scale": math.inf}}, {"query_changes": {"window": -1}},
-    {"query_changes": {"window": 5, "causal": 0}}, {"query_changes": {"mask_dev": 4096, "mask_dtype": _native.INT32}},
-    {"query_changes": {"mask_dev": 4097, "mask_dtype": _native.FLOAT16}},
-    {"query_changes": {"mask_dev": 4096, "mask_dtype": _native.INT8, "mask_len": -1}},
+    {"query_changes": {"window": 5, "causal": 0}},
+    {"batch_changes": WITH_ROWS, "query_changes": {"mask_dtype": _native.INT32}, "mask_dev": 4096},
+    {"batch_changes": WITH_ROWS, "query_changes": {"mask_dtype": _native.FLOAT16}, "mask_dev": 4097},
+    {"batch_changes": WITH_ROWS, "query_changes": {"mask_dtype": _native.INT8, "mask_len": -1}, "mask_dev": 4096},
+    {"batch_changes": WITH_ROWS, "q_dev": None}, {"batch_changes": WITH_ROWS, "q_dev": 4097},
+    {"batch_changes": WITH_ROWS, "out_dev": None}, {"batch_changes": WITH_ROWS, "out_dev": 4099},
 ])
 def test_c_abi_refuses(changes):
     assert call(**changes) == _native.EINVAL

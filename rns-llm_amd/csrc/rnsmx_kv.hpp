@@ -116,7 +116,8 @@ struct KvAttnArgs {
   int32_t causal, window, vec, out_vec;  // vec: q rows are read 16 bytes at a time; out_vec: out starts on 16 bytes
   int32_t chunk, splits, waves;  // waves of a workgroup of kv_rows_kernel
   int32_t tile_rows, row_tiles;  // rows of a workgroup (which says the kernel), workgroups over a sequence's rows
-  KvDiv by_group, by_splits, by_tiles, by_heads;
+  // group: query heads of a key/value head; units: a pair's workgroups; pairs: those that run side by side
+  KvDiv by_group, by_splits, by_units, by_heads, by_pairs;
   float scale;
 };
 
@@ -130,15 +131,35 @@ constexpr bool kv_wide(int row_bytes) { return row_bytes <= 160; }
 constexpr int64_t kv_row_floats(int row_bytes) { return kKvRows * (static_cast<int64_t>(row_bytes) + 2); }
 constexpr int64_t kv_tile_floats(int row_bytes) { return 256 * (static_cast<int64_t>(row_bytes) / 2 + 4); }
 
-// Workgroups go to the 8 XCDs in turn: the n-th of an XCD takes the n-th of a
-// contiguous part of the work, so that what shares keys shares an L2.  turn: of
-// work ordered from long to short and two workgroups to a CU, every other 32 (an
-// XCD's CUs) in reverse, so that the long ones share theirs with the short.
-__device__ __forceinline__ int32_t kv_xcd_order(uint32_t id, uint32_t count, bool turn = false) {
-  const uint32_t xcd = id & 7, per = count >> 3, more = count & 7, size = per + (xcd < more ? 1 : 0);
-  uint32_t n = id >> 3;
-  if (turn && (n & 32) && (n | 31) < size) n ^= 31;
-  return static_cast<int32_t>(xcd * per + min(xcd, more) + n);
+// A workgroup's part of the work: sequence and head (a pair), tile of rows,
+// split of the tokens; task numbers pairs' tiles.  Neighbours are different
+// pairs, so that each of the 8 XCDs, which workgroups go to in turn, gets as many
+// long and short parts as the others (72 pairs of sequences of 400 to 2500
+// tokens: 60 us with the pairs one after the other in eighths, 52 so), and where
+// the pairs divide by 8 each is one XCD's, whose L2 its tiles share.  Tiles run
+// from the longest down; with two workgroups to a CU (turn) every other 32 (an
+// XCD's CUs) are reversed, so that a long one shares its CU with a short one
+// (2048 tokens, 32 heads: 91 us without, 79 with).
+struct KvPlace {
+  int32_t seq, head, tile, split, task;
+};
+__device__ __forceinline__ KvPlace kv_place(const KvAttnArgs &a, uint32_t id, uint32_t count, bool turn) {
+  if (turn) {
+    const uint32_t xcd = id & 7, size = (count >> 3) + (xcd < (count & 7) ? 1 : 0);
+    uint32_t n = id >> 3;
+    if ((n & 32) && (n | 31) < size) id = (n ^ 31) << 3 | xcd;
+  }
+  uint32_t rest = id;
+  const uint32_t in_group = kv_rem(a.by_pairs, rest);
+  uint32_t unit = kv_rem(a.by_units, rest);
+  uint32_t pair = rest * a.by_pairs.d + in_group;
+  KvPlace p;
+  p.split = kv_rem(a.by_splits, unit);
+  p.tile = a.row_tiles - 1 - static_cast<int32_t>(unit);
+  p.task = pair * a.row_tiles + p.tile;
+  p.head = kv_rem(a.by_heads, pair);
+  p.seq = pair;
+  return p;
 }
 
 // rnsmx_kv_rows.hip, one object per row size

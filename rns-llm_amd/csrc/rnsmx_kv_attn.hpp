@@ -114,17 +114,20 @@ __device__ __forceinline__ int32_t kv_query_exponent(float top) {
 // on): loads that do not depend on each other or on what is seen.
 __device__ __forceinline__ void kv_mask_load(uint32_t (&m)[8], const KvAttnArgs &a, int64_t row, int32_t q_head, int32_t t) {
   const int64_t at = row * a.mask_rs + static_cast<int64_t>(q_head) * a.mask_hs;
-  kv_for<8>([&](auto J) {
-    const int64_t i = at + static_cast<int64_t>(min(t + J, a.mask_len - 1)) * a.mask_ts;
-    if (a.mask_len <= 0)
-      m[J] = 0;
-    else if (a.mask_dtype == RNSMX_INT8)
-      m[J] = static_cast<const uint8_t *>(a.mask)[i];
-    else if (a.mask_dtype == RNSMX_FLOAT32)
-      m[J] = static_cast<const uint32_t *>(a.mask)[i];
-    else
-      m[J] = static_cast<const uint16_t *>(a.mask)[i];
-  });
+  auto load = [&](auto *p) {
+    kv_for<8>([&](auto J) {
+      constexpr int j = J;
+      m[j] = p[at + static_cast<int64_t>(min(t + j, a.mask_len - 1)) * a.mask_ts];
+    });
+  };
+  if (a.mask_len <= 0)
+    kv_for<8>([&](auto J) { m[J] = 0; });
+  else if (a.mask_dtype == RNSMX_INT8)
+    load(static_cast<const uint8_t *>(a.mask));
+  else if (a.mask_dtype == RNSMX_FLOAT32)
+    load(static_cast<const uint32_t *>(a.mask));
+  else
+    load(static_cast<const uint16_t *>(a.mask));
 }
 // Whether it hides token t; an additive mask's value goes onto the score.
 __device__ __forceinline__ bool kv_mask_hides(const KvAttnArgs &a, uint32_t m, int32_t t, float &x) {

@@ -307,6 +307,16 @@ static void kv_split(KvAttnArgs &a) {
 // Up to so many rows of a sequence and key/value head run 16 to a workgroup.
 constexpr int64_t kFewRows = 64;
 
+// Pairs of sequences and heads whose workgroups run side by side: all, or where
+// there are many a divisor of their number, so that an XCD's part of them stays
+// in its L2 from one tile of rows to the next.
+static int64_t pairs_at_once(int64_t pairs) {
+  if (pairs <= 256) return std::max<int64_t>(pairs, 1);
+  for (int64_t n = 256; n >= 64; n -= 8)
+    if (pairs % n == 0) return n;
+  return pairs;
+}
+
 static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const rnsmx_kv_query_t *query,
                             KvAttnArgs &a) {
   if (int32_t rc = kv_batch_args(cache, batch, a.b)) return rc;
@@ -336,7 +346,8 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   kv_split(a);
   a.by_group = kv_div(query->q_heads / cache->heads);
   a.by_splits = kv_div(a.splits);
-  a.by_tiles = kv_div(std::max(a.row_tiles, 1));
+  a.by_units = kv_div(std::max(a.row_tiles, 1) * a.splits);
+  a.by_pairs = kv_div(static_cast<uint32_t>(pairs_at_once(static_cast<int64_t>(a.b.seqs) * cache->heads)));
   a.by_heads = kv_div(cache->heads);
   return RNSMX_OK;
 }

@@ -36,10 +36,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
   __shared__ int32_t last;
 
   const KvBatchArgs &b = a.b;
-  uint32_t id = kv_xcd_order(blockIdx.x, gridDim.x);
-  const int32_t split = kv_rem(a.by_splits, id), task = id;
-  const int32_t tile = a.row_tiles - 1 - static_cast<int32_t>(kv_rem(a.by_tiles, id));  // the longest first
-  const int32_t head = kv_rem(a.by_heads, id), seq = id, group = a.by_group.d;
+  const KvPlace place = kv_place(a, blockIdx.x, gridDim.x, false);
+  const int32_t split = place.split, task = place.task, tile = place.tile, head = place.head, seq = place.seq;
+  const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
   auto token_of = [&](int32_t r) { return static_cast<int32_t>(kv_quot(a.by_group, r)); };  // of a row
   const int32_t rows = q.n * group, row0 = tile * ROWS;

@@ -47,10 +47,9 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   __shared__ __attribute__((aligned(16))) float pages_of_step[2][4][4];  // key scale, log2 and reciprocal of the value scale, whether it is there
 
   const KvBatchArgs &b = a.b;
-  uint32_t id = kv_xcd_order(blockIdx.x, gridDim.x, true);
-  const int32_t split = kv_rem(a.by_splits, id), task = id;
-  const int32_t tile = a.row_tiles - 1 - static_cast<int32_t>(kv_rem(a.by_tiles, id));  // the longest first
-  const int32_t head = kv_rem(a.by_heads, id), seq = id, group = a.by_group.d;
+  const KvPlace place = kv_place(a, blockIdx.x, gridDim.x, true);
+  const int32_t split = place.split, task = place.task, tile = place.tile, head = place.head, seq = place.seq;
+  const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
   const int32_t rows = q.n * group, row0 = tile * kKvTileRows;
   if (row0 >= rows) return;

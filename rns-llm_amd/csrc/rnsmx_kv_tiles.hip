@@ -67,8 +67,6 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   const int32_t w_first = row0 + 32 * wave, w_last = min(w_first + 31, rows - 1);
   const bool w_any = w_first < rows;
   const int32_t t_first = kv_of(w_first), t_last = kv_of(w_last);
-  const int32_t w_hi = !w_any ? 0 : a.causal ? base + t_last + 1 : q.len;
-  const int32_t w_lo = a.window > 0 ? base + t_first + 1 - a.window : 0;
   const int32_t full_hi = a.causal ? base + t_first + 1 : q.len;
   const int32_t full_lo = a.window > 0 ? max(base + t_last + 1 - a.window, 0) : 0;
 
@@ -149,7 +147,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   int32_t page = 0;
   if (c0 < c1) {
     load_step(c0, page_of(c0));
-    page = page_of(c0 + kStep);
+    page = page_of(min(c0 + kStep, c1 - 1) & ~(kStep - 1));
   }
 
   h16x8 qf[QN][KS];
@@ -258,8 +256,10 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
         ml = nl;
       }
     }
-    h16x8 p[QN][4];
-    // a row without a reference has nothing but minus infinities (and not-a-numbers) so far
+    // A group's weights, then its products, whose time on the matrix cores the
+    // next group's weights fill (and the next step's codes after the last).
+    // A row without a reference has nothing but minus infinities (and
+    // not-a-numbers) so far.
     const float ref = mx == -INFINITY ? 0.0f : mx;
     kv_for<4>([&](auto G) {
       constexpr int g = G;
@@ -271,20 +271,18 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
         part += w[g][j];
       });
       sum = fmaf(part, rv[g], sum);
+      h16x8 p[QN];
       kv_for<8>([&](auto J) {
         constexpr int j = J;
         const _Float16 half = static_cast<_Float16>(w[g][j]);
-        p[0][g][j] = half;
-        if constexpr (SPLIT) p[1][g][j] = static_cast<_Float16>(w[g][j] - static_cast<float>(half));
+        p[0][j] = half;
+        if constexpr (SPLIT) p[1][j] = static_cast<_Float16>(w[g][j] - static_cast<float>(half));
       });
-    });
-    kv_for<DB>([&](auto I) {
-      constexpr int i = I;
-      const int32_t d = 32 * i + col, vswap = value_swap(d);
-      kv_for<4>([&](auto G) {
-        constexpr int g = G;
-        const h16x8 v = *reinterpret_cast<const h16x8 *>(&values[buf][d * kStep + ((2 * g + h) ^ vswap) * 8]);
-        kv_for<QN>([&](auto P) { o[i] = kv_mfma32(v, p[P][g], o[i]); });
+      kv_for<DB>([&](auto I) {
+        constexpr int i = I;
+        const int32_t d = 32 * i + col;
+        const h16x8 v = *reinterpret_cast<const h16x8 *>(&values[buf][d * kStep + ((2 * g + h) ^ value_swap(d)) * 8]);
+        kv_for<QN>([&](auto P) { o[i] = kv_mfma32(v, p[P], o[i]); });
       });
     });
   };
@@ -294,13 +292,14 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     int32_t buf = 0;
     for (int32_t t0 = c0; t0 < c1; t0 += kStep, buf ^= 1) {
       __syncthreads();  // this step is staged, and the other buffer's readers are done
-      const bool more = t0 + kStep < c1;
-      if (more) {
-        load_step(t0 + kStep, page);
-        page = page_of(t0 + 2 * kStep);
-      }
-      if (t0 < w_hi && t0 + kStep > w_lo) compute(buf, t0);
-      if (more) stage(buf ^ 1);
+      // The next step's codes (the last step's again after it: no branch parts
+      // the products from the conversions).  A wave whose rows see nothing of a
+      // step goes through it all the same, beside those that do.
+      const int32_t next = min(t0 + kStep, c1 - 1) & ~(kStep - 1);
+      load_step(next, page);
+      page = page_of(min(t0 + 2 * kStep, c1 - 1) & ~(kStep - 1));
+      compute(buf, t0);
+      stage(buf ^ 1);
     }
   }
   sum += __shfl_xor(sum, 32);

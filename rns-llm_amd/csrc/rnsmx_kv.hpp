@@ -114,7 +114,7 @@ struct KvAttnArgs {
   int64_t q_rs, q_hs, mask_rs, mask_hs, mask_ts;
   int32_t q_heads, dtype, mask_dtype, mask_len;
   int32_t causal, window, vec, out_vec;  // vec: q rows are read 16 bytes at a time; out_vec: out starts on 16 bytes
-  int32_t chunk, splits, waves;  // waves of a workgroup of kv_rows_kernel
+  int32_t chunk, splits, waves;  // waves of a workgroup, 4 or 8
   int32_t tile_rows, row_tiles;  // rows of a workgroup (which says the kernel), workgroups over a sequence's rows
   // group: query heads of a key/value head; units: a pair's workgroups; pairs: those that run side by side
   KvDiv by_group, by_splits, by_units, by_heads, by_pairs;
@@ -168,6 +168,8 @@ void launch_kv_rows(const KvAttnArgs &a, hipStream_t st);
 
 // rnsmx_kv_tiles.hip, one object per row size
 constexpr int kKvTileRows = 128;  // query rows of a workgroup of kv_tiles_kernel
+// Row sizes whose staged steps fit the shared memory twice run on eight waves too.
+constexpr int kv_tile_halves(int row_bytes) { return row_bytes <= 128 ? 2 : 1; }
 template <int DT>
 void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st);
 

@@ -110,10 +110,28 @@ __device__ __forceinline__ int32_t kv_query_exponent(float top) {
   return max(top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0, -120);
 }
 
-// Eight tokens of a mask's row from t on, as they are stored (0 from mask_len
-// on): loads that do not depend on each other or on what is seen.
-__device__ __forceinline__ void kv_mask_load(uint32_t (&m)[8], const KvAttnArgs &a, int64_t row, int32_t q_head, int32_t t) {
+// Eight tokens of a mask's row from t on, as they are stored: loads that do not
+// depend on each other or on what is seen.  Tokens in a row of a mask that covers
+// the step up to `end` come in one load or two; else one by one, the last
+// column's in the place of those past it (0 of a mask without columns).
+__device__ __forceinline__ void kv_mask_load(uint32_t (&m)[8], const KvAttnArgs &a, int64_t row, int32_t q_head, int32_t t,
+                                             int32_t end) {
   const int64_t at = row * a.mask_rs + static_cast<int64_t>(q_head) * a.mask_hs;
+  const int32_t size = a.mask_dtype == RNSMX_INT8 ? 1 : a.mask_dtype == RNSMX_FLOAT32 ? 4 : 2;
+  if (a.mask_ts == 1 && end <= a.mask_len) {
+    const uint8_t *p = static_cast<const uint8_t *>(a.mask) + (at + t) * size;
+    uint32_t w[8];
+    if (size == 1) {
+      __builtin_memcpy(w, p, 8);
+      kv_for<8>([&](auto J) { m[J] = w[J / 4] >> (8 * (J % 4)) & 0xFFu; });
+    } else if (size == 2) {
+      __builtin_memcpy(w, p, 16);
+      kv_for<8>([&](auto J) { m[J] = w[J / 2] >> (16 * (J % 2)) & 0xFFFFu; });
+    } else {
+      __builtin_memcpy(m, p, 32);
+    }
+    return;
+  }
   auto load = [&](auto *p) {
     kv_for<8>([&](auto J) {
       constexpr int j = J;
@@ -122,9 +140,9 @@ __device__ __forceinline__ void kv_mask_load(uint32_t (&m)[8], const KvAttnArgs 
   };
   if (a.mask_len <= 0)
     kv_for<8>([&](auto J) { m[J] = 0; });
-  else if (a.mask_dtype == RNSMX_INT8)
+  else if (size == 1)
     load(static_cast<const uint8_t *>(a.mask));
-  else if (a.mask_dtype == RNSMX_FLOAT32)
+  else if (size == 4)
     load(static_cast<const uint32_t *>(a.mask));
   else
     load(static_cast<const uint16_t *>(a.mask));
@@ -153,6 +171,23 @@ __device__ __forceinline__ void kv_higher(float &e, float &x, float &lv, float e
   e = take ? e2 : e;
   x = take ? x2 : x;
   lv = take ? lv2 : lv;
+}
+
+// Sums against different references: the higher of two, and what sums against
+// one are multiplied by to be against another.  Not-a-numbers of a part without
+// a reference go through the zero.
+template <bool MASK>
+__device__ __forceinline__ void kv_reference(float &mx, float &ml, float mx2, float ml2) {
+  constexpr float kNat = MASK ? kKvLog2e : 1.0f;
+  const float s1 = mx * kNat + ml, s2 = mx2 * kNat + ml2;
+  const bool take = mx2 > -INFINITY && (!(mx > -INFINITY) || s2 > s1 || (s2 == s1 && (mx2 > mx || (mx2 == mx && ml2 > ml))));
+  mx = take ? mx2 : mx;
+  ml = take ? ml2 : ml;
+}
+template <bool MASK>
+__device__ __forceinline__ float kv_factor(float mx, float ml, float to_mx, float to_ml) {
+  constexpr float kNat = MASK ? kKvLog2e : 1.0f;
+  return mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx - to_mx) * kNat + (ml - to_ml));
 }
 
 }  // namespace rnsmx

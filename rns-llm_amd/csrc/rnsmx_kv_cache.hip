@@ -11,13 +11,15 @@ struct KvAppendArgs {
   KvBatchArgs b;
   const void *src[2];
   int64_t row_stride[2], head_stride[2];
-  int32_t dtype, pages, vec;  // pages: most pages of one sequence that the rows touch
+  int32_t vec;              // rows are read 16 bytes at a time
+  KvDiv by_heads, by_pages;  // pages: most of one sequence that the rows touch
 };
 
 struct KvReadArgs {
   KvBatchArgs b;
   void *dst[2];
-  int32_t dtype, pages, vec;
+  int32_t vec;
+  KvDiv by_heads, by_pages;
 };
 
 constexpr float kKvMax = 127.0f;
@@ -28,51 +30,87 @@ __device__ __forceinline__ void kv_load8(float (&x)[8], const T *p, int32_t left
   if (vec) {
     if constexpr (sizeof(T) == 4) {
       const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
-      kv_for<4>([&](auto I_) { constexpr int I = decltype(I_)::value; x[I] = a[I], x[I + 4] = b[I]; });
+      kv_for<4>([&](auto I) {
+        constexpr int i = I;
+        x[i] = a[i];
+        x[i + 4] = b[i];
+      });
     } else {
       const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
-      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
-        const uint16_t bits = static_cast<uint16_t>(a[I / 2] >> (16 * (I % 2)));
+      kv_for<8>([&](auto I) {
+        constexpr int i = I;
+        const uint16_t bits = static_cast<uint16_t>(a[i / 2] >> (16 * (i % 2)));
         if constexpr (std::is_same<T, _Float16>::value)
-          x[I] = static_cast<float>(__builtin_bit_cast(_Float16, bits));
+          x[i] = static_cast<float>(__builtin_bit_cast(_Float16, bits));
         else
-          x[I] = kv_bf16(bits);
+          x[i] = kv_bf16(bits);
       });
     }
     return;
   }
-  kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
+  kv_for<8>([&](auto I) {
+    constexpr int i = I;
     float v = 0.0f;
-    if (I < left) {
+    if (i < left) {
       if constexpr (std::is_same<T, uint16_t>::value)
-        v = kv_bf16(p[I]);
+        v = kv_bf16(p[i]);
       else
-        v = static_cast<float>(p[I]);
+        v = static_cast<float>(p[i]);
     }
-    x[I] = v;
+    x[i] = v;
   });
 }
 
-// clamp(rint(x / s), +-127) + 128; a quotient that is not a number gives 128
-// (the scale then says that nothing of the page can be read).
-__device__ __forceinline__ uint32_t kv_code(float x, float s) {
-  const float r = rintf(x / s);
-  return r != r ? 128u : static_cast<uint32_t>(static_cast<int32_t>(fminf(fmaxf(r, -kKvMax), kKvMax)) + 128);
-}
-
+// Codes plus 128 of eight values at the scale s, each rint of the correctly
+// rounded quotient x / s.  With r the correctly rounded 1 / s, q = x r is within
+// an ulp of it and q + (x - q s) r, both products fused, is it (Markstein's
+// theorem); where the remainder underflows x / s is far below a half.  Adding 1.5
+// 2^23 leaves the integer in the low byte, rounded to even.  |x| <= 127.01 s, as s
+// comes from the largest: no code needs a clamp.  A quarter of what divisions and
+// conversions cost, which bound prompts (10454 tokens, 32 heads of 128: 87 us).
+// At a scale that is not finite every code is zero.
 __device__ __forceinline__ u32x2 kv_codes(const float (&x)[8], float s) {
-  u32x2 c = {0u, 0u};
-  kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; c[I / 4] |= kv_code(x[I], s) << (8 * (I % 4)); });
+  if (!(s < INFINITY)) return u32x2{0x80808080u, 0x80808080u};
+  const float r = 1.0f / s;
+  uint32_t n[8];
+  kv_for<8>([&](auto I) {
+    constexpr int i = I;
+    const float q = x[i] * r;
+    n[i] = __float_as_uint(fmaf(fmaf(-q, s, x[i]), r, q) + 12582912.0f);
+  });
+  u32x2 c;
+  kv_for<2>([&](auto I) {
+    constexpr int i = I;
+    const uint32_t lo = __builtin_amdgcn_perm(n[4 * i + 1], n[4 * i], 0x0C0C0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(n[4 * i + 3], n[4 * i + 2], 0x04000C0Cu);
+    c[i] = (lo | hi) ^ 0x80808080u;
+  });
   return c;
 }
 
 // code * scale in float32.  The product is kept apart from a conversion to
 // float16 after it: the compiler would join them into one operation, which
 // rounds once, where the definition has float32 values.
-__device__ __forceinline__ float kv_value(u32x2 c, int i, float s) {
-  float v = static_cast<float>(static_cast<int32_t>((c[i / 4] >> (8 * (i % 4))) & 0xFFu) - 128) * s;
+__device__ __forceinline__ float kv_value(uint32_t c, int i, float s) {
+  float v = static_cast<float>(static_cast<int32_t>((c >> (8 * i)) & 0xFFu) - 128) * s;
   asm("" : "+v"(v));
   return v;
+}
+
+// The tokens of one page that a sequence's rows are: `old` to end - 1, from row
+// `row` on; nothing where the page is past its end.
+struct KvSpan {
+  int32_t page, old, end, row;
+};
+__device__ __forceinline__ KvSpan kv_span(const KvBatchArgs &b, const KvSeq &q, int32_t seq, int32_t index) {
+  const int32_t from = max(q.len - q.n, 0), pg = (from >> b.log_page) + index, start = pg << b.log_page;
+  KvSpan r{-1, 0, 0, 0};
+  if (start >= q.len || q.n == 0) return r;
+  r.old = max(from - start, 0);
+  r.end = min(q.len - start, 1 << b.log_page);
+  r.row = q.row + (start + r.old) - (q.len - q.n);
+  r.page = ((const kv_const_i32 *)b.table)[seq * b.table_stride + pg];
+  return r;
 }
 
 // One workgroup for the new tokens of one page and head, keys or values.
@@ -81,111 +119,115 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
   constexpr int CPT = DT / 8;
   __shared__ uint32_t tops[16];
   const KvBatchArgs &b = a.b;
-  int32_t id = blockIdx.x;
+  uint32_t id = blockIdx.x;
   const int32_t part = id & 1;
   id >>= 1;
-  const int32_t head = id % b.heads;
-  id /= b.heads;
-  const int32_t seq = id / a.pages, index = id - seq * a.pages;
+  const int32_t head = kv_rem(a.by_heads, id), index = kv_rem(a.by_pages, id), seq = id;
   const KvSeq q = kv_seq(b, seq);
-  const int32_t page_size = 1 << b.log_page, from = max(q.len - q.n, 0);
-  const int32_t pg = (from >> b.log_page) + index, start = pg << b.log_page;
-  if (start >= q.len) return;
-  const int32_t id_page = b.table[seq * b.table_stride + pg];
-  if (static_cast<uint32_t>(id_page) >= static_cast<uint32_t>(b.blocks)) return;
-  const int32_t old = max(from - start, 0), end = min(q.len - start, page_size);  // tokens old..end-1 are new
-  const int64_t slot = static_cast<int64_t>(id_page) * b.heads + head;
+  const KvSpan p = kv_span(b, q, seq, index);
+  if (p.end == 0 || static_cast<uint32_t>(p.page) >= static_cast<uint32_t>(b.blocks)) return;
+  const int64_t slot = static_cast<int64_t>(p.page) * b.heads + head;
   uint8_t *page = (part ? b.v : b.k) + (slot << b.log_page) * DT;
-  const T *src = static_cast<const T *>(part ? a.src[1] : a.src[0]);
   const int64_t rs = part ? a.row_stride[1] : a.row_stride[0], hs = part ? a.head_stride[1] : a.head_stride[0];
-  const int32_t groups = (end - old) * CPT;
-  src += (q.row + (start + old) - (q.len - q.n)) * rs + head * hs;
+  const T *src = static_cast<const T *>(part ? a.src[1] : a.src[0]) + p.row * rs + head * hs;
+  const int32_t groups = (p.end - p.old) * CPT;
 
   float x[kKvHeld][8];
   uint32_t top = 0;  // of |x| as bits: ordered as the values are, a NaN above all
-  kv_for<kKvHeld>([&](auto J_) { constexpr int J = decltype(J_)::value;
-    const int32_t c = threadIdx.x + J * blockDim.x;
+  kv_for<kKvHeld>([&](auto J) {
+    constexpr int j = J;
+    const int32_t c = threadIdx.x + j * blockDim.x;
     const int32_t t = c / CPT, d = (c - t * CPT) * 8;
     if (c < groups && d < b.dim) {
-      kv_load8<T>(x[J], src + t * rs + d, b.dim - d, a.vec);
+      kv_load8<T>(x[j], src + t * rs + d, b.dim - d, a.vec);
     } else {
-      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; x[J][I] = 0.0f; });
+      kv_for<8>([&](auto I) { x[j][I] = 0.0f; });
     }
-    kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; top = max(top, __float_as_uint(x[J][I]) & 0x7FFFFFFFu); });
   });
   float *scale = b.scales + slot * 2 + part;
-  const float held = old > 0 ? *scale : 0.0f;
-  kv_for<6>([&](auto I_) { constexpr int I = decltype(I_)::value; top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1 << I))); });
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  for (uint32_t w = 0; w < (blockDim.x + 63) / 64; ++w) top = max(top, tops[w]);
+  const float held = p.old > 0 ? *scale : 0.0f;
+  kv_for<kKvHeld>([&](auto J) { kv_for<8>([&](auto I) { top = max(top, __float_as_uint(x[J][I]) & 0x7FFFFFFFu); }); });
+  kv_for<6>([&](auto I) { top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1 << I))); });
+  if (blockDim.x > 64) {
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (uint32_t w = 0; w < blockDim.x / 64; ++w) top = max(top, tops[w]);
+  }
   const float amax = __uint_as_float(top);
   float s = amax != amax ? amax : fmaxf(amax * (1.0f / kKvMax), 1.1920928955078125e-07f);
-  if (old > 0) s = (s != s || held != held) ? __builtin_nanf("") : fmaxf(s, held);
+  if (p.old > 0) s = (s != s || held != held) ? __builtin_nanf("") : fmaxf(s, held);
   if (threadIdx.x == 0) *scale = s;
-  kv_for<kKvHeld>([&](auto J_) { constexpr int J = decltype(J_)::value;
+  kv_for<kKvHeld>([&](auto J) {
     const int32_t c = threadIdx.x + J * blockDim.x;
-    if (c < groups) *reinterpret_cast<u32x2 *>(page + old * DT + c * 8) = kv_codes(x[J], s);
+    if (c < groups) *reinterpret_cast<u32x2 *>(page + p.old * DT + c * 8) = kv_codes(x[J], s);
   });
-  if (old > 0 && s != held)  // the older tokens' codes, to the larger scale
-    for (int32_t c = threadIdx.x; c < old * CPT; c += blockDim.x) {
-      u32x2 *p = reinterpret_cast<u32x2 *>(page + c * 8);
+  if (p.old > 0 && s != held)  // the older tokens' codes, to the larger scale
+    for (int32_t c = threadIdx.x; c < p.old * CPT; c += blockDim.x) {
+      u32x2 *at = reinterpret_cast<u32x2 *>(page + c * 8);
+      const u32x2 code = *at;
       float v[8];
-      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; v[I] = kv_value(*p, I, held); });
-      *p = kv_codes(v, s);
+      kv_for<8>([&](auto I) {
+        constexpr int i = I;
+        v[i] = kv_value(code[i / 4], i % 4, held);
+      });
+      *at = kv_codes(v, s);
     }
 }
 
-// One workgroup for the rows of one page and head, keys or values.
+// One workgroup for the rows of one page and head, keys and values: two groups of
+// eight of each in flight a thread.
 template <int DT, typename T>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
   constexpr int CPT = DT / 8;
   const KvBatchArgs &b = a.b;
-  int32_t id = blockIdx.x;
-  const int32_t part = id & 1;
-  id >>= 1;
-  const int32_t head = id % b.heads;
-  id /= b.heads;
-  const int32_t seq = id / a.pages, index = id - seq * a.pages;
+  uint32_t id = blockIdx.x;
+  const int32_t head = kv_rem(a.by_heads, id), index = kv_rem(a.by_pages, id), seq = id;
   const KvSeq q = kv_seq(b, seq);
-  const int32_t page_size = 1 << b.log_page, from = max(q.len - q.n, 0);
-  T *dst = static_cast<T *>(part ? a.dst[1] : a.dst[0]) + head * b.dim;
   const int64_t rs = static_cast<int64_t>(b.heads) * b.dim;
-  if (index == 0)  // rows that have no token
-    for (int32_t i = threadIdx.x; i < max(q.n - q.len, 0) * b.dim; i += 256) {
+  T *dst[2] = {static_cast<T *>(a.dst[0]) + head * b.dim, static_cast<T *>(a.dst[1]) + head * b.dim};
+  if (index == 0 && q.n > q.len)  // rows that have no token
+    for (int32_t i = threadIdx.x; i < (q.n - q.len) * b.dim; i += 256) {
       const int32_t r = i / b.dim;
-      dst[(q.row + r) * rs + (i - r * b.dim)] = static_cast<T>(0);
+      kv_for<2>([&](auto P) { dst[P][(q.row + r) * rs + (i - r * b.dim)] = static_cast<T>(0); });
     }
-  const int32_t pg = (from >> b.log_page) + index, start = pg << b.log_page;
-  if (start >= q.len || q.n == 0) return;
-  const int32_t id_page = b.table[seq * b.table_stride + pg];
-  const bool there = static_cast<uint32_t>(id_page) < static_cast<uint32_t>(b.blocks);
-  const int32_t old = max(from - start, 0), end = min(q.len - start, page_size);
-  const int64_t slot = static_cast<int64_t>(there ? id_page : 0) * b.heads + head;
-  const uint8_t *page = (part ? b.v : b.k) + (slot << b.log_page) * DT;
-  const float s = there ? b.scales[slot * 2 + part] : 0.0f;
-  dst += (q.row + (start + old) - (q.len - q.n)) * rs;
-  for (int32_t c = threadIdx.x; c < (end - old) * CPT; c += 256) {
-    const int32_t t = c / CPT, d = (c - t * CPT) * 8;
-    if (d >= b.dim) continue;
-    const u32x2 code = *reinterpret_cast<const u32x2 *>(page + old * DT + c * 8);
-    float x[8];
-    kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value; x[I] = there ? kv_value(code, I, s) : 0.0f; });
-    T *to = dst + t * rs + d;
-    T y[8];
-    kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
-      if constexpr (std::is_same<T, uint16_t>::value)
-        y[I] = kv_to_bf16(x[I]);
-      else
-        y[I] = static_cast<T>(x[I]);
+  const KvSpan p = kv_span(b, q, seq, index);
+  if (p.end == 0) return;
+  const bool there = static_cast<uint32_t>(p.page) < static_cast<uint32_t>(b.blocks);
+  const int64_t slot = static_cast<int64_t>(there ? p.page : 0) * b.heads + head;
+  const int64_t at = ((slot << b.log_page) + p.old) * DT;
+  const float scale[2] = {b.scales[slot * 2], b.scales[slot * 2 + 1]};
+  kv_for<2>([&](auto P) { dst[P] += p.row * rs; });
+  const int32_t groups = (p.end - p.old) * CPT;
+  for (int32_t c0 = threadIdx.x; c0 < groups; c0 += 512) {
+    u32x2 code[2][2];
+    kv_for<2>([&](auto U) {
+      const int32_t c = min(c0 + 256 * U, groups - 1);
+      code[0][U] = *reinterpret_cast<const u32x2 *>(b.k + at + c * 8);
+      code[1][U] = *reinterpret_cast<const u32x2 *>(b.v + at + c * 8);
     });
-    if (a.vec) {
-      kv_for<sizeof(T) / 2>([&](auto I_) { constexpr int I = decltype(I_)::value; reinterpret_cast<u32x4 *>(to)[I] = reinterpret_cast<u32x4 *>(y)[I]; });
-    } else {
-      kv_for<8>([&](auto I_) { constexpr int I = decltype(I_)::value;
-        if (d + I < b.dim) to[I] = y[I];
-      });
-    }
+    kv_for<2>([&](auto U) {
+      const int32_t c = c0 + 256 * U, t = c / CPT, d = (c - t * CPT) * 8;
+      if (c < groups && d < b.dim)
+        kv_for<2>([&](auto P) {
+          T y[8];
+          kv_for<8>([&](auto I) {
+            constexpr int i = I;
+            const float v = there ? kv_value(code[P][U][i / 4], i % 4, scale[P]) : 0.0f;
+            if constexpr (std::is_same<T, uint16_t>::value)
+              y[i] = kv_to_bf16(v);
+            else
+              y[i] = static_cast<T>(v);
+          });
+          T *to = dst[P] + t * rs + d;
+          if (a.vec) {
+            kv_for<sizeof(T) / 2>([&](auto I) { reinterpret_cast<u32x4 *>(to)[I] = reinterpret_cast<u32x4 *>(y)[I]; });
+          } else {
+            kv_for<8>([&](auto I) {
+              if (d + I < b.dim) to[I] = y[I];
+            });
+          }
+        });
+    });
   }
 }
 
@@ -286,18 +328,28 @@ static int32_t grid_of(int64_t groups, unsigned &grid) {
 // 69 with twice as many), and not below 1024 tokens each (32 heads, 1024 tokens:
 // 12.0 whole, 13.7 in two).
 constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWideTokens = 4096;
-constexpr int64_t kTileGroups = 768, kTileTokens = 512;
+// Prompts: eight waves where the tiles leave room for them (72 pairs of parts of
+// prompts, 288 tiles: 45 us, 56 with four) or are long (8192 tokens, 8 heads: 197,
+// 220), four where two workgroups to a CU hide each other's waits (2048 tokens, 32
+// heads: 73, 77 with eight; 2 x 1024 tokens, 8 heads of 4: 41, 51).  Tokens are
+// split only up to a workgroup a CU: a part is 64 KB at 128 values a head (16
+// heads of 128, 1024 masked tokens: 66 us in two, 99 whole; 16 heads of 256: 79 in
+// two, 73 whole).
+constexpr int64_t kTileGroups = 256, kTileTokens = 512, kHalvesTasks = 384;
 static void kv_split(KvAttnArgs &a) {
   const int64_t span = a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32)
                                     : a.b.max_length;
   const int64_t tasks = static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles;
   const bool few = a.tile_rows == kKvRows;
-  a.waves = few && kv_wide(a.b.row_bytes) && span > 128 && (tasks < kWideTasks || span >= kWideTokens) ? 8 : 4;
+  if (few)
+    a.waves = kv_wide(a.b.row_bytes) && span > 128 && (tasks < kWideTasks || span >= kWideTokens) ? 8 : 4;
+  else
+    a.waves = kv_tile_halves(a.b.row_bytes) == 2 && (tasks <= kHalvesTasks || span >= kWideTokens) ? 8 : 4;
   const int64_t unit = few ? 32 * a.waves : 64;
   const int64_t steps = std::max<int64_t>(1, (span + unit - 1) / unit);
   int64_t splits = 1;
   if (tasks > 0 && tasks <= RNSMX_KV_TICKETS)
-    splits = few ? std::min(span / kSplitTokens, kSplitGroups / tasks) : std::min(span / kTileTokens, kTileGroups / tasks);
+    splits = few ? std::min(span / kSplitTokens, kSplitGroups / tasks) : std::min(span / (a.b.row_bytes > 128 ? 2 * kTileTokens : kTileTokens), kTileGroups / tasks);
   splits = std::max<int64_t>(splits, 1);
   const int64_t each = (steps + splits - 1) / splits;
   a.chunk = static_cast<int32_t>(std::min<int64_t>(each * unit, 1 << 30));
@@ -385,11 +437,11 @@ int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *b
   a.row_stride[1] = v_row_stride;
   a.head_stride[0] = k_head_stride;
   a.head_stride[1] = v_head_stride;
-  a.dtype = dtype;
   a.vec = a.b.dim % 8 == 0 && aligned(k_dev, 16) && aligned(v_dev, 16) && k_row_stride * size % 16 == 0 &&
           v_row_stride * size % 16 == 0 && k_head_stride * size % 16 == 0 && v_head_stride * size % 16 == 0;
   const int64_t pages = pages_touched(a.b);
-  a.pages = static_cast<int32_t>(pages);
+  a.by_heads = kv_div(a.b.heads);
+  a.by_pages = kv_div(static_cast<uint32_t>(pages));
   unsigned grid;
   if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads * 2, grid)) return rc;
   // every thread holds kKvHeld groups of 8 values of the tokens that a page can get
@@ -419,12 +471,12 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
     return fail(RNSMX_EINVAL, "keys or values null or not aligned to their type");
   a.dst[0] = k_dev;
   a.dst[1] = v_dev;
-  a.dtype = dtype;
   a.vec = a.b.dim % 8 == 0 && aligned(k_dev, 16) && aligned(v_dev, 16);
   const int64_t pages = pages_touched(a.b);
-  a.pages = static_cast<int32_t>(pages);
+  a.by_heads = kv_div(a.b.heads);
+  a.by_pages = kv_div(static_cast<uint32_t>(pages));
   unsigned grid;
-  if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads * 2, grid)) return rc;
+  if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads, grid)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == RNSMX_FLOAT32) {
     RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, float>), dim3(grid), dim3(256), 0, st, a))

@@ -111,7 +111,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
     const F32x2 sc = *reinterpret_cast<const F32x2 *>(b.scales + slot_v * 2);
     s.ks = sc.x;
     s.vs = sc.y;
-    if constexpr (MASK) kv_mask_load(s.m, a, q.row + t_row, q_head, t0 + 8 * g);
+    if constexpr (MASK) kv_mask_load(s.m, a, q.row + t_row, q_head, t0 + 8 * g, t0 + 32);
   };
 
   // The first step's loads go out before the queries', one wait for both, where

@@ -34,26 +34,37 @@ __device__ __forceinline__ int32_t value_swap(int32_t d) { return (d & 7) ^ (d >
 // converted once; wave w loads and converts tokens 16 w .. 16 w + 15, which lie
 // in one page.  The products and the weights are as kv_rows_kernel's, with
 // 32 x 32 products: a row is one lane pair's.
-template <int DT, bool SPLIT, bool MASK>
-__global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(const KvAttnArgs a) {
+//
+// HALVES 2: eight waves, the second four with the same rows and every other
+// step, staged apart; they join in the shared memory at the end.  A step's chain
+// (load, products, weights, products, conversions: some 4000 cycles, twice that
+// of its longest part) is then run through half as often by the longest tiles,
+// which a call of few workgroups waits for.
+template <int DT, int HALVES, bool SPLIT, bool MASK>
+__global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(const KvAttnArgs a) {
   constexpr int KS = DT / 16, DB = DT / 32, QN = SPLIT ? 2 : 1;
   constexpr int KROW = (DT + 63) / 64 * 64;  // halves of a staged key
   constexpr int KR = DT / 32;                // loads of 8 codes a lane and step, keys
   constexpr int VD = DT == 64 ? 2 : DT == 256 ? 8 : 4;  // columns of 8 tokens that a lane converts
   constexpr int VG = DT / VD, VR = (2 * VG + 63) / 64;  // of a token group, and rounds
-  __shared__ __attribute__((aligned(128))) _Float16 keys[2][kStep * KROW];
-  __shared__ __attribute__((aligned(128))) _Float16 values[2][DT * kStep];
+  // each half's two buffers of keys and of values
+  constexpr int kKeys = kStep * KROW, kValues = DT * kStep;
+  __shared__ __attribute__((aligned(128))) _Float16 staged[HALVES][2 * kKeys + 2 * kValues];
+  // key scale, log2 and reciprocal of the value scale, whether it is there
+  __shared__ __attribute__((aligned(16))) float page_scales[HALVES][2][4][4];
   __shared__ int32_t last;
-  __shared__ __attribute__((aligned(16))) float pages_of_step[2][4][4];  // key scale, log2 and reciprocal of the value scale, whether it is there
 
   const KvBatchArgs &b = a.b;
-  const KvPlace place = kv_place(a, blockIdx.x, gridDim.x, true);
+  const KvPlace place = kv_place(a, blockIdx.x, gridDim.x, HALVES == 1);
   const int32_t split = place.split, task = place.task, tile = place.tile, head = place.head, seq = place.seq;
   const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
   const int32_t rows = q.n * group, row0 = tile * kKvTileRows;
   if (row0 >= rows) return;
-  const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t half = HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  _Float16 *const keys = staged[half], *const values = keys + 2 * kKeys;
+  float (*const pages_of_step)[4][4] = page_scales[half];
   const int32_t col = lane & 31, h = lane >> 5;
   const int32_t base = q.len - q.n;
   auto kv_of = [&](int32_t r) { return static_cast<int32_t>(kv_quot(a.by_group, r)); };  // the token of a row
@@ -67,12 +78,12 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   const int32_t w_first = row0 + 32 * wave, w_last = min(w_first + 31, rows - 1);
   const bool w_any = w_first < rows;
   const int32_t t_first = kv_of(w_first), t_last = kv_of(w_last);
-  const int32_t full_hi = a.causal ? base + t_first + 1 : q.len;
+  const int32_t full_hi = min(a.causal ? base + t_first + 1 : q.len, c1);
   const int32_t full_lo = a.window > 0 ? max(base + t_last + 1 - a.window, 0) : 0;
 
   const int32_t row = min(w_first + col, rows - 1);
   const int32_t t_row = kv_of(row), q_head = head * group + (row - t_row * group);
-  const int32_t end_row = a.causal ? base + t_row + 1 : q.len;
+  const int32_t end_row = min(a.causal ? base + t_row + 1 : q.len, c1);
   const int32_t begin_row = a.window > 0 ? max(base + t_row + 1 - a.window, 0) : 0;
 
   // loads of a step: this wave's 16 tokens
@@ -120,7 +131,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     kv_for<KR>([&](auto R) {
       constexpr int r = R;
       const int32_t item = lane + 64 * r, t = 16 * wave + item / (DT / 8), c = item % (DT / 8);
-      *reinterpret_cast<h16x8 *>(&keys[buf][t * KROW + (c ^ key_swap(t)) * 8]) = kv_row8(kr[r][0], kr[r][1]);
+      *reinterpret_cast<h16x8 *>(&keys[buf * kKeys + t * KROW + (c ^ key_swap(t)) * 8]) = kv_row8(kr[r][0], kr[r][1]);
     });
     kv_for<VR>([&](auto R) {
       constexpr int r = R;
@@ -132,7 +143,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
           const auto &v = vr[r];
           const h16x8 x = kv_join(kv_halves<byte, byte>(v[0][w], v[1][w]), kv_halves<byte, byte>(v[2][w], v[3][w]),
                                   kv_halves<byte, byte>(v[4][w], v[5][w]), kv_halves<byte, byte>(v[6][w], v[7][w]));
-          *reinterpret_cast<h16x8 *>(&values[buf][(d0 + i) * kStep + (group ^ value_swap(d0 + i)) * 8]) = x;
+          *reinterpret_cast<h16x8 *>(&values[buf * kValues + (d0 + i) * kStep + (group ^ value_swap(d0 + i)) * 8]) = x;
         });
       }
     });
@@ -144,10 +155,14 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     }
   };
 
+  // a half's steps; past the chunk's end it goes on with the last one, all hidden
+  constexpr int32_t kStride = HALVES * kStep;
+  auto step_at = [&](int32_t t0) { return min(t0, c1 - 1) & ~(kStep - 1); };
+  const int32_t first = c0 + kStep * half;
   int32_t page = 0;
   if (c0 < c1) {
-    load_step(c0, page_of(c0));
-    page = page_of(min(c0 + kStep, c1 - 1) & ~(kStep - 1));
+    load_step(step_at(first), page_of(step_at(first)));
+    page = page_of(step_at(first + kStride));
   }
 
   h16x8 qf[QN][KS];
@@ -188,7 +203,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
       constexpr int s = S;
       kv_for<2>([&](auto B) {
         constexpr int sub = B;
-        const h16x8 k = *reinterpret_cast<const h16x8 *>(&keys[buf][(32 * sub + kt) * KROW + (((2 * s + h)) ^ swap) * 8]);
+        const h16x8 k = *reinterpret_cast<const h16x8 *>(&keys[buf * kKeys + (32 * sub + kt) * KROW + (((2 * s + h)) ^ swap) * 8]);
         kv_for<QN>([&](auto P) { acc[sub] = kv_mfma32(k, qf[P][s], acc[sub]); });
       });
     });
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
         constexpr int g = G;
         const int32_t t8 = t0 + 16 * g + 8 * h;
         uint32_t m[8];
-        if constexpr (MASK) kv_mask_load(m, a, q.row + t_row, q_head, t8);
+        if constexpr (MASK) kv_mask_load(m, a, q.row + t_row, q_head, t8, t0 + kStep);
         bool any = false;
         kv_for<8>([&](auto J) {
           constexpr int j = J;
@@ -281,7 +296,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
       kv_for<DB>([&](auto I) {
         constexpr int i = I;
         const int32_t d = 32 * i + col;
-        const h16x8 v = *reinterpret_cast<const h16x8 *>(&values[buf][d * kStep + ((2 * g + h) ^ value_swap(d)) * 8]);
+        const h16x8 v = *reinterpret_cast<const h16x8 *>(&values[buf * kValues + d * kStep + ((2 * g + h) ^ value_swap(d)) * 8]);
         kv_for<QN>([&](auto P) { o[i] = kv_mfma32(v, p[P], o[i]); });
       });
     });
@@ -290,19 +305,52 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   if (c0 < c1) {
     stage(0);
     int32_t buf = 0;
-    for (int32_t t0 = c0; t0 < c1; t0 += kStep, buf ^= 1) {
+    for (int32_t at = c0; at < c1; at += kStride, buf ^= 1) {
       __syncthreads();  // this step is staged, and the other buffer's readers are done
       // The next step's codes (the last step's again after it: no branch parts
       // the products from the conversions).  A wave whose rows see nothing of a
       // step goes through it all the same, beside those that do.
-      const int32_t next = min(t0 + kStep, c1 - 1) & ~(kStep - 1);
-      load_step(next, page);
-      page = page_of(min(t0 + 2 * kStep, c1 - 1) & ~(kStep - 1));
+      const int32_t t0 = at + kStep * half;
+      load_step(step_at(t0 + kStride), page);
+      page = page_of(step_at(t0 + 2 * kStride));
       compute(buf, t0);
       stage(buf ^ 1);
     }
   }
   sum += __shfl_xor(sum, 32);
+
+  if constexpr (HALVES == 2) {
+    // the second half's sums as its lanes hold them, into the buffers of both
+    float *const sums = reinterpret_cast<float *>(staged[1]) + tid * 4;
+    float *const refs = reinterpret_cast<float *>(staged[0]) + tid;
+    static_assert(sizeof(staged[0]) >= 256 * 4 * 4 * DB * sizeof(float), "a half's sums");
+    __syncthreads();
+    if (half == 1) {
+      kv_for<4 * DB>([&](auto K) {
+        constexpr int k = K, i = k / 4, r = 4 * (k % 4);
+        *reinterpret_cast<f32x4 *>(sums + k * 1024) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+      });
+      refs[0] = mx;
+      refs[256] = ml;
+      refs[512] = sum;
+    }
+    __syncthreads();
+    if (half == 0) {
+      const float mx2 = refs[0], ml2 = refs[256], mx1 = mx, ml1 = ml;
+      kv_reference<MASK>(mx, ml, mx2, ml2);
+      const float f1 = kv_factor<MASK>(mx1, ml1, mx, ml), f2 = kv_factor<MASK>(mx2, ml2, mx, ml);
+      sum = sum * f1 + refs[512] * f2;
+      kv_for<4 * DB>([&](auto K) {
+        constexpr int k = K, i = k / 4, r = 4 * (k % 4);
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(sums + k * 1024);
+        kv_for<4>([&](auto J) {
+          constexpr int j = J;
+          o[i][r + j] = o[i][r + j] * f1 + v[j] * f2;
+        });
+      });
+    }
+  }
+  const bool mine = w_any && half == 0;  // the waves that go on with the rows
 
   // Split over its tokens, a workgroup leaves its sums in the workspace as the
   // lanes hold them, two at a time; the one that draws the task's last ticket
@@ -316,7 +364,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
                          static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
                          __HIP_MEMORY_SCOPE_AGENT);
     };
-    if (w_any) {
+    if (mine) {
       kv_for<DB>([&](auto I) {
         kv_for<8>([&](auto J) {
           constexpr int i = I, j = J;
@@ -328,13 +376,13 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (tid == 0) {
+    if (threadIdx.x == 0) {
       const uint32_t old = __hip_atomic_fetch_add(a.tickets + task, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       last = old == static_cast<uint32_t>(active - 1);
       if (last) __hip_atomic_store(a.tickets + task, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!last || !w_any) return;
+    if (!last || !mine) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     auto get = [&](int32_t s, int64_t i) { return *reinterpret_cast<const F32x2 *>(at + s * kPart + i); };
     // the highest reference of all, as kv_higher orders them
@@ -342,17 +390,13 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     ml = 0.0f;
     for (int32_t s = 0; s < active; ++s) {
       const F32x2 r = get(s, 8 * DB * 512);
-      const float s1 = mx * kNat + ml, s2 = r.x * kNat + r.y;
-      const bool take = r.x > -INFINITY && (!(mx > -INFINITY) || s2 > s1 || (s2 == s1 && (r.x > mx || (r.x == mx && r.y > ml))));
-      mx = take ? r.x : mx;
-      ml = take ? r.y : ml;
+      kv_reference<MASK>(mx, ml, r.x, r.y);
     }
     sum = 0.0f;
     kv_for<DB>([&](auto I) { kv_for<16>([&](auto J) { o[I][static_cast<int>(J)] = 0.0f; }); });
     for (int32_t s = 0; s < active; ++s) {
       const F32x2 r = get(s, 8 * DB * 512), t = get(s, (8 * DB + 1) * 512);
-      // not-a-numbers of a part without a reference go through
-      const float f = r.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((r.x - mx) * kNat + (r.y - ml));
+      const float f = kv_factor<MASK>(r.x, r.y, mx, ml);
       sum = fmaf(t.x, f, sum);
       kv_for<DB>([&](auto I) {
         kv_for<8>([&](auto J) {
@@ -365,7 +409,7 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
     }
   }
 
-  if (!w_any || w_first + col >= rows) return;
+  if (!mine || w_first + col >= rows) return;
   // l = sum 2^ml, and the codes' unit
   const float f = sum == 0.0f ? 0.0f : kKvUnit / sum;
   const int64_t out = (static_cast<int64_t>(q.row + t_row) * a.q_heads + q_head) * b.dim;
@@ -401,20 +445,28 @@ __global__ __launch_bounds__(256, (DT <= 128 ? 2 : 1)) void kv_tiles_kernel(cons
   });
 }
 
-template <int DT>
-void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles * a.splits)), block(256);
+template <int DT, int HALVES>
+static void launch_halves(const KvAttnArgs &a, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles * a.splits)), block(256 * HALVES);
   const bool split = a.dtype == RNSMX_FLOAT32;
   if (a.mask) {
     if (split)
-      hipLaunchKernelGGL((kv_tiles_kernel<DT, true, true>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((kv_tiles_kernel<DT, HALVES, true, true>), grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL((kv_tiles_kernel<DT, false, true>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((kv_tiles_kernel<DT, HALVES, false, true>), grid, block, 0, st, a);
   } else if (split) {
-    hipLaunchKernelGGL((kv_tiles_kernel<DT, true, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((kv_tiles_kernel<DT, HALVES, true, false>), grid, block, 0, st, a);
   } else {
-    hipLaunchKernelGGL((kv_tiles_kernel<DT, false, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((kv_tiles_kernel<DT, HALVES, false, false>), grid, block, 0, st, a);
   }
+}
+
+template <int DT>
+void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st) {
+  if (a.waves == 8)
+    launch_halves<DT, kv_tile_halves(DT)>(a, st);
+  else
+    launch_halves<DT, 1>(a, st);
 }
 
 template void launch_kv_tiles<RNSMX_KV_DIM>(const KvAttnArgs &a, hipStream_t st);

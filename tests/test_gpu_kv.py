@@ -238,6 +238,57 @@ def test_several_tokens(backend, dtype, group, dim, page, causal, window):
     w.check(news, dtype, 2 * group, **options)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads,group,dim,page", [(1, 1, 64, 16), (2, 2, 40, 64), (1, 3, 128, 32), (1, 1, 160, 16), (1, 2, 250, 128)])
+@pytest.mark.parametrize("window", [None, 300])
+def test_prompts_split_over_their_tokens(backend, dtype, heads, group, dim, page, window):
+    """Long histories and prompts of a few workgroups, whose tokens are split."""
+    lengths, news = [1500, 130, 700, 0], [150, 130, 65, 1]
+    w = World(backend, lengths=lengths, heads=heads, dim=dim, page=page, seed=dim + page)
+    w.append(lengths, dtype)
+    batch = w.batch(news)
+    need = w.backend.kv_attention_workspace_bytes(w.cache, batch, q_heads=heads * group, dtype=dtype)
+    assert need > 0 or dim > 128  # wider heads are split from twice as many tokens on
+    w.check(news, dtype, heads * group, **({} if window is None else {"window": window}))
+    space = torch.zeros(need, dtype=torch.uint8, device=DEV)
+    q = torch.randn((sum(news), heads * group, dim), generator=w.gen).to(dtype).to(DEV)
+    first = w.backend.kv_attention(q, w.cache, batch, workspace=space)
+    for _ in range(5):
+        assert torch.equal(w.backend.kv_attention(q, w.cache, batch, workspace=space), first)
+    assert (space[:4 * 16384] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [160, 256])
+def test_prompts_of_wide_heads_split(backend, dtype, dim):
+    w = World(backend, lengths=[3333, 90], heads=1, dim=dim, page=64, seed=dim)
+    w.append([3333, 90], dtype)
+    news = [129, 66]
+    assert w.backend.kv_attention_workspace_bytes(w.cache, w.batch(news), q_heads=1, dtype=dtype) > 0
+    w.check(news, dtype, 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_of_many_sequences(backend, dtype, dim):
+    """Enough workgroups that each runs on four waves."""
+    seqs = 150
+    lengths = [60 + 7 * (i % 15) for i in range(seqs)]
+    news = [66 + (i % 3) if n >= 70 else n for i, n in enumerate(lengths)]
+    w = World(backend, lengths=lengths, heads=8, dim=dim, page=32, seed=26)
+    w.append(lengths, dtype)
+    q = torch.randn((sum(news), 8, dim), generator=w.gen).to(dtype)
+    got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch(news)).cpu().double()
+    at = 0
+    for i, n in enumerate(news):
+        if i % 29 == 0:
+            k, there = w.k.values(w.table[i], lengths[i])
+            v, _ = w.v.values(w.table[i], lengths[i])
+            out, spread, reach = ko.attention(q[at:at + n], k, v, there)
+            assert ((got[at:at + n] - out).abs() <= bound(dtype, out, spread, reach, dim, lengths[i], None)).all()
+        at += n
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_scale_and_large_products(backend, dtype):
     w = World(backend, lengths=[190, 7], heads=2, dim=64, page=16, seed=12)

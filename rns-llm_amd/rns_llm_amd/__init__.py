@@ -1,6 +1,8 @@
 """rns_llm_amd: MI355X-native backend for the RNS linear / fused-QKV path of
 Nek1tt/rns-llm.  Public names mirror ``rns_llm`` (``src/rns_llm/__init__.py``,
-``backends/__init__.py``, ``layers/__init__.py``)."""
+``backends/__init__.py``, ``layers/__init__.py``), but for the 8-bit key/value
+cache (``KVCache``, ``KVBatch``, ``RNSCachedAttention``), which it has no
+counterpart of."""
 from .backends import (
     AdaptiveMetadata,
     HipRNSBackend,
@@ -15,6 +17,7 @@ from .backends import (
 from .layers import (
     CachedRNSQKV,
     InstalledQKVFusion,
+    RNSCachedAttention,
     RNSLinear,
     RNSQKVProjection,
     install_opt_qkv_fusion,
@@ -34,7 +37,7 @@ from .moduli import (
 __all__ = [
     "AdaptiveMetadata", "HipRNSBackend", "KVBatch", "KVCache", "PreparedAdaptiveRNSWeight", "PreparedRNSWeight",
     "RNSRequestBatchWorkspace", "RNSWorkspace", "hip_extension_available", "CachedRNSQKV",
-    "InstalledQKVFusion", "RNSLinear", "RNSQKVProjection", "install_opt_qkv_fusion",
+    "InstalledQKVFusion", "RNSCachedAttention", "RNSLinear", "RNSQKVProjection", "install_opt_qkv_fusion",
     "replace_opt_attention_blocks",
     "DENSE_COPRIME_MODULI", "LARGE_PRIME_MODULI", "SMALL_PRIME_MODULI", "choose_moduli_for_dot",
     "minimal_prefix_channels", "safe_l1_dot_bound", "signed_capacity", "validate_moduli",

@@ -221,11 +221,16 @@ class KVCacheOps:
         """The keys and values of the batch's rows, ``code * scale`` rounded to
         ``dtype``: two ``[rows, kv_heads, head_dim]`` tensors, in one launch.
         Rows that have no token, and those in pages that are not there, are zero."""
-        if dtype not in _FLOAT_CODES:
-            raise ValueError("dtype must be float32, float16 or bfloat16")
-        shape = (batch.rows, cache.kv_heads, cache.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=cache.device)
-        v = torch.empty(shape, dtype=dtype, device=cache.device)
+        key = (dtype, cache._shape)
+        like = batch._checked.get(key)
+        if like is None:
+            if dtype not in _FLOAT_CODES:
+                raise ValueError("dtype must be float32, float16 or bfloat16")
+            # one value's memory in the outputs' shape: what they are made like costs less than their sizes
+            like = torch.empty((1,), dtype=dtype, device=cache.device).expand(batch.rows, cache.kv_heads, cache.head_dim)
+            batch._checked[key] = like
+        k = torch.empty_like(like, memory_format=torch.contiguous_format)
+        v = torch.empty_like(like, memory_format=torch.contiguous_format)
         rc = self._lib.rnsmx_kv_read(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), _FLOAT_CODES[dtype],
                                      self._stream_of(cache.device))
         if rc:
@@ -261,7 +266,7 @@ class KVCacheOps:
             checked = batch._checked[key] = (query, ctypes.addressof(query), need)
         _, ref, need = checked
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
             raise ValueError("out must be contiguous and like q")
         stream = self._stream_of(cache.device)

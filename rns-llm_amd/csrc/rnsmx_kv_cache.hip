@@ -329,12 +329,12 @@ static int32_t grid_of(int64_t groups, unsigned &grid) {
 // 12.0 whole, 13.7 in two).
 constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWideTokens = 4096;
 // Prompts: eight waves where the tiles leave room for them (72 pairs of parts of
-// prompts, 288 tiles: 45 us, 56 with four) or are long (8192 tokens, 8 heads: 197,
-// 220), four where two workgroups to a CU hide each other's waits (2048 tokens, 32
-// heads: 73, 77 with eight; 2 x 1024 tokens, 8 heads of 4: 41, 51).  Tokens are
-// split only up to a workgroup a CU: a part is 64 KB at 128 values a head (16
-// heads of 128, 1024 masked tokens: 66 us in two, 99 whole; 16 heads of 256: 79 in
-// two, 73 whole).
+// prompts, 288 tiles: 47 us, 60 with four) or are few and long (8192 tokens, 8
+// heads, 512 tiles: 197, 220), four where two workgroups to a CU hide each other's
+// waits (8192 tokens, 32 heads: 654, 726 with eight; 2048 tokens, 32 heads: 73,
+// 77).  Tokens are split only up to a workgroup a CU: a part is 64 KB at 128
+// values a head (16 heads of 128, 1024 masked tokens: 59 us in two, 99 whole; 16
+// heads of 256: 60, 73; 2048 tokens, 32 heads, 512 tiles: 82 in two, 73 whole).
 constexpr int64_t kTileGroups = 256, kTileTokens = 512, kHalvesTasks = 384;
 static void kv_split(KvAttnArgs &a) {
   const int64_t span = a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32)
@@ -344,12 +344,15 @@ static void kv_split(KvAttnArgs &a) {
   if (few)
     a.waves = kv_wide(a.b.row_bytes) && span > 128 && (tasks < kWideTasks || span >= kWideTokens) ? 8 : 4;
   else
-    a.waves = kv_tile_halves(a.b.row_bytes) == 2 && (tasks <= kHalvesTasks || span >= kWideTokens) ? 8 : 4;
+    a.waves = kv_tile_halves(a.b.row_bytes) == 2 &&
+                      (tasks <= kHalvesTasks || (tasks <= 512 && span >= kWideTokens))
+                  ? 8
+                  : 4;
   const int64_t unit = few ? 32 * a.waves : 64;
   const int64_t steps = std::max<int64_t>(1, (span + unit - 1) / unit);
   int64_t splits = 1;
   if (tasks > 0 && tasks <= RNSMX_KV_TICKETS)
-    splits = few ? std::min(span / kSplitTokens, kSplitGroups / tasks) : std::min(span / (a.b.row_bytes > 128 ? 2 * kTileTokens : kTileTokens), kTileGroups / tasks);
+    splits = few ? std::min(span / kSplitTokens, kSplitGroups / tasks) : std::min(span / kTileTokens, kTileGroups / tasks);
   splits = std::max<int64_t>(splits, 1);
   const int64_t each = (steps + splits - 1) / splits;
   a.chunk = static_cast<int32_t>(std::min<int64_t>(each * unit, 1 << 30));

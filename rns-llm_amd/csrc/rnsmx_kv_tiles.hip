@@ -385,27 +385,44 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
     if (!last || !mine) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     auto get = [&](int32_t s, int64_t i) { return *reinterpret_cast<const F32x2 *>(at + s * kPart + i); };
-    // the highest reference of all, as kv_higher orders them
+    // the highest reference of all, the references of four parts at a time; then
+    // the parts in their order, this workgroup's own as it still holds it
+    f32x16 own[DB];
+    kv_for<DB>([&](auto I) {
+      own[I] = o[I];
+      kv_for<16>([&](auto J) { o[I][static_cast<int>(J)] = 0.0f; });
+    });
+    const float own_sum = sum;
     mx = -INFINITY;
-    ml = 0.0f;
+    ml = sum = 0.0f;
+    for (int32_t s0 = 0; s0 < active; s0 += 4) {
+      F32x2 r[4];
+      kv_for<4>([&](auto S) { r[S] = get(min(s0 + S, active - 1), 8 * DB * 512); });
+      kv_for<4>([&](auto S) { kv_reference<MASK>(mx, ml, r[S].x, r[S].y); });
+    }
     for (int32_t s = 0; s < active; ++s) {
       const F32x2 r = get(s, 8 * DB * 512);
-      kv_reference<MASK>(mx, ml, r.x, r.y);
-    }
-    sum = 0.0f;
-    kv_for<DB>([&](auto I) { kv_for<16>([&](auto J) { o[I][static_cast<int>(J)] = 0.0f; }); });
-    for (int32_t s = 0; s < active; ++s) {
-      const F32x2 r = get(s, 8 * DB * 512), t = get(s, (8 * DB + 1) * 512);
-      const float f = kv_factor<MASK>(r.x, r.y, mx, ml);
-      sum = fmaf(t.x, f, sum);
-      kv_for<DB>([&](auto I) {
-        kv_for<8>([&](auto J) {
-          constexpr int i = I, j = J;
-          const F32x2 v = get(s, (8 * i + j) * 512);
-          o[i][2 * j] = fmaf(v.x, f, o[i][2 * j]);
-          o[i][2 * j + 1] = fmaf(v.y, f, o[i][2 * j + 1]);
+      if (s == split) {
+        const float f = kv_factor<MASK>(r.x, r.y, mx, ml);
+        sum = fmaf(own_sum, f, sum);
+        kv_for<DB>([&](auto I) {
+          kv_for<16>([&](auto J) {
+            constexpr int i = I, j = J;
+            o[i][j] = fmaf(own[i][j], f, o[i][j]);
+          });
         });
-      });
+      } else {
+        const F32x2 t = get(s, (8 * DB + 1) * 512);
+        F32x2 v[8 * DB];
+        kv_for<8 * DB>([&](auto K) { v[K] = get(s, K * 512); });
+        const float f = kv_factor<MASK>(r.x, r.y, mx, ml);
+        sum = fmaf(t.x, f, sum);
+        kv_for<8 * DB>([&](auto K) {
+          constexpr int k = K, i = k / 8, j = 2 * (k % 8);
+          o[i][j] = fmaf(v[k].x, f, o[i][j]);
+          o[i][j + 1] = fmaf(v[k].y, f, o[i][j + 1]);
+        });
+      }
     }
   }
 

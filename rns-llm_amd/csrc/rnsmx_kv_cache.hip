@@ -336,9 +336,11 @@ constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWi
 // values a head (16 heads of 128, 1024 masked tokens: 59 us in two, 99 whole; 16
 // heads of 256: 60, 73; 2048 tokens, 32 heads, 512 tiles: 82 in two, 73 whole).
 constexpr int64_t kTileGroups = 256, kTileTokens = 512, kHalvesTasks = 384;
+static int64_t kv_tokens(const KvAttnArgs &a) {  // most that a sequence's rows see
+  return a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32) : a.b.max_length;
+}
 static void kv_split(KvAttnArgs &a) {
-  const int64_t span = a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32)
-                                    : a.b.max_length;
+  const int64_t span = kv_tokens(a);
   const int64_t tasks = static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles;
   const bool few = a.tile_rows == kKvRows;
   if (few)
@@ -359,8 +361,20 @@ static void kv_split(KvAttnArgs &a) {
   a.splits = static_cast<int32_t>((steps + each - 1) / each);
 }
 
-// Up to so many rows of a sequence and key/value head run 16 to a workgroup.
-constexpr int64_t kFewRows = 64;
+// Whether a call runs 16 rows to a workgroup: up to kFewRows rows of a sequence and
+// key/value head, and past them while the work is too little to fill the chip with
+// tiles of 128: kFewGroups workgroups of 16 rows, each seeing so many tokens that
+// together they see kFewTokens.  One sequence of 8000 tokens, 8 heads, 128 rows: 27
+// us so, 53 in tiles, 512 rows: 58 and 54; 32 sequences of 2000, 8 heads, 48 rows: 39
+// and 54, 96 rows: 65 and 55; 4 of 500, 12 heads of 64, 400 rows: 11 and 17; prompts
+// of 1024 in float32, 32 heads: 58 and 44.  Half as many groups of heads wider than
+// 160, whose waves are one to a SIMD (1024 tokens, 16 heads of 256: 70 and 60).
+constexpr int64_t kFewRows = 32, kFewGroups = 1280, kFewTokens = 1750000;
+static bool few_rows(const KvBatchArgs &b, int64_t rows, int64_t span) {
+  if (rows <= kFewRows) return true;
+  const int64_t groups = static_cast<int64_t>(b.seqs) * b.heads * ((rows + kKvRows - 1) / kKvRows);
+  return groups <= (kv_wide(b.row_bytes) ? kFewGroups : kFewGroups / 2) && groups * std::max<int64_t>(span - b.max_rows / 2, 1) <= kFewTokens;
+}
 
 // Pairs of sequences and heads whose workgroups run side by side: all, or where
 // there are many a divisor of their number, so that an XCD's part of them stays
@@ -394,7 +408,7 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   a.window = query->window;
   a.scale = query->scale;
   const int64_t rows = static_cast<int64_t>(a.b.max_rows) * (query->q_heads / cache->heads);
-  a.tile_rows = rows <= kFewRows ? kKvRows : kKvTileRows;
+  a.tile_rows = few_rows(a.b, rows, kv_tokens(a)) ? kKvRows : kKvTileRows;
   const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows;
   if (tiles > 0x7FFFFFFF) return fail(RNSMX_EINVAL, "too many rows");
   a.row_tiles = static_cast<int32_t>(tiles);

@@ -15,17 +15,23 @@ TYPES = [torch.float32, torch.float16, torch.bfloat16]
 ROUND = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
+# Sequences that hold nothing and ask nothing beside a test's own: with so many
+# the prompts' kernel runs what few rows' would.
+MANY = 170
+
+
 class World:
     """A cache on the GPU and its oracle, filled alike."""
 
-    def __init__(self, backend, *, lengths, heads, dim, page, seed, spare=2):
+    def __init__(self, backend, *, lengths, heads, dim, page, seed, spare=2, idle=0):
+        self.idle = idle
         self.backend, self.heads, self.dim, self.page = backend, heads, dim, page
         self.gen = torch.Generator().manual_seed(seed)
         pages = [max(1, -(-n // page)) for n in lengths]
         blocks = sum(pages) + spare
         order = torch.randperm(blocks, generator=self.gen, dtype=torch.int32)
         # entries past a sequence's end hold numbers that are no page's
-        self.table = torch.full((len(lengths), max(pages)), 2 ** 31 - 1, dtype=torch.int32)
+        self.table = torch.full((len(lengths) + idle, max(pages)), 2 ** 31 - 1, dtype=torch.int32)
         at = 0
         for i, n in enumerate(pages):
             self.table[i, :n] = order[at:at + n]
@@ -36,8 +42,9 @@ class World:
         self.lengths = list(lengths)
 
     def batch(self, news, lengths=None, **more):
-        return self.backend.kv_batch(self.cache, self.table.to(DEV), self.lengths if lengths is None else lengths,
-                                     query_lengths=news, **more)
+        lengths = self.lengths if lengths is None else lengths
+        return self.backend.kv_batch(self.cache, self.table.to(DEV), list(lengths) + [0] * self.idle,
+                                     query_lengths=list(news) + [0] * self.idle, **more)
 
     def tokens(self, rows, dtype, heads=None):
         x = torch.randn((rows, heads or self.heads, self.dim), generator=self.gen)
@@ -230,26 +237,38 @@ def test_single_tokens(backend, dtype, heads, group, dim, page):
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("group,dim,page", [(1, 64, 16), (3, 128, 32), (4, 80, 64)])
 @pytest.mark.parametrize("causal,window", [(True, None), (False, None), (True, 1), (True, 45)])
-def test_several_tokens(backend, dtype, group, dim, page, causal, window):
+@pytest.mark.parametrize("idle", [0, MANY])
+def test_several_tokens(backend, dtype, group, dim, page, causal, window, idle):
     lengths, news = [70, 5, 200, 0, 33, 128], [70, 5, 3, 2, 1, 37]
-    w = World(backend, lengths=lengths, heads=2, dim=dim, page=page, seed=dim + page)
+    w = World(backend, lengths=lengths, heads=2, dim=dim, page=page, seed=dim + page, idle=idle)
     w.append(lengths, dtype)
     options = {"causal": causal} if window is None else {"window": window}
     w.check(news, dtype, 2 * group, **options)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("heads,group,dim,page", [(1, 1, 64, 16), (2, 2, 40, 64), (1, 3, 128, 32), (1, 1, 160, 16), (1, 2, 250, 128)])
-@pytest.mark.parametrize("window", [None, 300])
-def test_prompts_split_over_their_tokens(backend, dtype, heads, group, dim, page, window):
-    """Long histories and prompts of a few workgroups, whose tokens are split."""
-    lengths, news = [1500, 130, 700, 0], [150, 130, 65, 1]
-    w = World(backend, lengths=lengths, heads=heads, dim=dim, page=page, seed=dim + page)
+@pytest.mark.parametrize("heads,dim,page", [(1, 1, 16), (3, 40, 32), (2, 65, 64), (1, 160, 16), (1, 192, 128), (1, 250, 64), (1, 256, 32)])
+def test_prompts_of_any_head(backend, dtype, heads, dim, page):
+    lengths, news = [129, 40, 190, 1, 64], [129, 40, 70, 1, 64]
+    w = World(backend, lengths=lengths, heads=heads, dim=dim, page=page, seed=dim, idle=MANY)
+    w.append(lengths, dtype)
+    w.check(news, dtype, heads)
+    w.check(news, dtype, 2 * heads, window=50)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads,group,dim,page,lengths,news,idle", [
+    (1, 1, 64, 16, [3000, 700], [640, 65], 18), (2, 2, 40, 64, [2600, 130], [300, 130], 8), (1, 3, 128, 32, [3000, 1], [600, 1], 5),
+    (1, 1, 160, 16, [3000, 0], [640, 1], 18), (1, 2, 250, 128, [3000, 90], [640, 66], 8),
+])
+def test_prompts_split_over_their_tokens(backend, dtype, heads, group, dim, page, lengths, news, idle):
+    """Long prompts of a few workgroups, whose tokens are split."""
+    w = World(backend, lengths=lengths, heads=heads, dim=dim, page=page, seed=dim + page, idle=idle)
     w.append(lengths, dtype)
     batch = w.batch(news)
     need = w.backend.kv_attention_workspace_bytes(w.cache, batch, q_heads=heads * group, dtype=dtype)
-    assert need > 0 or dim > 128  # wider heads are split from twice as many tokens on
-    w.check(news, dtype, heads * group, **({} if window is None else {"window": window}))
+    assert need > 0
+    w.check(news, dtype, heads * group)
     space = torch.zeros(need, dtype=torch.uint8, device=DEV)
     q = torch.randn((sum(news), heads * group, dim), generator=w.gen).to(dtype).to(DEV)
     first = w.backend.kv_attention(q, w.cache, batch, workspace=space)
@@ -259,13 +278,14 @@ def test_prompts_split_over_their_tokens(backend, dtype, heads, group, dim, page
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("dim", [160, 256])
-def test_prompts_of_wide_heads_split(backend, dtype, dim):
-    w = World(backend, lengths=[3333, 90], heads=1, dim=dim, page=64, seed=dim)
-    w.append([3333, 90], dtype)
-    news = [129, 66]
-    assert w.backend.kv_attention_workspace_bytes(w.cache, w.batch(news), q_heads=1, dtype=dtype) > 0
-    w.check(news, dtype, 1)
+@pytest.mark.parametrize("group,dim", [(1, 128), (4, 64), (1, 256)])
+def test_some_rows_split_over_their_tokens(backend, dtype, group, dim):
+    """Up to a few hundred rows of few sequences take 16 to a workgroup, split."""
+    lengths, news = [1500, 130, 700, 0], [150, 130, 65, 1]
+    w = World(backend, lengths=lengths, heads=1, dim=dim, page=16, seed=dim)
+    w.append(lengths, dtype)
+    w.check(news, dtype, group)
+    w.check(news, dtype, group, window=300)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -311,10 +331,11 @@ def test_values_of_very_different_pages(backend):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("dim,page,news", [(64, 16, [1, 1, 1, 1]), (96, 32, [5, 3, 1, 9]), (128, 64, [40, 21, 3, 2])])
-def test_bool_masks(backend, dtype, dim, page, news):
+@pytest.mark.parametrize("dim,page,news,idle", [(64, 16, [1, 1, 1, 1], 0), (96, 32, [5, 3, 1, 9], 0), (128, 64, [40, 21, 3, 2], 0),
+                                                (64, 32, [77, 21, 70, 2], MANY), (128, 16, [40, 21, 3, 2], MANY)])
+def test_bool_masks(backend, dtype, dim, page, news, idle):
     lengths = [77, 21, 150, 2]
-    w = World(backend, lengths=lengths, heads=2, dim=dim, page=page, seed=dim)
+    w = World(backend, lengths=lengths, heads=2, dim=dim, page=page, seed=dim, idle=idle)
     w.append(lengths, dtype)
     rows = sum(news)
     mask = torch.rand((rows, 4, 150), generator=w.gen) < 0.7
@@ -330,9 +351,10 @@ def test_bool_masks(backend, dtype, dim, page, news):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("mask_dtype", TYPES, ids=str)
-def test_additive_masks(backend, dtype, mask_dtype):
+@pytest.mark.parametrize("idle", [0, MANY])
+def test_additive_masks(backend, dtype, mask_dtype, idle):
     lengths, news = [90, 33, 140], [4, 33, 1]
-    w = World(backend, lengths=lengths, heads=2, dim=64, page=16, seed=14)
+    w = World(backend, lengths=lengths, heads=2, dim=64, page=16, seed=14, idle=idle)
     w.append(lengths, dtype)
     mask = torch.randn((38, 4, 140), generator=w.gen)
     mask[torch.rand(mask.shape, generator=w.gen) < 0.2] = -math.inf
@@ -343,29 +365,33 @@ def test_additive_masks(backend, dtype, mask_dtype):
 
 
 @pytest.mark.parametrize("mask_dtype", [torch.float32, torch.bfloat16], ids=str)
-def test_masks_of_the_lowest_value(backend, mask_dtype):
+@pytest.mark.parametrize("rows,idle", [(2, 0), (50, MANY)])
+def test_masks_of_the_lowest_value(backend, mask_dtype, rows, idle):
     """The type's lowest value swallows the score: where a row has others, the
     token has no weight; where it has none, all its tokens weigh the same."""
-    w = World(backend, lengths=[100, 61], heads=2, dim=64, page=16, seed=15)
+    w = World(backend, lengths=[100, 61], heads=2, dim=64, page=16, seed=15, idle=idle)
     w.append([100, 61], torch.float32)
     low = torch.finfo(mask_dtype).min
-    mask = torch.zeros((4, 1, 100), dtype=mask_dtype)
+    mask = torch.zeros((2 * rows, 1, 100), dtype=mask_dtype)
     mask[0, :, 40:] = low
     mask[1] = low
     mask[2, :, ::2] = low
-    mask[3] = low
-    w.check([2, 2], torch.float32, 2, mask=mask)
+    mask[3::5] = low
+    w.check([rows, rows], torch.float32, 2, mask=mask)
 
 
-def test_hidden_places_may_hold_anything(backend):
+@pytest.mark.parametrize("rows,idle", [(1, 0), (17, MANY)])
+def test_hidden_places_may_hold_anything(backend, rows, idle):
     """NaN, infinities and codes of other sequences past the lengths, in pages
     beside the sequence's and under the mask."""
-    w = World(backend, lengths=[50, 17], heads=2, dim=64, page=16, seed=16, spare=4)
+    w = World(backend, lengths=[50, 17], heads=2, dim=64, page=16, seed=16, spare=4, idle=idle)
     w.append([50, 17], torch.float32)
-    q = torch.randn((2, 4, 64), generator=w.gen)
-    mask = torch.ones((2, 1, 50), dtype=torch.bool)
-    mask[0, :, 16:32] = False
-    want = w.check([1, 1], torch.float32, 4, q=q, mask=mask)
+    heads = 4 if rows == 1 else 8  # enough rows for either kernel
+    news = [rows, rows]
+    q = torch.randn((2 * rows, heads, 64), generator=w.gen)
+    mask = torch.ones((2 * rows, 1, 50), dtype=torch.bool)
+    mask[:rows, :, 16:32] = False
+    want = w.check(news, torch.float32, heads, q=q, mask=mask)
     used = torch.cat([w.table[0, :4], w.table[1, :2]]).long()
     free = torch.ones(w.cache.blocks, dtype=torch.bool)
     free[used] = False
@@ -374,21 +400,22 @@ def test_hidden_places_may_hold_anything(backend):
     w.cache.k_codes[w.table[0, 3].item(), :, 2:] = 255
     w.cache.v_codes[w.table[0, 3].item(), :, 2:] = 0
     w.table[1, 2:] = int(free.nonzero()[0])  # past the end
-    hidden = mask.float().masked_fill(~mask, -math.inf)
-    hidden[1, :, 17:] = math.nan  # past the sequence's end
+    hidden = torch.where(mask, 0.0, -math.inf)
+    hidden[rows:, :, 17:] = math.nan  # past the sequence's end
     for m in (mask, hidden):
-        got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch([1, 1]), mask=m.to(DEV)).cpu().double()
+        got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch(news), mask=m.to(DEV)).cpu().double()
         assert got.isfinite().all()
         assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
 
 
-def test_infinite_masks_are_not_numbers(backend):
-    w = World(backend, lengths=[40], heads=1, dim=64, page=16, seed=17)
+@pytest.mark.parametrize("rows,idle", [(3, 0), (40, 700)])
+def test_infinite_masks_are_not_numbers(backend, rows, idle):
+    w = World(backend, lengths=[40], heads=1, dim=64, page=16, seed=17, idle=idle)
     w.append([40], torch.float32)
-    mask = torch.zeros((3, 1, 40))
-    mask[0, 0, 5], mask[1, 0, 7] = math.inf, math.nan
-    out = w.backend.kv_attention(torch.ones((3, 1, 64), device=DEV), w.cache, w.batch([3]), mask=mask.to(DEV)).cpu()
-    assert out[:2].isnan().all() and out[2].isfinite().all()
+    mask = torch.zeros((rows, 1, 40))
+    mask[0, 0, 0], mask[1, 0, 1] = math.inf, math.nan
+    out = w.backend.kv_attention(torch.ones((rows, 1, 64), device=DEV), w.cache, w.batch([rows]), mask=mask.to(DEV)).cpu()
+    assert out[:2].isnan().all() and out[2:].isfinite().all()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -147,15 +147,34 @@ __device__ __forceinline__ void kv_mask_load(uint32_t (&m)[8], const KvAttnArgs 
   else
     load(static_cast<const uint16_t *>(a.mask));
 }
-// Whether it hides token t; an additive mask's value goes onto the score.
-__device__ __forceinline__ bool kv_mask_hides(const KvAttnArgs &a, uint32_t m, int32_t t, float &x) {
-  if (t >= a.mask_len) return true;
-  if (a.mask_dtype == RNSMX_INT8) return m == 0;
-  const float v = a.mask_dtype == RNSMX_FLOAT32   ? __uint_as_float(m)
-                  : a.mask_dtype == RNSMX_FLOAT16 ? static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m)))
-                                                  : kv_bf16(static_cast<uint16_t>(m));
-  x += v;
-  return v == -INFINITY;
+// Which of eight tokens from t on the mask shows (bit j: token t + j); an additive
+// mask's values go onto the scores.  `end` as kv_mask_load had it.
+__device__ __forceinline__ uint32_t kv_mask_shows(const KvAttnArgs &a, const uint32_t (&m)[8], int32_t t, int32_t end,
+                                                  float (&x)[8]) {
+  uint32_t shown = 0;
+  if (a.mask_dtype == RNSMX_INT8) {
+    kv_for<8>([&](auto J) { shown |= m[J] != 0 ? 1u << J : 0u; });
+  } else {
+    float v[8];
+    if (a.mask_dtype == RNSMX_FLOAT32)
+      kv_for<8>([&](auto J) { v[J] = __uint_as_float(m[J]); });
+    else if (a.mask_dtype == RNSMX_FLOAT16)
+      kv_for<8>([&](auto J) { v[J] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m[J]))); });
+    else
+      kv_for<8>([&](auto J) { v[J] = kv_bf16(static_cast<uint16_t>(m[J])); });
+    kv_for<8>([&](auto J) {
+      x[J] += v[J];
+      shown |= v[J] != -INFINITY ? 1u << J : 0u;
+    });
+  }
+  if (end > a.mask_len) shown &= (1u << min(max(a.mask_len - t, 0), 8)) - 1u;
+  return shown;
+}
+
+// Bits of those of eight tokens from t on that lie in [begin, end).
+__device__ __forceinline__ uint32_t kv_between(int32_t t, int32_t begin, int32_t end) {
+  const uint32_t below = (1u << min(max(end - t, 0), 8)) - 1u, before = (1u << min(max(begin - t, 0), 8)) - 1u;
+  return below & ~before;
 }
 
 // One candidate (x, lv) for a row's reference against another, e and e2 being

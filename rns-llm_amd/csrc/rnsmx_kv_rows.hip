@@ -191,14 +191,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
       // scores of what is not seen are minus infinity; a lane that sees none of
       // its eight tokens does without their page's scales, which may be anything
       const int32_t t8 = t0 + 8 * g;
-      bool any = false;
-      kv_for<8>([&](auto J) {
-        constexpr int j = J;
-        bool see = s.there && t8 + j < end_row && t8 + j >= begin_row;
-        if constexpr (MASK) see = !kv_mask_hides(a, s.m[j], t8 + j, w[j]) && see;
-        w[j] = see ? w[j] : -INFINITY;
-        any |= see;
-      });
+      uint32_t seen = s.there ? kv_between(t8, begin_row, end_row) : 0u;
+      if constexpr (MASK) seen &= kv_mask_shows(a, s.m, t8, t0 + 32, w);
+      kv_for<8>([&](auto J) { w[J] = seen >> J & 1u ? w[J] : -INFINITY; });
+      const bool any = seen != 0;
       c = any ? c : 1.0f;
       lv = any ? lv : 0.0f;
       rv = any ? rv : 0.0f;

@@ -233,14 +233,10 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
         const int32_t t8 = t0 + 16 * g + 8 * h;
         uint32_t m[8];
         if constexpr (MASK) kv_mask_load(m, a, q.row + t_row, q_head, t8, t0 + kStep);
-        bool any = false;
-        kv_for<8>([&](auto J) {
-          constexpr int j = J;
-          bool see = there[g] && t8 + j < end_row && t8 + j >= begin_row;
-          if constexpr (MASK) see = !kv_mask_hides(a, m[j], t8 + j, w[g][j]) && see;
-          w[g][j] = see ? w[g][j] : -INFINITY;
-          any |= see;
-        });
+        uint32_t seen = there[g] ? kv_between(t8, begin_row, end_row) : 0u;
+        if constexpr (MASK) seen &= kv_mask_shows(a, m, t8, t0 + kStep, w[g]);
+        kv_for<8>([&](auto J) { w[g][J] = seen >> J & 1u ? w[g][J] : -INFINITY; });
+        const bool any = seen != 0;
         c[g] = any ? c[g] : 1.0f;
         lv[g] = any ? lv[g] : 0.0f;
         rv[g] = any ? rv[g] : 0.0f;

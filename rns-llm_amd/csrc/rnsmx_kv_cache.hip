@@ -267,7 +267,10 @@ static int32_t kv_batch_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch
   if (batch->max_length > 1 << 30) return fail(RNSMX_EINVAL, "sequences hold at most 2^30 tokens");
   if (batch->max_length > static_cast<int64_t>(batch->table_width) * cache->page)
     return fail(RNSMX_EINVAL, "max_length is past the block table");
+  if (static_cast<int64_t>(batch->seqs) * cache->heads > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many sequences and heads");
   if (batch->seqs > 0 && (!batch->table_dev || !batch->lengths_dev)) return fail(RNSMX_EINVAL, "null batch pointer");
+  if (!aligned(batch->table_dev, 4) || !aligned(batch->lengths_dev, 4) || !aligned(batch->starts_dev, 4))
+    return fail(RNSMX_EINVAL, "batch pointers are not on 4-byte boundaries");
   if (!batch->starts_dev && batch->rows != batch->seqs) return fail(RNSMX_EINVAL, "one row a sequence without row starts");
   a.k = cache->k_dev;
   a.v = cache->v_dev;
@@ -336,8 +339,10 @@ constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWi
 // values a head (16 heads of 128, 1024 masked tokens: 59 us in two, 99 whole; 16
 // heads of 256: 60, 73; 2048 tokens, 32 heads, 512 tiles: 82 in two, 73 whole).
 constexpr int64_t kTileGroups = 256, kTileTokens = 512, kHalvesTasks = 384;
-static int64_t kv_tokens(const KvAttnArgs &a) {  // most that a sequence's rows see
-  return a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 32) : a.b.max_length;
+// Most tokens between a workgroup's first and its last: a window's, the rows of one
+// sequence that it may have, and what its first step starts before them.
+static int64_t kv_tokens(const KvAttnArgs &a) {
+  return a.window > 0 ? std::min<int64_t>(a.b.max_length, static_cast<int64_t>(a.window) + a.b.max_rows + 64) : a.b.max_length;
 }
 static void kv_split(KvAttnArgs &a) {
   const int64_t span = kv_tokens(a);

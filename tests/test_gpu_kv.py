@@ -246,6 +246,19 @@ def test_several_tokens(backend, dtype, group, dim, page, causal, window, idle):
     w.check(news, dtype, 2 * group, **options)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("idle", [0, MANY])
+def test_windows_of_any_place_in_a_step(backend, dim, idle):
+    """A window's first step starts up to 63 tokens before it; its last tokens
+    are seen all the same, in a table that has room for many more."""
+    lengths = [286, 287, 285, 256, 320, 319, 190, 100]
+    news = [100, 100, 99, 100, 100, 100, 100, 100]
+    w = World(backend, lengths=lengths, heads=2, dim=dim, page=16, seed=27, idle=idle)
+    w.append(lengths, torch.float16)
+    for window in (1, 28, 29, 60, 61, 92, 93):
+        w.check(news, torch.float16, 2, window=window)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("heads,dim,page", [(1, 1, 16), (3, 40, 32), (2, 65, 64), (1, 160, 16), (1, 192, 128), (1, 250, 64), (1, 256, 32)])
 def test_prompts_of_any_head(backend, dtype, heads, dim, page):

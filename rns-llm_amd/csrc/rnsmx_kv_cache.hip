@@ -103,9 +103,10 @@ struct KvSpan {
   int32_t page, old, end, row;
 };
 __device__ __forceinline__ KvSpan kv_span(const KvBatchArgs &b, const KvSeq &q, int32_t seq, int32_t index) {
-  const int32_t from = max(q.len - q.n, 0), pg = (from >> b.log_page) + index, start = pg << b.log_page;
+  const int32_t from = max(q.len - q.n, 0), pg = (from >> b.log_page) + index;
   KvSpan r{-1, 0, 0, 0};
-  if (start >= q.len || q.n == 0) return r;
+  if (q.n == 0 || pg > (q.len - 1) >> b.log_page) return r;
+  const int32_t start = pg << b.log_page;
   r.old = max(from - start, 0);
   r.end = min(q.len - start, 1 << b.log_page);
   r.row = q.row + (start + r.old) - (q.len - q.n);
@@ -186,8 +187,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
   const int64_t rs = static_cast<int64_t>(b.heads) * b.dim;
   T *dst[2] = {static_cast<T *>(a.dst[0]) + head * b.dim, static_cast<T *>(a.dst[1]) + head * b.dim};
   if (index == 0 && q.n > q.len)  // rows that have no token
-    for (int32_t i = threadIdx.x; i < (q.n - q.len) * b.dim; i += 256) {
-      const int32_t r = i / b.dim;
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(q.n - q.len) * b.dim; i += 256) {
+      const int64_t r = i / b.dim;
       kv_for<2>([&](auto P) { dst[P][(q.row + r) * rs + (i - r * b.dim)] = static_cast<T>(0); });
     }
   const KvSpan p = kv_span(b, q, seq, index);

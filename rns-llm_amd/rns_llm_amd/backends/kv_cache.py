@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from dataclasses import dataclass, field
 from typing import Sequence
 
@@ -20,6 +21,7 @@ from .. import _native
 
 PAGE_SIZES = (16, 32, 64, 128)
 MAX_LENGTH = 1 << 30
+_MAX_ROWS = 2 ** 31 - 1
 _FLOAT_CODES = {torch.float32: _native.FLOAT32, torch.float16: _native.FLOAT16,
                 torch.bfloat16: _native.BFLOAT16}
 _MASK_CODES = {**_FLOAT_CODES, torch.bool: _native.INT8}
@@ -149,6 +151,8 @@ class KVCacheOps:
         seqs = int(lengths.shape[0])
         if int(table.shape[0]) != seqs:
             raise ValueError(f"block_table has {table.shape[0]} rows for {seqs} sequences")
+        if query_starts is None and (rows is not None or max_query is not None):
+            raise ValueError("rows and max_query go with query_starts")
         if query_lengths is not None:
             if query_starts is not None:
                 raise ValueError("rows are given by query_lengths or by query_starts, not both")
@@ -159,9 +163,7 @@ class KVCacheOps:
             for n in counts:
                 starts.append(starts[-1] + n)
             rows, max_query = starts[-1], max(counts, default=0)
-            if rows > 2 ** 31 - 1:
-                raise ValueError("too many rows")
-            if max_query != 1 or rows != seqs:
+            if rows <= _MAX_ROWS and (max_query != 1 or rows != seqs):
                 query_starts = torch.tensor(starts, dtype=torch.int32, device=device)
         elif query_starts is not None:
             query_starts = _device_ints(query_starts, "query_starts", 1, device)
@@ -171,6 +173,9 @@ class KVCacheOps:
                 raise ValueError(f"query_starts must have {seqs + 1} elements")
         else:
             rows, max_query = seqs, 1
+        if rows > _MAX_ROWS:
+            raise ValueError("too many rows")
+        max_query = min(max_query, rows)
         struct = _native.KVBatchStruct(table.data_ptr(), table.stride(0), lengths.data_ptr(),
                                        None if query_starts is None else query_starts.data_ptr(),
                                        seqs, width, int(rows), int(max_query), top)
@@ -181,8 +186,8 @@ class KVCacheOps:
     def _check_rows(x: torch.Tensor, name: str, batch: KVBatch, heads: int | None, cache: KVCache) -> torch.Tensor:
         if x.dtype not in _FLOAT_CODES:
             raise ValueError(f"{name} must be float32, float16 or bfloat16")
-        if x.device != cache.device:
-            raise ValueError(f"{name} must be on {cache.device}")
+        if x.device != cache.device or batch.lengths.device != cache.device:
+            raise ValueError(f"{name} and the batch must be on {cache.device}")
         shape = x.shape
         if len(shape) != 3 or shape[0] != batch.rows or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [{batch.rows}, {'heads' if heads is None else heads}, {cache.head_dim}], "
@@ -226,6 +231,8 @@ class KVCacheOps:
         if like is None:
             if dtype not in _FLOAT_CODES:
                 raise ValueError("dtype must be float32, float16 or bfloat16")
+            if batch.lengths.device != cache.device:
+                raise ValueError(f"the batch must be on {cache.device}")
             # one value's memory in the outputs' shape: what they are made like costs less than their sizes
             like = torch.empty((1,), dtype=dtype, device=cache.device).expand(batch.rows, cache.kv_heads, cache.head_dim)
             batch._checked[key] = like
@@ -252,8 +259,11 @@ class KVCacheOps:
         hides); tokens from T on are hidden, and T covers the lengths given as
         numbers.  What is hidden contributes nothing whatever it holds, and a row
         that sees no token is zero.  ``workspace``: zero-initialised uint8 of
-        ``kv_attention_workspace_bytes``, by default one kept per stream."""
-        key = (q.dtype, q.shape, q.stride(), q.device, cache._shape, scale, causal, window,
+        ``kv_attention_workspace_bytes``, by default one kept per stream (under
+        graph capture one of the graph's, cleared by each replay)."""
+        scale = None if scale is None else float(scale)
+        window = None if window is None else operator.index(window)
+        key = (q.dtype, q.shape, q.stride(), q.device, cache._shape, scale, bool(causal), window,
                None if mask is None else (mask.dtype, mask.shape, mask.stride(), mask.device))
         checked = batch._checked.get(key)
         if checked is None:
@@ -329,9 +339,14 @@ class KVCacheOps:
 
     def _kv_scratch_for(self, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
         """The stream's scratch, replaced by a larger one where a call needs it
-        (zeroed: its counters are zero between calls).  Captured graphs hold the
-        address of the one they ran with, so the older ones are kept (each less
-        than half the next)."""
+        (zeroed: its counters are zero between calls).  Work in flight may still
+        use the older ones, so they are kept (each less than half the next).
+        Under capture it is the graph's own memory, whose counters are cleared
+        on every replay: a graph may run beside other calls and other graphs."""
+        if torch.cuda.is_current_stream_capturing():
+            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+            scratch[:4 * _native.KV_TICKETS].zero_()
+            return scratch
         index = device.index if device.index is not None else torch.cuda.current_device()
         held = self._kv_scratch.setdefault((index, stream), [])
         if not held or held[-1].numel() < nbytes:

@@ -550,6 +550,32 @@ def test_a_captured_decode_step_advances(backend):
     assert torch.equal(w.cache.k_codes, twin.k_codes) and torch.equal(w.cache.scales, twin.scales)
 
 
+def test_graphs_have_scratch_of_their_own(backend):
+    """Two graphs captured with no call before them, the second replayed first,
+    eager calls on the capturing stream and others between."""
+    w = World(backend, lengths=[3000, 2500], heads=2, dim=64, page=16, seed=28)
+    w.append([3000, 2500], torch.float16)
+    batch = w.batch([1, 1])
+    qs = [torch.randn((2, 4, 64), generator=w.gen).half().to(DEV) for _ in range(2)]
+    assert w.backend.kv_attention_workspace_bytes(w.cache, batch, q_heads=4, dtype=torch.float16) > 0
+    wants = [w.backend.kv_attention(q, w.cache, batch) for q in qs]
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(w.backend.kv_attention(q, w.cache, batch))
+    for which in (1, 0, 1, 1, 0):
+        graphs[which].replay()
+        assert torch.equal(outs[which], wants[which])
+        assert torch.equal(w.backend.kv_attention(qs[which], w.cache, batch), wants[which])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            got = w.backend.kv_attention(qs[1 - which], w.cache, batch)
+        side.synchronize()
+        assert torch.equal(got, wants[1 - which])
+
+
 def test_empty_calls(backend):
     w = World(backend, lengths=[5], heads=2, dim=64, page=16, seed=24)
     none = torch.empty((0, 2, 64), device=DEV)

@@ -75,6 +75,44 @@ def test_batches_that_are_none(table, lengths, options, match):
         backend().kv_batch(cache(), table, lengths, **options)
 
 
+@pytest.mark.parametrize("options,match", [
+    ({"rows": 2}, "go with"), ({"max_query": 1}, "go with"), ({"query_lengths": [1, 1], "rows": 2}, "go with"),
+    ({"query_lengths": [2 ** 30, 2 ** 30]}, "too many rows"),
+    ({"query_starts": torch.zeros(3, dtype=torch.int32), "rows": 2 ** 32, "max_query": 1}, "too many rows"),
+])
+def test_rows_that_a_batch_does_not_take(options, match):
+    with pytest.raises(ValueError, match=match):
+        batch(**options)
+
+
+def test_most_rows_of_a_sequence_are_no_more_than_there_are():
+    starts = torch.zeros(3, dtype=torch.int32)
+    assert batch(query_starts=starts, rows=2, max_query=2 ** 32).max_query == 2
+
+
+def test_batches_of_another_device():
+    c = cache()
+    b = object.__new__(type(batch(c)))
+    for name, value in vars(batch(c)).items():
+        object.__setattr__(b, name, value)
+    object.__setattr__(b, "lengths", torch.empty(2, dtype=torch.int32, device="meta"))
+    for call in (lambda: backend().kv_append(c, b, rows(), rows()), lambda: backend().kv_read(c, b, dtype=torch.float16),
+                 lambda: backend().kv_attention(rows(heads=4), c, b)):
+        with pytest.raises(ValueError, match="batch must be on"):
+            call()
+
+
+def test_scales_and_windows_are_taken_by_value():
+    """Numbers of any kind: a tensor's value, not which tensor it is."""
+    c = cache()
+    with pytest.raises(ValueError, match="scale"):
+        backend().kv_attention(rows(heads=4), c, batch(c), scale=torch.tensor(-1.0))
+    with pytest.raises(ValueError, match="window"):
+        backend().kv_attention(rows(heads=4), c, batch(c), window=torch.tensor(0))
+    with pytest.raises(TypeError):
+        backend().kv_attention(rows(heads=4), c, batch(c), window=1.5)
+
+
 def test_batches_bind_their_rows():
     b = batch()
     assert (b.rows, b.max_query, b.max_length, b.query_starts, b.sequences) == (2, 1, 32, None, 2)

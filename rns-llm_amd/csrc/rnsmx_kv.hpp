@@ -82,6 +82,16 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatchArgs &a, int32_t s) {
   return r;
 }
 
+// STREAM: past the caches, for what one call reads or writes once and is too much
+// for them.
+template <bool STREAM, typename V>
+__device__ __forceinline__ V kv_fetch(const V *p) {
+  if constexpr (STREAM)
+    return __builtin_nontemporal_load(p);
+  else
+    return *p;
+}
+
 // Element access for float32 / float16 / bfloat16 rows (dtype: rnsmx_dtype).
 __device__ __forceinline__ float kv_bf16(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
 __device__ __forceinline__ float kv_load(const void *p, int64_t i, int32_t dtype) {
@@ -113,6 +123,7 @@ struct KvAttnArgs {
   uint32_t *tickets;  // one arrival counter per task
   int64_t q_rs, q_hs, mask_rs, mask_hs, mask_ts;
   int32_t q_heads, dtype, mask_dtype, mask_len;
+  int32_t stream;  // values' codes are read past the caches
   int32_t causal, window, vec, out_vec;  // vec: q rows are read 16 bytes at a time; out_vec: out starts on 16 bytes
   int32_t chunk, splits, waves;  // waves of a workgroup, 4 or 8
   int32_t tile_rows, row_tiles;  // rows of a workgroup (which says the kernel), workgroups over a sequence's rows

@@ -25,18 +25,18 @@ struct KvReadArgs {
 constexpr float kKvMax = 127.0f;
 constexpr int kKvHeld = 4;  // groups of 8 values a thread of kv_append_kernel holds
 
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void kv_load8(float (&x)[8], const T *p, int32_t left, bool vec) {
   if (vec) {
     if constexpr (sizeof(T) == 4) {
-      const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+      const f32x4 a = kv_fetch<STREAM>(reinterpret_cast<const f32x4 *>(p)), b = kv_fetch<STREAM>(reinterpret_cast<const f32x4 *>(p) + 1);
       kv_for<4>([&](auto I) {
         constexpr int i = I;
         x[i] = a[i];
         x[i + 4] = b[i];
       });
     } else {
-      const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
+      const u32x4 a = kv_fetch<STREAM>(reinterpret_cast<const u32x4 *>(p));
       kv_for<8>([&](auto I) {
         constexpr int i = I;
         const uint16_t bits = static_cast<uint16_t>(a[i / 2] >> (16 * (i % 2)));
@@ -115,7 +115,7 @@ __device__ __forceinline__ KvSpan kv_span(const KvBatchArgs &b, const KvSeq &q, 
 }
 
 // One workgroup for the new tokens of one page and head, keys or values.
-template <int DT, typename T>
+template <int DT, typename T, bool STREAM>
 __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
   constexpr int CPT = DT / 8;
   __shared__ uint32_t tops[16];
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
     const int32_t c = threadIdx.x + j * blockDim.x;
     const int32_t t = c / CPT, d = (c - t * CPT) * 8;
     if (c < groups && d < b.dim) {
-      kv_load8<T>(x[j], src + t * rs + d, b.dim - d, a.vec);
+      kv_load8<STREAM>(x[j], src + t * rs + d, b.dim - d, a.vec);
     } else {
       kv_for<8>([&](auto I) { x[j][I] = 0.0f; });
     }
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
 
 // One workgroup for the rows of one page and head, keys and values: two groups of
 // eight of each in flight a thread.
-template <int DT, typename T>
+template <int DT, typename T, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
   constexpr int CPT = DT / 8;
   const KvBatchArgs &b = a.b;
@@ -221,7 +221,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
           });
           T *to = dst[P] + t * rs + d;
           if (a.vec) {
-            kv_for<sizeof(T) / 2>([&](auto I) { reinterpret_cast<u32x4 *>(to)[I] = reinterpret_cast<u32x4 *>(y)[I]; });
+            kv_for<sizeof(T) / 2>([&](auto I) {
+              if constexpr (STREAM)
+                __builtin_nontemporal_store(reinterpret_cast<u32x4 *>(y)[I], reinterpret_cast<u32x4 *>(to) + I);
+              else
+                reinterpret_cast<u32x4 *>(to)[I] = reinterpret_cast<u32x4 *>(y)[I];
+            });
           } else {
             kv_for<8>([&](auto I) {
               if (d + I < b.dim) to[I] = y[I];
@@ -297,6 +302,33 @@ static int32_t kv_batch_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch
 static int64_t pages_touched(const KvBatchArgs &a) {
   const int64_t page = 1 << a.log_page, n = std::min(a.max_rows, a.max_length);
   return n < 1 ? 1 : (n + page - 2) / page + 1;
+}
+
+// Whether a call's bytes go past the caches, where they would only push out what
+// others come back to: from twice the size of the L2s on.  Keys and values of 10454
+// tokens, 32 heads of 128 (171 MB): appended and read 90 us so, 109 through the
+// caches; 16 histories read 190, 196; attention of one row over 131071 tokens, 8
+// heads (268 MB): 56, 61.  Below, the next reader finds less: with an elementwise
+// pass before and after 8192 tokens, 8 heads (34 MB) take 54.8 so, 53.0 through the
+// caches, and attention of one row over 1024 tokens, 32 heads (8 MB), 12.2 and 10.9.
+constexpr int64_t kStreamBytes = 64ll << 20;
+static bool streams(int64_t bytes) { return bytes >= kStreamBytes; }
+
+// f(a value of the type, whether past the caches as a constant)
+template <typename F>
+static void kv_of_type(int32_t dtype, bool stream, F &&f) {
+  auto with = [&](auto t) {
+    if (stream)
+      f(t, std::true_type{});
+    else
+      f(t, std::false_type{});
+  };
+  if (dtype == RNSMX_FLOAT32)
+    with(float{});
+  else if (dtype == RNSMX_FLOAT16)
+    with(_Float16{});
+  else
+    with(uint16_t{});
 }
 
 static int32_t grid_of(int64_t groups, unsigned &grid) {
@@ -472,13 +504,10 @@ int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *b
   const int64_t groups = (tokens * (a.b.row_bytes / 8) + kKvHeld - 1) / kKvHeld;
   const unsigned threads = static_cast<unsigned>(std::max<int64_t>(64, (groups + 63) / 64 * 64));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == RNSMX_FLOAT32) {
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, float>), dim3(grid), dim3(threads), 0, st, a))
-  } else if (dtype == RNSMX_FLOAT16) {
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, _Float16>), dim3(grid), dim3(threads), 0, st, a))
-  } else {
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, uint16_t>), dim3(grid), dim3(threads), 0, st, a))
-  }
+  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim), [&](auto t, auto stream) {
+    using T = decltype(t);
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, T, decltype(stream)::value>), dim3(grid), dim3(threads), 0, st, a))
+  });
   return kv_check("kv_append");
 }
 
@@ -501,13 +530,10 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
   unsigned grid;
   if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads, grid)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == RNSMX_FLOAT32) {
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, float>), dim3(grid), dim3(256), 0, st, a))
-  } else if (dtype == RNSMX_FLOAT16) {
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, _Float16>), dim3(grid), dim3(256), 0, st, a))
-  } else {
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, uint16_t>), dim3(grid), dim3(256), 0, st, a))
-  }
+  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim), [&](auto t, auto stream) {
+    using T = decltype(t);
+    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, T, decltype(stream)::value>), dim3(grid), dim3(256), 0, st, a))
+  });
   return kv_check("kv_read");
 }
 
@@ -547,6 +573,8 @@ int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t
     a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace_dev) + RNSMX_KV_TICKETS * 4);
   }
   a.out = out_dev;
+  // each code is read by one workgroup alone
+  a.stream = a.row_tiles == 1 && streams(2ll * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a));
   unsigned grid;
   if (int32_t rc = grid_of(kv_tasks(a) * a.splits, grid)) return rc;
   if (grid == 0) return RNSMX_OK;

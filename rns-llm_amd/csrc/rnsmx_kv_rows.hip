@@ -22,7 +22,10 @@ __device__ __forceinline__ f32x4 kv_mfma(h16x8 a, h16x8 b, f32x4 c) {
 // added to them: with lv = log2(value scale),
 //   w = 2^(x - mx + lv - ml),  O += w code,  l += w / value scale = 2^(x - mx - ml)
 // where x is the product in powers of two and (mx, ml) a row's reference.
-template <int DT, int NW, bool SPLIT, bool MASK>
+// STREAM: the values' codes are read past the caches; the keys' are not, as a load
+// takes half a line of 128, which has to stay for the other half (62 sequences of
+// up to 4096 tokens, 32 heads: 212 us through the caches, 200 so, 219 with the keys).
+template <int DT, int NW, bool SPLIT, bool MASK, bool STREAM>
 __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows_kernel(const KvAttnArgs a) {
   constexpr int C64 = DT / 64, C32 = DT / 32 % 2;  // 64-value chunks of a row, and whether 32 are left
   constexpr int KS = DT / 32;                      // products' steps
@@ -94,19 +97,19 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
       constexpr int j = J;
       const uint8_t *p = vp + j * DT;
       if constexpr (W16 != 0) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(p + 16 * col);
+        const u32x4 w = kv_fetch<STREAM>(reinterpret_cast<const u32x4 *>(p + 16 * col));
         kv_for<4>([&](auto W) { s.v[j][W] = w[static_cast<int>(W)]; });
       }
       if constexpr (W8 != 0) {
-        const u32x2 w = *reinterpret_cast<const u32x2 *>(p + 256 * W16 + 8 * col);
+        const u32x2 w = kv_fetch<STREAM>(reinterpret_cast<const u32x2 *>(p + 256 * W16 + 8 * col));
         s.v[j][4 * W16] = w[0];
         s.v[j][4 * W16 + 1] = w[1];
       }
       if constexpr (W4 != 0)
-        s.v[j][4 * W16 + 2 * W8] = *reinterpret_cast<const uint32_t *>(p + 256 * W16 + 128 * W8 + 4 * col);
+        s.v[j][4 * W16 + 2 * W8] = kv_fetch<STREAM>(reinterpret_cast<const uint32_t *>(p + 256 * W16 + 128 * W8 + 4 * col));
       if constexpr (W2 != 0)
         s.v[j][4 * W16 + 2 * W8 + W4] =
-            *reinterpret_cast<const uint16_t *>(p + 256 * W16 + 128 * W8 + 64 * W4 + 2 * col);
+            kv_fetch<STREAM>(reinterpret_cast<const uint16_t *>(p + 256 * W16 + 128 * W8 + 64 * W4 + 2 * col));
     });
     const F32x2 sc = *reinterpret_cast<const F32x2 *>(b.scales + slot_v * 2);
     s.ks = sc.x;
@@ -371,17 +374,19 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
 template <int DT, int NW>
 static void launch_waves(const KvAttnArgs &a, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles * a.splits)), block(64 * NW);
-  const bool split = a.dtype == RNSMX_FLOAT32;
-  if (a.mask) {
-    if (split)
-      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, true, true>), grid, block, 0, st, a);
+  auto launch = [&](auto split) {
+    constexpr bool S = decltype(split)::value;
+    if (a.mask)
+      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, true, false>), grid, block, 0, st, a);
+    else if (a.stream)
+      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, false, true>), grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, false, true>), grid, block, 0, st, a);
-  } else if (split) {
-    hipLaunchKernelGGL((kv_rows_kernel<DT, NW, true, false>), grid, block, 0, st, a);
-  } else {
-    hipLaunchKernelGGL((kv_rows_kernel<DT, NW, false, false>), grid, block, 0, st, a);
-  }
+      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, false, false>), grid, block, 0, st, a);
+  };
+  if (a.dtype == RNSMX_FLOAT32)
+    launch(std::true_type{});
+  else
+    launch(std::false_type{});
 }
 
 template <int DT>

@@ -136,6 +136,9 @@ constexpr int kKvRows = 16;          // query rows of a workgroup of kv_rows_ker
 // Whether it is built with eight waves: row sizes whose waves are two to a SIMD.
 constexpr bool kv_wide(int row_bytes) { return row_bytes <= 160; }
 
+// Whether its values' codes are loaded in pieces of 64 bytes and more.
+constexpr bool kv_whole(int row_bytes) { return row_bytes % 64 == 0; }
+
 // Floats of one split's partial result.  Of kv_rows_kernel: rows of row_bytes
 // values, then each row's reference and sum; of kv_tiles_kernel: what the 256
 // lanes hold, row_bytes / 2 values, a reference of two and a sum each.

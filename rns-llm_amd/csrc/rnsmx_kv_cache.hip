@@ -29,7 +29,7 @@ template <bool STREAM, typename T>
 __device__ __forceinline__ void kv_load8(float (&x)[8], const T *p, int32_t left, bool vec) {
   if (vec) {
     if constexpr (sizeof(T) == 4) {
-      const f32x4 a = kv_fetch<STREAM>(reinterpret_cast<const f32x4 *>(p)), b = kv_fetch<STREAM>(reinterpret_cast<const f32x4 *>(p) + 1);
+      const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
       kv_for<4>([&](auto I) {
         constexpr int i = I;
         x[i] = a[i];
@@ -304,15 +304,18 @@ static int64_t pages_touched(const KvBatchArgs &a) {
   return n < 1 ? 1 : (n + page - 2) / page + 1;
 }
 
-// Whether a call's bytes go past the caches, where they would only push out what
-// others come back to: from twice the size of the L2s on.  Keys and values of 10454
-// tokens, 32 heads of 128 (171 MB): appended and read 90 us so, 109 through the
-// caches; 16 histories read 190, 196; attention of one row over 131071 tokens, 8
-// heads (268 MB): 56, 61.  Below, the next reader finds less: with an elementwise
-// pass before and after 8192 tokens, 8 heads (34 MB) take 54.8 so, 53.0 through the
-// caches, and attention of one row over 1024 tokens, 32 heads (8 MB), 12.2 and 10.9.
-constexpr int64_t kStreamBytes = 64ll << 20;
-static bool streams(int64_t bytes) { return bytes >= kStreamBytes; }
+// Whether a call's bytes go past the caches: where the 256 MB behind the L2s would
+// not keep them for the next reader, and a load or store takes its lines whole.  Keys
+// and values of 20736 tokens, 32 heads of 128 (340 MB) in bfloat16: appended 95 us so,
+// 105 through the caches, read 81 and 105; of 10368 tokens (170 MB) appended and read
+// after each other 92 and 101, of 7296 tokens (120 MB) 73 both.  Float32 goes through
+// them (a load takes half of its lines: 14592 tokens, 8 heads of 128, appended 36, 27
+// through them, read 59, 29), and so do rows of other sizes (46848 tokens, 8 heads of
+// 80: 53, 50 and 64, 35; rows of 192 bytes appended 114, 109, but read 81, 134).
+// Attention (codes of 134 MB, 16 sequences of 4096 tokens, 8 heads of 128): 36 so, 40
+// through the caches; rows of 64: 27, 30; of 160: 117, 107 (48 sequences).
+constexpr int64_t kStreamBytes = 128ll << 20;
+static bool streams(int64_t bytes, bool whole) { return whole && bytes >= kStreamBytes; }
 
 // f(a value of the type, whether past the caches as a constant)
 template <typename F>
@@ -324,7 +327,7 @@ static void kv_of_type(int32_t dtype, bool stream, F &&f) {
       f(t, std::false_type{});
   };
   if (dtype == RNSMX_FLOAT32)
-    with(float{});
+    f(float{}, std::false_type{});
   else if (dtype == RNSMX_FLOAT16)
     with(_Float16{});
   else
@@ -504,7 +507,9 @@ int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *b
   const int64_t groups = (tokens * (a.b.row_bytes / 8) + kKvHeld - 1) / kKvHeld;
   const unsigned threads = static_cast<unsigned>(std::max<int64_t>(64, (groups + 63) / 64 * 64));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim), [&](auto t, auto stream) {
+  const bool whole = size == 2 && a.vec && a.b.dim % 64 == 0 && aligned(k_dev, 128) && aligned(v_dev, 128) &&
+                     k_row_stride % 64 == 0 && v_row_stride % 64 == 0 && k_head_stride % 64 == 0 && v_head_stride % 64 == 0;
+  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim, whole), [&](auto t, auto stream) {
     using T = decltype(t);
     RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, T, decltype(stream)::value>), dim3(grid), dim3(threads), 0, st, a))
   });
@@ -530,7 +535,8 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
   unsigned grid;
   if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads, grid)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim), [&](auto t, auto stream) {
+  const bool whole = size == 2 && a.vec && a.b.dim % 32 == 0 && aligned(k_dev, 64) && aligned(v_dev, 64);
+  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim, whole), [&](auto t, auto stream) {
     using T = decltype(t);
     RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, T, decltype(stream)::value>), dim3(grid), dim3(256), 0, st, a))
   });
@@ -574,7 +580,8 @@ int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t
   }
   a.out = out_dev;
   // each code is read by one workgroup alone
-  a.stream = a.row_tiles == 1 && streams(2ll * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a));
+  a.stream = !a.mask && a.row_tiles == 1 &&
+             streams(2ll * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a), kv_whole(a.b.row_bytes));
   unsigned grid;
   if (int32_t rc = grid_of(kv_tasks(a) * a.splits, grid)) return rc;
   if (grid == 0) return RNSMX_OK;

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
         s.v[j][4 * W16 + 2 * W8] = kv_fetch<STREAM>(reinterpret_cast<const uint32_t *>(p + 256 * W16 + 128 * W8 + 4 * col));
       if constexpr (W2 != 0)
         s.v[j][4 * W16 + 2 * W8 + W4] =
-            kv_fetch<STREAM>(reinterpret_cast<const uint16_t *>(p + 256 * W16 + 128 * W8 + 64 * W4 + 2 * col));
+            *reinterpret_cast<const uint16_t *>(p + 256 * W16 + 128 * W8 + 64 * W4 + 2 * col);
     });
     const F32x2 sc = *reinterpret_cast<const F32x2 *>(b.scales + slot_v * 2);
     s.ks = sc.x;
@@ -379,7 +379,7 @@ static void launch_waves(const KvAttnArgs &a, hipStream_t st) {
     if (a.mask)
       hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, true, false>), grid, block, 0, st, a);
     else if (a.stream)
-      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, false, true>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, false, kv_whole(DT)>), grid, block, 0, st, a);
     else
       hipLaunchKernelGGL((kv_rows_kernel<DT, NW, S, false, false>), grid, block, 0, st, a);
   };

@@ -495,11 +495,13 @@ def test_cache_past_four_gigabytes(backend):
     assert ((out - want).abs() <= bound(torch.float16, want, spread, reach, dim, 300, None)).all()
 
 
-@pytest.mark.parametrize("dtype,lengths", [(torch.float32, [300, 213]), (torch.bfloat16, [601, 423])], ids=str)
-def test_rows_past_the_caches(backend, dtype, lengths):
-    """Keys and values of 64 MB and more."""
-    w = World(backend, lengths=lengths, heads=64, dim=256, page=32, seed=29)
-    k, v = w.append(lengths, dtype)
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 128), (torch.float16, 128), (torch.bfloat16, 256), (torch.bfloat16, 96)], ids=str)
+def test_rows_past_the_caches(backend, dtype, dim):
+    """Keys and values of 128 MB and more."""
+    rows = 2 ** 27 // (2 * dtype.itemsize * 64 * dim) + 1
+    lengths = [rows - 213, 213]
+    w = World(backend, lengths=lengths, heads=64, dim=dim, page=32, seed=29)
+    w.append(lengths, dtype)
     w.same()
     got = backend.kv_read(w.cache, w.batch(lengths), dtype=dtype)
     at = 0
@@ -512,11 +514,11 @@ def test_rows_past_the_caches(backend, dtype, lengths):
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("group,dim", [(1, 40), (8, 64), (2, 96), (1, 128), (4, 160), (2, 256)])
 def test_attention_past_the_caches(backend, dtype, group, dim):
-    """Tables with room for 64 MB of codes and more; what is in them is short."""
+    """Tables with room for 128 MB of codes and more; what is in them is short."""
     lengths = [300, 1, 0, 33, 1100, 70, 129, 64]
     w = World(backend, lengths=lengths, heads=2, dim=dim, page=16, seed=dim + 30)
     w.append(lengths, dtype)
-    w.table = torch.cat((w.table, torch.full((len(lengths), 4096), -1, dtype=torch.int32)), dim=1)
+    w.table = torch.cat((w.table, torch.full((len(lengths), 8192), -1, dtype=torch.int32)), dim=1)
     w.check([1] * len(lengths), dtype, 2 * group)
 
 

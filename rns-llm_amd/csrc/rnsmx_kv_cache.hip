@@ -67,7 +67,8 @@ __device__ __forceinline__ void kv_load8(float (&x)[8], const T *p, int32_t left
 // theorem); where the remainder underflows x / s is far below a half.  Adding 1.5
 // 2^23 leaves the integer in the low byte, rounded to even.  |x| <= 127.01 s, as s
 // comes from the largest: no code needs a clamp.  A quarter of what divisions and
-// conversions cost, which bound prompts (10454 tokens, 32 heads of 128: 87 us).
+// conversions cost, which bounded prompts (10454 tokens, 32 heads of 128: 87 us with
+// them, 66 so).
 // At a scale that is not finite every code is zero.
 __device__ __forceinline__ u32x2 kv_codes(const float (&x)[8], float s) {
   if (!(s < INFINITY)) return u32x2{0x80808080u, 0x80808080u};
@@ -114,7 +115,14 @@ __device__ __forceinline__ KvSpan kv_span(const KvBatchArgs &b, const KvSeq &q, 
   return r;
 }
 
-// One workgroup for the new tokens of one page and head, keys or values.
+// One workgroup for the new tokens of one page and head, keys or values: a page's
+// scale is one maximum over them, so they are read once and wait for it in registers,
+// up to four groups of eight a thread (two: 1 % slower), and only a page that held
+// tokens before and whose scale grows is read and written again.  Bound by memory:
+// two or four bytes read and one written a value, 10454 tokens, 32 heads of 128 in
+// bfloat16 (257 MB) in 49 us, 5.2 TB/s, waves waiting for loads 69 % of their time; a
+// single token of 12 heads takes 3.2 us, which is the launch and three loads in turn
+// (length, page, values).
 template <int DT, typename T, bool STREAM>
 __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
   constexpr int CPT = DT / 8;
@@ -176,7 +184,9 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
 }
 
 // One workgroup for the rows of one page and head, keys and values: two groups of
-// eight of each in flight a thread.
+// eight of each in flight a thread, as a page of 64 tokens of 128 values gives 256
+// threads four.  Bound by memory: 16 sequences of up to 4095 tokens, 32 heads of 128 to
+// bfloat16 (979 MB) in 190 us, 5.2 TB/s, a copy's rate; 257 tokens of 12 heads 3.1 us.
 template <int DT, typename T, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
   constexpr int CPT = DT / 8;
@@ -359,21 +369,21 @@ static int32_t grid_of(int64_t groups, unsigned &grid) {
 
 // How a call's tokens are split over waves and workgroups (device time, 32-wide
 // pages and up).  Eight waves take a step of 256 tokens where the workgroups
-// leave room for them on the chip (24 x 8 heads of 80, window 1023: 13.6 us, 15.3
-// with four) or sequences are long (62 x 32 heads of 128, up to 4096 tokens: 222,
-// 230); many short ones take four (256 x 12 heads of 64, 512 tokens: 34.7, 44.2
+// leave room for them on the chip (24 x 8 heads of 80, window 1023: 13.5 us, 15.3
+// with four) or sequences are long (62 x 32 heads of 128, up to 4096 tokens: 200,
+// 204); many short ones take four (256 x 12 heads of 64, 512 tokens: 29.3, 39.7
 // with eight).  Splitting costs the parts' way through memory and the ticket's,
-// some 5 us: not past a workgroup a CU (one token against 131071, 8 heads: 61 us,
-// 69 with twice as many), and not below 1024 tokens each (32 heads, 1024 tokens:
-// 12.0 whole, 13.7 in two).
+// some 5 us: not past a workgroup a CU (one token against 131071, 8 heads: 58 us,
+// 65 with twice as many), and not below 1024 tokens each (32 heads, 1024 tokens:
+// 11.0 whole, 14.2 in two).
 constexpr int64_t kSplitGroups = 256, kSplitTokens = 1024, kWideTasks = 512, kWideTokens = 4096;
 // Prompts: eight waves where the tiles leave room for them (72 pairs of parts of
-// prompts, 288 tiles: 47 us, 60 with four) or are few and long (8192 tokens, 8
-// heads, 512 tiles: 197, 220), four where two workgroups to a CU hide each other's
-// waits (8192 tokens, 32 heads: 654, 726 with eight; 2048 tokens, 32 heads: 73,
-// 77).  Tokens are split only up to a workgroup a CU: a part is 64 KB at 128
-// values a head (16 heads of 128, 1024 masked tokens: 59 us in two, 99 whole; 16
-// heads of 256: 60, 73; 2048 tokens, 32 heads, 512 tiles: 82 in two, 73 whole).
+// prompts, 288 tiles: 44 us, 56 with four) or are few and long (8192 tokens, 8
+// heads, 512 tiles: 195, 212), four where two workgroups to a CU hide each other's
+// waits (8192 tokens, 32 heads: 654, 726 with eight; 2048 tokens, 32 heads: 69,
+// 75).  Tokens are split only up to a workgroup a CU: a part is 64 KB at 128
+// values a head (16 heads of 256, 1024 tokens, 128 tiles: 57 us in two, 72 whole;
+// 2048 tokens, 32 heads, 512 tiles: 72 in two, 69 whole).
 constexpr int64_t kTileGroups = 256, kTileTokens = 512, kHalvesTasks = 384;
 // Most tokens between a workgroup's first and its last: a window's, the rows of one
 // sequence that it may have, and what its first step starts before them.

@@ -35,6 +35,13 @@ __device__ __forceinline__ int32_t value_swap(int32_t d) { return (d & 7) ^ (d >
 // in one page.  The products and the weights are as kv_rows_kernel's, with
 // 32 x 32 products: a row is one lane pair's.
 //
+// Bound by what surrounds the products (weights, conversions, waits) more than by
+// them: at 8192 tokens, 32 heads of 128 (550 GFLOP) 654 us, 0.84 PFLOP/s of the 1.23
+// that a large library product reaches here, vector units busy half of the time, matrix
+// units and shared memory a third each.  2048 tokens, 32 heads (34 GFLOP) take 62 to 69
+// us: 512 tiles go in one round, so the longest chain decides, 32 steps of some 4200
+// cycles; waves wait 30 % of their time and are issue-blocked 25 %.
+//
 // HALVES 2: eight waves, the second four with the same rows and every other
 // step, staged apart; they join in the shared memory at the end.  A step's chain
 // (load, products, weights, products, conversions: some 4000 cycles, twice that

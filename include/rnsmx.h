@@ -497,7 +497,8 @@ typedef struct rnsmx_kv_cache {
  * with fewer tokens than rows: the empty slot of a batch of fixed size) has no
  * token.  A page number outside [0, blocks) is a page that is not there: not
  * written, read as zeros, not attended to.  Lengths past max_length and rows
- * past max_rows or `rows` are cut off; nothing out of range is accessed.
+ * past max_rows or `rows` are cut off; nothing out of range is accessed.  Rows
+ * that are no sequence's are neither read nor written.
  */
 typedef struct rnsmx_kv_batch {
   const int32_t *table_dev;

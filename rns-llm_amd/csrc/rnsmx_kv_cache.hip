@@ -459,10 +459,9 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   a.window = query->window;
   a.scale = query->scale;
   const int64_t rows = static_cast<int64_t>(a.b.max_rows) * (query->q_heads / cache->heads);
+  if (rows > 0x7FFFFFFF - kKvTileRows) return fail(RNSMX_EINVAL, "too many rows");  // of 32 bits in the kernels
   a.tile_rows = few_rows(a.b, rows, kv_tokens(a)) ? kKvRows : kKvTileRows;
-  const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows;
-  if (tiles > 0x7FFFFFFF) return fail(RNSMX_EINVAL, "too many rows");
-  a.row_tiles = static_cast<int32_t>(tiles);
+  a.row_tiles = static_cast<int32_t>((rows + a.tile_rows - 1) / a.tile_rows);
   kv_split(a);
   a.by_group = kv_div(query->q_heads / cache->heads);
   a.by_splits = kv_div(a.splits);

@@ -65,7 +65,8 @@ class KVBatch:
     The tensors are read by the device on each call and may be written in
     between, as a decode loop (or a captured graph) does that advances
     ``lengths``; ``rows``, ``max_query`` and ``max_length`` bound what they may
-    hold, and what goes past them is cut off."""
+    hold, and what goes past them is cut off.  Rows that ``query_starts`` gives to
+    no sequence are not written in a call's outputs."""
 
     block_table: torch.Tensor
     lengths: torch.Tensor

@@ -189,6 +189,7 @@ WITH_ROWS = {"seqs": 1, "rows": 1}  # past the call of zero sequences; refused b
     {"batch_changes": {"rows": -1}}, {"batch_changes": {"table_width": 0}}, {"batch_changes": {"max_length": 33}},
     {"batch_changes": {"seqs": 65536}, "cache_changes": {"heads": 65536}, "query_changes": {"q_heads": 65536}},
     {"batch_changes": {"seqs": 2 ** 31 - 1}, "cache_changes": {"heads": 2 ** 30}, "query_changes": {"q_heads": 2 ** 30}},
+    {"batch_changes": {"rows": 2 ** 30, "max_rows": 2 ** 30}, "query_changes": {"q_heads": 8}},
     {"batch_changes": {"lengths_dev": 4098}}, {"batch_changes": {"table_dev": 4097}}, {"batch_changes": {"starts_dev": 4099}},
     {"batch_changes": {"seqs": 2, "lengths_dev": None}}, {"batch_changes": {"seqs": 2, "starts_dev": None, "rows": 3}},
     {"query_changes": {"dtype": _native.INT8}}, {"query_changes": {"q_heads": 3}}, {"query_changes": {"q_heads": 0}},

@@ -149,11 +149,12 @@ constexpr int64_t kv_tile_floats(int row_bytes) { return 256 * (static_cast<int6
 // split of the tokens; task numbers pairs' tiles.  Neighbours are different
 // pairs, so that each of the 8 XCDs, which workgroups go to in turn, gets as many
 // long and short parts as the others (72 pairs of sequences of 400 to 2500
-// tokens: 60 us with the pairs one after the other in eighths, 52 so), and where
-// the pairs divide by 8 each is one XCD's, whose L2 its tiles share.  Tiles run
-// from the longest down; with two workgroups to a CU (turn) every other 32 (an
-// XCD's CUs) are reversed, so that a long one shares its CU with a short one
-// (2048 tokens, 32 heads: 91 us without, 79 with).
+// tokens: 78 us with the pairs one after the other in eighths, 44 so; a prompt of
+// 2048, 32 heads: 84, 69), and where the pairs divide by 8 each is one XCD's, whose
+// L2 its tiles share.  Tiles run from the longest down; with two workgroups to a CU
+// (turn) every other 32 (an XCD's CUs) are reversed, so that a long one shares its
+// CU with a short one (two prompts of 1024, 32 heads on 8: 39.7 us without, 38.0
+// with).
 struct KvPlace {
   int32_t seq, head, tile, split, task;
 };

@@ -289,8 +289,10 @@ class KVCacheOps:
         elif need > 0:
             scratch = self._kv_scratch_for(need, cache.device, stream)
             space, size = scratch.data_ptr(), scratch.numel()
-        rc = self._lib.rnsmx_kv_attention(cache._ref, batch._ref, ref, q.data_ptr(),
-                                          None if mask is None else mask.data_ptr(), space, size, out.data_ptr(), stream)
+        # a mask without columns has no address, and hides everything all the same
+        hides = None if mask is None else mask.data_ptr() or cache.scales.data_ptr()
+        rc = self._lib.rnsmx_kv_attention(cache._ref, batch._ref, ref, q.data_ptr(), hides, space, size, out.data_ptr(),
+                                          stream)
         if rc:
             _native.check(rc)
         self._stats["kv_attention_calls"] += 1

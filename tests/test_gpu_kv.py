@@ -377,6 +377,29 @@ def test_additive_masks(backend, dtype, mask_dtype, idle):
     assert (got[3::7] == 0).all()
 
 
+@pytest.mark.parametrize("kind", [torch.bool, torch.float32, torch.float16])
+@pytest.mark.parametrize("rows,idle", [(1, 0), (60, MANY)])
+@pytest.mark.parametrize("columns", [0, 1, 37, 64, 130, 199])
+def test_masks_that_end_before_the_tokens(backend, kind, rows, idle, columns):
+    """With lengths on the device a mask may be shorter: what is past it is
+    hidden, to the bit as by a mask that says so."""
+    w = World(backend, lengths=[200, 150], heads=2, dim=72, page=16, seed=31, idle=idle)
+    w.append([200, 150], torch.float16)
+    news = [rows, rows] + [0] * idle
+    starts = torch.tensor([0] + news, dtype=torch.int32).cumsum(0).to(dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([200, 150] + [0] * idle, dtype=torch.int32, device=DEV)
+    batch = backend.kv_batch(w.cache, w.table.to(DEV), lengths, query_starts=starts, rows=2 * rows, max_query=rows)
+    q = torch.randn((2 * rows, 4, 72), generator=w.gen).half().to(DEV)
+    whole = torch.rand((2 * rows, 1, 208), generator=w.gen) < 0.7
+    whole[:, :, columns:] = False
+    if kind != torch.bool:
+        whole = torch.where(whole, torch.randn(whole.shape, generator=w.gen), torch.tensor(-torch.inf)).to(kind)
+    got = backend.kv_attention(q, w.cache, batch, mask=whole[:, :, :columns].contiguous().to(DEV))
+    assert torch.equal(got, backend.kv_attention(q, w.cache, batch, mask=whole.to(DEV)))
+    if columns == 0:
+        assert (got == 0).all()
+
+
 @pytest.mark.parametrize("mask_dtype", [torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("rows,idle", [(2, 0), (50, MANY)])
 def test_masks_of_the_lowest_value(backend, mask_dtype, rows, idle):

@@ -195,6 +195,12 @@ class KVCacheOps:
                              f"got {tuple(shape)}")
         return x if x.stride(2) == 1 or shape[2] == 1 else x.contiguous()
 
+    @staticmethod
+    def _check_gpu(cache: KVCache) -> None:
+        """A cache may be made and bound on the host, but a kernel reads none there."""
+        if cache.device.type != "cuda":
+            raise ValueError(f"the cache must be on the GPU, it is on {cache.device}")
+
     def kv_append(self, cache: KVCache, batch: KVBatch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Quantises the batch's rows, ``k`` and ``v`` ``[rows, kv_heads,
         head_dim]`` of any strides, into the cache, in one launch.
@@ -215,6 +221,7 @@ class KVCacheOps:
                 raise ValueError("k and v must have one dtype")
             if plain_k is not k or plain_v is not v:
                 return self.kv_append(cache, batch, plain_k, plain_v)
+            self._check_gpu(cache)
             args = (_FLOAT_CODES[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
             batch._checked[key] = args
         rc = self._lib.rnsmx_kv_append(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), *args,
@@ -234,6 +241,7 @@ class KVCacheOps:
                 raise ValueError("dtype must be float32, float16 or bfloat16")
             if batch.lengths.device != cache.device:
                 raise ValueError(f"the batch must be on {cache.device}")
+            self._check_gpu(cache)
             # one value's memory in the outputs' shape: what they are made like costs less than their sizes
             like = torch.empty((1,), dtype=dtype, device=cache.device).expand(batch.rows, cache.kv_heads, cache.head_dim)
             batch._checked[key] = like
@@ -262,6 +270,8 @@ class KVCacheOps:
         that sees no token is zero.  ``workspace``: zero-initialised uint8 of
         ``kv_attention_workspace_bytes``, by default one kept per stream (under
         graph capture one of the graph's, cleared by each replay)."""
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()):
+            raise ValueError("out must be contiguous and like q")
         scale = None if scale is None else float(scale)
         window = None if window is None else operator.index(window)
         key = (q.dtype, q.shape, q.stride(), q.device, cache._shape, scale, bool(causal), window,
@@ -273,13 +283,12 @@ class KVCacheOps:
                 return self.kv_attention(plain, cache, batch, scale=scale, causal=causal, window=window, mask=mask,
                                          out=out, workspace=workspace)
             query = self._query_of(q, cache, batch, scale, causal, window, mask)
+            self._check_gpu(cache)
             need = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ctypes.addressof(query)))
             checked = batch._checked[key] = (query, ctypes.addressof(query), need)
         _, ref, need = checked
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-            raise ValueError("out must be contiguous and like q")
         stream = self._stream_of(cache.device)
         space, size = None, 0
         if workspace is not None:

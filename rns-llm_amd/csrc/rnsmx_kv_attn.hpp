@@ -171,6 +171,12 @@ __device__ __forceinline__ uint32_t kv_mask_shows(const KvAttnArgs &a, const uin
   return shown;
 }
 
+// The first token that a row at position p sees.  A row before its sequence's
+// first token lies below zero, where p + 1 - window would pass 32 bits.
+__device__ __forceinline__ int32_t kv_window_begin(const KvAttnArgs &a, int32_t p) {
+  return a.window > 0 ? max(p + 1, a.window) - a.window : 0;
+}
+
 // Bits of those of eight tokens from t on that lie in [begin, end).
 __device__ __forceinline__ uint32_t kv_between(int32_t t, int32_t begin, int32_t end) {
   const uint32_t below = (1u << min(max(end - t, 0), 8)) - 1u, before = (1u << min(max(begin - t, 0), 8)) - 1u;

@@ -59,9 +59,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
   const int32_t base = q.len - q.n;  // position of the sequence's first row
   const int32_t t_first = token_of(row0), t_last = token_of(min(row0 + ROWS, rows) - 1);
   const int32_t hi = max(a.causal ? base + t_last + 1 : q.len, 0);
-  const int32_t lo = a.window > 0 ? max(base + t_first + 1 - a.window, 0) & ~31 : 0;
+  const int32_t lo = kv_window_begin(a, base + t_first) & ~31;
   const int32_t full_hi = a.causal ? base + t_first + 1 : q.len;                    // seen by every row: below it
-  const int32_t full_lo = a.window > 0 ? max(base + t_last + 1 - a.window, 0) : 0;  // and from it on
+  const int32_t full_lo = kv_window_begin(a, base + t_last);              // and from it on
   const int32_t c0 = lo + split * a.chunk;
   if (split > 0 && c0 >= hi) return;
   const int32_t c1 = min(hi, c0 + a.chunk);
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
   // this lane's row: its place and what it sees
   const int32_t row = min(row0 + col, rows - 1), t_row = token_of(row), q_head = head * group + (row - t_row * group);
   const int32_t end_row = a.causal ? base + t_row + 1 : q.len;
-  const int32_t begin_row = a.window > 0 ? max(base + t_row + 1 - a.window, 0) : 0;
+  const int32_t begin_row = kv_window_begin(a, base + t_row);
 
   struct Step {
     u32x4 k[2][C64];

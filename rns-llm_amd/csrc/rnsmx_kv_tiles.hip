@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
   // what the workgroup's rows see, and this wave's
   const int32_t last_row = min(row0 + kKvTileRows, rows) - 1;
   const int32_t hi = max(a.causal ? base + kv_of(last_row) + 1 : q.len, 0);
-  const int32_t lo = a.window > 0 ? max(base + kv_of(row0) + 1 - a.window, 0) & ~(kStep - 1) : 0;
+  const int32_t lo = kv_window_begin(a, base + kv_of(row0)) & ~(kStep - 1);
   const int32_t c0 = lo + split * a.chunk;
   if (split > 0 && c0 >= hi) return;
   const int32_t c1 = min(hi, c0 + a.chunk);
@@ -86,12 +86,12 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
   const bool w_any = w_first < rows;
   const int32_t t_first = kv_of(w_first), t_last = kv_of(w_last);
   const int32_t full_hi = min(a.causal ? base + t_first + 1 : q.len, c1);
-  const int32_t full_lo = a.window > 0 ? max(base + t_last + 1 - a.window, 0) : 0;
+  const int32_t full_lo = kv_window_begin(a, base + t_last);
 
   const int32_t row = min(w_first + col, rows - 1);
   const int32_t t_row = kv_of(row), q_head = head * group + (row - t_row * group);
   const int32_t end_row = min(a.causal ? base + t_row + 1 : q.len, c1);
-  const int32_t begin_row = a.window > 0 ? max(base + t_row + 1 - a.window, 0) : 0;
+  const int32_t begin_row = kv_window_begin(a, base + t_row);
 
   // loads of a step: this wave's 16 tokens
   u32x2 kr[KR];

@@ -496,9 +496,14 @@ typedef struct rnsmx_kv_cache {
  * row s alone), are its last tokens; a row before its first token (a sequence
  * with fewer tokens than rows: the empty slot of a batch of fixed size) has no
  * token.  A page number outside [0, blocks) is a page that is not there: not
- * written, read as zeros, not attended to.  Lengths past max_length and rows
- * past max_rows or `rows` are cut off; nothing out of range is accessed.  Rows
- * that are no sequence's are neither read nor written.
+ * written, read as zeros, not attended to.
+ *
+ * What the device holds past max_length and max_rows is dropped, and nothing else
+ * moves: tokens from max_length on are not there, as those of a page that is not;
+ * of a sequence's rows the first max_rows count, at the positions that all of them
+ * give, and the others are not appended and zero in outputs.  Row starts are cut
+ * to [0, rows].  Nothing out of range is accessed.  Rows that are no sequence's are
+ * neither read nor written.
  */
 typedef struct rnsmx_kv_batch {
   const int32_t *table_dev;
@@ -537,8 +542,8 @@ int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *b
                         int64_t v_row_stride, int64_t v_head_stride, void *stream);
 
 /* The values of the batch's rows, code * scale rounded to dtype, ->
- * k_dev and v_dev [rows][heads][head_dim] contiguous (zeros in rows that have
- * no token or whose page is not there). */
+ * k_dev and v_dev [rows][heads][head_dim] contiguous (zeros in rows whose token
+ * or page is not there). */
 int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
                       void *k_dev, void *v_dev, int32_t dtype, void *stream);
 

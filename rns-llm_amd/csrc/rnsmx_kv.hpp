@@ -63,22 +63,28 @@ struct KvBatchArgs {
   int32_t seqs, table_width, rows, max_rows, max_length;
 };
 
-// One sequence's length and rows, cut to what the host was told.
+// One sequence: its tokens and rows as far as the host was told of them.  `base`,
+// the position of its first row, is that of what the device holds, so that a cut
+// drops tokens or rows and moves none.
 struct KvSeq {
-  int32_t len, row, n;
+  int32_t len, row, n, base;
+  int32_t all;  // its rows, those past max_rows too
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvBatchArgs &a, int32_t s) {
   KvSeq r;
   // through the scalar cache: s is one for the workgroup
   const kv_const_i32 *lengths = (const kv_const_i32 *)a.lengths, *starts = (const kv_const_i32 *)a.starts;
-  r.len = min(max(lengths[s], 0), a.max_length);
+  const int32_t length = max(lengths[s], 0);
+  r.len = min(length, a.max_length);
   if (a.starts) {
     r.row = min(max(starts[s], 0), a.rows);
-    r.n = min(max(starts[s + 1] - r.row, 0), min(a.max_rows, a.rows - r.row));
+    r.all = min(max(starts[s + 1], r.row), a.rows) - r.row;
   } else {
     r.row = s;
-    r.n = 1;
+    r.all = 1;
   }
+  r.n = min(r.all, a.max_rows);
+  r.base = length - r.all;
   return r;
 }
 

@@ -177,6 +177,20 @@ __device__ __forceinline__ int32_t kv_window_begin(const KvAttnArgs &a, int32_t 
   return a.window > 0 ? max(p + 1, a.window) - a.window : 0;
 }
 
+// Where a row at position p sees tokens of its sequence up to.
+__device__ __forceinline__ int32_t kv_causal_end(const KvAttnArgs &a, const KvSeq &q, int32_t p) {
+  return a.causal ? min(p + 1, q.len) : q.len;
+}
+
+// Zeros for a sequence's rows past max_rows.
+__device__ __forceinline__ void kv_zero_rows(const KvAttnArgs &a, const KvSeq &q, int32_t head) {
+  const int64_t wide = static_cast<int64_t>(a.by_group.d) * a.b.dim, count = (q.all - q.n) * wide;
+  for (int64_t i = threadIdx.x; i < count; i += blockDim.x) {
+    const int64_t r = i / wide;
+    kv_store(a.out, (q.row + q.n + r) * a.q_heads * a.b.dim + head * wide + (i - r * wide), a.dtype, 0.0f);
+  }
+}
+
 // Bits of those of eight tokens from t on that lie in [begin, end).
 __device__ __forceinline__ uint32_t kv_between(int32_t t, int32_t begin, int32_t end) {
   const uint32_t below = (1u << min(max(end - t, 0), 8)) - 1u, before = (1u << min(max(begin - t, 0), 8)) - 1u;

@@ -98,19 +98,22 @@ __device__ __forceinline__ float kv_value(uint32_t c, int i, float s) {
   return v;
 }
 
+// The end of those of a sequence's tokens that its rows are, up to max_rows of them.
+__device__ __forceinline__ int32_t kv_rows_end(const KvSeq &q) { return min(q.base + q.n, q.len); }
+
 // The tokens of one page that a sequence's rows are: `old` to end - 1, from row
-// `row` on; nothing where the page is past its end.
+// `row` on; nothing where the page is past their end.
 struct KvSpan {
   int32_t page, old, end, row;
 };
 __device__ __forceinline__ KvSpan kv_span(const KvBatchArgs &b, const KvSeq &q, int32_t seq, int32_t index) {
-  const int32_t from = max(q.len - q.n, 0), pg = (from >> b.log_page) + index;
+  const int32_t from = max(q.base, 0), to = kv_rows_end(q), pg = (from >> b.log_page) + index;
   KvSpan r{-1, 0, 0, 0};
-  if (q.n == 0 || pg > (q.len - 1) >> b.log_page) return r;
+  if (to <= from || pg > (to - 1) >> b.log_page) return r;
   const int32_t start = pg << b.log_page;
   r.old = max(from - start, 0);
-  r.end = min(q.len - start, 1 << b.log_page);
-  r.row = q.row + (start + r.old) - (q.len - q.n);
+  r.end = min(to - start, 1 << b.log_page);
+  r.row = q.row + (start + r.old) - q.base;
   r.page = ((const kv_const_i32 *)b.table)[seq * b.table_stride + pg];
   return r;
 }
@@ -196,11 +199,14 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
   const KvSeq q = kv_seq(b, seq);
   const int64_t rs = static_cast<int64_t>(b.heads) * b.dim;
   T *dst[2] = {static_cast<T *>(a.dst[0]) + head * b.dim, static_cast<T *>(a.dst[1]) + head * b.dim};
-  if (index == 0 && q.n > q.len)  // rows that have no token
-    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(q.n - q.len) * b.dim; i += 256) {
-      const int64_t r = i / b.dim;
-      kv_for<2>([&](auto P) { dst[P][(q.row + r) * rs + (i - r * b.dim)] = static_cast<T>(0); });
+  if (index == 0) {  // rows that have no token: `none` before the first, and those after the last
+    const int32_t none = min(max(-q.base, 0), q.all), last = max(kv_rows_end(q) - q.base, none);
+    const int32_t empty = none + q.all - last;
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(empty) * b.dim; i += 256) {
+      const int64_t e = i / b.dim, r = e < none ? e : last + (e - none);
+      kv_for<2>([&](auto P) { dst[P][(q.row + r) * rs + (i - e * b.dim)] = static_cast<T>(0); });
     }
+  }
   const KvSpan p = kv_span(b, q, seq, index);
   if (p.end == 0) return;
   const bool there = static_cast<uint32_t>(p.page) < static_cast<uint32_t>(b.blocks);
@@ -463,9 +469,10 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   a.tile_rows = few_rows(a.b, rows, kv_tokens(a)) ? kKvRows : kKvTileRows;
   a.row_tiles = static_cast<int32_t>((rows + a.tile_rows - 1) / a.tile_rows);
   kv_split(a);
+  a.row_tiles = std::max(a.row_tiles, 1);  // what zeroes a sequence's rows past max_rows 0
   a.by_group = kv_div(query->q_heads / cache->heads);
   a.by_splits = kv_div(a.splits);
-  a.by_units = kv_div(std::max(a.row_tiles, 1) * a.splits);
+  a.by_units = kv_div(a.row_tiles * a.splits);
   a.by_pairs = kv_div(static_cast<uint32_t>(pairs_at_once(static_cast<int64_t>(a.b.seqs) * cache->heads)));
   a.by_heads = kv_div(cache->heads);
   return RNSMX_OK;

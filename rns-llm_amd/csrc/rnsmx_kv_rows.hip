@@ -52,23 +52,24 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
   const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
   auto token_of = [&](int32_t r) { return static_cast<int32_t>(kv_quot(a.by_group, r)); };  // of a row
+  if (q.all > q.n && tile == 0 && split == 0) kv_zero_rows(a, q, head);
   const int32_t rows = q.n * group, row0 = tile * ROWS;
   if (row0 >= rows) return;
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t col = lane & 15, g = lane >> 4;
-  const int32_t base = q.len - q.n;  // position of the sequence's first row
+  const int32_t base = q.base;
   const int32_t t_first = token_of(row0), t_last = token_of(min(row0 + ROWS, rows) - 1);
-  const int32_t hi = max(a.causal ? base + t_last + 1 : q.len, 0);
-  const int32_t lo = kv_window_begin(a, base + t_first) & ~31;
-  const int32_t full_hi = a.causal ? base + t_first + 1 : q.len;                    // seen by every row: below it
-  const int32_t full_lo = kv_window_begin(a, base + t_last);              // and from it on
+  const int32_t hi = max(kv_causal_end(a, q, base + t_last), 0);
+  const int32_t lo = min(kv_window_begin(a, base + t_first), q.len) & ~31;
+  const int32_t full_hi = kv_causal_end(a, q, base + t_first);  // seen by every row: below it
+  const int32_t full_lo = kv_window_begin(a, base + t_last);    // and from it on
   const int32_t c0 = lo + split * a.chunk;
   if (split > 0 && c0 >= hi) return;
   const int32_t c1 = min(hi, c0 + a.chunk);
 
   // this lane's row: its place and what it sees
   const int32_t row = min(row0 + col, rows - 1), t_row = token_of(row), q_head = head * group + (row - t_row * group);
-  const int32_t end_row = a.causal ? base + t_row + 1 : q.len;
+  const int32_t end_row = kv_causal_end(a, q, base + t_row);
   const int32_t begin_row = kv_window_begin(a, base + t_row);
 
   struct Step {

@@ -66,6 +66,7 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
   const int32_t split = place.split, task = place.task, tile = place.tile, head = place.head, seq = place.seq;
   const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
+  if (q.all > q.n && tile == 0 && split == 0) kv_zero_rows(a, q, head);
   const int32_t rows = q.n * group, row0 = tile * kKvTileRows;
   if (row0 >= rows) return;
   const int32_t tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -73,24 +74,24 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
   _Float16 *const keys = staged[half], *const values = keys + 2 * kKeys;
   float (*const pages_of_step)[4][4] = page_scales[half];
   const int32_t col = lane & 31, h = lane >> 5;
-  const int32_t base = q.len - q.n;
+  const int32_t base = q.base;
   auto kv_of = [&](int32_t r) { return static_cast<int32_t>(kv_quot(a.by_group, r)); };  // the token of a row
   // what the workgroup's rows see, and this wave's
   const int32_t last_row = min(row0 + kKvTileRows, rows) - 1;
-  const int32_t hi = max(a.causal ? base + kv_of(last_row) + 1 : q.len, 0);
-  const int32_t lo = kv_window_begin(a, base + kv_of(row0)) & ~(kStep - 1);
+  const int32_t hi = max(kv_causal_end(a, q, base + kv_of(last_row)), 0);
+  const int32_t lo = min(kv_window_begin(a, base + kv_of(row0)), q.len) & ~(kStep - 1);
   const int32_t c0 = lo + split * a.chunk;
   if (split > 0 && c0 >= hi) return;
   const int32_t c1 = min(hi, c0 + a.chunk);
   const int32_t w_first = row0 + 32 * wave, w_last = min(w_first + 31, rows - 1);
   const bool w_any = w_first < rows;
   const int32_t t_first = kv_of(w_first), t_last = kv_of(w_last);
-  const int32_t full_hi = min(a.causal ? base + t_first + 1 : q.len, c1);
+  const int32_t full_hi = min(kv_causal_end(a, q, base + t_first), c1);
   const int32_t full_lo = kv_window_begin(a, base + t_last);
 
   const int32_t row = min(w_first + col, rows - 1);
   const int32_t t_row = kv_of(row), q_head = head * group + (row - t_row * group);
-  const int32_t end_row = min(a.causal ? base + t_row + 1 : q.len, c1);
+  const int32_t end_row = min(kv_causal_end(a, q, base + t_row), c1);
   const int32_t begin_row = kv_window_begin(a, base + t_row);
 
   // loads of a step: this wave's 16 tokens

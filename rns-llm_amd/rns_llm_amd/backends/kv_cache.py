@@ -65,8 +65,11 @@ class KVBatch:
     The tensors are read by the device on each call and may be written in
     between, as a decode loop (or a captured graph) does that advances
     ``lengths``; ``rows``, ``max_query`` and ``max_length`` bound what they may
-    hold, and what goes past them is cut off.  Rows that ``query_starts`` gives to
-    no sequence are not written in a call's outputs."""
+    hold.  What goes past them is dropped and moves nothing: tokens from
+    ``max_length`` on are not there, and a sequence's rows past its first
+    ``max_query`` are not appended and zero in outputs (starts are cut to
+    ``rows``).  Rows that ``query_starts`` gives to no sequence are not written in
+    a call's outputs."""
 
     block_table: torch.Tensor
     lengths: torch.Tensor

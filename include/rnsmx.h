@@ -583,8 +583,9 @@ int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const 
  * out[row][head] = sum_t softmax_t(scale * q . k_t + mask) v_t over the tokens
  * the row sees -> out_dev [rows][q_heads][head_dim] contiguous.  Products of
  * the queries and codes and of the softmax weights and codes run on the matrix
- * cores in float16 (FLOAT32 queries: two halves each, 22 bits), with float32
- * sums, maxima and exponentials.
+ * cores in float16, with float32 sums, maxima and exponentials.  Weights have 11
+ * bits down to 2^-24 of a row's largest (FLOAT32 queries: queries and weights go in
+ * two halves, 22 bits) and lose them below, the last at 2^-35 (2^-46).
  */
 int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
                            const rnsmx_kv_query_t *query, const void *q_dev,

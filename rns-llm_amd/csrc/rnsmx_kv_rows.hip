@@ -244,13 +244,14 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
       constexpr int j = J;
       const _Float16 h = static_cast<_Float16>(w[j]);
       p[0][j] = h;
-      if constexpr (SPLIT) p[1][j] = static_cast<_Float16>(w[j] - static_cast<float>(h));
+      if constexpr (SPLIT) p[1][j] = kv_low(w[j], h);
     });
     kv_for<VW>([&](auto I) {
       constexpr int i = I, word = i / 4, byte = i % 4;
       const h16x8 v = kv_join(kv_halves<byte, byte>(s.v[0][word], s.v[1][word]), kv_halves<byte, byte>(s.v[2][word], s.v[3][word]),
                               kv_halves<byte, byte>(s.v[4][word], s.v[5][word]), kv_halves<byte, byte>(s.v[6][word], s.v[7][word]));
-      kv_for<QN>([&](auto P) { o[i] = kv_mfma(v, p[P], o[i]); });
+      o[i] = kv_mfma(v, p[0], o[i]);
+      if constexpr (SPLIT) o[i] = kv_mfma(kv_low_codes(v), p[1], o[i]);
     });
   };
 

@@ -295,13 +295,14 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
         constexpr int j = J;
         const _Float16 half = static_cast<_Float16>(w[g][j]);
         p[0][j] = half;
-        if constexpr (SPLIT) p[1][j] = static_cast<_Float16>(w[g][j] - static_cast<float>(half));
+        if constexpr (SPLIT) p[1][j] = kv_low(w[g][j], half);
       });
       kv_for<DB>([&](auto I) {
         constexpr int i = I;
         const int32_t d = 32 * i + col;
         const h16x8 v = *reinterpret_cast<const h16x8 *>(&values[buf * kValues + d * kStep + ((2 * g + h) ^ value_swap(d)) * 8]);
-        kv_for<QN>([&](auto P) { o[i] = kv_mfma32(v, p[P], o[i]); });
+        o[i] = kv_mfma32(v, p[0], o[i]);
+        if constexpr (SPLIT) o[i] = kv_mfma32(kv_low_codes(v), p[1], o[i]);
       });
     });
   };

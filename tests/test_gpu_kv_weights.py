@@ -1,0 +1,47 @@
+"""Softmax weights far below a row's largest, where they are what its result is
+made of: a first token, say, that has nearly all the weight and next to no value."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_kv import DEV, MANY, ROUND, TYPES, World
+
+pytestmark = pytest.mark.gpu
+
+
+def most_off(dtype, out, spread, length, largest):
+    """What each element may be off by.  Scores of up to 64 in powers of two have
+    24 bits, a few times over on the way to a weight: less than 2^-15 of it.  A
+    weight has 11 bits, or 22 in two halves (float32), and float16's spacing of
+    2^-24 ends both where the largest weight is 2^10 or more: 2^-35 of it, and 2^11
+    less for the second half; `largest`: the largest value of the sequence, which
+    the largest weight goes with."""
+    weights, ends = (2.0 ** -21, 2.0 ** -46) if dtype == torch.float32 else (2.0 ** -11, 2.0 ** -35)
+    return ROUND[dtype] * out.abs() + (weights + 2.0 ** -15) * spread + length * ends * largest + 1e-30
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("gap", [10, 16])
+@pytest.mark.parametrize("length,at,rows,dim,idle", [
+    (1100, 0, 1, 64, 0), (1100, 700, 3, 128, 0), (6000, 3, 1, 128, 0), (6000, 5990, 2, 40, 0),
+    (700, 0, 60, 64, MANY), (700, 333, 60, 128, MANY), (1500, 20, 60, 160, MANY), (3000, 1, 600, 64, 8),
+])
+@pytest.mark.parametrize("masked", [False, True])
+def test_small_weights_count(backend, dtype, gap, length, at, rows, dim, idle, masked):
+    w = World(backend, lengths=[length], heads=1, dim=dim, page=16, seed=gap + dim, idle=idle)
+    q = torch.randn((1, 1, dim), generator=w.gen) + 0.02 * torch.randn((rows, 1, dim), generator=w.gen)
+    k, v = (torch.randn((length, 1, dim), generator=w.gen) for _ in range(2))
+    # its score: some four deviations for the largest of the others, and the gap
+    k[at] = (4 + gap) * math.sqrt(dim) * q[0] / (q[0] ** 2).sum()
+    v[at] = 0.01 * v[at]
+    v[at, :, ::2] = 0
+    w.append([length], torch.float32, k=k, v=v)
+    news, q = [rows], q.to(dtype)
+    mask = torch.zeros((1, 1, length)) if masked else None
+    got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch(news), mask=None if mask is None else mask.to(DEV)).cpu().double()
+    some = [0, rows - 1, rows // 2]
+    out, spread, _ = (x[some] for x in w.want(q, news))
+    most = most_off(dtype, out, spread, length, v.abs().max())
+    off = (got[some] - out).abs()
+    assert (off <= most).all(), f"off by {float((off / most).max()):.3g} of the bound, {float(off.norm() / out.norm()):.3g} of the result"

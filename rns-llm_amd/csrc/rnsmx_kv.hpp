@@ -5,6 +5,7 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "rnsmx_common.hpp"
@@ -47,6 +48,16 @@ __device__ __forceinline__ uint32_t kv_rem(const KvDiv &v, uint32_t &n) {
   const uint32_t q = kv_quot(v, n), r = n - q * v.d;
   n = q;
   return r;
+}
+
+// A launch has fewer than 2^32 threads, which a prompt beside many sequences passes
+// (128 of them, 32 heads, 131072 tokens in pages of 16): f(first workgroup, how many)
+// for each launch of a call's, all but the last a multiple of 512, so that kv_place's
+// order goes on from one to the next.
+template <typename F>
+inline void kv_launches(uint32_t groups, uint32_t threads, F &&f) {
+  const uint32_t most = (0xFFFFFFFFu / threads) & ~511u;
+  for (uint32_t first = 0; first < groups; first += std::min(most, groups - first)) f(first, std::min(most, groups - first));
 }
 
 // Row sizes the attention kernels are built for; a head dimension takes the
@@ -135,6 +146,7 @@ struct KvAttnArgs {
   int32_t tile_rows, row_tiles;  // rows of a workgroup (which says the kernel), workgroups over a sequence's rows
   // group: query heads of a key/value head; units: a pair's workgroups; pairs: those that run side by side
   KvDiv by_group, by_splits, by_units, by_heads, by_pairs;
+  uint32_t first, groups;  // a launch's first workgroup, and those of all the call's launches
   float scale;
 };
 
@@ -164,7 +176,9 @@ constexpr int64_t kv_tile_floats(int row_bytes) { return 256 * (static_cast<int6
 struct KvPlace {
   int32_t seq, head, tile, split, task;
 };
-__device__ __forceinline__ KvPlace kv_place(const KvAttnArgs &a, uint32_t id, uint32_t count, bool turn) {
+__device__ __forceinline__ KvPlace kv_place(const KvAttnArgs &a, bool turn) {
+  const uint32_t count = a.groups;
+  uint32_t id = a.first + blockIdx.x;
   if (turn) {
     const uint32_t xcd = id & 7, size = (count >> 3) + (xcd < (count & 7) ? 1 : 0);
     uint32_t n = id >> 3;
@@ -185,13 +199,13 @@ __device__ __forceinline__ KvPlace kv_place(const KvAttnArgs &a, uint32_t id, ui
 
 // rnsmx_kv_rows.hip, one object per row size
 template <int DT>
-void launch_kv_rows(const KvAttnArgs &a, hipStream_t st);
+void launch_kv_rows(const KvAttnArgs &a, uint32_t groups, hipStream_t st);
 
 // rnsmx_kv_tiles.hip, one object per row size
 constexpr int kKvTileRows = 128;  // query rows of a workgroup of kv_tiles_kernel
 // Row sizes whose staged steps fit the shared memory twice run on eight waves too.
 constexpr int kv_tile_halves(int row_bytes) { return row_bytes <= 128 ? 2 : 1; }
 template <int DT>
-void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st);
+void launch_kv_tiles(const KvAttnArgs &a, uint32_t groups, hipStream_t st);
 
 }  // namespace rnsmx

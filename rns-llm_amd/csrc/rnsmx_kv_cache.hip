@@ -13,6 +13,7 @@ struct KvAppendArgs {
   int64_t row_stride[2], head_stride[2];
   int32_t vec;              // rows are read 16 bytes at a time
   KvDiv by_heads, by_pages;  // pages: most of one sequence that the rows touch
+  uint32_t first;            // a launch's first workgroup
 };
 
 struct KvReadArgs {
@@ -20,6 +21,7 @@ struct KvReadArgs {
   void *dst[2];
   int32_t vec;
   KvDiv by_heads, by_pages;
+  uint32_t first;
 };
 
 constexpr float kKvMax = 127.0f;
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(1024) void kv_append_kernel(const KvAppendArgs a) {
   constexpr int CPT = DT / 8;
   __shared__ uint32_t tops[16];
   const KvBatchArgs &b = a.b;
-  uint32_t id = blockIdx.x;
+  uint32_t id = a.first + blockIdx.x;
   const int32_t part = id & 1;
   id >>= 1;
   const int32_t head = kv_rem(a.by_heads, id), index = kv_rem(a.by_pages, id), seq = id;
@@ -194,7 +196,7 @@ template <int DT, typename T, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
   constexpr int CPT = DT / 8;
   const KvBatchArgs &b = a.b;
-  uint32_t id = blockIdx.x;
+  uint32_t id = a.first + blockIdx.x;
   const int32_t head = kv_rem(a.by_heads, id), index = kv_rem(a.by_pages, id), seq = id;
   const KvSeq q = kv_seq(b, seq);
   const int64_t rs = static_cast<int64_t>(b.heads) * b.dim;
@@ -351,7 +353,7 @@ static void kv_of_type(int32_t dtype, bool stream, F &&f) {
 }
 
 static int32_t grid_of(int64_t groups, unsigned &grid) {
-  if (groups > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many sequences, pages and heads for one launch");
+  if (groups > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many sequences, pages and heads for one call");
   grid = static_cast<unsigned>(groups);
   return RNSMX_OK;
 }
@@ -527,7 +529,10 @@ int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *b
                      k_row_stride % 64 == 0 && v_row_stride % 64 == 0 && k_head_stride % 64 == 0 && v_head_stride % 64 == 0;
   kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim, whole), [&](auto t, auto stream) {
     using T = decltype(t);
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, T, decltype(stream)::value>), dim3(grid), dim3(threads), 0, st, a))
+    kv_launches(grid, threads, [&](uint32_t first, uint32_t groups) {
+      a.first = first;
+      RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_append_kernel<DT, T, decltype(stream)::value>), dim3(groups), dim3(threads), 0, st, a))
+    });
   });
   return kv_check("kv_append");
 }
@@ -554,7 +559,10 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
   const bool whole = size == 2 && a.vec && a.b.dim % 32 == 0 && aligned(k_dev, 64) && aligned(v_dev, 64);
   kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim, whole), [&](auto t, auto stream) {
     using T = decltype(t);
-    RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, T, decltype(stream)::value>), dim3(grid), dim3(256), 0, st, a))
+    kv_launches(grid, 256, [&](uint32_t first, uint32_t groups) {
+      a.first = first;
+      RNSMX_KV_DIMS(a.b.row_bytes, hipLaunchKernelGGL((kv_read_kernel<DT, T, decltype(stream)::value>), dim3(groups), dim3(256), 0, st, a))
+    });
   });
   return kv_check("kv_read");
 }
@@ -603,11 +611,15 @@ int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t
   if (grid == 0) return RNSMX_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   a.out_vec = aligned(out_dev, 16);
-  if (a.tile_rows == kKvTileRows) {
-    RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_tiles<DT>(a, st))
-  } else {
-    RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_rows<DT>(a, st))
-  }
+  a.groups = grid;
+  kv_launches(grid, 64 * a.waves, [&](uint32_t first, uint32_t groups) {
+    a.first = first;
+    if (a.tile_rows == kKvTileRows) {
+      RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_tiles<DT>(a, groups, st))
+    } else {
+      RNSMX_KV_DIMS(a.b.row_bytes, launch_kv_rows<DT>(a, groups, st))
+    }
+  });
   return kv_check("kv_attention");
 }
 

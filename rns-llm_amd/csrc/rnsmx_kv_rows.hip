@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
   __shared__ int32_t last;
 
   const KvBatchArgs &b = a.b;
-  const KvPlace place = kv_place(a, blockIdx.x, gridDim.x, false);
+  const KvPlace place = kv_place(a, false);
   const int32_t split = place.split, task = place.task, tile = place.tile, head = place.head, seq = place.seq;
   const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
@@ -382,8 +382,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
 }
 
 template <int DT, int NW>
-static void launch_waves(const KvAttnArgs &a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles * a.splits)), block(64 * NW);
+static void launch_waves(const KvAttnArgs &a, uint32_t groups, hipStream_t st) {
+  const dim3 grid(groups), block(64 * NW);
   auto launch = [&](auto split) {
     constexpr bool S = decltype(split)::value;
     if (a.mask)
@@ -400,13 +400,13 @@ static void launch_waves(const KvAttnArgs &a, hipStream_t st) {
 }
 
 template <int DT>
-void launch_kv_rows(const KvAttnArgs &a, hipStream_t st) {
+void launch_kv_rows(const KvAttnArgs &a, uint32_t groups, hipStream_t st) {
   if (a.waves == 8 && kv_wide(DT))
-    launch_waves<DT, kv_wide(DT) ? 8 : 4>(a, st);
+    launch_waves<DT, kv_wide(DT) ? 8 : 4>(a, groups, st);
   else
-    launch_waves<DT, 4>(a, st);
+    launch_waves<DT, 4>(a, groups, st);
 }
 
-template void launch_kv_rows<RNSMX_KV_DIM>(const KvAttnArgs &a, hipStream_t st);
+template void launch_kv_rows<RNSMX_KV_DIM>(const KvAttnArgs &a, uint32_t groups, hipStream_t st);
 
 }  // namespace rnsmx

@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
   __shared__ int32_t last;
 
   const KvBatchArgs &b = a.b;
-  const KvPlace place = kv_place(a, blockIdx.x, gridDim.x, HALVES == 1);
+  const KvPlace place = kv_place(a, HALVES == 1);
   const int32_t split = place.split, task = place.task, tile = place.tile, head = place.head, seq = place.seq;
   const int32_t group = a.by_group.d;
   const KvSeq q = kv_seq(b, seq);
@@ -468,8 +468,8 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
 }
 
 template <int DT, int HALVES>
-static void launch_halves(const KvAttnArgs &a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles * a.splits)), block(256 * HALVES);
+static void launch_halves(const KvAttnArgs &a, uint32_t groups, hipStream_t st) {
+  const dim3 grid(groups), block(256 * HALVES);
   const bool split = a.dtype == RNSMX_FLOAT32;
   if (a.mask) {
     if (split)
@@ -484,13 +484,13 @@ static void launch_halves(const KvAttnArgs &a, hipStream_t st) {
 }
 
 template <int DT>
-void launch_kv_tiles(const KvAttnArgs &a, hipStream_t st) {
+void launch_kv_tiles(const KvAttnArgs &a, uint32_t groups, hipStream_t st) {
   if (a.waves == 8)
-    launch_halves<DT, kv_tile_halves(DT)>(a, st);
+    launch_halves<DT, kv_tile_halves(DT)>(a, groups, st);
   else
-    launch_halves<DT, 1>(a, st);
+    launch_halves<DT, 1>(a, groups, st);
 }
 
-template void launch_kv_tiles<RNSMX_KV_DIM>(const KvAttnArgs &a, hipStream_t st);
+template void launch_kv_tiles<RNSMX_KV_DIM>(const KvAttnArgs &a, uint32_t groups, hipStream_t st);
 
 }  // namespace rnsmx

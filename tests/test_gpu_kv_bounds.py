@@ -182,3 +182,52 @@ def test_row_starts_of_any_number(backend, starts):
     backend.kv_read(cache, batch, dtype=torch.float16)
     torch.cuda.synchronize()
     assert (edge[0] == 0).all() and (edge[2] == 0).all() and edge.isfinite().all()
+
+
+def test_calls_of_more_threads_than_a_launch_has(backend):
+    """A prompt beside many sequences that hold nothing: 2^32 threads and more
+    are several launches."""
+    heads, rows, seqs = 1024, 2048, 2050
+    pages = rows // 16
+    cache, twin = (backend.create_kv_cache(device=GPU, blocks=pages, block_size=16, kv_heads=heads, head_dim=1) for _ in range(2))
+    table = torch.full((seqs, pages), -1, dtype=torch.int32, device=DEV)
+    gen = torch.Generator().manual_seed(33)
+    k, v, q = (torch.randn((rows, heads, 1), generator=gen).half().to(DEV) for _ in range(3))
+    for at in (0, seqs // 2, seqs - 1):  # in the first launch, one between, the last
+        table.fill_(-1)
+        table[at] = torch.randperm(pages, generator=gen, dtype=torch.int32)
+        counts = [0] * seqs
+        counts[at] = rows
+        batch = backend.kv_batch(cache, table, counts, query_lengths=counts)
+        alone = backend.kv_batch(twin, table[at:at + 1], [rows], query_lengths=[rows])
+        backend.kv_append(cache, batch, k, v)
+        backend.kv_append(twin, alone, k, v)
+        for a, b in ((twin.k_codes, cache.k_codes), (twin.v_codes, cache.v_codes), (twin.scales, cache.scales)):
+            assert torch.equal(a, b)
+            a.zero_()
+            b.zero_()
+        backend.kv_append(cache, batch, k, v)
+        backend.kv_append(twin, alone, k, v)
+        for x, y in zip(backend.kv_read(cache, batch, dtype=torch.float16), backend.kv_read(twin, alone, dtype=torch.float16)):
+            assert torch.equal(x, y)
+        got, want = backend.kv_attention(q, cache, batch), backend.kv_attention(q, twin, alone)
+        torch.testing.assert_close(got, want, rtol=2e-3, atol=2e-3)
+
+
+def test_single_rows_of_more_threads_than_a_launch_has(backend):
+    heads, seqs = 1024, 16500
+    cache = backend.create_kv_cache(device=GPU, blocks=4, block_size=16, kv_heads=heads, head_dim=1)
+    table = torch.full((seqs, 1), -1, dtype=torch.int32, device=DEV)
+    real = [0, 8000, 16383, seqs - 1]
+    table[real, 0] = torch.arange(4, dtype=torch.int32, device=DEV)
+    counts = torch.zeros(seqs, dtype=torch.int32, device=DEV)
+    counts[real] = 1
+    q, k, v = (torch.randn((seqs, heads, 1), device=DEV).half() for _ in range(3))
+    batch = backend.kv_batch(cache, table, counts)
+    backend.kv_append(cache, batch, k, v)
+    out = torch.full_like(q, torch.nan)
+    backend.kv_attention(q, cache, batch, out=out)
+    assert torch.equal(out[real], backend.kv_read(cache, batch, dtype=torch.float16)[1][real])  # one token has all the weight
+    empty = torch.ones(seqs, dtype=torch.bool, device=DEV)
+    empty[real] = False
+    assert (out[empty] == 0).all()

@@ -22,6 +22,7 @@ from .. import _native
 PAGE_SIZES = (16, 32, 64, 128)
 MAX_LENGTH = 1 << 30
 _MAX_ROWS = 2 ** 31 - 1
+_MAX_CHECKED = 64  # shapes a batch remembers; a mask that grows by a column each step brings ever new ones
 _FLOAT_CODES = {torch.float32: _native.FLOAT32, torch.float16: _native.FLOAT16,
                 torch.bfloat16: _native.BFLOAT16}
 _MASK_CODES = {**_FLOAT_CODES, torch.bool: _native.INT8}
@@ -86,6 +87,12 @@ class KVBatch:
     @property
     def sequences(self) -> int:
         return int(self.lengths.shape[0])
+
+    def _remember(self, key: tuple, value):
+        if len(self._checked) >= _MAX_CHECKED:
+            self._checked.clear()
+        self._checked[key] = value
+        return value
 
 
 def _device_ints(values: torch.Tensor, name: str, ndim: int, device: torch.device) -> torch.Tensor:
@@ -225,8 +232,7 @@ class KVCacheOps:
             if plain_k is not k or plain_v is not v:
                 return self.kv_append(cache, batch, plain_k, plain_v)
             self._check_gpu(cache)
-            args = (_FLOAT_CODES[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-            batch._checked[key] = args
+            args = batch._remember(key, (_FLOAT_CODES[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1)))
         rc = self._lib.rnsmx_kv_append(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), *args,
                                        self._stream_of(cache.device))
         if rc:
@@ -247,7 +253,7 @@ class KVCacheOps:
             self._check_gpu(cache)
             # one value's memory in the outputs' shape: what they are made like costs less than their sizes
             like = torch.empty((1,), dtype=dtype, device=cache.device).expand(batch.rows, cache.kv_heads, cache.head_dim)
-            batch._checked[key] = like
+            batch._remember(key, like)
         k = torch.empty_like(like, memory_format=torch.contiguous_format)
         v = torch.empty_like(like, memory_format=torch.contiguous_format)
         rc = self._lib.rnsmx_kv_read(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), _FLOAT_CODES[dtype],
@@ -288,7 +294,7 @@ class KVCacheOps:
             query = self._query_of(q, cache, batch, scale, causal, window, mask)
             self._check_gpu(cache)
             need = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ctypes.addressof(query)))
-            checked = batch._checked[key] = (query, ctypes.addressof(query), need)
+            checked = batch._remember(key, (query, ctypes.addressof(query), need))
         _, ref, need = checked
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)

@@ -47,3 +47,30 @@ def test_caches_in_host_memory_reach_no_kernel(call, monkeypatch):
     for _ in range(2):
         with pytest.raises(ValueError, match="on the GPU"):
             call(b, cache(), x, q)
+
+
+def test_a_batch_remembers_few_shapes(monkeypatch):
+    """A mask that grows with the sequence is a new shape each step; what a batch
+    keeps of them does not grow."""
+
+    class Counts:
+        rnsmx_kv_attention_workspace_bytes = staticmethod(lambda *args: 0)
+        masks = []
+
+        def rnsmx_kv_attention(self, cache, batch, query, *args):
+            self.masks.append(_native.KVQueryStruct.from_address(query).mask_len)
+            return 0
+
+    b = backend()
+    b._lib, b._stats = Counts(), {"kv_attention_calls": 0}
+    monkeypatch.setattr(type(b), "_stream_of", staticmethod(lambda device: 0))
+    monkeypatch.setattr(type(b), "_check_gpu", staticmethod(lambda cache: None))
+    c = cache()
+    step = backend().kv_batch(c, torch.zeros((2, 2), dtype=torch.int32), torch.ones(2, dtype=torch.int32))
+    q, most = torch.zeros((2, 4, 40), dtype=torch.float16), 0
+    for n in range(1, 1000):
+        b.kv_attention(q, c, step, mask=torch.zeros((1, 1, n)))
+        b.kv_attention(q, c, step)
+        most = max(most, len(step._checked))
+    assert b._lib.masks == [m for n in range(1, 1000) for m in (n, 0)]
+    assert most <= 64

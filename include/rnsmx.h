@@ -579,6 +579,22 @@ typedef struct rnsmx_kv_query {
 int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
                                            const rnsmx_kv_query_t *query);
 
+/* How rnsmx_kv_attention runs a call. */
+typedef struct rnsmx_kv_plan {
+  int32_t tile_rows; /* query rows of a workgroup: 16 or, prompts, 128 */
+  int32_t row_tiles; /* workgroups over the rows of a sequence         */
+  int32_t waves;     /* of a workgroup, 4 or 8                         */
+  int32_t splits;    /* workgroups over the tokens of a sequence       */
+  int32_t chunk;     /* tokens of each                                 */
+  int32_t stream;    /* 1: 16 rows: values' codes are read past the caches */
+} rnsmx_kv_plan_t;
+
+/* The plan of a call with a mask (masked 1) or without.  It follows from sizes
+ * alone: host code only (no GPU call, no stream), nothing of the pointers is read.
+ * For tests and tuning, as rnsmx_gemm_plan. */
+int32_t rnsmx_kv_attention_plan(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                                const rnsmx_kv_query_t *query, int32_t masked, rnsmx_kv_plan_t *out);
+
 /*
  * out[row][head] = sum_t softmax_t(scale * q . k_t + mask) v_t over the tokens
  * the row sees -> out_dev [rows][q_heads][head_dim] contiguous.  Products of

@@ -480,6 +480,12 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
   return RNSMX_OK;
 }
 
+// Each code is read by one workgroup alone, and they are many.
+static bool kv_past_caches(const KvAttnArgs &a, bool masked) {
+  return !masked && a.tile_rows == kKvRows && a.row_tiles == 1 &&
+         streams(2ll * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a), kv_whole(a.b.row_bytes));
+}
+
 static int64_t kv_tasks(const KvAttnArgs &a) { return static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles; }
 
 static int64_t kv_workspace(const KvAttnArgs &a) {
@@ -575,6 +581,16 @@ int64_t rnsmx_kv_attention_workspace_bytes(const rnsmx_kv_cache_t *cache, const 
   return kv_workspace(a);
 }
 
+int32_t rnsmx_kv_attention_plan(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch,
+                                const rnsmx_kv_query_t *query, int32_t masked, rnsmx_kv_plan_t *out) {
+  clear_error();
+  if (!out) return fail(RNSMX_EINVAL, "null plan");
+  KvAttnArgs a{};
+  if (int32_t rc = kv_attn_args(cache, batch, query, a)) return rc;
+  *out = rnsmx_kv_plan_t{a.tile_rows, a.row_tiles, a.waves, a.splits, a.chunk, kv_past_caches(a, masked != 0)};
+  return RNSMX_OK;
+}
+
 int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *batch, const rnsmx_kv_query_t *query,
                            const void *q_dev, const void *mask_dev, void *workspace_dev, int64_t workspace_bytes,
                            void *out_dev, void *stream) {
@@ -603,9 +619,7 @@ int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t
     a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace_dev) + RNSMX_KV_TICKETS * 4);
   }
   a.out = out_dev;
-  // each code is read by one workgroup alone
-  a.stream = !a.mask && a.row_tiles == 1 &&
-             streams(2ll * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a), kv_whole(a.b.row_bytes));
+  a.stream = kv_past_caches(a, a.mask != nullptr);
   unsigned grid;
   if (int32_t rc = grid_of(kv_tasks(a) * a.splits, grid)) return rc;
   if (grid == 0) return RNSMX_OK;

@@ -53,6 +53,7 @@ EXPORTED_SYMBOLS = (
     "rnsmx_kv_append",
     "rnsmx_kv_read",
     "rnsmx_kv_attention_workspace_bytes",
+    "rnsmx_kv_attention_plan",
     "rnsmx_kv_attention",
 )
 
@@ -178,6 +179,22 @@ class KVQueryStruct(ctypes.Structure):
     ]
 
 
+class KVPlan(ctypes.Structure):
+    """Mirror of ``rnsmx_kv_plan_t``."""
+
+    _fields_ = [
+        ("tile_rows", ctypes.c_int32),
+        ("row_tiles", ctypes.c_int32),
+        ("waves", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+        ("chunk", ctypes.c_int32),
+        ("stream", ctypes.c_int32),
+    ]
+
+    def as_tuple(self) -> tuple[int, ...]:
+        return tuple(getattr(self, name) for name, _ in self._fields_)
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -228,10 +245,11 @@ _SIGNATURES = {
     "rnsmx_kv_append": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _P]),
     "rnsmx_kv_read": (_I32, [_P, _P, _P, _P, _I32, _P]),
     "rnsmx_kv_attention_workspace_bytes": (_I64, [_P, _P, _P]),
+    "rnsmx_kv_attention_plan": (_I32, [_P, _P, _P, _I32, _P]),
     "rnsmx_kv_attention": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _P, _P]),
 }
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 
 class NativeError(RuntimeError):

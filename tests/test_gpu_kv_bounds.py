@@ -5,6 +5,7 @@ import ctypes
 import pytest
 import torch
 
+from kv_plans import plan_of
 from rns_llm_amd import _native
 
 pytestmark = pytest.mark.gpu
@@ -45,6 +46,7 @@ def test_windows_of_any_number(backend, window, idle):
     cache, table, gen = filled(backend, [1, 40, 1], idle=idle)
     batch = backend.kv_batch(cache, table, lengths + [0] * idle, query_lengths=news + [0] * idle)
     q = torch.randn((sum(news), 4, 64), generator=gen).half().to(DEV)
+    assert plan_of(cache, batch, 4, torch.float16).tile_rows == (128 if idle else 16)
     want = backend.kv_attention(q, cache, batch)
     assert (want[:39] == 0).all() and (want[39:80].abs().amax(dim=(1, 2)) > 0).all()
     query = _native.KVQueryStruct(q.stride(0), q.stride(1), 0, 0, 0, _native.FLOAT16, 4, 0, 0, 1, window, 0.125)
@@ -125,6 +127,7 @@ def test_rows_past_max_query_move_no_others(backend, idle, most):
     rest = torch.ones(42, dtype=torch.bool, device=DEV)
     rest[pick] = False
     q = torch.randn((42, 4, 64), generator=gen).half().to(DEV)
+    assert plan_of(cache, batch, 4, torch.float16).tile_rows == (128 if idle and most == 33 else 16)
     for window in (None, 21):
         out = torch.full_like(q, torch.nan)
         backend.kv_attention(q, cache, batch, window=window, out=out)
@@ -145,18 +148,19 @@ def test_rows_past_max_query_move_no_others(backend, idle, most):
         assert torch.equal(x[pick], y) and (x[rest] == 0).all()
 
 
-@pytest.mark.parametrize("idle", [0, MANY])
+@pytest.mark.parametrize("idle,rows", [(0, 5), (0, 35), (MANY, 35)])
 @pytest.mark.parametrize("over", [1, 4, 200, 2 ** 31 - 1 - 40])
-def test_rows_past_max_length_see_what_is_there(backend, idle, over):
+def test_rows_past_max_length_see_what_is_there(backend, idle, rows, over):
     """Rows keep their positions: the window of one past the bound ends where it
     stands, whatever of it is there."""
-    top, rows = 40, 5
+    top = 40
     cache, table, gen = filled(backend, [48, 48], idle=idle)
     length = top + over
     starts = torch.cat([ints(0, rows), ints(*[2 * rows] * (1 + idle))])
     batch = backend.kv_batch(cache, table, ints(length, 40, *[0] * idle), query_starts=starts, rows=2 * rows, max_query=rows,
                              max_length=top)
     q = torch.randn((2 * rows, 4, 64), generator=gen).half().to(DEV)
+    assert plan_of(cache, batch, 4, torch.float16).tile_rows == (128 if idle else 16)
     whole = backend.kv_batch(cache, table, [40, 40] + [0] * idle, query_lengths=[rows, rows] + [0] * idle)
     at = torch.arange(rows).view(-1, 1, 1) + length - rows
     token = torch.arange(40).view(1, 1, 40)

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from kv_plans import plan_of
 from test_gpu_kv import DEV, MANY, ROUND, TYPES, World
 
 pytestmark = pytest.mark.gpu
@@ -26,6 +27,7 @@ def most_off(dtype, out, spread, length, largest):
 @pytest.mark.parametrize("length,at,rows,dim,idle", [
     (1100, 0, 1, 64, 0), (1100, 700, 3, 128, 0), (6000, 3, 1, 128, 0), (6000, 5990, 2, 40, 0),
     (700, 0, 60, 64, MANY), (700, 333, 60, 128, MANY), (1500, 20, 60, 160, MANY), (3000, 1, 600, 64, 8),
+    (700, 0, 130, 64, MANY), (700, 333, 130, 128, MANY), (1500, 20, 130, 160, MANY), (3000, 1, 640, 64, 18), (3000, 2900, 640, 40, 18),
 ])
 @pytest.mark.parametrize("masked", [False, True])
 def test_small_weights_count(backend, dtype, gap, length, at, rows, dim, idle, masked):
@@ -39,9 +41,25 @@ def test_small_weights_count(backend, dtype, gap, length, at, rows, dim, idle, m
     w.append([length], torch.float32, k=k, v=v)
     news, q = [rows], q.to(dtype)
     mask = torch.zeros((1, 1, length)) if masked else None
+    kernel = plan_of(w.cache, w.batch(news), 1, dtype, masked=masked)
+    assert kernel.tile_rows == (128 if rows in (130, 640) else 16) and (kernel.splits > 1) == (length == 6000 or rows == 640)
     got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch(news), mask=None if mask is None else mask.to(DEV)).cpu().double()
     some = [0, rows - 1, rows // 2]
     out, spread, _ = (x[some] for x in w.want(q, news))
     most = most_off(dtype, out, spread, length, v.abs().max())
     off = (got[some] - out).abs()
     assert (off <= most).all(), f"off by {float((off / most).max()):.3g} of the bound, {float(off.norm() / out.norm()):.3g} of the result"
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,group,dim", [(150, 1, 128), (60, 4, 64), (150, 1, 256)])
+@pytest.mark.parametrize("window", [None, 2500])
+def test_tiles_of_16_rows_are_split(backend, dtype, rows, group, dim, window):
+    """Several tiles of 16 rows to a sequence and several splits to a tile, beside
+    sequences that need fewer of either."""
+    lengths, news = [4100, 130, 2700, 0], [rows, min(130, rows), rows // 2, 1]
+    w = World(backend, lengths=lengths, heads=1, dim=dim, page=16, seed=dim)
+    w.append(lengths, dtype)
+    kernel = plan_of(w.cache, w.batch(news), group, dtype, window=window)
+    assert kernel.tile_rows == 16 and kernel.row_tiles > 1 and kernel.splits > 1
+    w.check(news, dtype, group, **({} if window is None else {"window": window}))

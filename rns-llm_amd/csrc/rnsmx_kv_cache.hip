@@ -333,7 +333,9 @@ static int64_t pages_touched(const KvBatchArgs &a) {
 // Attention (codes of 134 MB, 16 sequences of 4096 tokens, 8 heads of 128): 36 so, 40
 // through the caches; rows of 64: 27, 30; of 160: 117, 107 (48 sequences).
 constexpr int64_t kStreamBytes = 128ll << 20;
-static bool streams(int64_t bytes, bool whole) { return whole && bytes >= kStreamBytes; }
+static bool streams(double bytes, bool whole) { return whole && bytes >= kStreamBytes; }
+// Values of a call's rows, keys or values: past 64 bits for sizes that the checks take.
+static double kv_values(const KvBatchArgs &b) { return static_cast<double>(b.rows) * b.heads * b.dim; }
 
 // f(a value of the type, whether past the caches as a constant)
 template <typename F>
@@ -483,7 +485,7 @@ static int32_t kv_attn_args(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_
 // Each code is read by one workgroup alone, and they are many.
 static bool kv_past_caches(const KvAttnArgs &a, bool masked) {
   return !masked && a.tile_rows == kKvRows && a.row_tiles == 1 &&
-         streams(2ll * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a), kv_whole(a.b.row_bytes));
+         streams(2.0 * a.b.row_bytes * a.b.heads * a.b.seqs * kv_tokens(a), kv_whole(a.b.row_bytes));
 }
 
 static int64_t kv_tasks(const KvAttnArgs &a) { return static_cast<int64_t>(a.b.seqs) * a.b.heads * a.row_tiles; }
@@ -533,7 +535,7 @@ int32_t rnsmx_kv_append(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *b
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool whole = size == 2 && a.vec && a.b.dim % 64 == 0 && aligned(k_dev, 128) && aligned(v_dev, 128) &&
                      k_row_stride % 64 == 0 && v_row_stride % 64 == 0 && k_head_stride % 64 == 0 && v_head_stride % 64 == 0;
-  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim, whole), [&](auto t, auto stream) {
+  kv_of_type(dtype, streams(2.0 * size * kv_values(a.b), whole), [&](auto t, auto stream) {
     using T = decltype(t);
     kv_launches(grid, threads, [&](uint32_t first, uint32_t groups) {
       a.first = first;
@@ -563,7 +565,7 @@ int32_t rnsmx_kv_read(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t *bat
   if (int32_t rc = grid_of(a.b.seqs * pages * a.b.heads, grid)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool whole = size == 2 && a.vec && a.b.dim % 32 == 0 && aligned(k_dev, 64) && aligned(v_dev, 64);
-  kv_of_type(dtype, streams(2 * size * a.b.rows * a.b.heads * a.b.dim, whole), [&](auto t, auto stream) {
+  kv_of_type(dtype, streams(2.0 * size * kv_values(a.b), whole), [&](auto t, auto stream) {
     using T = decltype(t);
     kv_launches(grid, 256, [&](uint32_t first, uint32_t groups) {
       a.first = first;

@@ -86,6 +86,12 @@ def test_tests_of_prompts_run_their_kernel(sizes, options, split):
         assert got[0] == 128 and (got[3] > 1) == split
 
 
+@pytest.mark.parametrize("seqs,heads", [(2 ** 22, 2 ** 8), (2 ** 15, 2 ** 15), (2 ** 25, 1)])
+def test_plans_of_more_bytes_than_64_bits_count(seqs, heads):
+    """2^69 and 2^64 bytes of codes in the widest tables that the checks take."""
+    assert plan(seqs, heads, heads, 1, 2 ** 30, 256, page=128)[5] == 1
+
+
 def test_plans_follow_the_refusals():
     with pytest.raises(ValueError):
         plan(1, 3, 4, 1, 16, 64)

@@ -95,6 +95,18 @@ class KVBatch:
         return value
 
 
+class _WithoutGradient(torch.autograd.Function):
+    """An output as it is; a backward pass that reaches it says that it ends there."""
+
+    @staticmethod
+    def forward(ctx, out, *inputs):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, *gradients):
+        raise RuntimeError("kv_attention has no gradient: detach its queries and mask, or call it under torch.no_grad()")
+
+
 def _device_ints(values: torch.Tensor, name: str, ndim: int, device: torch.device) -> torch.Tensor:
     if values.dtype != torch.int32 or values.ndim != ndim or values.device != device:
         raise ValueError(f"{name} must be a {ndim}-dimensional int32 tensor on {device}")
@@ -221,7 +233,8 @@ class KVCacheOps:
         larger of its scale and the new tokens'; where that is larger than its
         own, its older codes are quantised again from the values they stood for.
         A value that is not finite makes every value of its page and head read
-        as NaN.  Sequences of one call must not share pages that it writes to."""
+        as NaN.  Sequences of one call must not share pages that it writes to.  No
+        gradient goes through the cache."""
         key = (k.dtype, k.shape, k.stride(), k.device, v.dtype, v.shape, v.stride(), v.device, cache._shape)
         args = batch._checked.get(key)
         if args is None:
@@ -278,7 +291,10 @@ class KVCacheOps:
         numbers.  What is hidden contributes nothing whatever it holds, and a row
         that sees no token is zero.  ``workspace``: zero-initialised uint8 of
         ``kv_attention_workspace_bytes``, by default one kept per stream (under
-        graph capture one of the graph's, cleared by each replay)."""
+        graph capture one of the graph's, cleared by each replay).
+
+        There is no gradient: where queries or mask require one, a backward pass
+        through the result raises (a given ``out`` holds numbers alone)."""
         if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()):
             raise ValueError("out must be contiguous and like q")
         scale = None if scale is None else float(scale)
@@ -296,6 +312,7 @@ class KVCacheOps:
             need = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ctypes.addressof(query)))
             checked = batch._remember(key, (query, ctypes.addressof(query), need))
         _, ref, need = checked
+        wanted = out is None and (q.requires_grad or mask is not None and mask.requires_grad) and torch.is_grad_enabled()
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         stream = self._stream_of(cache.device)
@@ -314,7 +331,7 @@ class KVCacheOps:
         if rc:
             _native.check(rc)
         self._stats["kv_attention_calls"] += 1
-        return out
+        return _WithoutGradient.apply(out, q, mask) if wanted else out
 
     def _query_of(self, q: torch.Tensor, cache: KVCache, batch: KVBatch, scale, causal, window, mask):
         """The checked arguments of ``kv_attention`` as the library takes them."""

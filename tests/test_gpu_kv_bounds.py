@@ -235,3 +235,24 @@ def test_single_rows_of_more_threads_than_a_launch_has(backend):
     empty = torch.ones(seqs, dtype=torch.bool, device=DEV)
     empty[real] = False
     assert (out[empty] == 0).all()
+
+
+@pytest.mark.parametrize("which", ["q", "mask"])
+def test_a_backward_pass_that_gets_here_says_so(backend, which):
+    cache, table, gen = filled(backend, [40, 17])
+    batch = backend.kv_batch(cache, table, [40, 17], query_lengths=[3, 2])
+    q = torch.randn((5, 4, 64), generator=gen).to(DEV)
+    mask = torch.randn((1, 1, 40), generator=gen).to(DEV)
+    want = backend.kv_attention(q, cache, batch, mask=mask)
+    assert not want.requires_grad
+    asks = {"q": q, "mask": mask}[which].requires_grad_()
+    got = backend.kv_attention(q, cache, batch, mask=mask)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        got.sum().backward()
+    assert asks.grad is None
+    with torch.no_grad():
+        assert not backend.kv_attention(q, cache, batch, mask=mask).requires_grad
+    out = torch.empty_like(want)
+    assert backend.kv_attention(q, cache, batch, mask=mask, out=out) is out and not out.requires_grad
+    assert not backend.kv_attention(q.detach(), cache, batch, mask=mask.detach()).requires_grad

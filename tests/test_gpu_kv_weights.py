@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from kv_plans import plan_of
-from test_gpu_kv import DEV, MANY, ROUND, TYPES, World
+from test_gpu_kv import DEV, MANY, ROUND, TYPES, World, bound
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,40 @@ def test_tiles_of_16_rows_are_split(backend, dtype, rows, group, dim, window):
     kernel = plan_of(w.cache, w.batch(news), group, dtype, window=window)
     assert kernel.tile_rows == 16 and kernel.row_tiles > 1 and kernel.splits > 1
     w.check(news, dtype, group, **({} if window is None else {"window": window}))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("mask_dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,idle,dim", [(2, 0, 64), (50, MANY, 64), (50, MANY, 128), (20, 0, 200)])
+@pytest.mark.parametrize("heads_apart", [False, True])
+def test_the_lowest_value_hides_as_minus_infinity_does(backend, dtype, mask_dtype, rows, idle, dim, heads_apart):
+    """Within the bound of the same call without a mask: tokens at the type's lowest
+    value have no weight where a row has others; where it has none, what it sees
+    weighs the same."""
+    lengths = [100, 61]
+    w = World(backend, lengths=lengths, heads=2, dim=dim, page=16, seed=35, idle=idle)
+    w.append(lengths, dtype)
+    news = [rows, rows]
+    q = torch.randn((2 * rows, 4, dim), generator=w.gen).to(dtype)
+    low = torch.rand((2 * rows, 4 if heads_apart else 1, 100), generator=w.gen) < 0.4
+    low[1::4] = True
+    low[3::8] = False
+    kernel = plan_of(w.cache, w.batch(news), 4, dtype, masked=True)
+    assert kernel.tile_rows == (128 if idle else 16)
+    mask = torch.where(low, torch.finfo(mask_dtype).min, 0.0).to(mask_dtype)
+    got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch(news), mask=mask.to(DEV)).cpu().double()
+    out, spread, reach = w.want(q, news, mask=~low)
+    at = 0
+    for i, n in enumerate(lengths):
+        k, _ = w.k.values(w.table[i], n)
+        v, _ = w.v.values(w.table[i], n)
+        v = v.repeat_interleave(2, dim=1)
+        for r in range(rows):
+            seen = n - rows + r + 1
+            full = low[at + r].expand(4, 100)[:, :seen].all(dim=1)  # heads whose tokens are all at the lowest
+            out[at + r, full] = v[:seen].mean(dim=0)[full]
+            spread[at + r, full] = v[:seen].abs().mean(dim=0)[full]
+            reach[at + r, full] = 0.0
+        at += rows
+    most = bound(dtype, out, spread, reach, dim, 100, None)
+    assert ((got - out).abs() <= most).all(), f"off by {float(((got - out).abs() / most).max()):.3g} of the bound"

@@ -531,7 +531,9 @@ int32_t rnsmx_kv_row_bytes(int32_t head_dim);
  *   scale = max(max|x| * fl32(1/127), 2^-23), code = clamp(rint(x / scale), +-127)
  * over its new tokens, in float32.  A page that held tokens of the sequence
  * before keeps the larger of its scale and the new tokens'; where that is
- * larger than its own its older codes are quantised again, from code * scale.
+ * larger than its own its older codes are quantised again, from code * scale.  A
+ * scale grows until the page's first token is written anew: one that was appended
+ * and is taken back leaves it as it made it.
  * A value that is not finite makes the scale of its page and head so: every
  * value there reads as NaN.  Rows of one call must not share a page with
  * another sequence's.

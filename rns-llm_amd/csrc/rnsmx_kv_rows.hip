@@ -23,8 +23,8 @@ __device__ __forceinline__ f32x4 kv_mfma(h16x8 a, h16x8 b, f32x4 c) {
 //   w = 2^(x - mx + lv - ml),  O += w code,  l += w / value scale = 2^(x - mx - ml)
 // where x is the product in powers of two and (mx, ml) a row's reference.
 // Bound by memory where codes are many: 62 sequences of up to 4096 tokens, 32 heads of
-// 128 (1181 MB) in 192 to 203 us, 5.8 to 6.2 TB/s, one row of 8 heads over 131071 tokens (268
-// MB) in 51 to 57, its waves waiting 46 to 48 % of their time.  The 16 rows cost what
+// 128 (1181 MB) in 189 to 202 us, 5.8 to 6.2 TB/s, one row of 8 heads over 131071 tokens (268
+// MB) in 50 to 57, its waves waiting 46 to 48 % of their time.  The 16 rows cost what
 // one does, as a product of 16 x 16 has no smaller form, so grouped heads and drafted
 // tokens come for nothing.  Codes are loaded from memory into the operands' places,
 // without a pass through shared memory: no wave reads what another does.  Small calls

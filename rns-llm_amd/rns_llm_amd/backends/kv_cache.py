@@ -231,7 +231,8 @@ class KVCacheOps:
         2**-23)`` over its new tokens, ``code = clamp(round(x / scale), ±127)``,
         in float32.  A page that held tokens of the sequence before keeps the
         larger of its scale and the new tokens'; where that is larger than its
-        own, its older codes are quantised again from the values they stood for.
+        own, its older codes are quantised again from the values they stood for;
+        a token that is taken back leaves its page's scale as it made it.
         A value that is not finite makes every value of its page and head read
         as NaN.  Sequences of one call must not share pages that it writes to.  No
         gradient goes through the cache."""

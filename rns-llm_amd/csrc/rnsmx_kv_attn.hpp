@@ -45,6 +45,19 @@ constexpr float kKvBelow = 10.0f, kKvAbove = 15.75f;
 // products again (decode 200 us to 214, one token of 131072 56.8 to 58.8, a prompt
 // of 2048 71 to 92); float32 queries have it.
 //
+// A weight's exponent is fma(product, page's factor, page's part - reference): the
+// product is not rounded, its row's largest was when it became the reference, and
+// past 2^27 that half of a last place alone takes a weight past float16.  Rows whose
+// reference has 2^20 (a last place of 2^-3) and more take the product as the reference
+// had it, rounded, and the difference before the page's part.
+constexpr float kKvFar = 1048576.0f;
+__device__ __forceinline__ bool kv_far(float reference) { return fabsf(reference) >= kKvFar && reference > -INFINITY; }
+__device__ __forceinline__ float kv_apart(float product, float factor, float reference) {
+  float x = product * factor;
+  asm("" : "+v"(x));  // kept from joining the subtraction
+  return x - reference;
+}
+
 // Float32 calls have weights in two halves: h, and what is left of w times 2^11,
 // as large as h was, against codes times 2^-11, which float16 holds exactly (code
 // 2^-20).  22 bits down to 2^-24 of the largest, 11 down to 2^-35; at the same
@@ -220,14 +233,15 @@ __device__ __forceinline__ uint32_t kv_between(int32_t t, int32_t begin, int32_t
 
 // One candidate (x, lv) for a row's reference against another, e and e2 being
 // how far each lies above the present one: of those that pass kKvAbove the one
-// with the larger sum, of equals the larger x, then the larger lv, so that lanes
-// that exchange theirs take the same one.
+// with the larger sum, by the differences, as sums lose what is less than a last
+// place of x; of equals the larger x, then the larger lv, so that lanes that exchange
+// theirs take the same one.
 template <bool MASK>
 __device__ __forceinline__ void kv_higher(float &e, float &x, float &lv, float e2, float x2, float lv2) {
   constexpr float kNat = MASK ? kKvLog2e : 1.0f;
-  const float s1 = x * kNat + lv, s2 = x2 * kNat + lv2;
+  const float more = (x2 - x) * kNat + (lv2 - lv);
   const bool take = !(e > kKvAbove) ? e2 > kKvAbove
-                                    : (e2 > kKvAbove && (s2 > s1 || (s2 == s1 && (x2 > x || (x2 == x && lv2 > lv)))));
+                                    : (e2 > kKvAbove && (more > 0.0f || (more == 0.0f && (x2 > x || (x2 == x && lv2 > lv)))));
   e = take ? e2 : e;
   x = take ? x2 : x;
   lv = take ? lv2 : lv;
@@ -239,8 +253,9 @@ __device__ __forceinline__ void kv_higher(float &e, float &x, float &lv, float e
 template <bool MASK>
 __device__ __forceinline__ void kv_reference(float &mx, float &ml, float mx2, float ml2) {
   constexpr float kNat = MASK ? kKvLog2e : 1.0f;
-  const float s1 = mx * kNat + ml, s2 = mx2 * kNat + ml2;
-  const bool take = mx2 > -INFINITY && (!(mx > -INFINITY) || s2 > s1 || (s2 == s1 && (mx2 > mx || (mx2 == mx && ml2 > ml))));
+  const float more = (mx2 - mx) * kNat + (ml2 - ml);
+  const bool take =
+      mx2 > -INFINITY && (!(mx > -INFINITY) || more > 0.0f || (more == 0.0f && (mx2 > mx || (mx2 == mx && ml2 > ml))));
   mx = take ? mx2 : mx;
   ml = take ? ml2 : ml;
 }

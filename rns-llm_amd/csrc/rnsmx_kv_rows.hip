@@ -215,7 +215,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
     kv_for<7>([&](auto J) { xm = fmaxf(xm, w[J + 1]); });
     if constexpr (!MASK) xm *= c;
     const float em = (xm - mx) * kNat + (lv - ml);
-    if (__any(em > kKvAbove)) {
+    bool apart = false;
+    if (__any(em > kKvAbove || (!MASK && kv_far(mx)))) {
       float best = em, bx = xm, bl = lv;
       kv_for<2>([&](auto I) {
         constexpr int step = 16 << I;
@@ -229,9 +230,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
         mx = bx;
         ml = nl;
       }
+      if constexpr (!MASK) {
+        apart = __any(kv_far(mx));
+        if (apart) {
+          kv_for<8>([&](auto J) { w[J] = kv_apart(w[J], c, mx == -INFINITY ? 0.0f : mx); });
+          c = 1.0f;
+        }
+      }
     }
     // a row without a reference has nothing but minus infinities (and not-a-numbers) so far
-    const float ref = mx == -INFINITY ? 0.0f : mx, off = MASK ? lv - ml : lv - ml - ref;
+    const float ref = apart || mx == -INFINITY ? 0.0f : mx, off = MASK ? lv - ml : lv - ml - ref;
     float part = 0.0f;
     kv_for<8>([&](auto J) {
       constexpr int j = J;

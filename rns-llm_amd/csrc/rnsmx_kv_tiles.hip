@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
       if constexpr (!MASK) xm[g] *= c[g];
     });
     float em[4];
-    bool above = false;
+    bool above = !MASK && kv_far(mx), apart = false;
     kv_for<4>([&](auto G) {
       constexpr int g = G;
       em[g] = (xm[g] - mx) * kNat + (lv[g] - ml);
@@ -274,12 +274,21 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
         mx = bx;
         ml = nl;
       }
+      if constexpr (!MASK) {
+        apart = __any(kv_far(mx));
+        if (apart)
+          kv_for<4>([&](auto G) {
+            constexpr int g = G;
+            kv_for<8>([&](auto J) { w[g][J] = kv_apart(w[g][J], c[g], mx == -INFINITY ? 0.0f : mx); });
+            c[g] = 1.0f;
+          });
+      }
     }
     // A group's weights, then its products, whose time on the matrix cores the
     // next group's weights fill (and the next step's codes after the last).
     // A row without a reference has nothing but minus infinities (and
     // not-a-numbers) so far.
-    const float ref = mx == -INFINITY ? 0.0f : mx;
+    const float ref = apart || mx == -INFINITY ? 0.0f : mx;
     kv_for<4>([&](auto G) {
       constexpr int g = G;
       const float off = MASK ? lv[g] - ml : lv[g] - ml - ref;

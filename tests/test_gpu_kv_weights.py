@@ -100,3 +100,42 @@ def test_the_lowest_value_hides_as_minus_infinity_does(backend, dtype, mask_dtyp
         at += rows
     most = bound(dtype, out, spread, reach, dim, 100, None)
     assert ((got - out).abs() <= most).all(), f"off by {float(((got - out).abs() / most).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 13, 2.0 ** 15, 2.0 ** 30])
+@pytest.mark.parametrize("lengths,rows,dim,idle,masked", [
+    ([300, 70], 1, 64, 0, False), ([300, 70], 3, 128, 0, True), ([4100, 1], 1, 128, 0, False), ([300, 70], 70, 64, MANY, False),
+    ([300, 170], 170, 128, MANY, False), ([300, 70], 70, 128, MANY, True), ([1100, 700], 20, 256, 0, False),
+])
+def test_scores_of_any_size(backend, dtype, size, lengths, rows, dim, idle, masked):
+    """Scores of 2^16 to 2^60, each one that float32 holds: a row's result is the
+    value of its largest, which is ahead of the next by far."""
+    w = World(backend, lengths=lengths, heads=2, dim=dim, page=16, seed=41, idle=idle)
+    total = sum(lengths)
+    k, v = (torch.randn((total, 2, dim), generator=w.gen) for _ in range(2))
+    v = v * 2.0 ** torch.randint(-9, 9, (total, 1, 1), generator=w.gen)  # pages of different scales
+    w.append(lengths, torch.float32, k=size * k, v=v)
+    news = [min(rows, n) for n in lengths]
+    q = (size * torch.randn((sum(news), 4, dim), generator=w.gen)).to(dtype)
+    mask = torch.zeros((1, 1, max(lengths))) if masked else None
+    got = w.backend.kv_attention(q.to(DEV), w.cache, w.batch(news), mask=None if mask is None else mask.to(DEV)).cpu().double()
+    assert got.isfinite().all()
+    at, checked = 0, 0
+    for i, (n, m) in enumerate(zip(lengths, news)):
+        kk, _ = w.k.values(w.table[i], n)
+        vv, _ = w.v.values(w.table[i], n)
+        for r in range(0, m, max(1, m // 7)):
+            for h in range(4):
+                seen = n - m + r + 1
+                x = kk[:seen, h // 2] @ q[at + r, h].double() / math.sqrt(dim)
+                top = x.sort(descending=True)
+                # as far ahead as the scores' own roundings, and 64 for the next to have no weight
+                if seen > 1 and top.values[0] - top.values[1] < 64 + 2.0 ** -18 * x.abs().max():
+                    continue
+                want = vv[int(top.indices[0]), h // 2]
+                most = ROUND[dtype] * want.abs() + 2.0 ** (-20 if dtype == torch.float32 else -10) * want.abs().max()
+                assert ((got[at + r, h] - want).abs() <= most).all(), (i, r, h)
+                checked += 1
+        at += m
+    assert checked

@@ -48,10 +48,10 @@ constexpr float kKvBelow = 10.0f, kKvAbove = 15.75f;
 // A weight's exponent is fma(product, page's factor, page's part - reference): the
 // product is not rounded, its row's largest was when it became the reference, and
 // past 2^27 that half of a last place alone takes a weight past float16.  Rows whose
-// reference has 2^20 (a last place of 2^-3) and more take the product as the reference
-// had it, rounded, and the difference before the page's part.
+// reference has 2^20 (a last place of 2^-3) and more, and a wave's others with them,
+// take the product as the reference had it, rounded, and the difference before the
+// page's part.
 constexpr float kKvFar = 1048576.0f;
-__device__ __forceinline__ bool kv_far(float reference) { return fabsf(reference) >= kKvFar && reference > -INFINITY; }
 __device__ __forceinline__ float kv_apart(float product, float factor, float reference) {
   float x = product * factor;
   asm("" : "+v"(x));  // kept from joining the subtraction

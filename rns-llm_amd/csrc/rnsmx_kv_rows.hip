@@ -176,6 +176,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
   kv_for<VW>([&](auto I) { o[I] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; });
   // the row's reference, and its weights over the value scales, in units of 2^-ml
   float mx = -INFINITY, ml = 0.0f, sum = 0.0f;
+  // what its products are less: mx; 0 of a row without a reference, which has nothing
+  // but minus infinities (and not-a-numbers) so far, and of a wave that has far ones.
+  // Kept from step to step, but in masked calls, which lack the register.
+  float held = 0.0f;
+  uint64_t far = 0;
 
   auto compute = [&](const Step &s, int32_t t0) {
     f32x4 acc[2];
@@ -215,8 +220,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
     kv_for<7>([&](auto J) { xm = fmaxf(xm, w[J + 1]); });
     if constexpr (!MASK) xm *= c;
     const float em = (xm - mx) * kNat + (lv - ml);
-    bool apart = false;
-    if (__any(em > kKvAbove || (!MASK && kv_far(mx)))) {
+    if ((__ballot(em > kKvAbove) | far) != 0) {
       float best = em, bx = xm, bl = lv;
       kv_for<2>([&](auto I) {
         constexpr int step = 16 << I;
@@ -231,15 +235,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DT <= 160 ? 2 : 1) void kv_rows
         ml = nl;
       }
       if constexpr (!MASK) {
-        apart = __any(kv_far(mx));
-        if (apart) {
-          kv_for<8>([&](auto J) { w[J] = kv_apart(w[J], c, mx == -INFINITY ? 0.0f : mx); });
+        held = mx == -INFINITY ? 0.0f : mx;
+        far |= __ballot(fabsf(held) >= kKvFar);
+        if (far != 0) {
+          kv_for<8>([&](auto J) { w[J] = kv_apart(w[J], c, held); });
           c = 1.0f;
+          held = 0.0f;
         }
       }
     }
-    // a row without a reference has nothing but minus infinities (and not-a-numbers) so far
-    const float ref = apart || mx == -INFINITY ? 0.0f : mx, off = MASK ? lv - ml : lv - ml - ref;
+    const float ref = !MASK ? held : mx == -INFINITY ? 0.0f : mx, off = MASK ? lv - ml : lv - ml - ref;
     float part = 0.0f;
     kv_for<8>([&](auto J) {
       constexpr int j = J;

@@ -201,6 +201,9 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
   kv_for<DB>([&](auto I) { kv_for<16>([&](auto J) { o[I][static_cast<int>(J)] = 0.0f; }); });
   // the row's reference and its weights' sum over the value scale, in units of 2^ml
   float mx = -INFINITY, ml = 0.0f, sum = 0.0f;
+  // what its products are less (kv_rows_kernel has which)
+  float held = 0.0f;
+  uint64_t far = 0;
   constexpr float kNat = MASK ? kKvLog2e : 1.0f;
 
   auto compute = [&](int32_t buf, int32_t t0) {
@@ -256,13 +259,13 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
       if constexpr (!MASK) xm[g] *= c[g];
     });
     float em[4];
-    bool above = !MASK && kv_far(mx), apart = false;
+    bool above = false;
     kv_for<4>([&](auto G) {
       constexpr int g = G;
       em[g] = (xm[g] - mx) * kNat + (lv[g] - ml);
       above |= em[g] > kKvAbove;
     });
-    if (__any(above)) {
+    if ((__ballot(above) | far) != 0) {
       float best = em[0], bx = xm[0], bl = lv[0];
       kv_for<3>([&](auto G) { kv_higher<MASK>(best, bx, bl, em[G + 1], xm[G + 1], lv[G + 1]); });
       kv_higher<MASK>(best, bx, bl, __shfl_xor(best, 32), __shfl_xor(bx, 32), __shfl_xor(bl, 32));
@@ -275,20 +278,21 @@ __global__ __launch_bounds__(256 * HALVES, (DT <= 128 ? 2 : 1)) void kv_tiles_ke
         ml = nl;
       }
       if constexpr (!MASK) {
-        apart = __any(kv_far(mx));
-        if (apart)
+        held = mx == -INFINITY ? 0.0f : mx;
+        far |= __ballot(fabsf(held) >= kKvFar);
+        if (far != 0) {
           kv_for<4>([&](auto G) {
             constexpr int g = G;
-            kv_for<8>([&](auto J) { w[g][J] = kv_apart(w[g][J], c[g], mx == -INFINITY ? 0.0f : mx); });
+            kv_for<8>([&](auto J) { w[g][J] = kv_apart(w[g][J], c[g], held); });
             c[g] = 1.0f;
           });
+          held = 0.0f;
+        }
       }
     }
     // A group's weights, then its products, whose time on the matrix cores the
     // next group's weights fill (and the next step's codes after the last).
-    // A row without a reference has nothing but minus infinities (and
-    // not-a-numbers) so far.
-    const float ref = apart || mx == -INFINITY ? 0.0f : mx;
+    const float ref = !MASK ? held : mx == -INFINITY ? 0.0f : mx;
     kv_for<4>([&](auto G) {
       constexpr int g = G;
       const float off = MASK ? lv[g] - ml : lv[g] - ml - ref;

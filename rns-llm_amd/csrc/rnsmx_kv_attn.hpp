@@ -35,8 +35,8 @@ constexpr float kKvLog2e = 1.44269504088896340736f;
 // What is far below the largest matters where that has small values: 4095 tokens
 // 16 below one whose codes are zero come out within 1e-3 of themselves so, and
 // with the largest at 2^4 (limit 2^12) within 8e-2.  The room above decides how
-// often rows are rescaled: one prompt of 2048, 32 heads of 128, takes 67.8 us with
-// 8 of it, 68.6 so, 71.2 with 4.
+// often rows are rescaled: one prompt of 2048, 32 heads of 128, in short runs takes
+// 67.8 us with 8 of it, 68.6 so, 71.2 with 4.
 constexpr float kKvBelow = 10.0f, kKvAbove = 15.75f;
 
 // 16-bit calls round their weights to float16's 11 bits, three more than bfloat16

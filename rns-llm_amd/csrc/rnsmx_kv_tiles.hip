@@ -36,7 +36,7 @@ __device__ __forceinline__ int32_t value_swap(int32_t d) { return (d & 7) ^ (d >
 // 32 x 32 products: a row is one lane pair's.
 //
 // Bound by what surrounds the products (weights, conversions, waits) more than by
-// them: at 8192 tokens, 32 heads of 128 (550 GFLOP) 630 to 680 us, 0.81 to 0.87 PFLOP/s of the 1.23
+// them: at 8192 tokens, 32 heads of 128 (550 GFLOP) 630 to 700 us, 0.79 to 0.87 PFLOP/s of the 1.23
 // that a large library product reaches here, vector units busy half of the time, matrix
 // units and shared memory a third each.  2048 tokens, 32 heads (34 GFLOP) take 62 to 70
 // us: 512 tiles go in one round, so the longest chain decides, 32 steps of some 4200

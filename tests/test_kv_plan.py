@@ -73,7 +73,7 @@ def test_rules(sizes, options, want):
     ((5 + MANY, 1, 1, 129, 256, 192), {"page": 128}, False), ((5 + MANY, 1, 1, 129, 192, 256), {"page": 32}, False),
     ((20, 1, 1, 640, 3008, 64), {}, True), ((10, 2, 4, 300, 2624, 40), {"page": 64}, True),
     ((7, 1, 3, 600, 3008, 128), {"page": 32}, True), ((20, 1, 1, 640, 3008, 160), {}, True),
-    ((10, 1, 2, 640, 3072, 250), {"page": 128}, True), ((150, 8, 8, 68, 160, 64), {"page": 32}, False),
+    ((10, 1, 2, 640, 3008, 250), {"page": 64}, True), ((150, 8, 8, 68, 160, 64), {"page": 32}, False),
     ((4 + MANY, 2, 4, 77, 160, 64), {"page": 32, "masked": True}, False),
     ((4 + MANY, 2, 4, 40, 160, 128), {"masked": True}, False), ((4 + MANY, 2, 4, 40, 160, 128), {"window": 30}, False),
     ((3 + MANY, 2, 4, 33, 144, 64), {"masked": True}, False), ((2 + MANY, 2, 4, 60, 208, 72), {"masked": True}, False),

@@ -610,6 +610,143 @@ int32_t rnsmx_kv_attention(const rnsmx_kv_cache_t *cache, const rnsmx_kv_batch_t
                            const void *mask_dev, void *workspace_dev,
                            int64_t workspace_bytes, void *out_dev, void *stream);
 
+/*
+ * Pages handed out on the device.  seqs sequences, each with a row of `width`
+ * page numbers (-1 past its pages) and a length; a page is held by any number of
+ * sequences.  Everything lies on the device and is changed there, so a captured
+ * step hands out pages on each replay.  Calls on one pool follow each other on one
+ * stream (or are ordered by events).  No counterpart in the reference.
+ */
+typedef struct rnsmx_kv_pool {
+  int32_t *table_dev;   /* [seqs][width], -1 where there is no page           */
+  int32_t *lengths_dev; /* [seqs] tokens                                      */
+  int32_t *refs_dev;    /* [blocks] holders of each page                      */
+  uint32_t *free_dev;   /* [(blocks + 31) / 32] bit b % 32 of word b / 32: nobody holds b */
+  int32_t *scratch_dev; /* rnsmx_kv_pool_scratch_words: [blocks] of 0, [blocks] of 2^31 - 1, the
+                           rest of any value; every call leaves them so          */
+  int32_t blocks;
+  int32_t page;         /* tokens a page: 16, 32, 64 or 128                    */
+  int32_t seqs;
+  int32_t width;        /* pages a sequence may have, of 2^30 tokens at most   */
+} rnsmx_kv_pool_t;
+
+/* Host only.  32-bit words of scratch_dev; -1 for sizes that no pool has. */
+int64_t rnsmx_kv_pool_scratch_words(int32_t blocks, int32_t seqs, int32_t width);
+
+/* What rnsmx_kv_assign writes for the calls of a step: its rnsmx_kv_batch_t has
+ * the pool's table, lengths_dev and starts_dev. */
+typedef struct rnsmx_kv_step {
+  int32_t *lengths_dev; /* [seqs] tokens with the new ones; 0 of a sequence that has none new */
+  int32_t *starts_dev;  /* [seqs + 1] its rows; null: one row a sequence, which has 0 or 1 new */
+  int32_t *copies_dev;  /* [seqs][3] page copied, page it is copied to, tokens; -1, -1, 0: none */
+  int32_t *missing_dev; /* [1] 0, pages that the pool lacks, or -1, -2 (below) */
+  int32_t rows;         /* most rows of the call                              */
+  int32_t max_rows;     /* most new tokens of a sequence                      */
+  int32_t max_length;   /* most tokens of a sequence                          */
+} rnsmx_kv_step_t;
+
+/*
+ * Gives every sequence pages for its new tokens (new_dev [seqs], cut to 0 and
+ * max_rows; null: one each) and adds them to its length.  Pages are the lowest that
+ * nobody holds, given to the sequences in their order and to a sequence in its
+ * columns' order.  A page that is partly filled, goes on being filled and is held by
+ * others is replaced by a page of the sequence's own, copied by rnsmx_kv_copy; where
+ * all its holders go on in it, the first of them keeps it.  A call that lacks pages
+ * (*missing_dev: how many), has a sequence that passes its table's row or max_length (-1)
+ * or more rows than the step (-2, whatever else) changes nothing in the pool, and its step
+ * has no tokens (lengths 0).
+ */
+int32_t rnsmx_kv_assign(const rnsmx_kv_pool_t *pool, const rnsmx_kv_step_t *step,
+                        const int32_t *new_dev, void *stream);
+
+/* Cuts every sequence to lengths_dev [seqs] tokens (one that has no more stays as it
+ * is; below 0 is 0) and lets go of the pages past them. */
+int32_t rnsmx_kv_trim(const rnsmx_kv_pool_t *pool, const int32_t *lengths_dev, void *stream);
+
+/* Every sequence s becomes what sequence parents_dev[s] was, whose pages it holds
+ * too; empty where that is none of the pool's. */
+int32_t rnsmx_kv_reorder(const rnsmx_kv_pool_t *pool, const int32_t *parents_dev, void *stream);
+
+/* Where a batch's rows lie (pages of `page` tokens, numbers below `blocks`):
+ * positions_dev [rows] of their tokens in their sequences and slots_dev [rows] = page
+ * number * page + place in the page.  A row without a token (of no sequence, or before
+ * its sequence's first) is at position 0, slot -1; one whose token is dropped or whose
+ * page is not there has slot -1. */
+int32_t rnsmx_kv_slots(const rnsmx_kv_batch_t *batch, int32_t blocks, int32_t page,
+                       int32_t *positions_dev, int64_t *slots_dev, void *stream);
+
+/* Copies the first tokens of pages, keys, values and scales of all heads:
+ * copies_dev [count][3], page copied, page it is copied to, tokens.  One whose
+ * numbers are no page's copies nothing.  No page is copied to twice, or to and from. */
+int32_t rnsmx_kv_copy(const rnsmx_kv_cache_t *cache, const int32_t *copies_dev, int32_t count, void *stream);
+
+/*
+ * Rotary positions: of each head of head_dim values the first 2 pairs, as pairs
+ * (i, i + pairs) or, interleaved, (2 i, 2 i + 1).  A pair (u, v) at position p becomes
+ *   magnitude (u cos t - v sin t), magnitude (v cos t + u sin t),
+ *   t = 2 pi p steps_dev[i] / 2^64,
+ * the fraction of a turn being exact in 64 bits; the values past them stay.
+ */
+#define RNSMX_ROTARY_MAX_DIM 1024
+#define RNSMX_ROTARY_MAX_HEADS 4096
+typedef struct rnsmx_rotary {
+  const uint64_t *steps_dev; /* [pairs] turns a position, in 2^-64 of one     */
+  int32_t pairs;
+  int32_t interleaved;
+  float magnitude;
+} rnsmx_rotary_t;
+
+typedef struct rnsmx_rotary_rows {
+  int64_t rows;
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride; /* elements */
+  int64_t q_out_row_stride, q_out_head_stride, k_out_row_stride, k_out_head_stride;
+  int32_t q_heads, k_heads; /* either may be 0, its pointers are not read then */
+  int32_t head_dim;
+  int32_t dtype;           /* FLOAT32, FLOAT16, BFLOAT16                       */
+  int32_t positions_dtype; /* INT32, INT64                                     */
+  int32_t back;            /* 1: by the angles' negatives (the gradient)       */
+} rnsmx_rotary_rows_t;
+
+/* Turns queries and keys [rows][heads][head_dim] by positions_dev [rows], in float32,
+ * rounded once.  An output is its input (the same pointer and strides) or shares no
+ * memory with either; no value of an output is another's. */
+int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *rows,
+                     const void *positions_dev, const void *q_dev, const void *k_dev,
+                     void *q_out_dev, void *k_out_dev, void *stream);
+
+/*
+ * Beam search's selection: for each request the k best continuations of its beams,
+ *   score(b, v) = scores[b] + (x[v] - log sum_u exp x[u]),  x the logits of beam b,
+ * compared in 64 bits; of equal ones the lower beam's go first, within a beam the
+ * larger logit, then the lower token.  A finished beam goes on as it is, once, with
+ * end_token; its logits are not read.  What is not finite is no candidate, and a beam
+ * whose logits hold a not-a-number or plus infinity, or nothing above minus infinity,
+ * has none.  A place without a candidate has score minus infinity, end_token
+ * (0 where that is negative) and its own beam (its number modulo beams) as its parent.
+ */
+#define RNSMX_BEAMS_MAX 64
+typedef struct rnsmx_beams {
+  int64_t request_stride, beam_stride; /* of the logits, elements           */
+  int32_t dtype;                       /* FLOAT32, FLOAT16, BFLOAT16         */
+  int32_t requests, beams, vocabulary; /* beams, k: 1 to RNSMX_BEAMS_MAX     */
+  int32_t k;
+  int32_t end_token;
+} rnsmx_beams_t;
+
+/* Bytes of workspace; -1 for sizes that rnsmx_beam_select refuses.  Its first
+ * RNSMX_KV_TICKETS 32-bit counters are those of the key/value attention: zero when it is
+ * first used, and every call leaves them zero. */
+int64_t rnsmx_beam_workspace_bytes(const rnsmx_beams_t *beams);
+
+/* logits_dev [requests][beams][vocabulary], scores_dev [requests][beams],
+ * finished_dev the same in bytes (null: none) -> [requests][k] each: scores, tokens and
+ * parents, a parent being request * beams + beam. */
+int32_t rnsmx_beam_select(const rnsmx_beams_t *beams, const void *logits_dev,
+                          const float *scores_dev, const uint8_t *finished_dev,
+                          void *workspace_dev, int64_t workspace_bytes,
+                          float *out_scores_dev, int32_t *out_tokens_dev,
+                          int32_t *out_parents_dev, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,545 @@
+// Pages handed out on the device: block tables, reference counts and slot maps
+// of sequences that grow, shrink and share, and copies of shared pages.
+#include <algorithm>
+#include <climits>
+
+#include "rnsmx_kv.hpp"
+
+namespace rnsmx {
+
+struct PoolArgs {
+  int32_t *table, *lengths, *refs;
+  uint32_t *free;               // a bit a page that nobody holds
+  int32_t *going, *first;       // scratch, [blocks] each: zeros and INT32_MAX between calls
+  int32_t *spare, *spare_lengths;  // scratch of kv_reorder: a table and lengths
+  int32_t blocks, words, log_page, seqs, width;
+};
+
+struct AssignArgs {
+  PoolArgs p;
+  const int32_t *asked;  // new tokens of each sequence; null: one each
+  int32_t *seen, *starts, *copies, *missing;
+  int32_t rows, max_rows, max_length;
+};
+
+__device__ __forceinline__ int32_t pool_pages(const PoolArgs &p, int32_t n) {  // that n tokens lie in
+  return static_cast<int32_t>((static_cast<uint32_t>(n) + (1u << p.log_page) - 1u) >> p.log_page);
+}
+__device__ __forceinline__ bool pool_has(const PoolArgs &p, int32_t page) {
+  return static_cast<uint32_t>(page) < static_cast<uint32_t>(p.blocks);
+}
+// A holder less; a page without one is free.
+__device__ __forceinline__ void pool_drop(const PoolArgs &p, int32_t page) {
+  if (!pool_has(p, page)) return;
+  if (__hip_atomic_fetch_add(p.refs + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 1)
+    __hip_atomic_fetch_or(p.free + (page >> 5), 1u << (page & 31), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Sums of N values a thread over the threads before it, and over all.
+template <int N>
+__device__ __forceinline__ void pool_scan(int64_t (&before)[N], int64_t (&all)[N], int64_t (*wave)[N]) {
+  const int32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  int64_t sum[N];
+  kv_for<N>([&](auto K) { sum[K] = before[K]; });
+  kv_for<6>([&](auto I) {
+    constexpr int step = 1 << I;
+    kv_for<N>([&](auto K) {
+      const int64_t other = __shfl_up(static_cast<long long>(sum[K]), step);
+      if (lane >= step) sum[K] += other;
+    });
+  });
+  __syncthreads();
+  if (lane == 63) kv_for<N>([&](auto K) { wave[w][K] = sum[K]; });
+  __syncthreads();
+  kv_for<N>([&](auto K) {
+    int64_t past = 0, total = 0;
+    for (int32_t i = 0; i < waves; ++i) {
+      const int64_t v = wave[i][K];
+      past += i < w ? v : 0;
+      total += v;
+    }
+    before[K] = past + sum[K] - before[K];
+    all[K] = total;
+  });
+}
+
+constexpr int32_t kPoolPicked = 12288;  // page numbers of a round, 48 KB
+constexpr int32_t kPoolOwn = 2;         // pages of a sequence that its thread enters, a wave together the others
+constexpr int32_t kPoolMost = INT_MAX;
+
+// One workgroup for a call, as the pages of every sequence depend on those of all
+// before it.  What a call needs is counted before anything is changed, so one that
+// the pool has no room for changes nothing.
+// Bound by its chain: lengths, tails' entries and counts, a sum over the workgroup,
+// page numbers through shared memory into the tables.
+__global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
+  __shared__ int32_t picked[kPoolPicked];
+  __shared__ int64_t sums[16][3];
+  __shared__ int32_t any, past;
+  const PoolArgs &p = a.p;
+  const int32_t threads = blockDim.x, tid = threadIdx.x, lane = tid & 63;
+  const int32_t page = 1 << p.log_page, room = min(p.width << p.log_page, a.max_length);
+  const bool once = p.seqs <= threads;  // a sequence a thread, kept in registers
+
+  struct Info {
+    int32_t seq, old, n, inside;  // tokens held, new, and of the held ones those on the last page
+    int32_t source;               // the page copied, -1: none
+    int32_t begin, need;          // pages wanted from column `begin` on
+    int32_t rank;                 // the first of them among all
+  };
+  auto held = [&](int32_t s) {
+    Info i{s, 0, 0, 0, -1, 0, 0, 0};
+    if (s < p.seqs) {
+      i.old = min(max(p.lengths[s], 0), p.width << p.log_page);
+      i.n = min(a.asked ? max(a.asked[s], 0) : 1, a.max_rows);
+      i.inside = i.old & (page - 1);
+    }
+    return i;
+  };
+  // its last page where it goes on in it and others hold it too
+  auto tail_of = [&](const Info &i) {
+    if (i.n == 0 || i.inside == 0) return -1;
+    const int32_t t = p.table[static_cast<int64_t>(i.seq) * p.width + (i.old >> p.log_page)];
+    return pool_has(p, t) && p.refs[t] > 1 ? t : -1;
+  };
+  auto want = [&](Info &i) {
+    i.begin = pool_pages(p, i.old) - (i.source >= 0 ? 1 : 0);
+    i.need = i.n > 0 && i.n <= room - i.old ? pool_pages(p, i.old + i.n) - i.begin : 0;
+  };
+
+  // this thread's words of the free pages
+  const int32_t each = (p.words + threads - 1) / threads;
+  const int32_t word0 = min(tid * each, p.words), word1 = min(word0 + each, p.words);
+  if (tid == 0) any = past = 0;
+  __syncthreads();
+  Info mine{};
+  for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
+    mine = held(s0 + tid);
+    mine.source = tail_of(mine);
+    if (mine.n > 0 && mine.n > room - mine.old) past = 1;
+    if (mine.source >= 0) {
+      any = 1;
+      __hip_atomic_fetch_add(p.going + mine.source, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_fetch_min(p.first + mine.source, mine.seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  int64_t wanted = 0, rows = 0, free_before = 0, free_all = 0;
+  for (int32_t w = word0; w < word1; ++w) free_before += __popc(p.free[w]);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  const bool shared = any != 0;
+  for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
+    if (!once) {
+      mine = held(s0 + tid);
+      mine.source = tail_of(mine);
+    }
+    if (shared && mine.source >= 0) {
+      // the first of a page's holders keeps it if all of them go on
+      const int32_t going = __hip_atomic_load(p.going + mine.source, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int32_t first = __hip_atomic_load(p.first + mine.source, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (going == p.refs[mine.source] && first == mine.seq) mine.source = -1;
+    }
+    want(mine);
+    int64_t before[3] = {mine.need, mine.n, s0 == 0 ? free_before : 0}, total[3];
+    pool_scan(before, total, sums);
+    if (s0 == 0) {
+      free_before = before[2];
+      free_all = total[2];
+    }
+    mine.rank = static_cast<int32_t>(min(wanted + before[0], static_cast<int64_t>(kPoolMost)));
+    if (mine.seq < p.seqs) {
+      if (a.starts) a.starts[mine.seq] = static_cast<int32_t>(min(rows + before[1], static_cast<int64_t>(kPoolMost)));
+      if (!once) {  // what was settled waits in the outputs
+        int32_t *c = a.copies + 3 * static_cast<int64_t>(mine.seq);
+        c[0] = mine.source;
+        c[1] = mine.rank;
+      }
+    }
+    wanted += total[0];
+    rows += total[1];
+  }
+  const int32_t missing = rows > a.rows ? -2
+                          : past != 0   ? -1
+                                        : static_cast<int32_t>(min(max(wanted - free_all, static_cast<int64_t>(0)), static_cast<int64_t>(kPoolMost)));
+  if (tid == 0) {
+    if (a.starts) a.starts[p.seqs] = static_cast<int32_t>(min(rows, static_cast<int64_t>(kPoolMost)));
+    *a.missing = missing;
+  }
+  __syncthreads();  // marks and counts are read by all before they change
+  if (shared)
+    for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
+      const Info i = held(s0 + tid);
+      const int32_t t = tail_of(i);
+      if (t >= 0) {
+        p.going[t] = 0;
+        p.first[t] = INT_MAX;
+      }
+    }
+  __syncthreads();
+
+  const bool ok = missing == 0;
+  const int32_t count = ok ? static_cast<int32_t>(wanted) : 0;
+  auto settled = [&](int32_t s) {
+    Info i = held(s);
+    if (s < p.seqs) {
+      i.source = a.copies[3 * static_cast<int64_t>(s)];
+      i.rank = a.copies[3 * static_cast<int64_t>(s) + 1];
+    }
+    want(i);
+    return i;
+  };
+  for (int32_t base = 0; base < count; base += kPoolPicked) {
+    const int32_t end = min(count, base + kPoolPicked);
+    int64_t rank = free_before;
+    for (int32_t w = word0; w < word1 && rank < end; ++w) {
+      uint32_t bits = p.free[w];
+      const int32_t n = __popc(bits);
+      if (rank + n > base)
+        for (int64_t r = rank; bits != 0 && r < end; ++r, bits &= bits - 1)
+          if (r >= base) {
+            const int32_t number = 32 * w + __ffs(bits) - 1;
+            picked[r - base] = number;
+            p.refs[number] = 1;
+          }
+      rank += n;
+    }
+    __syncthreads();
+    for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
+      if (!once) mine = settled(s0 + tid);
+      auto enter = [&](int32_t s, int32_t column, int32_t r) {
+        if (r >= base && r < end) p.table[static_cast<int64_t>(s) * p.width + column] = picked[r - base];
+      };
+      kv_for<kPoolOwn>([&](auto J) {
+        if (J < mine.need) enter(mine.seq, mine.begin + J, mine.rank + J);
+      });
+      uint64_t many = __ballot(mine.need > kPoolOwn);
+      while (many != 0) {
+        const int32_t l = __ffsll(static_cast<unsigned long long>(many)) - 1;
+        many &= many - 1;
+        const int32_t s = __shfl(mine.seq, l), begin = __shfl(mine.begin, l), need = __shfl(mine.need, l), first = __shfl(mine.rank, l);
+        // those of the round
+        const int32_t j1 = min(need, end - first);
+        for (int32_t j = max(kPoolOwn, base - first) + lane; j < j1; j += 64) enter(s, begin + j, first + j);
+      }
+    }
+    __syncthreads();
+  }
+  // the pages taken are not free any more
+  if (count > 0) {
+    int64_t rank = free_before;
+    for (int32_t w = word0; w < word1 && rank < count; ++w) {
+      uint32_t bits = p.free[w];
+      const int32_t n = __popc(bits);
+      for (int64_t r = rank; bits != 0 && r < count; ++r) bits &= bits - 1;
+      p.free[w] = bits;
+      rank += n;
+    }
+  }
+  for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
+    if (!once) mine = settled(s0 + tid);
+    const int32_t s = mine.seq;
+    if (s >= p.seqs) continue;
+    const bool copied = ok && mine.source >= 0;
+    int32_t *c = a.copies + 3 * static_cast<int64_t>(s);
+    c[0] = copied ? mine.source : -1;
+    c[1] = copied ? p.table[static_cast<int64_t>(s) * p.width + mine.begin] : -1;
+    c[2] = copied ? mine.inside : 0;
+    if (copied) __hip_atomic_fetch_add(p.refs + mine.source, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    a.seen[s] = ok && mine.n > 0 ? mine.old + mine.n : 0;
+    if (ok && mine.n > 0) p.lengths[s] = mine.old + mine.n;
+  }
+}
+
+// A workgroup for a sequence: the pages past `to` tokens are let go.
+__global__ __launch_bounds__(256) void kv_trim_kernel(const PoolArgs p, const int32_t *to) {
+  const int32_t s = blockIdx.x;
+  const int32_t old = min(max(p.lengths[s], 0), p.width << p.log_page), n = min(old, max(to[s], 0));
+  if (n == old) return;
+  int32_t *row = p.table + static_cast<int64_t>(s) * p.width;
+  for (int32_t w = pool_pages(p, n) + threadIdx.x; w < pool_pages(p, old); w += blockDim.x) {
+    const int32_t page = row[w];
+    row[w] = -1;
+    pool_drop(p, page);
+  }
+  __syncthreads();  // every thread has read the length
+  if (threadIdx.x == 0) p.lengths[s] = n;
+}
+
+// A sequence that goes on from itself is left alone, and a page that stays where it
+// was is neither counted up nor down.
+__device__ __forceinline__ int32_t pool_parent(const PoolArgs &p, const int32_t *parents, int32_t s) {
+  const int32_t from = parents[s];
+  return static_cast<uint32_t>(from) < static_cast<uint32_t>(p.seqs) ? from : -1;
+}
+// Two launches, a workgroup for a sequence each: what every sequence becomes is laid
+// aside and held once more; then it takes its place and what was there is let go, after all
+// that stays is held.
+__global__ __launch_bounds__(256) void kv_gather_kernel(const PoolArgs p, const int32_t *parents) {
+  const int32_t s = blockIdx.x, from = pool_parent(p, parents, s);
+  if (from == s) return;
+  const int32_t *row = p.table + static_cast<int64_t>(s) * p.width, *source = p.table + static_cast<int64_t>(max(from, 0)) * p.width;
+  int32_t *to = p.spare + static_cast<int64_t>(s) * p.width;
+  for (int32_t w = threadIdx.x; w < p.width; w += blockDim.x) {
+    const int32_t page = from < 0 ? -1 : source[w];
+    to[w] = page;
+    if (page != row[w] && pool_has(p, page)) __hip_atomic_fetch_add(p.refs + page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (threadIdx.x == 0) p.spare_lengths[s] = from < 0 ? 0 : p.lengths[from];
+}
+__global__ __launch_bounds__(256) void kv_settle_kernel(const PoolArgs p, const int32_t *parents) {
+  const int32_t s = blockIdx.x, from = pool_parent(p, parents, s);
+  if (from == s) return;
+  int32_t *row = p.table + static_cast<int64_t>(s) * p.width;
+  const int32_t *source = p.spare + static_cast<int64_t>(s) * p.width;
+  for (int32_t w = threadIdx.x; w < p.width; w += blockDim.x) {
+    const int32_t page = source[w], old = row[w];
+    if (page == old) continue;
+    row[w] = page;
+    pool_drop(p, old);
+  }
+  if (threadIdx.x == 0) p.lengths[s] = p.spare_lengths[s];
+}
+
+constexpr int32_t kSlotStarts = 4096;  // row starts held in shared memory
+
+// A thread a row; its sequence is found by halving among the row starts, which a
+// workgroup reads once where they fit.
+__global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int32_t *positions, int64_t *slots) {
+  __shared__ int32_t held[kSlotStarts];
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const bool few = b.starts && b.seqs < kSlotStarts;
+  if (few) {
+    for (int32_t i = threadIdx.x; i <= b.seqs; i += 256) held[i] = b.starts[i];
+    __syncthreads();
+  }
+  if (r >= b.rows) return;
+  const int32_t row = static_cast<int32_t>(r);
+  int32_t seq = row;
+  if (b.starts) {
+    const int32_t *starts = few ? held : b.starts;
+    // the last sequence that starts at the row or before it
+    int32_t low = -1, high = b.seqs;
+    while (high - low > 1) {
+      const int32_t mid = (low + high) >> 1;
+      if (starts[mid] <= row)
+        low = mid;
+      else
+        high = mid;
+    }
+    seq = low;
+  }
+  int32_t position = 0;
+  int64_t slot = -1;
+  if (seq >= 0 && seq < b.seqs) {
+    const int32_t length = max(b.lengths[seq], 0);
+    int32_t first = row, all = 1;
+    if (b.starts) {
+      first = min(max(b.starts[seq], 0), b.rows);
+      all = min(max(b.starts[seq + 1], first), b.rows) - first;
+    }
+    const int32_t i = row - first, at = length - all + i;
+    if (i < all) {
+      position = max(at, 0);
+      if (at >= 0 && i < b.max_rows && at < b.max_length) {
+        const int32_t page = b.table[seq * b.table_stride + (at >> b.log_page)];
+        if (static_cast<uint32_t>(page) < static_cast<uint32_t>(b.blocks))
+          slot = (static_cast<int64_t>(page) << b.log_page) + (at & ((1 << b.log_page) - 1));
+      }
+    }
+  }
+  positions[r] = position;
+  slots[r] = slot;
+}
+
+struct CopyArgs {
+  uint8_t *k, *v;
+  float *scales;
+  const int32_t *copies;
+  int32_t blocks, log_page, heads, row_bytes;
+  KvDiv by_heads;
+  uint32_t first;
+};
+
+// A workgroup for a sequence's copy of one head: the page's first tokens, keys and
+// values, and its scales.  Bound by memory; most workgroups of a step find nothing to copy.
+__global__ __launch_bounds__(256) void kv_copy_kernel(const CopyArgs a) {
+  uint32_t id = a.first + blockIdx.x;
+  const int32_t head = kv_rem(a.by_heads, id);
+  const kv_const_i32 *c = (const kv_const_i32 *)a.copies + 3 * static_cast<int64_t>(id);
+  const int32_t source = c[0], target = c[1], tokens = min(c[2], 1 << a.log_page);
+  if (static_cast<uint32_t>(source) >= static_cast<uint32_t>(a.blocks) || static_cast<uint32_t>(target) >= static_cast<uint32_t>(a.blocks) ||
+      source == target)
+    return;
+  const int64_t from = static_cast<int64_t>(source) * a.heads + head, to = static_cast<int64_t>(target) * a.heads + head;
+  const int64_t size = static_cast<int64_t>(a.row_bytes) << a.log_page;
+  const u32x4 *ks = reinterpret_cast<const u32x4 *>(a.k + from * size), *vs = reinterpret_cast<const u32x4 *>(a.v + from * size);
+  u32x4 *kt = reinterpret_cast<u32x4 *>(a.k + to * size), *vt = reinterpret_cast<u32x4 *>(a.v + to * size);
+  const int32_t count = tokens * a.row_bytes / 16;
+  if (threadIdx.x < 2) a.scales[2 * to + threadIdx.x] = a.scales[2 * from + threadIdx.x];
+  for (int32_t i = threadIdx.x; i < count; i += 512) {
+    const int32_t j = i + 256;
+    const u32x4 k0 = ks[i], v0 = vs[i];
+    if (j < count) {
+      const u32x4 k1 = ks[j], v1 = vs[j];
+      kt[j] = k1;
+      vt[j] = v1;
+    }
+    kt[i] = k0;
+    vt[i] = v0;
+  }
+}
+
+static int32_t pages_check(const char *what) {
+  const hipError_t err = hipGetLastError();
+  if (err == hipSuccess) return RNSMX_OK;
+  set_error("%s: %s", what, hipGetErrorString(err));
+  return RNSMX_ELAUNCH;
+}
+static bool on(const void *p, int64_t n) { return p && reinterpret_cast<uintptr_t>(p) % n == 0; }
+static int32_t log_of(int32_t page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
+
+static int64_t scratch_words(int32_t blocks, int32_t seqs, int32_t width) {
+  return 2 * static_cast<int64_t>(blocks) + static_cast<int64_t>(seqs) * width + seqs;
+}
+
+static int32_t pool_args(const rnsmx_kv_pool_t *pool, PoolArgs &a) {
+  if (!pool) return fail(RNSMX_EINVAL, "null pool");
+  a.log_page = log_of(pool->page);
+  if (a.log_page < 0) return fail(RNSMX_EINVAL, "a page holds 16, 32, 64 or 128 tokens");
+  if (pool->blocks < 1 || pool->seqs < 1 || pool->width < 1) return fail(RNSMX_EINVAL, "a pool has pages, sequences and a table");
+  if ((static_cast<int64_t>(pool->width) << a.log_page) > 1 << 30) return fail(RNSMX_EINVAL, "sequences hold at most 2^30 tokens");
+  if (!on(pool->table_dev, 4) || !on(pool->lengths_dev, 4) || !on(pool->refs_dev, 4) || !on(pool->free_dev, 4) || !on(pool->scratch_dev, 4))
+    return fail(RNSMX_EINVAL, "a pool's pointer is null or not on a 4-byte boundary");
+  a.table = pool->table_dev;
+  a.lengths = pool->lengths_dev;
+  a.refs = pool->refs_dev;
+  a.free = pool->free_dev;
+  a.going = pool->scratch_dev;
+  a.first = a.going + pool->blocks;
+  a.spare = a.first + pool->blocks;
+  a.spare_lengths = a.spare + static_cast<int64_t>(pool->seqs) * pool->width;
+  a.blocks = pool->blocks;
+  a.words = static_cast<int32_t>((static_cast<int64_t>(pool->blocks) + 31) / 32);
+  a.seqs = pool->seqs;
+  a.width = pool->width;
+  return RNSMX_OK;
+}
+
+// Threads for a sequence's row of the table.
+static unsigned row_threads(const PoolArgs &a) { return a.width <= 64 ? 64 : 256; }
+
+}  // namespace rnsmx
+
+using namespace rnsmx;
+
+extern "C" {
+
+int64_t rnsmx_kv_pool_scratch_words(int32_t blocks, int32_t seqs, int32_t width) {
+  return blocks < 1 || seqs < 1 || width < 1 ? -1 : scratch_words(blocks, seqs, width);
+}
+
+int32_t rnsmx_kv_assign(const rnsmx_kv_pool_t *pool, const rnsmx_kv_step_t *step, const int32_t *new_dev, void *stream) {
+  clear_error();
+  AssignArgs a{};
+  if (int32_t rc = pool_args(pool, a.p)) return rc;
+  if (!step) return fail(RNSMX_EINVAL, "null step");
+  if (step->rows < 0 || step->max_rows < 0 || step->max_length < 0) return fail(RNSMX_EINVAL, "bad step sizes");
+  if (!on(step->lengths_dev, 4) || !on(step->copies_dev, 4) || !on(step->missing_dev, 4) ||
+      (step->starts_dev && !on(step->starts_dev, 4)) || (new_dev && !on(new_dev, 4)))
+    return fail(RNSMX_EINVAL, "a step's pointer is null or not on a 4-byte boundary");
+  a.asked = new_dev;
+  a.seen = step->lengths_dev;
+  a.starts = step->starts_dev;
+  a.copies = step->copies_dev;
+  a.missing = step->missing_dev;
+  a.rows = step->rows;
+  a.max_rows = step->max_rows;
+  a.max_length = step->max_length;
+  // a sequence and two words of free pages a thread
+  const int64_t work = std::max<int64_t>({a.p.seqs, a.p.words / 2, a.rows >> a.p.log_page});
+  const unsigned threads = static_cast<unsigned>(std::min<int64_t>(1024, (work + 63) / 64 * 64));
+  hipLaunchKernelGGL(kv_assign_kernel, dim3(1), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
+  return pages_check("kv_assign");
+}
+
+int32_t rnsmx_kv_trim(const rnsmx_kv_pool_t *pool, const int32_t *lengths_dev, void *stream) {
+  clear_error();
+  PoolArgs a{};
+  if (int32_t rc = pool_args(pool, a)) return rc;
+  if (!on(lengths_dev, 4)) return fail(RNSMX_EINVAL, "lengths null or not on a 4-byte boundary");
+  hipLaunchKernelGGL(kv_trim_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, static_cast<hipStream_t>(stream), a, lengths_dev);
+  return pages_check("kv_trim");
+}
+
+int32_t rnsmx_kv_reorder(const rnsmx_kv_pool_t *pool, const int32_t *parents_dev, void *stream) {
+  clear_error();
+  PoolArgs a{};
+  if (int32_t rc = pool_args(pool, a)) return rc;
+  if (!on(parents_dev, 4)) return fail(RNSMX_EINVAL, "parents null or not on a 4-byte boundary");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(kv_gather_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, st, a, parents_dev);
+  hipLaunchKernelGGL(kv_settle_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, st, a, parents_dev);
+  return pages_check("kv_reorder");
+}
+
+int32_t rnsmx_kv_slots(const rnsmx_kv_batch_t *batch, int32_t blocks, int32_t page, int32_t *positions_dev, int64_t *slots_dev,
+                       void *stream) {
+  clear_error();
+  if (!batch) return fail(RNSMX_EINVAL, "null batch");
+  KvBatchArgs b{};
+  b.log_page = log_of(page);
+  if (b.log_page < 0) return fail(RNSMX_EINVAL, "a page holds 16, 32, 64 or 128 tokens");
+  if (blocks < 1 || batch->seqs < 0 || batch->rows < 0 || batch->max_rows < 0 || batch->max_length < 0 || batch->table_width < 1 ||
+      batch->table_stride < 0)
+    return fail(RNSMX_EINVAL, "bad batch sizes");
+  if (batch->max_length > 1 << 30 || batch->max_length > static_cast<int64_t>(batch->table_width) << b.log_page)
+    return fail(RNSMX_EINVAL, "max_length is past the block table");
+  if (!batch->starts_dev && batch->rows != batch->seqs) return fail(RNSMX_EINVAL, "one row a sequence without row starts");
+  if (batch->rows == 0) return RNSMX_OK;
+  if (batch->seqs > 0 && (!on(batch->table_dev, 4) || !on(batch->lengths_dev, 4)))
+    return fail(RNSMX_EINVAL, "a batch's pointer is null or not on a 4-byte boundary");
+  if ((batch->starts_dev && !on(batch->starts_dev, 4)) || !on(positions_dev, 4) || !on(slots_dev, 8))
+    return fail(RNSMX_EINVAL, "starts, positions or slots null or not aligned to their type");
+  b.table = batch->table_dev;
+  b.lengths = batch->lengths_dev;
+  b.starts = batch->starts_dev;
+  b.table_stride = batch->table_stride;
+  b.blocks = blocks;
+  b.seqs = batch->seqs;
+  b.rows = batch->rows;
+  b.max_rows = batch->starts_dev ? batch->max_rows : 1;
+  b.max_length = batch->max_length;
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(b.rows) + 255) / 256);
+  hipLaunchKernelGGL(kv_slots_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), b, positions_dev, slots_dev);
+  return pages_check("kv_slots");
+}
+
+int32_t rnsmx_kv_copy(const rnsmx_kv_cache_t *cache, const int32_t *copies_dev, int32_t count, void *stream) {
+  clear_error();
+  if (!cache) return fail(RNSMX_EINVAL, "null cache");
+  CopyArgs a{};
+  a.log_page = log_of(cache->page);
+  if (a.log_page < 0 || cache->blocks < 1 || cache->heads < 1 || cache->row_bytes != rnsmx_kv_row_bytes(cache->head_dim) ||
+      cache->row_bytes < 1)
+    return fail(RNSMX_EINVAL, "bad cache sizes");
+  if (!on(cache->k_dev, 16) || !on(cache->v_dev, 16) || !on(cache->scales_dev, 8))
+    return fail(RNSMX_EINVAL, "codes start on 16-byte boundaries, scales on 8-byte ones");
+  if (count < 0 || static_cast<int64_t>(count) * cache->heads > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many copies and heads for one call");
+  if (count == 0) return RNSMX_OK;
+  if (!on(copies_dev, 4)) return fail(RNSMX_EINVAL, "copies null or not on a 4-byte boundary");
+  a.k = cache->k_dev;
+  a.v = cache->v_dev;
+  a.scales = cache->scales_dev;
+  a.copies = copies_dev;
+  a.blocks = cache->blocks;
+  a.heads = cache->heads;
+  a.row_bytes = cache->row_bytes;
+  a.by_heads = kv_div(cache->heads);
+  kv_launches(static_cast<uint32_t>(count) * cache->heads, 256, [&](uint32_t first, uint32_t groups) {
+    a.first = first;
+    hipLaunchKernelGGL(kv_copy_kernel, dim3(groups), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  });
+  return pages_check("kv_copy");
+}
+
+}  // extern "C"

@@ -1,0 +1,300 @@
+// Rotary positions: queries and keys turned by their positions' angles.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "rnsmx_kv_attn.hpp"
+
+namespace rnsmx {
+
+// One of the two tensors of a call: heads of `dim` values at its strides.
+struct RotaryPart {
+  const void *src;
+  void *dst;
+  int64_t src_rs, src_hs, dst_rs, dst_hs;
+};
+
+struct RotaryArgs {
+  RotaryPart part[2];
+  const uint64_t *steps;
+  const void *positions;
+  int64_t rows, first;  // a launch's first row
+  int32_t wide;  // positions of 64 bits
+  int32_t q_heads, heads, pairs, dim;
+  int32_t pieces;     // of a head: its pairs by eights, then what is copied by sixteens
+  int32_t turning;    // of them those of pairs
+  int32_t per_row;    // pieces of a row
+  int32_t row_tile;   // rows of a workgroup
+  int32_t head_tile;  // heads of a workgroup
+  KvDiv by_pieces, by_row, by_pairs;
+  float magnitude, sign;
+};
+
+constexpr int kRotaryTable = 1024;  // angles of a workgroup
+
+// Cosine and sine of a position's angle.  position * step mod 2^64 is the fraction
+// of a turn, exact but for the step's own last place (2^-65 turns a position): no
+// position is too far.  Its upper half is cut into quarters, so that what
+// is converted to float32 is below an eighth of a turn and keeps its bits.
+__device__ __forceinline__ F32x2 rotary_angle(int64_t position, uint64_t step) {
+  const uint32_t turn = static_cast<uint32_t>((static_cast<uint64_t>(position) * step) >> 32);
+  const uint32_t quarter = (turn + 0x20000000u) >> 30;
+  const float x = static_cast<float>(static_cast<int32_t>(turn - (quarter << 30))) * 4.656612873077393e-10f;  // 2^-31
+  float s, c;
+  sincospif(x, &s, &c);
+  const float co = quarter & 1 ? s : c, si = quarter & 1 ? c : s;
+  return F32x2{(quarter == 1 || quarter == 2) ? -co : co, quarter >= 2 ? -si : si};
+}
+
+template <typename T>
+__device__ __forceinline__ float rotary_load(T v) {
+  if constexpr (std::is_same<T, uint16_t>::value)
+    return kv_bf16(v);
+  else
+    return static_cast<float>(v);
+}
+template <typename T>
+__device__ __forceinline__ T rotary_round(float v) {
+  if constexpr (std::is_same<T, uint16_t>::value)
+    return kv_to_bf16(v);
+  else
+    return static_cast<T>(v);
+}
+
+// Eight values at p, those from `left` on not there.
+template <bool VEC, typename T>
+__device__ __forceinline__ void rotary_get(T (&x)[8], const T *p, int32_t left) {
+  if constexpr (VEC) {
+    kv_for<sizeof(T) / 2>([&](auto I) { reinterpret_cast<u32x4 *>(x)[I] = reinterpret_cast<const u32x4 *>(p)[I]; });
+  } else {
+    kv_for<8>([&](auto I) { x[I] = I < left ? p[I] : T(0); });
+  }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void rotary_put(T *p, const T (&x)[8], int32_t left) {
+  if constexpr (VEC) {
+    kv_for<sizeof(T) / 2>([&](auto I) { reinterpret_cast<u32x4 *>(p)[I] = reinterpret_cast<const u32x4 *>(x)[I]; });
+  } else {
+    kv_for<8>([&](auto I) {
+      if (I < left) p[I] = x[I];
+    });
+  }
+}
+
+// A workgroup takes some rows and heads: the rows' angles once into shared memory,
+// then eight pairs a thread and step.  A thread reads what it writes before it writes
+// it, so a call may be in place.
+template <typename T, bool VEC, bool NEIGHBOURS>
+__global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
+  __shared__ __attribute__((aligned(16))) F32x2 angles[kRotaryTable];
+  const int64_t row0 = a.first + static_cast<int64_t>(blockIdx.x) * a.row_tile;
+  const int32_t rows = static_cast<int32_t>(min(static_cast<int64_t>(a.row_tile), a.rows - row0));
+  const int32_t head0 = blockIdx.y * a.head_tile;
+  const int32_t count = rows * a.per_row;
+  const int32_t half = a.pairs;
+
+  struct Piece {
+    T x[2][8];
+    const T *from;
+    T *to;
+    int32_t at[2], left[2], row, first;  // columns and how many of them are there
+    bool there, turned;
+  };
+  auto load = [&](Piece &p, int32_t i) {
+    p.there = i < count;
+    uint32_t n = static_cast<uint32_t>(min(i, count - 1));
+    const int32_t in_row = kv_rem(a.by_row, n);
+    p.row = n;
+    n = in_row;
+    const int32_t piece = kv_rem(a.by_pieces, n), head = head0 + n;
+    const bool second = head >= a.q_heads;
+    p.there = p.there && head < a.q_heads + a.heads;
+    const int32_t h = p.there ? head - (second ? a.q_heads : 0) : 0;
+    const int64_t row = row0 + p.row;
+    const RotaryPart &u = a.part[0], &v = a.part[1];
+    p.from = static_cast<const T *>(second ? v.src : u.src) + (row * (second ? v.src_rs : u.src_rs) + h * (second ? v.src_hs : u.src_hs));
+    p.to = static_cast<T *>(second ? v.dst : u.dst) + (row * (second ? v.dst_rs : u.dst_rs) + h * (second ? v.dst_hs : u.dst_hs));
+    p.turned = piece < a.turning;
+    p.first = 8 * piece;
+    if (p.turned && !NEIGHBOURS) {
+      p.at[0] = 8 * piece;
+      p.at[1] = half + 8 * piece;
+      p.left[0] = p.left[1] = half - 8 * piece;
+    } else {
+      p.at[0] = p.turned ? 16 * piece : 2 * half + 16 * (piece - a.turning);
+      p.at[1] = p.at[0] + 8;
+      const int32_t end = p.turned ? 2 * half : a.dim;
+      p.left[0] = end - p.at[0];
+      p.left[1] = end - p.at[1];
+    }
+    kv_for<2>([&](auto K) {
+      // whole or not at all where they are eights
+      if (p.there && p.left[K] > 0) rotary_get<VEC>(p.x[K], p.from + p.at[K], p.left[K]);
+    });
+  };
+  auto store = [&](Piece &p) {
+    if (!p.there) return;
+    if (p.turned) {
+      const F32x2 *t = angles + p.row * half + p.first;
+      kv_for<8>([&](auto I) {
+        constexpr int i = I;
+        // neighbours: pair i lies in values 2 i, 2 i + 1 of the sixteen
+        constexpr int ka = NEIGHBOURS ? (2 * i) / 8 : 0, ia = NEIGHBOURS ? (2 * i) % 8 : i;
+        constexpr int kb = NEIGHBOURS ? (2 * i + 1) / 8 : 1, ib = NEIGHBOURS ? (2 * i + 1) % 8 : i;
+        const F32x2 cs = VEC || p.first + i < half ? t[i] : F32x2{1.0f, 0.0f};
+        const float u = rotary_load(p.x[ka][ia]), v = rotary_load(p.x[kb][ib]);
+        p.x[ka][ia] = rotary_round<T>(fmaf(u, cs.x, -(v * cs.y)));
+        p.x[kb][ib] = rotary_round<T>(fmaf(v, cs.x, u * cs.y));
+      });
+    }
+    kv_for<2>([&](auto K) {
+      if (p.left[K] > 0) rotary_put<VEC>(p.to + p.at[K], p.x[K], p.left[K]);
+    });
+  };
+
+  Piece first;
+  load(first, threadIdx.x);
+  for (int32_t i = threadIdx.x; i < rows * half; i += 256) {
+    uint32_t r = i;
+    const int32_t pair = kv_rem(a.by_pairs, r);
+    const int64_t row = row0 + r;
+    const int64_t position = a.wide ? static_cast<const int64_t *>(a.positions)[row] : static_cast<const int32_t *>(a.positions)[row];
+    const F32x2 t = rotary_angle(position, a.steps[pair]);
+    angles[i] = F32x2{t.x * a.magnitude, t.y * (a.magnitude * a.sign)};
+  }
+  __syncthreads();
+  store(first);
+  for (int32_t i = threadIdx.x + 256; i < count; i += 512) {
+    Piece p, q;
+    load(p, i);
+    load(q, i + 256);
+    store(p);
+    store(q);
+  }
+}
+
+static bool rotary_vec(const rnsmx_rotary_rows_t &r, int64_t size, const void *p, int64_t rs, int64_t hs) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && rs * size % 16 == 0 && hs * size % 16 == 0;
+}
+
+// Bytes from the first to past the last of a tensor's rows.
+static int64_t rotary_extent(int64_t rows, int64_t heads, int64_t dim, int64_t rs, int64_t hs, int64_t size) {
+  return ((rows - 1) * rs + (heads - 1) * hs + dim) * size;
+}
+
+}  // namespace rnsmx
+
+using namespace rnsmx;
+
+extern "C" {
+
+int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *rows, const void *positions_dev, const void *q_dev,
+                     const void *k_dev, void *q_out_dev, void *k_out_dev, void *stream) {
+  clear_error();
+  if (!rotary || !rows) return fail(RNSMX_EINVAL, "null rotary or rows");
+  if (rows->dtype != RNSMX_FLOAT32 && rows->dtype != RNSMX_FLOAT16 && rows->dtype != RNSMX_BFLOAT16)
+    return fail(RNSMX_EINVAL, "queries and keys are float32, float16 or bfloat16");
+  if (rows->positions_dtype != RNSMX_INT32 && rows->positions_dtype != RNSMX_INT64)
+    return fail(RNSMX_EINVAL, "positions are int32 or int64");
+  if (rows->rows < 0 || rows->q_heads < 0 || rows->k_heads < 0 || rows->head_dim < 1 || rows->head_dim > RNSMX_ROTARY_MAX_DIM ||
+      static_cast<int64_t>(rows->q_heads) + rows->k_heads > RNSMX_ROTARY_MAX_HEADS)
+    return fail(RNSMX_EINVAL, "bad row sizes");
+  if (rotary->pairs < 1 || 2 * static_cast<int64_t>(rotary->pairs) > rows->head_dim)
+    return fail(RNSMX_EINVAL, "the pairs are more than a head has");
+  if (!std::isfinite(rotary->magnitude)) return fail(RNSMX_EINVAL, "the magnitude is not finite");
+  for (const int64_t s : {rows->q_row_stride, rows->q_head_stride, rows->k_row_stride, rows->k_head_stride, rows->q_out_row_stride,
+                          rows->q_out_head_stride, rows->k_out_row_stride, rows->k_out_head_stride})
+    if (s < 0) return fail(RNSMX_EINVAL, "negative strides");
+  const int32_t heads = rows->q_heads + rows->k_heads;
+  if (rows->rows == 0 || heads == 0) return RNSMX_OK;
+  if (rows->rows > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many rows");
+  const int64_t size = rows->dtype == RNSMX_FLOAT32 ? 4 : 2;
+  if (!rotary->steps_dev || reinterpret_cast<uintptr_t>(rotary->steps_dev) % 8 != 0 || !positions_dev ||
+      reinterpret_cast<uintptr_t>(positions_dev) % (rows->positions_dtype == RNSMX_INT64 ? 8 : 4) != 0)
+    return fail(RNSMX_EINVAL, "steps or positions null or not aligned to their type");
+
+  RotaryArgs a{};
+  a.part[0] = {q_dev, q_out_dev, rows->q_row_stride, rows->q_head_stride, rows->q_out_row_stride, rows->q_out_head_stride};
+  a.part[1] = {k_dev, k_out_dev, rows->k_row_stride, rows->k_head_stride, rows->k_out_row_stride, rows->k_out_head_stride};
+  const int32_t part_heads[2] = {rows->q_heads, rows->k_heads};
+  bool vec = rotary->pairs % 8 == 0 && rows->head_dim % 8 == 0, copied = false;
+  for (int i = 0; i < 2; ++i) {
+    if (part_heads[i] == 0) continue;
+    const RotaryPart &p = a.part[i];
+    if (!p.src || !p.dst || reinterpret_cast<uintptr_t>(p.src) % size != 0 || reinterpret_cast<uintptr_t>(p.dst) % size != 0)
+      return fail(RNSMX_EINVAL, "queries, keys or outputs null or not aligned to their type");
+    const bool in_place = p.src == p.dst && p.src_rs == p.dst_rs && p.src_hs == p.dst_hs;
+    copied = copied || !in_place;
+    vec = vec && rotary_vec(*rows, size, p.src, p.src_rs, p.src_hs) && rotary_vec(*rows, size, p.dst, p.dst_rs, p.dst_hs);
+    // Outputs meet an input's memory only where they are it; columns of one
+    // product interleave without sharing a value, which ranges cannot tell.
+    for (int j = 0; j < 2; ++j)
+      if (part_heads[j] > 0 && !in_place &&
+          ranges_meet(p.dst, rotary_extent(rows->rows, part_heads[i], rows->head_dim, p.dst_rs, p.dst_hs, size), a.part[j].src,
+                      rotary_extent(rows->rows, part_heads[j], rows->head_dim, a.part[j].src_rs, a.part[j].src_hs, size)))
+        return fail(RNSMX_EINVAL, "outputs lie over queries or keys without being them");
+  }
+  a.steps = rotary->steps_dev;
+  a.positions = positions_dev;
+  a.rows = rows->rows;
+  a.wide = rows->positions_dtype == RNSMX_INT64;
+  a.q_heads = rows->q_heads;
+  a.heads = rows->k_heads;
+  a.pairs = rotary->pairs;
+  a.dim = rows->head_dim;
+  a.magnitude = rotary->magnitude;
+  a.sign = rows->back ? -1.0f : 1.0f;
+  a.turning = (a.pairs + 7) / 8;
+  a.pieces = a.turning + (copied ? (a.dim - 2 * a.pairs + 15) / 16 : 0);
+
+  // A workgroup's rows share the angles' cost and are as many as leave the chip
+  // kRotaryGroups workgroups; where rows are fewer than that their heads are split.
+  constexpr int64_t kRotaryGroups = 1024;
+  const int64_t most_rows = std::min<int64_t>(kRotaryTable / a.pairs, 8);
+  a.row_tile = static_cast<int32_t>(std::max<int64_t>(1, std::min(most_rows, a.rows / kRotaryGroups)));
+  const int64_t row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
+  a.head_tile = heads;
+  if (row_tiles < 256) {
+    // down to a piece a thread
+    const int64_t least = std::max<int64_t>(1, 256 / a.pieces), parts = std::max<int64_t>(1, std::min<int64_t>(512 / row_tiles, heads / least));
+    a.head_tile = static_cast<int32_t>((heads + parts - 1) / parts);
+  }
+  a.per_row = a.head_tile * a.pieces;
+  a.by_pieces = kv_div(a.pieces);
+  a.by_row = kv_div(a.per_row);
+  a.by_pairs = kv_div(a.pairs);
+  const unsigned head_tiles = (heads + a.head_tile - 1) / a.head_tile;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto launch = [&](auto t) {
+    using T = decltype(t);
+    auto with = [&](auto vector) {
+      constexpr bool V = decltype(vector)::value;
+      // a launch has fewer than 2^32 threads
+      const int64_t most = (1 << 23) / head_tiles;
+      for (int64_t tile = 0; tile < row_tiles; tile += most) {
+        a.first = tile * a.row_tile;
+        const dim3 grid(static_cast<unsigned>(std::min(most, row_tiles - tile)), head_tiles);
+        if (rotary->interleaved)
+          hipLaunchKernelGGL((rotate_kernel<T, V, true>), grid, dim3(256), 0, st, a);
+        else
+          hipLaunchKernelGGL((rotate_kernel<T, V, false>), grid, dim3(256), 0, st, a);
+      }
+    };
+    if (vec)
+      with(std::true_type{});
+    else
+      with(std::false_type{});
+  };
+  if (rows->dtype == RNSMX_FLOAT32)
+    launch(float{});
+  else if (rows->dtype == RNSMX_FLOAT16)
+    launch(_Float16{});
+  else
+    launch(uint16_t{});
+  const hipError_t err = hipGetLastError();
+  if (err == hipSuccess) return RNSMX_OK;
+  set_error("rotate: %s", hipGetErrorString(err));
+  return RNSMX_ELAUNCH;
+}
+
+}  // extern "C"

@@ -23,7 +23,9 @@ KV_DIMS = (64, 96, 128, 160, 192, 256)  # row sizes of the key/value cache
 # (source, object name, extra flags)
 UNITS = [("rnsmx_kernels.hip", "rnsmx_kernels", []), ("rnsmx_bytes.hip", "rnsmx_bytes", []),
          ("rnsmx_linear.hip", "rnsmx_linear", []), ("rnsmx_units.hip", "rnsmx_units", []),
-         ("rnsmx_kv_cache.hip", "rnsmx_kv_cache", []), ("rnsmx_host.cpp", "rnsmx_host", [])] + [
+         ("rnsmx_kv_cache.hip", "rnsmx_kv_cache", []), ("rnsmx_pages.hip", "rnsmx_pages", []),
+         ("rnsmx_rotary.hip", "rnsmx_rotary", []), ("rnsmx_beams.hip", "rnsmx_beams", []),
+         ("rnsmx_host.cpp", "rnsmx_host", [])] + [
     (f"rnsmx_kv_{part}.hip", f"rnsmx_kv_{part}_{d}", [f"-DRNSMX_KV_DIM={d}"])
     for part in ("rows", "tiles") for d in KV_DIMS] + [
     ("rnsmx_gemm_part.hip", f"rnsmx_gemm_r{r}_p{p}", [f"-DRNSMX_RCAP={r}", f"-DRNSMX_PART={p}"])

@@ -55,11 +55,23 @@ EXPORTED_SYMBOLS = (
     "rnsmx_kv_attention_workspace_bytes",
     "rnsmx_kv_attention_plan",
     "rnsmx_kv_attention",
+    "rnsmx_kv_pool_scratch_words",
+    "rnsmx_kv_assign",
+    "rnsmx_kv_trim",
+    "rnsmx_kv_reorder",
+    "rnsmx_kv_slots",
+    "rnsmx_kv_copy",
+    "rnsmx_rotate",
+    "rnsmx_beam_workspace_bytes",
+    "rnsmx_beam_select",
 )
 
 QUANT_SCRATCH = 1025  # RNSMX_QUANT_SCRATCH
 KV_MAX_DIM = 256  # RNSMX_KV_MAX_DIM
 KV_TICKETS = 16384  # RNSMX_KV_TICKETS
+ROTARY_MAX_DIM = 1024  # RNSMX_ROTARY_MAX_DIM
+ROTARY_MAX_HEADS = 4096  # RNSMX_ROTARY_MAX_HEADS
+BEAMS_MAX = 64  # RNSMX_BEAMS_MAX
 
 
 class Moduli(ctypes.Structure):
@@ -195,6 +207,84 @@ class KVPlan(ctypes.Structure):
         return tuple(getattr(self, name) for name, _ in self._fields_)
 
 
+class KVPoolStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_kv_pool_t``."""
+
+    _fields_ = [
+        ("table_dev", ctypes.c_void_p),
+        ("lengths_dev", ctypes.c_void_p),
+        ("refs_dev", ctypes.c_void_p),
+        ("free_dev", ctypes.c_void_p),
+        ("scratch_dev", ctypes.c_void_p),
+        ("blocks", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("seqs", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+    ]
+
+
+class KVStepStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_kv_step_t``."""
+
+    _fields_ = [
+        ("lengths_dev", ctypes.c_void_p),
+        ("starts_dev", ctypes.c_void_p),
+        ("copies_dev", ctypes.c_void_p),
+        ("missing_dev", ctypes.c_void_p),
+        ("rows", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+        ("max_length", ctypes.c_int32),
+    ]
+
+
+class RotaryStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_rotary_t``."""
+
+    _fields_ = [
+        ("steps_dev", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+    ]
+
+
+class RotaryRowsStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_rotary_rows_t``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("q_out_row_stride", ctypes.c_int64),
+        ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_row_stride", ctypes.c_int64),
+        ("k_out_head_stride", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("positions_dtype", ctypes.c_int32),
+        ("back", ctypes.c_int32),
+    ]
+
+
+class BeamsStruct(ctypes.Structure):
+    """Mirror of ``rnsmx_beams_t``."""
+
+    _fields_ = [
+        ("request_stride", ctypes.c_int64),
+        ("beam_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("requests", ctypes.c_int32),
+        ("beams", ctypes.c_int32),
+        ("vocabulary", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("end_token", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -247,6 +337,15 @@ _SIGNATURES = {
     "rnsmx_kv_attention_workspace_bytes": (_I64, [_P, _P, _P]),
     "rnsmx_kv_attention_plan": (_I32, [_P, _P, _P, _I32, _P]),
     "rnsmx_kv_attention": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _P, _P]),
+    "rnsmx_kv_pool_scratch_words": (_I64, [_I32, _I32, _I32]),
+    "rnsmx_kv_assign": (_I32, [_P, _P, _P, _P]),
+    "rnsmx_kv_trim": (_I32, [_P, _P, _P]),
+    "rnsmx_kv_reorder": (_I32, [_P, _P, _P]),
+    "rnsmx_kv_slots": (_I32, [_P, _I32, _I32, _P, _P, _P]),
+    "rnsmx_kv_copy": (_I32, [_P, _P, _I32, _P]),
+    "rnsmx_rotate": (_I32, [_P, _P, _P, _P, _P, _P, _P, _P]),
+    "rnsmx_beam_workspace_bytes": (_I64, [_P]),
+    "rnsmx_beam_select": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _P]),
 }
 
 ABI_VERSION = 7

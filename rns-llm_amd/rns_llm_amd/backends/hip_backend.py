@@ -42,7 +42,10 @@ from ..moduli import (
     safe_l1_dot_bound,
     validate_moduli,
 )
+from .beams import BeamOps
 from .kv_cache import KVCacheOps
+from .kv_pool import KVPoolOps
+from .rotary import RotaryOps
 
 KERNEL_NAME = "mfma"
 
@@ -302,10 +305,12 @@ class LinearCall:
         return AdaptiveMetadata(meta, self._full_moduli, stats)
 
 
-class HipRNSBackend(KVCacheOps):
+class HipRNSBackend(KVCacheOps, KVPoolOps, RotaryOps, BeamOps):
     """RNS backend on MI355X: one MFMA GEMM launch for all residue channels
     with the modular reduction, Garner reconstruction and signed correction
-    in its epilogue; and the 8-bit key/value cache (``kv_cache.py``)."""
+    in its epilogue; the 8-bit key/value cache (``kv_cache.py``), its pages handed out
+    on the device (``kv_pool.py``), rotary positions (``rotary.py``) and beam search's
+    selection (``beams.py``)."""
 
     name = "hip-rns-mfma"
 
@@ -320,6 +325,16 @@ class HipRNSBackend(KVCacheOps):
         self._stats: Counter[str] = Counter()
 
     _stream_of = staticmethod(_stream_handle)
+
+    def _on_device(self, device: torch.device, call, *args) -> None:
+        """A library call on `device`'s current stream, with that device the current one."""
+        if device.index is not None and device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                rc = call(*args, _stream_handle(device))
+        else:
+            rc = call(*args, _stream_handle(device))
+        if rc:
+            _native.check(rc)
 
     # ------------------------------------------------------------------
     # Stats (cuda_backend.py:129-135)

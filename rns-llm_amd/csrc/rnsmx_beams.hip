@@ -1,5 +1,6 @@
 // Beam search's selection: the best continuations of each request's beams.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -12,21 +13,20 @@ struct BeamArgs {
   const float *scores;
   const uint8_t *finished;
   int64_t request_stride, beam_stride;
-  uint64_t *partial;   // [requests * beams][splits][k + 2]
+  uint64_t *partial;   // [requests * beams][splits][k + 2]: the chunk's best, then its reference and sum
   uint32_t *tickets;   // an arrival counter a request of the launch
   float *out_scores;
   int32_t *out_tokens, *out_parents;
   int32_t first;       // a launch's first request
-  int32_t beams, vocabulary, k, splits, end_token;
-  KvDiv by_splits, by_beams;
+  int32_t beams, vocabulary, k, end_token;
+  int32_t chunk, splits;  // values of a workgroup, and workgroups of a beam
+  KvDiv by_splits, by_beams, by_k;
 };
 
-constexpr int kBeamValues = 16;                    // of a thread
-constexpr int kBeamChunk = 256 * kBeamValues;      // of a workgroup
-constexpr int kBeamLists = 16384;                  // chunks of a request
-// Entries of a workgroup's list: no more than kBeamValues of each of k lanes of its four
-// waves lie above their common bound, and k at it.
-constexpr int beam_list(int k) { return (4 * kBeamValues + 1) * k; }
+constexpr int kBeamMost = 256 * 64;  // values of a workgroup at most
+constexpr int kBeamList = 512;    // of a workgroup's or request's values those that reach its bound
+constexpr int kBeamChunks = 1024; // of a request at most
+constexpr int kBeamHeld = 1024;   // results of a request that shared memory holds all
 
 // Numbers whose order as unsigned ones is that of the values; zeros are one.
 __device__ __forceinline__ uint32_t beam_key(float x) {
@@ -36,159 +36,250 @@ __device__ __forceinline__ uint32_t beam_key(float x) {
 __device__ __forceinline__ float beam_logit(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+constexpr uint32_t kBeamNone = 0x007FFFFFu;  // of minus infinity, which is no candidate
 __device__ __forceinline__ uint64_t beam_score_key(double x) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
   return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | 0x8000000000000000ull);
 }
-
-__device__ __forceinline__ uint64_t beam_shuffle(uint64_t v, int lanes) {
-  return static_cast<uint64_t>(__shfl_xor(static_cast<long long>(v), lanes));
+__device__ __forceinline__ double beam_score(uint64_t key) {
+  return __builtin_bit_cast(double, key >> 63 ? key ^ 0x8000000000000000ull : ~key);
 }
 
-// One workgroup for a chunk of one beam's logits: read once into registers, they give
-// the largest, the sum of exponentials against it and the chunk's k best.  A bound that
-// at least k of them reach is the k-th largest of a wave's 64 lane maxima, the highest of
-// the four waves'; the few that reach it are put in order by counting.  The workgroup that
-// comes last of a request's joins the chunks.
+// The largest of a wave's numbers, in every lane: rows of 16, then across them.
+__device__ __forceinline__ uint32_t beam_wave_max(uint32_t v) {
+  auto step = [&](auto ctrl, auto rows) {
+    constexpr int c = ctrl, r = rows;
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), c, r, 0xF, false)));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr:1
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+
+// A number that at least k lanes' reach (0 if fewer have any), no higher than the
+// k-th largest: its bits from the highest down until just k are left.
+__device__ __forceinline__ uint32_t beam_bound(uint32_t v, int32_t k) {
+  uint32_t bound = 0;
+  for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+    const int32_t n = __popcll(__ballot(v >= (bound | bit)));
+    if (n >= k) bound |= bit;
+    if (n == k) break;
+  }
+  return bound;
+}
+
+// How many of n numbers in shared memory are larger than one, each of four neighbouring
+// lanes asking a quarter of them.
+__device__ __forceinline__ int32_t beam_larger(const uint64_t *of, int32_t n, uint64_t one) {
+  int32_t larger = 0;
+  for (int32_t j0 = threadIdx.x & 3; j0 < n; j0 += 16) {
+    uint64_t v[4];
+    kv_for<4>([&](auto U) { v[U] = of[min(j0 + 4 * U, n - 1)]; });
+    kv_for<4>([&](auto U) { larger += j0 + 4 * U < n && v[U] > one ? 1 : 0; });
+  }
+  kv_for<2>([&](auto I) { larger += __shfl_xor(larger, 1 << I); });
+  return larger;
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void beam_kernel(const BeamArgs a) {
-  constexpr int G = 16 / sizeof(T), N = kBeamValues / G;  // values of a load, loads of a thread
-  extern __shared__ uint64_t list[];  // and, once it is written out, how many of each chunk's are taken
-  uint8_t *const taken = reinterpret_cast<uint8_t *>(list);
-  __shared__ uint32_t wave_key[4], wave_bound[4];
-  __shared__ double wave_sum[4], total[64];
-  __shared__ int32_t count, last;
+__device__ __forceinline__ float beam_float(T v) {
+  if constexpr (std::is_same<T, uint16_t>::value)
+    return kv_bf16(v);
+  else
+    return static_cast<float>(v);
+}
+// A value of a load's raw words.
+template <typename T>
+__device__ __forceinline__ float beam_value(const u32x4 &raw, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i]);
+  const uint32_t w = raw[i / 2];
+  if constexpr (std::is_same<T, uint16_t>::value) return __uint_as_float(i % 2 ? w & 0xFFFF0000u : w << 16);
+  return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(i % 2 ? w >> 16 : w)));
+}
+
+// One workgroup for a chunk of one beam's logits, which are read once, all loads in
+// flight, and stay in registers as they are stored.  They give the largest, the sum of
+// exponentials against it and the chunk's k best.  A bound that at least k of them
+// reach: the k-th largest of 64 maxima, one for each lane over the four waves; of what lies
+// below it nothing more is asked, eight values at a time.  The few that reach it are put
+// in order by counting.  Where they are many (logits that are equal, or in an order that puts
+// the largest side by side) the k-th largest itself is found by halving.  The workgroup
+// that comes last of a request's joins the chunks, in the same manner.
+template <typename T, int N>
+__global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
+  constexpr int G = 16 / sizeof(T);  // values of a load, of which a thread has N
+  extern __shared__ uint64_t shared[];
+  uint64_t *const list = shared;
+  u32x4 *const load_of = reinterpret_cast<u32x4 *>(list + kBeamList);
+  int32_t *const load_at = reinterpret_cast<int32_t *>(load_of + kBeamList);
+  __shared__ uint32_t column[4][64];
+  __shared__ double wave_sum[4], total[64], score[64];
+  __shared__ bool over[64];
+  __shared__ uint32_t shared_bound;
+  __shared__ uint64_t result[RNSMX_BEAMS_MAX + 2];
+  __shared__ int32_t count, loads, digit[4], last;
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t id = blockIdx.x;
   const int32_t split = kv_rem(a.by_splits, id), beam = kv_rem(a.by_beams, id), place = id, request = a.first + place;
   const int32_t k = a.k, lists = a.beams * a.splits;
-  const int64_t row = static_cast<int64_t>(request) * a.beams + beam;
+  const int64_t row = static_cast<int64_t>(request) * a.beams + beam, row0 = static_cast<int64_t>(request) * a.beams;
   uint64_t *to = a.partial + (row * a.splits + split) * (k + 2);
-  auto put = [&](int32_t i, uint64_t v) { __hip_atomic_store(to + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  if (tid == 0) count = loads = 0;
 
   if (!(a.finished && a.finished[row])) {
     const T *p = static_cast<const T *>(a.logits) + request * a.request_stride + beam * a.beam_stride;
     const int32_t before = static_cast<int32_t>(reinterpret_cast<uintptr_t>(p) / sizeof(T) % G);  // to the load's boundary
-    const int64_t first = static_cast<int64_t>(split) * kBeamChunk - before;
-    float x[kBeamValues];
-    uint32_t there = 0;  // a bit a value
+    const int64_t first = static_cast<int64_t>(split) * a.chunk - before;
+    const int64_t end = min(first + a.chunk, static_cast<int64_t>(a.vocabulary));
+    // what is past the row's ends is as little a candidate as minus infinity
+    constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, uint16_t>::value ? 0xFF80FF80u : 0xFC00FC00u;
+    u32x4 raw[N];
+    const T *const base = p + first;
+    const int32_t low = first < 0 ? 1 : 0, high = static_cast<int32_t>(end - first) - G;  // where whole loads may start
     kv_for<N>([&](auto J) {
-      constexpr int j = J;
-      const int64_t e = first + (j * 256 + tid) * G;
-      T v[G];
-      if (e >= 0 && e + G <= a.vocabulary) {
-        *reinterpret_cast<u32x4 *>(v) = *reinterpret_cast<const u32x4 *>(p + e);
-        there |= ((1u << G) - 1u) << (j * G);
-      } else {
-        kv_for<G>([&](auto I) {
-          const bool in = e + I >= 0 && e + I < a.vocabulary;
-          v[I] = in ? p[e + I] : T(0);
-          there |= in ? 1u << (j * G + I) : 0u;
-        });
-      }
-      kv_for<G>([&](auto I) {
-        if constexpr (std::is_same<T, uint16_t>::value)
-          x[j * G + I] = kv_bf16(v[I]);
-        else
-          x[j * G + I] = static_cast<float>(v[I]);
+      const int32_t e = (J * 256 + tid) * G;
+      raw[J] = u32x4{none, none, none, none};
+      if (e >= low && e <= high) raw[J] = *reinterpret_cast<const u32x4 *>(base + e);
+    });
+    // the values before the row's first whole load and after its last, one a lane
+    float edge = -INFINITY;
+    int64_t edge_at = 0;
+    {
+      const int64_t head = before ? min(static_cast<int64_t>(G - before), end) : 0;  // values of the first
+      const int64_t tail = (end + before) / G * G - before;                           // where the last begin
+      edge_at = lane < 16 ? lane : tail + lane - 16;
+      const bool there = lane < 16 ? split == 0 && edge_at < head : split == a.splits - 1 && tail >= head && edge_at < end;
+      if (wave == 0 && there) edge = beam_float(p[edge_at]);
+    }
+    auto place_of = [&](int j, int i) { return (j * 256 + tid) * G + i; };  // in the chunk
+    const int32_t edge_place = static_cast<int32_t>(edge_at - first);
+    // f(value, place in the chunk)
+    auto each = [&](auto &&f) {
+      kv_for<N>([&](auto J) { kv_for<G>([&](auto I) { f(beam_value<T>(raw[J], I), place_of(J, I)); }); });
+      f(edge, edge_place);
+    };
+    float top[N], most = -INFINITY;
+    kv_for<N>([&](auto J) {
+      top[J] = beam_value<T>(raw[J], 0);
+      kv_for<G - 1>([&](auto I) { top[J] = fmaxf(top[J], beam_value<T>(raw[J], I + 1)); });
+      most = fmaxf(most, top[J]);
+    });
+    most = fmaxf(most, edge);
+    column[wave][lane] = beam_key(most);
+    // The values stay as they are stored, and what is asked of them is asked anew each time:
+    // 64 values or answers more would halve the waves that the registers hold.
+    auto keep_raw = [&]() {
+      kv_for<N>([&](auto J) {
+        u32x4 &words = raw[J];
+        asm volatile("" : "+v"(words));
       });
-    });
-    uint32_t top = 0;
-    kv_for<kBeamValues>([&](auto I) { top = max(top, there >> I & 1u ? beam_key(x[I]) : 0u); });
-    uint32_t most = top;
-    kv_for<6>([&](auto I) { most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 1 << I))); });
-    // the k-th largest lane maximum, from its highest bit down
-    uint32_t bound = 0;
-    for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
-      const int32_t n = __popcll(__ballot(top >= (bound | bit)));
-      if (n >= k) bound |= bit;
-      if (n == k) break;
-    }
-    if (lane == 0) {
-      wave_key[wave] = most;
-      wave_bound[wave] = bound;
-    }
-    if (tid == 0) count = 0;
+    };
+    keep_raw();
     __syncthreads();
-    most = max(max(wave_key[0], wave_key[1]), max(wave_key[2], wave_key[3]));
-    bound = max(max(wave_bound[0], wave_bound[1]), max(wave_bound[2], wave_bound[3]));
-    const float largest = most == 0 ? -INFINITY : beam_logit(most), reference = largest == -INFINITY ? 0.0f : largest;
-    float part = 0.0f;
-    kv_for<kBeamValues>([&](auto I) {
-      part += there >> I & 1u ? __builtin_amdgcn_exp2f((x[I] - reference) * kKvLog2e) : 0.0f;
-    });
-    double sum = part;
+    const uint32_t mine = max(max(column[0][lane], column[1][lane]), max(column[2][lane], column[3][lane]));
+    const float largest = beam_logit(beam_wave_max(mine)), reference = largest == -INFINITY ? 0.0f : largest;
+    if (wave == 0) {
+      const uint32_t bound = beam_bound(mine, k);
+      if (lane == 0) shared_bound = bound;
+    }
+    float part[2] = {0.0f, 0.0f};
+    each([&](float x, int32_t at) { part[at & 1] += __builtin_amdgcn_exp2f((x - reference) * kKvLog2e); });
+    double sum = static_cast<double>(part[0]) + part[1];
     kv_for<6>([&](auto I) { sum += __shfl_xor(sum, 1 << I); });
     if (lane == 0) wave_sum[wave] = sum;
-    // those above the bound, and, where they are few, those at it
-    uint32_t above = 0, equal = 0;
-    kv_for<kBeamValues>([&](auto I) {
-      const uint32_t key = beam_key(x[I]);
-      above |= (there >> I & 1u) && key > bound ? 1u << I : 0u;
-      equal |= (there >> I & 1u) && key == bound ? 1u << I : 0u;
-    });
-    auto token = [&](int32_t i) { return static_cast<uint32_t>(first + ((i / G) * 256 + tid) * G + i % G); };
-    auto enter = [&](uint32_t which) {
-      if (which != 0) {
-        int32_t at = atomicAdd(&count, __popc(which));
-        kv_for<kBeamValues>([&](auto I) {
-          if (which >> I & 1u) list[at++] = static_cast<uint64_t>(beam_key(x[I])) << 32 | ~token(I);
-        });
-      }
+    keep_raw();
+    __syncthreads();
+    auto enter = [&](float x, int32_t place) {
+      const int32_t at = atomicAdd(&count, 1);
+      if (at < kBeamList) list[at] = static_cast<uint64_t>(beam_key(x)) << 32 | ~static_cast<uint32_t>(first + place);
     };
-    enter(above);
-    __syncthreads();
-    const int32_t larger = count;
-    const double chunk_sum = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
-    __syncthreads();
-    // equal ones: as many as there are, counted together with the larger
-    if (larger < k) {
-      if (equal != 0) atomicAdd(&count, __popc(equal));
-      __syncthreads();
-      const int32_t all = count;
-      __syncthreads();
-      if (tid == 0) count = larger;
-      __syncthreads();
-      if (all > beam_list(k)) {
-        // too many: the k lowest tokens of them, by halving
-        int32_t low = -1, high = kBeamChunk - 1;  // in the chunk; k of them lie up to `high`
-        while (high - low > 1) {
-          const int32_t mid = (low + high) >> 1;
-          int32_t n = 0;
-          kv_for<kBeamValues>([&](auto I) {
-            constexpr int i = I;
-            n += (equal >> i & 1u) && ((i / G) * 256 + tid) * G + i % G <= mid ? 1 : 0;
-          });
-          if (tid == 0) last = 0;
-          __syncthreads();
-          if (n != 0) atomicAdd(&last, n);
-          __syncthreads();
-          if (last >= k)
-            high = mid;
-          else
-            low = mid;
-          __syncthreads();
+    // whole loads with one that reaches the bound, then their values, one a thread
+    const float least = shared_bound > kBeamNone ? beam_logit(shared_bound) : -INFINITY;
+    kv_for<N>([&](auto J) {
+      if (top[J] >= least && top[J] > -INFINITY) {
+        const int32_t at = atomicAdd(&loads, 1);
+        if (at < kBeamList) {
+          load_of[at] = raw[J];
+          load_at[at] = J * 256 + tid;
         }
-        kv_for<kBeamValues>([&](auto I) {
-          constexpr int i = I;
-          if (((i / G) * 256 + tid) * G + i % G > high) equal &= ~(1u << i);
-        });
       }
-      enter(equal);
+    });
+    if (edge >= least && edge > -INFINITY) enter(edge, edge_place);
+    __syncthreads();
+    const int32_t held = loads;
+    for (int32_t i = tid; i < min(held, kBeamList) * G; i += 256) {
+      const float x = beam_float(reinterpret_cast<const T *>(load_of)[i]);
+      if (x >= least && x > -INFINITY) enter(x, load_at[i / G] * G + i % G);
+    }
+    __syncthreads();
+    int32_t n = count;
+    if (held > kBeamList || n > kBeamList) {
+      // Digit by digit the key of the k-th largest, and how many that are it belong to the k.
+      const int32_t size = static_cast<int32_t>(end - first);
+      auto key_at = [&](int32_t i) {
+        const int64_t e = first + i;
+        return e >= 0 && i < size ? beam_key(beam_float(p[e])) : 0u;
+      };
+      int32_t *const bins = reinterpret_cast<int32_t *>(column);
+      uint32_t kth = 0;
+      int32_t wanted = k;
+      for (int32_t shift = 24; shift >= 0; shift -= 8) {
+        bins[tid] = 0;
+        __syncthreads();
+        for (int32_t i = tid; i < size; i += 256) {
+          const uint32_t key = key_at(i);
+          if (key > kBeamNone && (shift == 24 || key >> (shift + 8) == kth >> (shift + 8))) atomicAdd(&bins[key >> shift & 255], 1);
+        }
+        __syncthreads();
+        int32_t larger = 0;
+        for (int32_t j = tid + 1; j < 256; ++j) larger += bins[j];
+        if (larger < wanted && wanted <= larger + bins[tid]) {
+          digit[0] = tid;
+          digit[1] = wanted - larger;
+        }
+        __syncthreads();
+        kth |= static_cast<uint32_t>(digit[0]) << shift;
+        wanted = digit[1];
+      }
+      if (tid == 0) count = 0;
       __syncthreads();
+      // the larger ones, and in the order of the tokens as many equal ones as are wanted
+      int32_t before_these = 0;
+      for (int32_t i0 = 0; i0 < size; i0 += 256) {
+        const uint32_t key = key_at(i0 + tid);
+        if (key > kth) enter(beam_logit(key), i0 + tid);
+        if (before_these >= wanted) continue;
+        const uint64_t equal = __ballot(key == kth);
+        __syncthreads();
+        if (lane == 0) digit[wave] = __popcll(equal);
+        __syncthreads();
+        int32_t rank = before_these + __popcll(equal & ((1ull << lane) - 1));
+        for (int32_t w = 0; w < 4; ++w) {
+          rank += w < wave ? digit[w] : 0;
+          before_these += digit[w];
+        }
+        if (key == kth && rank < wanted) enter(beam_logit(key), i0 + tid);
+      }
+      __syncthreads();
+      n = count;
     }
-    const int32_t n = count;
-    for (int32_t i = tid; i < n; i += 256) {
-      const uint64_t mine = list[i];
-      int32_t rank = 0;
-      for (int32_t j = 0; j < n; ++j) rank += list[j] > mine ? 1 : 0;
-      if (rank < k) put(rank, mine);
+    for (int32_t i = tid >> 2; i < n; i += 64) {  // four lanes an item
+      const uint64_t item = list[i];
+      const int32_t rank = beam_larger(list, n, item);
+      if (rank < k && (tid & 3) == 0) result[rank] = item;
     }
-    for (int32_t i = n + tid; i < k; i += 256) put(i, 0);
+    if (tid >= n && tid < k) result[tid] = 0;
     if (tid == 0) {
-      put(k, __float_as_uint(largest));
-      put(k + 1, __builtin_bit_cast(uint64_t, chunk_sum));
+      result[k] = __float_as_uint(largest);
+      result[k + 1] = __builtin_bit_cast(uint64_t, wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3]);
     }
+    __syncthreads();
+    if (tid < k + 2) __hip_atomic_store(to + tid, result[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 
   // The last workgroup of a request (kv_rows_kernel has the protocol).
@@ -198,108 +289,244 @@ __global__ __launch_bounds__(256) void beam_kernel(const BeamArgs a) {
     const uint32_t old = __hip_atomic_fetch_add(a.tickets + place, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     last = old == static_cast<uint32_t>(lists - 1);
     if (last) __hip_atomic_store(a.tickets + place, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    count = 0;
   }
   __syncthreads();
   if (!last) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  const int64_t row0 = static_cast<int64_t>(request) * a.beams;
+  // The chunks' results are read past this XCD's caches, each once: a fence that drops what
+  // the caches hold would cost some 20 us with 64 requests joining at once.
   const uint64_t *from = a.partial + row0 * a.splits * (k + 2);
-
-  // each beam's logarithm of its exponentials' sum; not a number: no candidates
-  for (int32_t b = wave; b < a.beams; b += 4) {
-    if (a.finished && a.finished[row0 + b]) continue;
-    float largest = -INFINITY;
-    bool bad = false;
-    for (int32_t s = lane; s < a.splits; s += 64) {
-      const float m = __uint_as_float(static_cast<uint32_t>(from[(b * a.splits + s) * static_cast<int64_t>(k + 2) + k]));
-      bad = bad || m != m;
-      largest = fmaxf(largest, m);
-    }
-    kv_for<6>([&](auto I) { largest = fmaxf(largest, __shfl_xor(largest, 1 << I)); });
-    double sum = 0.0;
-    for (int32_t s = lane; s < a.splits; s += 64) {
-      const uint64_t *e = from + (b * a.splits + s) * static_cast<int64_t>(k + 2) + k;
-      const float m = __uint_as_float(static_cast<uint32_t>(e[0]));
-      const double v = __builtin_bit_cast(double, e[1]);
-      sum += m == -INFINITY ? v : v * exp(static_cast<double>(m) - static_cast<double>(largest));
-    }
-    kv_for<6>([&](auto I) { sum += __shfl_xor(sum, 1 << I); });
-    const bool dead = __any(bad) || !(fabsf(largest) < INFINITY);
-    if (lane == 0) total[b] = dead ? __builtin_nan("") : static_cast<double>(largest) + log(sum);
+  auto get = [&](int32_t i, int32_t n) {
+    return __hip_atomic_load(from + static_cast<int64_t>(i) * (k + 2) + n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  const int64_t out = static_cast<int64_t>(request) * k;
+  // few results are all held in shared memory, of many each chunk's best
+  const bool whole = lists * (k + 2) <= kBeamHeld;
+  const int32_t each_held = whole ? k + 2 : 1;
+  uint64_t *const held = shared, *const key_of = held + lists * each_held, *const item_of = key_of + kBeamList;
+  double *const sums = reinterpret_cast<double *>(item_of + kBeamList);
+  float *const tops = reinterpret_cast<float *>(sums + lists);
+  int32_t *const beam_of = reinterpret_cast<int32_t *>(tops + lists), *const chosen = beam_of + kBeamList;
+  if (whole) {
+    for (int32_t i = tid; i < lists * (k + 2); i += 256)
+      held[i] = __hip_atomic_load(from + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
   }
-  for (int32_t i = tid; i < lists; i += 256) taken[i] = 0;
+  auto item_at = [&](int32_t i, int32_t n) { return whole ? held[i * (k + 2) + n] : n == 0 ? held[i] : get(i, n); };
+  for (int32_t i = tid; i < lists; i += 256) {
+    uint32_t b = i;
+    const int32_t s = kv_rem(a.by_splits, b);
+    if (a.finished && a.finished[row0 + b]) {  // one candidate, the beam itself
+      held[i * each_held] = s == 0 ? ~static_cast<uint32_t>(a.end_token) : 0;
+    } else {
+      const uint64_t m = whole ? held[i * (k + 2) + k] : get(i, k), v = whole ? held[i * (k + 2) + k + 1] : get(i, k + 1);
+      if (!whole) held[i] = get(i, 0);
+      tops[i] = __uint_as_float(static_cast<uint32_t>(m));
+      sums[i] = __builtin_bit_cast(double, v);
+    }
+  }
   __syncthreads();
 
-  // k rounds: each thread offers the best of its chunks' next ones
+  // each beam's logarithm of its exponentials' sum, by sixteen lanes
+  for (int32_t b0 = 0; b0 < a.beams; b0 += 16) {
+    const int32_t b = b0 + (tid >> 4), in_group = tid & 15;
+    const bool ended = b < a.beams && a.finished && a.finished[row0 + b];
+    const int32_t first = b * a.splits, chunks = b < a.beams && !ended ? a.splits : 0;
+    float largest = -INFINITY;
+    for (int32_t s = in_group; s < chunks; s += 16) largest = fmaxf(largest, tops[first + s]);
+    kv_for<4>([&](auto I) { largest = fmaxf(largest, __shfl_xor(largest, 1 << I)); });
+    double sum = 0.0;
+    for (int32_t s = in_group; s < chunks; s += 16) {
+      const float m = tops[first + s];
+      // a chunk without anything above minus infinity has a sum of 0, or not-a-numbers
+      sum += m == -INFINITY ? sums[first + s] : sums[first + s] * exp(static_cast<double>(m) - static_cast<double>(largest));
+    }
+    kv_for<4>([&](auto I) { sum += __shfl_xor(sum, 1 << I); });
+    if (in_group == 0 && b < a.beams) {
+      total[b] = static_cast<double>(largest) + log(sum);
+      score[b] = a.scores[row0 + b];
+      over[b] = ended;
+    }
+  }
+  __syncthreads();
+
   struct Offer {
     uint64_t key;   // of the score, 0: none
-    uint64_t item;  // key of the logit and the token, as the lists have them
-    int32_t beam, list;
+    uint64_t item;  // key of the logit and the token, as the chunks have them
+    int32_t beam, chunk;
   };
   auto better = [](const Offer &p, const Offer &q) {
     if (p.key != q.key) return p.key > q.key;
     if (p.beam != q.beam) return p.beam < q.beam;
     return p.item > q.item;
   };
-  auto offer = [&]() {
-    Offer best{0, 0, INT_MAX, 0};
-    for (int32_t i = tid; i < lists; i += 256) {
-      const int32_t b = i / a.splits, s = i - b * a.splits, n = taken[i];
-      const double score = a.scores[row0 + b];
-      Offer o{0, 0, b, i};
-      if (a.finished && a.finished[row0 + b]) {
-        if (s != 0 || n != 0) continue;
-        o.item = ~static_cast<uint32_t>(a.end_token);
-        o.key = fabs(score) < INFINITY ? beam_score_key(score) : 0;
-      } else {
-        if (n >= k) continue;
-        o.item = from[i * static_cast<int64_t>(k + 2) + n];
-        const double v = score + (static_cast<double>(beam_logit(static_cast<uint32_t>(o.item >> 32))) - total[b]);
-        o.key = o.item != 0 && fabs(v) < INFINITY ? beam_score_key(v) : 0;
-      }
-      if (o.key != 0 && better(o, best)) best = o;
-    }
-    return best;
+  auto offer = [&](int32_t i, uint64_t item) {  // an item of chunk i
+    const int32_t b = static_cast<int32_t>(kv_quot(a.by_splits, i));
+    Offer o{0, item, b, i};
+    if (item == 0) return o;
+    const double v = over[b] ? score[b] : score[b] + (static_cast<double>(beam_logit(static_cast<uint32_t>(item >> 32))) - total[b]);
+    o.key = fabs(v) < INFINITY ? beam_score_key(v) : 0;
+    return o;
   };
-  Offer mine = offer();
+  auto write = [&](int32_t j, const Offer &o) {
+    a.out_scores[out + j] = static_cast<float>(beam_score(o.key));
+    a.out_tokens[out + j] = static_cast<int32_t>(~static_cast<uint32_t>(o.item));
+    a.out_parents[out + j] = static_cast<int32_t>(row0) + o.beam;
+  };
+
+  // The chunks' best give the bound where they are as many as are wanted; only chunks whose
+  // best reaches it are looked at further.
+  auto settle = [&](uint32_t most) {
+    column[wave][lane] = most;
+    __syncthreads();
+    if (wave == 0) {
+      const uint32_t bound =
+          beam_bound(max(max(column[0][lane], column[1][lane]), max(column[2][lane], column[3][lane])), k);
+      if (lane == 0) shared_bound = max(bound, 1u);
+    }
+    __syncthreads();
+  };
+  uint32_t most_here = 0;
+  for (int32_t i = tid; i < lists; i += 256)
+    most_here = max(most_here, static_cast<uint32_t>(offer(i, held[i * each_held]).key >> 32));
+  if (tid == 0) loads = 0;
+  settle(most_here);
+  for (int32_t i = tid; i < lists; i += 256)
+    if (static_cast<uint32_t>(offer(i, held[i * each_held]).key >> 32) >= shared_bound) chosen[atomicAdd(&loads, 1)] = i;
+  __syncthreads();
+  // f(offer) for every result of the chunks chosen, four loads at a time
+  const int32_t offers = loads * k;
+  auto offered = [&](auto &&f) {
+    for (int32_t i0 = tid; i0 < offers; i0 += 4 * 256) {
+      uint64_t item[4];
+      int32_t chunk[4];
+      kv_for<4>([&](auto U) {
+        uint32_t q = min(i0 + 256 * U, offers - 1);
+        const int32_t n = kv_rem(a.by_k, q);
+        chunk[U] = chosen[q];
+        item[U] = n > 0 && over[kv_quot(a.by_splits, chunk[U])] ? 0 : item_at(chunk[U], n);
+      });
+      kv_for<4>([&](auto U) {
+        if (i0 + 256 * U < offers) f(offer(chunk[U], item[U]));
+      });
+    }
+  };
+  auto collect = [&]() {
+    const uint32_t least = shared_bound;
+    offered([&](const Offer &o) {
+      if (static_cast<uint32_t>(o.key >> 32) >= least) {
+        const int32_t at = atomicAdd(&count, 1);
+        if (at < kBeamList) {
+          key_of[at] = o.key;
+          item_of[at] = o.item;
+          beam_of[at] = o.beam;
+        }
+      }
+    });
+    __syncthreads();
+  };
+  collect();
+  if (count > kBeamList) {  // few chunks more than are wanted give a low bound: all of theirs a higher one
+    most_here = 0;
+    offered([&](const Offer &o) { most_here = max(most_here, static_cast<uint32_t>(o.key >> 32)); });
+    __syncthreads();
+    if (tid == 0) count = 0;
+    settle(most_here);
+    collect();
+  }
+  const int32_t n = count;
+  if (n <= kBeamList) {
+    if (n > 64) {  // what the best of a lane's each reach, k of them, is as high as needs be
+      most_here = 0;
+      for (int32_t i = tid; i < n; i += 256) most_here = max(most_here, static_cast<uint32_t>(key_of[i] >> 32));
+      settle(most_here);
+    }
+    for (int32_t i = tid >> 2; i < n; i += 64) {  // four lanes an offer
+      const Offer o{key_of[i], item_of[i], beam_of[i], 0};
+      if (static_cast<uint32_t>(o.key >> 32) < shared_bound) continue;
+      int32_t rank = 0;
+      for (int32_t j0 = tid & 3; j0 < n; j0 += 16) {
+        uint64_t key[4];
+        kv_for<4>([&](auto U) { key[U] = key_of[min(j0 + 4 * U, n - 1)]; });
+        kv_for<4>([&](auto U) {
+          const int32_t j = j0 + 4 * U;
+          if (j < n) rank += key[U] > o.key || (key[U] == o.key && better(Offer{key[U], item_of[j], beam_of[j], 0}, o)) ? 1 : 0;
+        });
+      }
+      kv_for<2>([&](auto I) { rank += __shfl_xor(rank, 1 << I); });
+      if (rank < k && (tid & 3) == 0) write(rank, o);
+    }
+    for (int32_t j = n + tid; j < k; j += 256) {
+      a.out_scores[out + j] = -INFINITY;
+      a.out_tokens[out + j] = max(a.end_token, 0);
+      a.out_parents[out + j] = static_cast<int32_t>(row0) + j % a.beams;
+    }
+    return;
+  }
+  // Too many that are equal, and more than are wanted: k rounds, in which each thread
+  // offers the best of its chunks' next ones.
+  int32_t *const taken = chosen;
+  __syncthreads();
+  for (int32_t i = tid; i < lists; i += 256) taken[i] = 0;
+  __syncthreads();
+  auto next = [&]() {
+    Offer most{0, 0, INT_MAX, 0};
+    for (int32_t i = tid; i < lists; i += 256)
+      if (taken[i] < (over[kv_quot(a.by_splits, i)] ? 1 : k)) {
+        const Offer o = offer(i, item_at(i, taken[i]));
+        if (o.key != 0 && better(o, most)) most = o;
+      }
+    return most;
+  };
+  Offer mine = next();
   __shared__ Offer wave_best[4];
   for (int32_t j = 0; j < k; ++j) {
-    Offer best = mine;
+    Offer most = mine;
     kv_for<6>([&](auto I) {
-      Offer o{beam_shuffle(best.key, 1 << I), beam_shuffle(best.item, 1 << I), __shfl_xor(best.beam, 1 << I), __shfl_xor(best.list, 1 << I)};
-      if (better(o, best)) best = o;
+      auto other = [&](uint64_t v) { return static_cast<uint64_t>(__shfl_xor(static_cast<long long>(v), 1 << I)); };
+      const Offer o{other(most.key), other(most.item), __shfl_xor(most.beam, 1 << I), __shfl_xor(most.chunk, 1 << I)};
+      if (better(o, most)) most = o;
     });
-    if (lane == 0) wave_best[wave] = best;
+    if (lane == 0) wave_best[wave] = most;
     __syncthreads();
     kv_for<4>([&](auto W) {
-      if (better(wave_best[W], best)) best = wave_best[W];
+      if (better(wave_best[W], most)) most = wave_best[W];
     });
-    const int64_t at = static_cast<int64_t>(request) * k + j;
-    if (best.key == 0) {  // nothing left: this place and those after it have none
-      if (tid < k - j) {
-        a.out_scores[at + tid] = -INFINITY;
-        a.out_tokens[at + tid] = max(a.end_token, 0);
-        a.out_parents[at + tid] = static_cast<int32_t>(row0) + (j + tid) % a.beams;
-      }
-      break;
-    }
-    if (tid == 0) {
-      const uint64_t u = best.key;
-      a.out_scores[at] = static_cast<float>(__builtin_bit_cast(double, u >> 63 ? u ^ 0x8000000000000000ull : ~u));
-      a.out_tokens[at] = static_cast<int32_t>(~static_cast<uint32_t>(best.item));
-      a.out_parents[at] = static_cast<int32_t>(row0) + best.beam;
-    }
-    if (best.list == mine.list && mine.key != 0) {
-      ++taken[mine.list];
-      mine = offer();
+    if (tid == 0) write(j, most);
+    if (most.chunk == mine.chunk && mine.key != 0) {
+      ++taken[mine.chunk];
+      mine = next();
     }
     __syncthreads();
   }
 }
 
-static int32_t beam_splits(int32_t vocabulary) {
-  // a row starts up to seven values into its first load
-  return static_cast<int32_t>((static_cast<int64_t>(vocabulary) + 7 + kBeamChunk - 1) / kBeamChunk);
+// Bytes of a workgroup's shared memory: what its own values need, or the join of `lists` chunks.
+static size_t beam_shared(int64_t lists, int32_t k) {
+  const int64_t held = lists * (k + 2) <= kBeamHeld ? lists * (k + 2) : lists;
+  return std::max<size_t>(kBeamList * (8 + 16 + 4), held * 8 + lists * (8 + 4 + 4) + kBeamList * (8 + 8 + 4));
+}
+
+// Chunks of a beam: as many as give the chip kBeamGroups workgroups, but no smaller than
+// kBeamLeast values and no larger than the registers hold.
+constexpr int64_t kBeamGroups = 1024, kBeamLeast = 4096;
+static void beam_chunks(const rnsmx_beams_t &b, int32_t &chunk, int32_t &splits) {
+  const int64_t per = b.dtype == RNSMX_FLOAT32 ? 4 : 8, values = b.vocabulary + per;  // a row may start inside a load
+  const int64_t rows = std::max<int64_t>(static_cast<int64_t>(b.requests) * b.beams, 1);
+  const int64_t least = (values + kBeamMost - 1) / kBeamMost, most = (values + kBeamLeast - 1) / kBeamLeast;
+  const int64_t n = std::max(least, std::min({most, kBeamGroups / rows, kBeamChunks / static_cast<int64_t>(b.beams)}));
+  chunk = static_cast<int32_t>(round_up((values + n - 1) / n, per));
+  splits = static_cast<int32_t>((values + chunk - 1) / chunk);
+}
+
+// The kernel of the fewest loads a thread that take a chunk, by eighths of the most.
+template <typename T, int N = kBeamMost / 256 * static_cast<int>(sizeof(T)) / 16>
+static void launch_beams(const BeamArgs &a, dim3 grid, size_t shared, hipStream_t st) {
+  constexpr int step = sizeof(T) == 4 ? 2 : 1, values = 256 * 16 / static_cast<int>(sizeof(T));
+  if constexpr (N > step) {
+    if (a.chunk <= (N - step) * values) return launch_beams<T, N - step>(a, grid, shared, st);
+  }
+  hipLaunchKernelGGL((beam_kernel<T, N>), grid, dim3(256), shared, st, a);
 }
 
 static int32_t beam_check(const rnsmx_beams_t *b) {
@@ -309,7 +536,9 @@ static int32_t beam_check(const rnsmx_beams_t *b) {
   if (b->requests < 0 || b->beams < 1 || b->beams > RNSMX_BEAMS_MAX || b->vocabulary < 1 || b->k < 1 || b->k > RNSMX_BEAMS_MAX)
     return fail(RNSMX_EINVAL, "1 to 64 beams, 1 to 64 continuations, at least one token");
   if (b->request_stride < 0 || b->beam_stride < 0) return fail(RNSMX_EINVAL, "negative strides");
-  if (static_cast<int64_t>(b->beams) * beam_splits(b->vocabulary) > kBeamLists) return fail(RNSMX_EINVAL, "too many tokens and beams");
+  int32_t chunk, splits;
+  beam_chunks(*b, chunk, splits);
+  if (static_cast<int64_t>(b->beams) * splits > kBeamChunks) return fail(RNSMX_EINVAL, "too many tokens and beams");
   if (static_cast<int64_t>(b->requests) * b->beams > 0x7FFFFFFFLL) return fail(RNSMX_EINVAL, "too many requests and beams");
   return RNSMX_OK;
 }
@@ -323,8 +552,9 @@ extern "C" {
 int64_t rnsmx_beam_workspace_bytes(const rnsmx_beams_t *beams) {
   clear_error();
   if (beam_check(beams)) return -1;
-  return RNSMX_KV_TICKETS * 4 +
-         static_cast<int64_t>(beams->requests) * beams->beams * beam_splits(beams->vocabulary) * (beams->k + 2) * 8;
+  int32_t chunk, splits;
+  beam_chunks(*beams, chunk, splits);
+  return RNSMX_KV_TICKETS * 4 + static_cast<int64_t>(beams->requests) * beams->beams * splits * (beams->k + 2) * 8;
 }
 
 int32_t rnsmx_beam_select(const rnsmx_beams_t *beams, const void *logits_dev, const float *scores_dev, const uint8_t *finished_dev,
@@ -356,10 +586,11 @@ int32_t rnsmx_beam_select(const rnsmx_beams_t *beams, const void *logits_dev, co
   a.beams = beams->beams;
   a.vocabulary = beams->vocabulary;
   a.k = beams->k;
-  a.splits = beam_splits(beams->vocabulary);
+  beam_chunks(*beams, a.chunk, a.splits);
   a.end_token = beams->end_token;
   a.by_splits = kv_div(a.splits);
   a.by_beams = kv_div(a.beams);
+  a.by_k = kv_div(a.k);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t lists = static_cast<int64_t>(a.beams) * a.splits;
   // a ticket a request, and fewer than 2^32 threads
@@ -367,13 +598,13 @@ int32_t rnsmx_beam_select(const rnsmx_beams_t *beams, const void *logits_dev, co
   for (int64_t first = 0; first < beams->requests; first += most) {
     a.first = static_cast<int32_t>(first);
     const dim3 grid(static_cast<unsigned>(std::min(most, beams->requests - first) * lists));
-    const size_t shared = std::max<size_t>(static_cast<size_t>(beam_list(a.k)) * 8, lists);
+    const size_t shared = beam_shared(lists, a.k);
     if (beams->dtype == RNSMX_FLOAT32)
-      hipLaunchKernelGGL(beam_kernel<float>, grid, dim3(256), shared, st, a);
+      launch_beams<float>(a, grid, shared, st);
     else if (beams->dtype == RNSMX_FLOAT16)
-      hipLaunchKernelGGL(beam_kernel<_Float16>, grid, dim3(256), shared, st, a);
+      launch_beams<_Float16>(a, grid, shared, st);
     else
-      hipLaunchKernelGGL(beam_kernel<uint16_t>, grid, dim3(256), shared, st, a);
+      launch_beams<uint16_t>(a, grid, shared, st);
   }
   const hipError_t err = hipGetLastError();
   if (err == hipSuccess) return RNSMX_OK;

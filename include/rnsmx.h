@@ -621,7 +621,8 @@ typedef struct rnsmx_kv_pool {
   int32_t *table_dev;   /* [seqs][width], -1 where there is no page           */
   int32_t *lengths_dev; /* [seqs] tokens                                      */
   int32_t *refs_dev;    /* [blocks] holders of each page                      */
-  uint32_t *free_dev;   /* [(blocks + 31) / 32] bit b % 32 of word b / 32: nobody holds b */
+  uint8_t *free_dev;    /* [blocks, rounded up to 16] 1: nobody holds the page; 0 past the last.
+                           On a 16-byte boundary                              */
   int32_t *scratch_dev; /* rnsmx_kv_pool_scratch_words: [blocks] of 0, [blocks] of 2^31 - 1, the
                            rest of any value; every call leaves them so          */
   int32_t blocks;

@@ -9,10 +9,11 @@ namespace rnsmx {
 
 struct PoolArgs {
   int32_t *table, *lengths, *refs;
-  uint32_t *free;               // a bit a page that nobody holds
-  int32_t *going, *first;       // scratch, [blocks] each: zeros and INT32_MAX between calls
+  uint8_t *free;                   // 1 where nobody holds a page, by sixteens (0 past the last)
+  int32_t *going, *first;          // scratch, [blocks] each: zeros and INT32_MAX between calls
+  int32_t *before;                 // scratch, [blocks]: free pages before each word of them
   int32_t *spare, *spare_lengths;  // scratch of kv_reorder: a table and lengths
-  int32_t blocks, words, log_page, seqs, width;
+  int32_t blocks, words, log_page, seqs, width;  // words: sixteens of pages
 };
 
 struct AssignArgs {
@@ -28,11 +29,13 @@ __device__ __forceinline__ int32_t pool_pages(const PoolArgs &p, int32_t n) {  /
 __device__ __forceinline__ bool pool_has(const PoolArgs &p, int32_t page) {
   return static_cast<uint32_t>(page) < static_cast<uint32_t>(p.blocks);
 }
-// A holder less; a page without one is free.
+// A holder less; a page without one is free.  A byte a page: bits would be set by
+// atomics, some 30 to a word where pages lie side by side, as those of prompts do (515
+// sequences with 18800 pages cut to nothing: 11.8 us).
 __device__ __forceinline__ void pool_drop(const PoolArgs &p, int32_t page) {
   if (!pool_has(p, page)) return;
   if (__hip_atomic_fetch_add(p.refs + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 1)
-    __hip_atomic_fetch_or(p.free + (page >> 5), 1u << (page & 31), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    p.free[page] = 1;
 }
 
 // Sums of N values a thread over the threads before it, and over all.
@@ -63,59 +66,74 @@ __device__ __forceinline__ void pool_scan(int64_t (&before)[N], int64_t (&all)[N
   });
 }
 
-constexpr int32_t kPoolPicked = 12288;  // page numbers of a round, 48 KB
-constexpr int32_t kPoolOwn = 2;         // pages of a sequence that its thread enters, a wave together the others
+constexpr int32_t kPoolPicked = 4096;  // page numbers in shared memory
+constexpr int32_t kPoolOwn = 2;        // pages of a sequence that its thread enters, a wave together the others
 constexpr int32_t kPoolMost = INT_MAX;
+
+// The free ones of sixteen pages, a bit each.
+__device__ __forceinline__ uint32_t pool_free(const PoolArgs &p, int32_t w) {
+  const u32x4 v = reinterpret_cast<const u32x4 *>(p.free)[w];
+  uint32_t bits = 0;
+  kv_for<4>([&](auto I) {  // bytes of 0 or 1 to four bits
+    constexpr int i = I;
+    bits |= ((v[i] | v[i] >> 7 | v[i] >> 14 | v[i] >> 21) & 15u) << (4 * i);
+  });
+  return bits;
+}
+
+struct PoolInfo {
+  int32_t seq, old, n, inside;  // tokens held, new, and of the held ones those on the last page
+  int32_t source;               // the page copied, -1: none
+  int32_t begin, need;          // pages wanted from column `begin` on
+  int32_t rank;                 // the first of them among all
+};
+__device__ __forceinline__ int32_t pool_room(const AssignArgs &a) { return min(a.p.width << a.p.log_page, a.max_length); }
+__device__ __forceinline__ PoolInfo pool_held(const AssignArgs &a, int32_t s) {
+  PoolInfo i{s, 0, 0, 0, -1, 0, 0, 0};
+  if (s < a.p.seqs) {
+    i.old = min(max(a.p.lengths[s], 0), a.p.width << a.p.log_page);
+    i.n = min(a.asked ? max(a.asked[s], 0) : 1, a.max_rows);
+    i.inside = i.old & ((1 << a.p.log_page) - 1);
+  }
+  return i;
+}
+// Its last page where it goes on in it and others hold it too.
+__device__ __forceinline__ int32_t pool_tail(const PoolArgs &p, const PoolInfo &i) {
+  if (i.n == 0 || i.inside == 0) return -1;
+  const int32_t t = p.table[static_cast<int64_t>(i.seq) * p.width + (i.old >> p.log_page)];
+  return pool_has(p, t) && p.refs[t] > 1 ? t : -1;
+}
+__device__ __forceinline__ void pool_want(const AssignArgs &a, PoolInfo &i) {
+  i.begin = pool_pages(a.p, i.old) - (i.source >= 0 ? 1 : 0);
+  i.need = i.n > 0 && i.n <= pool_room(a) - i.old ? pool_pages(a.p, i.old + i.n) - i.begin : 0;
+}
 
 // One workgroup for a call, as the pages of every sequence depend on those of all
 // before it.  What a call needs is counted before anything is changed, so one that
-// the pool has no room for changes nothing.
+// the pool has no room for changes nothing.  LOCAL: the page numbers go through shared
+// memory into the tables; else, where they may be more than it holds, through memory, and
+// kv_enter_kernel enters them.
 // Bound by its chain: lengths, tails' entries and counts, a sum over the workgroup,
-// page numbers through shared memory into the tables.
+// page numbers into the tables.
+template <bool LOCAL>
 __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
-  __shared__ int32_t picked[kPoolPicked];
+  __shared__ int32_t held[LOCAL ? kPoolPicked : 1];
   __shared__ int64_t sums[16][3];
   __shared__ int32_t any, past;
   const PoolArgs &p = a.p;
   const int32_t threads = blockDim.x, tid = threadIdx.x, lane = tid & 63;
-  const int32_t page = 1 << p.log_page, room = min(p.width << p.log_page, a.max_length);
+  const int32_t room = pool_room(a);
   const bool once = p.seqs <= threads;  // a sequence a thread, kept in registers
-
-  struct Info {
-    int32_t seq, old, n, inside;  // tokens held, new, and of the held ones those on the last page
-    int32_t source;               // the page copied, -1: none
-    int32_t begin, need;          // pages wanted from column `begin` on
-    int32_t rank;                 // the first of them among all
-  };
-  auto held = [&](int32_t s) {
-    Info i{s, 0, 0, 0, -1, 0, 0, 0};
-    if (s < p.seqs) {
-      i.old = min(max(p.lengths[s], 0), p.width << p.log_page);
-      i.n = min(a.asked ? max(a.asked[s], 0) : 1, a.max_rows);
-      i.inside = i.old & (page - 1);
-    }
-    return i;
-  };
-  // its last page where it goes on in it and others hold it too
-  auto tail_of = [&](const Info &i) {
-    if (i.n == 0 || i.inside == 0) return -1;
-    const int32_t t = p.table[static_cast<int64_t>(i.seq) * p.width + (i.old >> p.log_page)];
-    return pool_has(p, t) && p.refs[t] > 1 ? t : -1;
-  };
-  auto want = [&](Info &i) {
-    i.begin = pool_pages(p, i.old) - (i.source >= 0 ? 1 : 0);
-    i.need = i.n > 0 && i.n <= room - i.old ? pool_pages(p, i.old + i.n) - i.begin : 0;
-  };
 
   // this thread's words of the free pages
   const int32_t each = (p.words + threads - 1) / threads;
   const int32_t word0 = min(tid * each, p.words), word1 = min(word0 + each, p.words);
   if (tid == 0) any = past = 0;
   __syncthreads();
-  Info mine{};
+  PoolInfo mine{};
   for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
-    mine = held(s0 + tid);
-    mine.source = tail_of(mine);
+    mine = pool_held(a, s0 + tid);
+    mine.source = pool_tail(p, mine);
     if (mine.n > 0 && mine.n > room - mine.old) past = 1;
     if (mine.source >= 0) {
       any = 1;
@@ -124,14 +142,14 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
     }
   }
   int64_t wanted = 0, rows = 0, free_before = 0, free_all = 0;
-  for (int32_t w = word0; w < word1; ++w) free_before += __popc(p.free[w]);
+  for (int32_t w = word0; w < word1; ++w) free_before += __popc(pool_free(p, w));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   const bool shared = any != 0;
   for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
     if (!once) {
-      mine = held(s0 + tid);
-      mine.source = tail_of(mine);
+      mine = pool_held(a, s0 + tid);
+      mine.source = pool_tail(p, mine);
     }
     if (shared && mine.source >= 0) {
       // the first of a page's holders keeps it if all of them go on
@@ -139,7 +157,7 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
       const int32_t first = __hip_atomic_load(p.first + mine.source, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (going == p.refs[mine.source] && first == mine.seq) mine.source = -1;
     }
-    want(mine);
+    pool_want(a, mine);
     int64_t before[3] = {mine.need, mine.n, s0 == 0 ? free_before : 0}, total[3];
     pool_scan(before, total, sums);
     if (s0 == 0) {
@@ -165,11 +183,13 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
     if (a.starts) a.starts[p.seqs] = static_cast<int32_t>(min(rows, static_cast<int64_t>(kPoolMost)));
     *a.missing = missing;
   }
+  const bool ok = missing == 0;
+  const int32_t count = ok ? static_cast<int32_t>(wanted) : 0;
   __syncthreads();  // marks and counts are read by all before they change
   if (shared)
     for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
-      const Info i = held(s0 + tid);
-      const int32_t t = tail_of(i);
+      const PoolInfo i = pool_held(a, s0 + tid);
+      const int32_t t = pool_tail(p, i);
       if (t >= 0) {
         p.going[t] = 0;
         p.first[t] = INT_MAX;
@@ -177,77 +197,90 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
     }
   __syncthreads();
 
-  const bool ok = missing == 0;
-  const int32_t count = ok ? static_cast<int32_t>(wanted) : 0;
-  auto settled = [&](int32_t s) {
-    Info i = held(s);
-    if (s < p.seqs) {
-      i.source = a.copies[3 * static_cast<int64_t>(s)];
-      i.rank = a.copies[3 * static_cast<int64_t>(s) + 1];
-    }
-    want(i);
-    return i;
-  };
-  for (int32_t base = 0; base < count; base += kPoolPicked) {
-    const int32_t end = min(count, base + kPoolPicked);
+  // the lowest free pages, in their order
+  if constexpr (LOCAL) {
     int64_t rank = free_before;
-    for (int32_t w = word0; w < word1 && rank < end; ++w) {
-      uint32_t bits = p.free[w];
-      const int32_t n = __popc(bits);
-      if (rank + n > base)
-        for (int64_t r = rank; bits != 0 && r < end; ++r, bits &= bits - 1)
-          if (r >= base) {
-            const int32_t number = 32 * w + __ffs(bits) - 1;
-            picked[r - base] = number;
-            p.refs[number] = 1;
-          }
-      rank += n;
-    }
+    for (int32_t w = word0; w < word1 && rank < count; ++w)
+      for (uint32_t bits = pool_free(p, w); bits != 0 && rank < count; bits &= bits - 1) {
+        const int32_t number = 16 * w + __ffs(bits) - 1;
+        held[rank++] = number;
+        p.refs[number] = 1;
+        p.free[number] = 0;
+      }
     __syncthreads();
-    for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
-      if (!once) mine = settled(s0 + tid);
-      auto enter = [&](int32_t s, int32_t column, int32_t r) {
-        if (r >= base && r < end) p.table[static_cast<int64_t>(s) * p.width + column] = picked[r - base];
-      };
+  } else {
+    int64_t rank = free_before;
+    for (int32_t w = word0; w < word1; ++w) {
+      p.before[w] = static_cast<int32_t>(rank);
+      rank += __popc(pool_free(p, w));
+    }
+    if (tid == 0) p.spare[p.seqs] = count;
+  }
+  for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
+    if (!once) {
+      mine = pool_held(a, s0 + tid);
+      if (mine.seq < p.seqs) {
+        mine.source = a.copies[3 * static_cast<int64_t>(mine.seq)];
+        mine.rank = a.copies[3 * static_cast<int64_t>(mine.seq) + 1];
+      }
+      pool_want(a, mine);
+    }
+    if (count == 0) mine.need = 0;
+    if constexpr (LOCAL) {
       kv_for<kPoolOwn>([&](auto J) {
-        if (J < mine.need) enter(mine.seq, mine.begin + J, mine.rank + J);
+        if (J < mine.need) p.table[static_cast<int64_t>(mine.seq) * p.width + mine.begin + J] = held[mine.rank + J];
       });
       uint64_t many = __ballot(mine.need > kPoolOwn);
       while (many != 0) {
         const int32_t l = __ffsll(static_cast<unsigned long long>(many)) - 1;
         many &= many - 1;
-        const int32_t s = __shfl(mine.seq, l), begin = __shfl(mine.begin, l), need = __shfl(mine.need, l), first = __shfl(mine.rank, l);
-        // those of the round
-        const int32_t j1 = min(need, end - first);
-        for (int32_t j = max(kPoolOwn, base - first) + lane; j < j1; j += 64) enter(s, begin + j, first + j);
+        const int32_t need = __shfl(mine.need, l), first = __shfl(mine.rank, l);
+        int32_t *to = p.table + static_cast<int64_t>(__shfl(mine.seq, l)) * p.width + __shfl(mine.begin, l);
+        for (int32_t j = kPoolOwn + lane; j < need; j += 64) to[j] = held[first + j];
       }
     }
-    __syncthreads();
-  }
-  // the pages taken are not free any more
-  if (count > 0) {
-    int64_t rank = free_before;
-    for (int32_t w = word0; w < word1 && rank < count; ++w) {
-      uint32_t bits = p.free[w];
-      const int32_t n = __popc(bits);
-      for (int64_t r = rank; bits != 0 && r < count; ++r) bits &= bits - 1;
-      p.free[w] = bits;
-      rank += n;
-    }
-  }
-  for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
-    if (!once) mine = settled(s0 + tid);
     const int32_t s = mine.seq;
     if (s >= p.seqs) continue;
     const bool copied = ok && mine.source >= 0;
     int32_t *c = a.copies + 3 * static_cast<int64_t>(s);
     c[0] = copied ? mine.source : -1;
-    c[1] = copied ? p.table[static_cast<int64_t>(s) * p.width + mine.begin] : -1;
+    c[1] = -1;
+    if constexpr (LOCAL)
+      if (copied) c[1] = held[mine.rank];
     c[2] = copied ? mine.inside : 0;
     if (copied) __hip_atomic_fetch_add(p.refs + mine.source, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     a.seen[s] = ok && mine.n > 0 ? mine.old + mine.n : 0;
     if (ok && mine.n > 0) p.lengths[s] = mine.old + mine.n;
+    if constexpr (!LOCAL) p.spare[s] = mine.rank;
   }
+}
+
+// A thread a page: the free ones of the lowest ranks are taken, each by the sequence in whose
+// part of the ranks it lies.
+__global__ __launch_bounds__(256) void kv_enter_kernel(const AssignArgs a) {
+  const PoolArgs &p = a.p;
+  const int64_t b = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int32_t w = static_cast<int32_t>(b >> 4), count = p.spare[p.seqs];
+  if (w >= p.words || count == 0) return;
+  const uint32_t bits = pool_free(p, w);
+  const int32_t bit = static_cast<int32_t>(b & 15), rank = p.before[w] + __popc(bits & ((1u << bit) - 1u));
+  if (!(bits >> bit & 1u) || rank >= count) return;
+  const int32_t page = static_cast<int32_t>(b);
+  // the last sequence whose part begins at the rank or before it
+  int32_t low = 0, high = p.seqs;
+  while (high - low > 1) {
+    const int32_t mid = (low + high) >> 1;
+    if (p.spare[mid] <= rank)
+      low = mid;
+    else
+      high = mid;
+  }
+  const int32_t first = p.spare[low], need = p.spare[low + 1] - first;
+  p.refs[page] = 1;
+  p.free[page] = 0;
+  p.table[static_cast<int64_t>(low) * p.width + (pool_pages(p, p.lengths[low]) - need) + (rank - first)] = page;
+  int32_t *c = a.copies + 3 * static_cast<int64_t>(low);
+  if (rank == first && c[0] >= 0) c[1] = page;
 }
 
 // A workgroup for a sequence: the pages past `to` tokens are let go.
@@ -300,25 +333,66 @@ __global__ __launch_bounds__(256) void kv_settle_kernel(const PoolArgs p, const 
   if (threadIdx.x == 0) p.lengths[s] = p.spare_lengths[s];
 }
 
+// Small tables in one launch of one workgroup, which holds what every sequence becomes in
+// registers until all that stays is held (4 sequences of 17 columns 2.9 + 2.9 us in two
+// launches; 256 of 25 columns 3.1 + 3.0).
+constexpr int kReorderEach = 8;
+__global__ __launch_bounds__(1024) void kv_reorder_kernel(const PoolArgs p, const int32_t *parents, const KvDiv by_width) {
+  const int32_t threads = blockDim.x, count = p.seqs * p.width;
+  int32_t page[kReorderEach], old[kReorderEach], length[kReorderEach];
+  kv_for<kReorderEach>([&](auto J) {
+    const int32_t e = threadIdx.x + J * threads;
+    page[J] = old[J] = length[J] = -1;
+    if (e < count) {
+      uint32_t s = e;
+      const int32_t w = kv_rem(by_width, s), from = pool_parent(p, parents, s);
+      old[J] = p.table[e];
+      page[J] = from < 0 ? -1 : p.table[static_cast<int64_t>(from) * p.width + w];
+      if (page[J] != old[J] && pool_has(p, page[J]))
+        __hip_atomic_fetch_add(p.refs + page[J], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (e < p.seqs) {
+      const int32_t from = pool_parent(p, parents, e);
+      length[J] = from < 0 ? 0 : p.lengths[from];
+    }
+  });
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  kv_for<kReorderEach>([&](auto J) {
+    const int32_t e = threadIdx.x + J * threads;
+    if (e < count && page[J] != old[J]) {
+      p.table[e] = page[J];
+      pool_drop(p, old[J]);
+    }
+    if (e < p.seqs) p.lengths[e] = length[J];
+  });
+}
+
 constexpr int32_t kSlotStarts = 4096;  // row starts held in shared memory
 
-// A thread a row; its sequence is found by halving among the row starts, which a
-// workgroup reads once where they fit.
+// A wave for GROUPS groups of 64 rows.  A group whose rows are all of one sequence, which
+// those of prompts mostly are, asks once for it; else each row finds its own by halving among
+// the row starts, which a workgroup reads once where they fit.
+template <int GROUPS>
 __global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int32_t *positions, int64_t *slots) {
   __shared__ int32_t held[kSlotStarts];
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const bool few = b.starts && b.seqs < kSlotStarts;
   if (few) {
-    for (int32_t i = threadIdx.x; i <= b.seqs; i += 256) held[i] = b.starts[i];
+    for (int32_t i0 = threadIdx.x; i0 <= b.seqs; i0 += 1024) {  // four loads at a time
+      int32_t v[4];
+      kv_for<4>([&](auto U) { v[U] = b.starts[min(i0 + 256 * U, b.seqs)]; });
+      kv_for<4>([&](auto U) {
+        if (i0 + 256 * U <= b.seqs) held[i0 + 256 * U] = v[U];
+      });
+    }
     __syncthreads();
   }
-  if (r >= b.rows) return;
-  const int32_t row = static_cast<int32_t>(r);
-  int32_t seq = row;
-  if (b.starts) {
-    const int32_t *starts = few ? held : b.starts;
-    // the last sequence that starts at the row or before it
-    int32_t low = -1, high = b.seqs;
+  const int32_t *const starts = few ? held : b.starts;
+  const int32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t wave_row = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * (64 * GROUPS);
+  // the last sequence that starts at the row or before it, from `low` on, which does
+  auto find = [&](int32_t low, int64_t row) {
+    int32_t high = b.seqs;
     while (high - low > 1) {
       const int32_t mid = (low + high) >> 1;
       if (starts[mid] <= row)
@@ -326,29 +400,54 @@ __global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int3
       else
         high = mid;
     }
-    seq = low;
-  }
-  int32_t position = 0;
-  int64_t slot = -1;
-  if (seq >= 0 && seq < b.seqs) {
-    const int32_t length = max(b.lengths[seq], 0);
-    int32_t first = row, all = 1;
-    if (b.starts) {
-      first = min(max(b.starts[seq], 0), b.rows);
-      all = min(max(b.starts[seq + 1], first), b.rows) - first;
+    return low;
+  };
+  if (wave_row >= b.rows) return;
+  // sequences of all groups first, then their lengths, then their pages: loads that wait for
+  // each other do so once
+  int32_t seq[GROUPS], length[GROUPS], page[GROUPS], place[GROUPS], position[GROUPS];
+  int32_t known = b.starts ? __builtin_amdgcn_readfirstlane(find(-1, wave_row)) : 0;
+  kv_for<GROUPS>([&](auto I) {
+    const int64_t row0 = wave_row + 64 * I, row = row0 + lane;
+    seq[I] = b.starts ? known : static_cast<int32_t>(min(row, static_cast<int64_t>(b.seqs)));
+    if (b.starts && !(known >= 0 && known + 1 < b.seqs && starts[known + 1] > row0 + 63)) {
+      seq[I] = find(known, row);
+      known = __builtin_amdgcn_readlane(seq[I], 63);
     }
-    const int32_t i = row - first, at = length - all + i;
-    if (i < all) {
-      position = max(at, 0);
-      if (at >= 0 && i < b.max_rows && at < b.max_length) {
-        const int32_t page = b.table[seq * b.table_stride + (at >> b.log_page)];
-        if (static_cast<uint32_t>(page) < static_cast<uint32_t>(b.blocks))
-          slot = (static_cast<int64_t>(page) << b.log_page) + (at & ((1 << b.log_page) - 1));
+    const bool any = seq[I] >= 0 && seq[I] < b.seqs && row < b.rows;
+    if (!any) seq[I] = -1;
+    length[I] = any ? max(b.lengths[seq[I]], 0) : 0;
+  });
+  kv_for<GROUPS>([&](auto I) {
+    const int64_t row = wave_row + 64 * I + lane;
+    position[I] = 0;
+    place[I] = 0;
+    page[I] = -1;
+    if (seq[I] >= 0) {
+      int32_t first = static_cast<int32_t>(row), all = 1;
+      if (b.starts) {
+        first = min(max(starts[seq[I]], 0), b.rows);
+        all = min(max(starts[seq[I] + 1], first), b.rows) - first;
+      }
+      const int32_t n = static_cast<int32_t>(row) - first, at = length[I] - all + n;
+      if (n < all) {
+        position[I] = max(at, 0);
+        if (at >= 0 && n < b.max_rows && at < b.max_length) {
+          page[I] = b.table[seq[I] * b.table_stride + (at >> b.log_page)];
+          place[I] = at & ((1 << b.log_page) - 1);
+        }
       }
     }
-  }
-  positions[r] = position;
-  slots[r] = slot;
+  });
+  kv_for<GROUPS>([&](auto I) {
+    const int64_t row = wave_row + 64 * I + lane;
+    if (row < b.rows) {
+      positions[row] = position[I];
+      slots[row] = static_cast<uint32_t>(page[I]) < static_cast<uint32_t>(b.blocks)
+                       ? (static_cast<int64_t>(page[I]) << b.log_page) + place[I]
+                       : -1;
+    }
+  });
 }
 
 struct CopyArgs {
@@ -399,7 +498,7 @@ static bool on(const void *p, int64_t n) { return p && reinterpret_cast<uintptr_
 static int32_t log_of(int32_t page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
 
 static int64_t scratch_words(int32_t blocks, int32_t seqs, int32_t width) {
-  return 2 * static_cast<int64_t>(blocks) + static_cast<int64_t>(seqs) * width + seqs;
+  return 3 * static_cast<int64_t>(blocks) + static_cast<int64_t>(seqs) * width + static_cast<int64_t>(seqs);
 }
 
 static int32_t pool_args(const rnsmx_kv_pool_t *pool, PoolArgs &a) {
@@ -408,18 +507,19 @@ static int32_t pool_args(const rnsmx_kv_pool_t *pool, PoolArgs &a) {
   if (a.log_page < 0) return fail(RNSMX_EINVAL, "a page holds 16, 32, 64 or 128 tokens");
   if (pool->blocks < 1 || pool->seqs < 1 || pool->width < 1) return fail(RNSMX_EINVAL, "a pool has pages, sequences and a table");
   if ((static_cast<int64_t>(pool->width) << a.log_page) > 1 << 30) return fail(RNSMX_EINVAL, "sequences hold at most 2^30 tokens");
-  if (!on(pool->table_dev, 4) || !on(pool->lengths_dev, 4) || !on(pool->refs_dev, 4) || !on(pool->free_dev, 4) || !on(pool->scratch_dev, 4))
-    return fail(RNSMX_EINVAL, "a pool's pointer is null or not on a 4-byte boundary");
+  if (!on(pool->table_dev, 4) || !on(pool->lengths_dev, 4) || !on(pool->refs_dev, 4) || !on(pool->free_dev, 16) || !on(pool->scratch_dev, 4))
+    return fail(RNSMX_EINVAL, "a pool's pointer is null or not on a 4-byte (free_dev 16-byte) boundary");
   a.table = pool->table_dev;
   a.lengths = pool->lengths_dev;
   a.refs = pool->refs_dev;
   a.free = pool->free_dev;
   a.going = pool->scratch_dev;
   a.first = a.going + pool->blocks;
-  a.spare = a.first + pool->blocks;
+  a.before = a.first + pool->blocks;
+  a.spare = a.before + pool->blocks;
   a.spare_lengths = a.spare + static_cast<int64_t>(pool->seqs) * pool->width;
   a.blocks = pool->blocks;
-  a.words = static_cast<int32_t>((static_cast<int64_t>(pool->blocks) + 31) / 32);
+  a.words = static_cast<int32_t>((static_cast<int64_t>(pool->blocks) + 15) / 16);
   a.seqs = pool->seqs;
   a.width = pool->width;
   return RNSMX_OK;
@@ -456,9 +556,18 @@ int32_t rnsmx_kv_assign(const rnsmx_kv_pool_t *pool, const rnsmx_kv_step_t *step
   a.max_rows = step->max_rows;
   a.max_length = step->max_length;
   // a sequence and two words of free pages a thread
-  const int64_t work = std::max<int64_t>({a.p.seqs, a.p.words / 2, a.rows >> a.p.log_page});
+  const int64_t work = std::max<int64_t>(a.p.seqs, a.p.words / 2);
   const unsigned threads = static_cast<unsigned>(std::min<int64_t>(1024, (work + 63) / 64 * 64));
-  hipLaunchKernelGGL(kv_assign_kernel, dim3(1), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
+  // Most pages that a call can hand out: those of whole pages of rows, and for each sequence a
+  // copy and a page that its rows begin or end.
+  const int64_t most = std::min<int64_t>(a.p.blocks, (a.rows >> a.p.log_page) + 2 * std::min<int64_t>(a.p.seqs, a.rows));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (most <= kPoolPicked) {
+    hipLaunchKernelGGL(kv_assign_kernel<true>, dim3(1), dim3(threads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(kv_assign_kernel<false>, dim3(1), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(kv_enter_kernel, dim3((a.p.words + 15) / 16), dim3(256), 0, st, a);
+  }
   return pages_check("kv_assign");
 }
 
@@ -477,6 +586,12 @@ int32_t rnsmx_kv_reorder(const rnsmx_kv_pool_t *pool, const int32_t *parents_dev
   if (int32_t rc = pool_args(pool, a)) return rc;
   if (!on(parents_dev, 4)) return fail(RNSMX_EINVAL, "parents null or not on a 4-byte boundary");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t entries = static_cast<int64_t>(a.seqs) * a.width;
+  if (entries <= kReorderEach * 1024) {
+    const unsigned threads = static_cast<unsigned>(std::min<int64_t>(1024, (entries + 63) / 64 * 64));
+    hipLaunchKernelGGL(kv_reorder_kernel, dim3(1), dim3(threads), 0, st, a, parents_dev, kv_div(a.width));
+    return pages_check("kv_reorder");
+  }
   hipLaunchKernelGGL(kv_gather_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, st, a, parents_dev);
   hipLaunchKernelGGL(kv_settle_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, st, a, parents_dev);
   return pages_check("kv_reorder");
@@ -509,8 +624,13 @@ int32_t rnsmx_kv_slots(const rnsmx_kv_batch_t *batch, int32_t blocks, int32_t pa
   b.rows = batch->rows;
   b.max_rows = batch->starts_dev ? batch->max_rows : 1;
   b.max_length = batch->max_length;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(b.rows) + 255) / 256);
-  hipLaunchKernelGGL(kv_slots_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), b, positions_dev, slots_dev);
+  // a group a wave where that leaves some of the chip's waves free
+  const int64_t each = 256 * (b.rows >= 1 << 18 ? 4 : 1);
+  const dim3 grid(static_cast<unsigned>((b.rows + each - 1) / each));
+  if (each > 256)
+    hipLaunchKernelGGL(kv_slots_kernel<4>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), b, positions_dev, slots_dev);
+  else
+    hipLaunchKernelGGL(kv_slots_kernel<1>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), b, positions_dev, slots_dev);
   return pages_check("kv_slots");
 }
 

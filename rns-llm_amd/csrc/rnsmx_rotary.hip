@@ -21,7 +21,7 @@ struct RotaryArgs {
   int64_t rows, first;  // a launch's first row
   int32_t wide;  // positions of 64 bits
   int32_t q_heads, heads, pairs, dim;
-  int32_t pieces;     // of a head: its pairs by eights, then what is copied by sixteens
+  int32_t pieces;     // of a head: its pairs, then what is copied
   int32_t turning;    // of them those of pairs
   int32_t per_row;    // pieces of a row
   int32_t row_tile;   // rows of a workgroup
@@ -61,31 +61,32 @@ __device__ __forceinline__ T rotary_round(float v) {
     return static_cast<T>(v);
 }
 
-// Eight values at p, those from `left` on not there.
-template <bool VEC, typename T>
-__device__ __forceinline__ void rotary_get(T (&x)[8], const T *p, int32_t left) {
+// 16 bytes at p, of whose values those from `left` on are not there.
+template <bool VEC, typename T, int N>
+__device__ __forceinline__ void rotary_get(T (&x)[N], const T *p, int32_t left) {
   if constexpr (VEC) {
-    kv_for<sizeof(T) / 2>([&](auto I) { reinterpret_cast<u32x4 *>(x)[I] = reinterpret_cast<const u32x4 *>(p)[I]; });
+    *reinterpret_cast<u32x4 *>(x) = *reinterpret_cast<const u32x4 *>(p);
   } else {
-    kv_for<8>([&](auto I) { x[I] = I < left ? p[I] : T(0); });
+    kv_for<N>([&](auto I) { x[I] = I < left ? p[I] : T(0); });
   }
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void rotary_put(T *p, const T (&x)[8], int32_t left) {
+template <bool VEC, typename T, int N>
+__device__ __forceinline__ void rotary_put(T *p, const T (&x)[N], int32_t left) {
   if constexpr (VEC) {
-    kv_for<sizeof(T) / 2>([&](auto I) { reinterpret_cast<u32x4 *>(p)[I] = reinterpret_cast<const u32x4 *>(x)[I]; });
+    *reinterpret_cast<u32x4 *>(p) = *reinterpret_cast<const u32x4 *>(x);
   } else {
-    kv_for<8>([&](auto I) {
+    kv_for<N>([&](auto I) {
       if (I < left) p[I] = x[I];
     });
   }
 }
 
 // A workgroup takes some rows and heads: the rows' angles once into shared memory,
-// then eight pairs a thread and step.  A thread reads what it writes before it writes
+// then a piece a thread and step: the pairs of two loads of 16 bytes.  A thread reads what it writes before it writes
 // it, so a call may be in place.
 template <typename T, bool VEC, bool NEIGHBOURS>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
+  constexpr int N = 16 / sizeof(T);  // values of a load, pairs of a piece
   __shared__ __attribute__((aligned(16))) F32x2 angles[kRotaryTable];
   const int64_t row0 = a.first + static_cast<int64_t>(blockIdx.x) * a.row_tile;
   const int32_t rows = static_cast<int32_t>(min(static_cast<int64_t>(a.row_tile), a.rows - row0));
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
   const int32_t half = a.pairs;
 
   struct Piece {
-    T x[2][8];
+    alignas(16) T x[2][N];
     const T *from;
     T *to;
     int32_t at[2], left[2], row, first;  // columns and how many of them are there
@@ -115,20 +116,20 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
     p.from = static_cast<const T *>(second ? v.src : u.src) + (row * (second ? v.src_rs : u.src_rs) + h * (second ? v.src_hs : u.src_hs));
     p.to = static_cast<T *>(second ? v.dst : u.dst) + (row * (second ? v.dst_rs : u.dst_rs) + h * (second ? v.dst_hs : u.dst_hs));
     p.turned = piece < a.turning;
-    p.first = 8 * piece;
+    p.first = N * piece;
     if (p.turned && !NEIGHBOURS) {
-      p.at[0] = 8 * piece;
-      p.at[1] = half + 8 * piece;
-      p.left[0] = p.left[1] = half - 8 * piece;
+      p.at[0] = N * piece;
+      p.at[1] = half + N * piece;
+      p.left[0] = p.left[1] = half - N * piece;
     } else {
-      p.at[0] = p.turned ? 16 * piece : 2 * half + 16 * (piece - a.turning);
-      p.at[1] = p.at[0] + 8;
+      p.at[0] = p.turned ? 2 * N * piece : 2 * half + 2 * N * (piece - a.turning);
+      p.at[1] = p.at[0] + N;
       const int32_t end = p.turned ? 2 * half : a.dim;
       p.left[0] = end - p.at[0];
       p.left[1] = end - p.at[1];
     }
     kv_for<2>([&](auto K) {
-      // whole or not at all where they are eights
+      // whole or not at all where loads are
       if (p.there && p.left[K] > 0) rotary_get<VEC>(p.x[K], p.from + p.at[K], p.left[K]);
     });
   };
@@ -136,11 +137,11 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
     if (!p.there) return;
     if (p.turned) {
       const F32x2 *t = angles + p.row * half + p.first;
-      kv_for<8>([&](auto I) {
+      kv_for<N>([&](auto I) {
         constexpr int i = I;
-        // neighbours: pair i lies in values 2 i, 2 i + 1 of the sixteen
-        constexpr int ka = NEIGHBOURS ? (2 * i) / 8 : 0, ia = NEIGHBOURS ? (2 * i) % 8 : i;
-        constexpr int kb = NEIGHBOURS ? (2 * i + 1) / 8 : 1, ib = NEIGHBOURS ? (2 * i + 1) % 8 : i;
+        // neighbours: pair i lies in values 2 i, 2 i + 1 of the piece
+        constexpr int ka = NEIGHBOURS ? (2 * i) / N : 0, ia = NEIGHBOURS ? (2 * i) % N : i;
+        constexpr int kb = NEIGHBOURS ? (2 * i + 1) / N : 1, ib = NEIGHBOURS ? (2 * i + 1) % N : i;
         const F32x2 cs = VEC || p.first + i < half ? t[i] : F32x2{1.0f, 0.0f};
         const float u = rotary_load(p.x[ka][ia]), v = rotary_load(p.x[kb][ib]);
         p.x[ka][ia] = rotary_round<T>(fmaf(u, cs.x, -(v * cs.y)));
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
   }
 }
 
-static bool rotary_vec(const rnsmx_rotary_rows_t &r, int64_t size, const void *p, int64_t rs, int64_t hs) {
+static bool rotary_vec(int64_t size, const void *p, int64_t rs, int64_t hs) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && rs * size % 16 == 0 && hs * size % 16 == 0;
 }
 
@@ -217,7 +218,8 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   a.part[0] = {q_dev, q_out_dev, rows->q_row_stride, rows->q_head_stride, rows->q_out_row_stride, rows->q_out_head_stride};
   a.part[1] = {k_dev, k_out_dev, rows->k_row_stride, rows->k_head_stride, rows->k_out_row_stride, rows->k_out_head_stride};
   const int32_t part_heads[2] = {rows->q_heads, rows->k_heads};
-  bool vec = rotary->pairs % 8 == 0 && rows->head_dim % 8 == 0, copied = false;
+  const int32_t step = static_cast<int32_t>(16 / size);  // values of a load
+  bool vec = rotary->pairs % step == 0 && rows->head_dim % step == 0, copied = false;
   for (int i = 0; i < 2; ++i) {
     if (part_heads[i] == 0) continue;
     const RotaryPart &p = a.part[i];
@@ -225,7 +227,7 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
       return fail(RNSMX_EINVAL, "queries, keys or outputs null or not aligned to their type");
     const bool in_place = p.src == p.dst && p.src_rs == p.dst_rs && p.src_hs == p.dst_hs;
     copied = copied || !in_place;
-    vec = vec && rotary_vec(*rows, size, p.src, p.src_rs, p.src_hs) && rotary_vec(*rows, size, p.dst, p.dst_rs, p.dst_hs);
+    vec = vec && rotary_vec(size, p.src, p.src_rs, p.src_hs) && rotary_vec(size, p.dst, p.dst_rs, p.dst_hs);
     // Outputs meet an input's memory only where they are it; columns of one
     // product interleave without sharing a value, which ranges cannot tell.
     for (int j = 0; j < 2; ++j)
@@ -244,8 +246,8 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   a.dim = rows->head_dim;
   a.magnitude = rotary->magnitude;
   a.sign = rows->back ? -1.0f : 1.0f;
-  a.turning = (a.pairs + 7) / 8;
-  a.pieces = a.turning + (copied ? (a.dim - 2 * a.pairs + 15) / 16 : 0);
+  a.turning = (a.pairs + step - 1) / step;
+  a.pieces = a.turning + (copied ? (a.dim - 2 * a.pairs + 2 * step - 1) / (2 * step) : 0);
 
   // A workgroup's rows share the angles' cost and are as many as leave the chip
   // kRotaryGroups workgroups; where rows are fewer than that their heads are split.

@@ -14,6 +14,7 @@ import torch
 from .. import _native
 from .kv_cache import _FLOAT_CODES
 
+_MAX_CHECKED = 64
 
 class _WithoutGradient(torch.autograd.Function):
     """Scores as they are; a backward pass that reaches them says that it ends there."""
@@ -47,6 +48,34 @@ class BeamOps:
         infinity, ``end_token`` (0 without one) and its own number modulo the beams as its
         parent's.  There is no gradient: a backward pass through the scores raises."""
         k = operator.index(k)
+        key = (logits.dtype, logits.shape, logits.stride(), logits.device, scores.dtype, scores.shape, scores.stride(), scores.device,
+               k, None if finished is None else (finished.dtype, finished.shape, finished.stride(), finished.device), end_token)
+        checked = self._beam_checked.get(key)
+        if checked is None:
+            plain = self._plain_beams(logits, scores, k, finished, end_token)
+            if any(x is not y for x, y in zip(plain, (logits, scores, finished))):
+                return self.beam_select(plain[0], plain[1], k, finished=plain[2], end_token=end_token)
+            checked = self._beam_call(logits, k, end_token)
+            if len(self._beam_checked) >= _MAX_CHECKED:
+                self._beam_checked.clear()
+            self._beam_checked[key] = checked
+        _, ref, need, like = checked
+        device = logits.device
+        space = self._kv_scratch_for(need, device, self._stream_of(device))
+        out = torch.empty_like(like[0], memory_format=torch.contiguous_format)
+        tokens = torch.empty_like(like[1], memory_format=torch.contiguous_format)
+        parents = torch.empty_like(like[1], memory_format=torch.contiguous_format)
+        self._on_device(device, self._lib.rnsmx_beam_select, ref, logits.data_ptr(), scores.data_ptr(),
+                        None if finished is None else finished.data_ptr(), space.data_ptr(), space.numel(), out.data_ptr(),
+                        tokens.data_ptr(), parents.data_ptr())
+        self._stats["beam_select_calls"] += 1
+        if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+            out = _WithoutGradient.apply(out, logits, scores)
+        return out, tokens, parents
+
+    @staticmethod
+    def _plain_beams(logits: torch.Tensor, scores: torch.Tensor, k: int, finished: torch.Tensor | None, end_token: int | None):
+        """The checked tensors as the library takes them: values of a row, scores and flags side by side."""
         if logits.dtype not in _FLOAT_CODES or logits.ndim != 3:
             raise ValueError("logits must be [requests, beams, vocabulary] in float32, float16 or bfloat16")
         requests, beams, vocabulary = logits.shape
@@ -55,32 +84,29 @@ class BeamOps:
             raise ValueError(f"scores must be float32 [{requests}, {beams}] on {device}")
         if not 1 <= beams <= _native.BEAMS_MAX or not 1 <= k <= _native.BEAMS_MAX:
             raise ValueError(f"1 to {_native.BEAMS_MAX} beams and continuations, got {beams} and {k}")
+        if vocabulary < 1:
+            raise ValueError("a vocabulary has at least one token")
         if finished is not None:
             if finished.dtype != torch.bool or finished.shape != scores.shape or finished.device != device:
                 raise ValueError(f"finished must be bool [{requests}, {beams}] on {device}")
             if end_token is None:
                 raise ValueError("finished beams need an end_token")
-        if end_token is not None and not 0 <= end_token < vocabulary:
+        if end_token is not None and not 0 <= operator.index(end_token) < vocabulary:
             raise ValueError(f"end_token must be a token of the vocabulary, got {end_token}")
         if device.type != "cuda":
             raise ValueError(f"logits must be on the GPU, they are on {device}")
-        wanted = torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad)
-        rows = logits if logits.stride(2) == 1 or vocabulary == 1 else logits.contiguous()
-        plain = scores if scores.is_contiguous() else scores.contiguous()
-        if finished is not None and not finished.is_contiguous():
-            finished = finished.contiguous()
-        struct = _native.BeamsStruct(rows.stride(0), rows.stride(1), _FLOAT_CODES[logits.dtype], requests, beams, vocabulary, k,
-                                     -1 if end_token is None else int(end_token))
+        return (logits if logits.stride(2) == 1 else logits.contiguous(), scores if scores.is_contiguous() else scores.contiguous(),
+                finished if finished is None or finished.is_contiguous() else finished.contiguous())
+
+    def _beam_call(self, logits: torch.Tensor, k: int, end_token: int | None):
+        requests, beams, vocabulary = logits.shape
+        struct = _native.BeamsStruct(logits.stride(0), logits.stride(1), _FLOAT_CODES[logits.dtype], requests, beams, vocabulary, k,
+                                     -1 if end_token is None else operator.index(end_token))
         ref = ctypes.addressof(struct)
         need = int(self._lib.rnsmx_beam_workspace_bytes(ref))
         if need < 0:
             _native.check(_native.EINVAL)
-        space = self._kv_scratch_for(need, device, self._stream_of(device))
-        out = torch.empty((requests, k), dtype=torch.float32, device=device)
-        tokens = torch.empty((requests, k), dtype=torch.int32, device=device)
-        parents = torch.empty_like(tokens)
-        self._on_device(device, self._lib.rnsmx_beam_select, ref, rows.data_ptr(), plain.data_ptr(),
-                        None if finished is None else finished.data_ptr(), space.data_ptr(), space.numel(), out.data_ptr(),
-                        tokens.data_ptr(), parents.data_ptr())
-        self._stats["beam_select_calls"] += 1
-        return (_WithoutGradient.apply(out, logits, scores) if wanted else out), tokens, parents
+        # one number's memory in the outputs' shape: what they are made like costs less than their sizes
+        like = tuple(torch.empty((1,), dtype=dtype, device=logits.device).expand(requests, k)
+                     for dtype in (torch.float32, torch.int32))
+        return struct, ref, need, like

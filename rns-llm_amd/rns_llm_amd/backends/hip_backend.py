@@ -322,6 +322,7 @@ class HipRNSBackend(KVCacheOps, KVPoolOps, RotaryOps, BeamOps):
         self._quant_scratch: dict[tuple[int, int], torch.Tensor] = {}
         self._ws_bytes: dict[tuple[int, int, int], int] = {}
         self._kv_scratch: dict[tuple[int, int], list[torch.Tensor]] = {}
+        self._beam_checked: dict[tuple, tuple] = {}
         self._stats: Counter[str] = Counter()
 
     _stream_of = staticmethod(_stream_handle)

@@ -26,7 +26,7 @@ class KVPool:
 
     ``table``: int32 ``[sequences, width]``, each sequence's pages, -1 past them;
     ``lengths``: int32 ``[sequences]``; ``refs``: int32 ``[blocks]``, how many sequences
-    hold a page; ``free``: int32, a bit a page that nobody holds.  Calls on a pool
+    hold a page; ``free``: uint8, 1 for a page that nobody holds.  Calls on a pool
     change it in their order, so they belong on one stream (or behind its events)."""
 
     table: torch.Tensor
@@ -78,9 +78,8 @@ class KVPoolOps:
         table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
         lengths = torch.zeros((sequences,), dtype=torch.int32, device=device)
         refs = torch.zeros((blocks,), dtype=torch.int32, device=device)
-        free = torch.full((-(-blocks // 32),), -1, dtype=torch.int32, device=device)
-        if blocks % 32:
-            free[-1] = (1 << blocks % 32) - 1
+        free = torch.ones((-(-blocks // 16) * 16,), dtype=torch.uint8, device=device)
+        free[blocks:] = 0
         scratch = torch.zeros((int(self._lib.rnsmx_kv_pool_scratch_words(blocks, sequences, width)),), dtype=torch.int32,
                               device=device)
         scratch[blocks:2 * blocks] = 2 ** 31 - 1
@@ -171,14 +170,20 @@ class KVPoolOps:
         place in the page (int64 ``[rows]``), in one launch.  A row without a token is at
         position 0; its slot is -1, as is that of a token that the batch drops or
         whose page is not there."""
-        if batch.lengths.device != pages.device:
-            raise ValueError(f"the batch must be on {pages.device}")
-        if pages.device.type != "cuda":
-            raise ValueError(f"the pages must be on the GPU, they are on {pages.device}")
-        if batch.max_length > batch.block_table.shape[1] * pages.block_size:
-            raise ValueError("the batch is of larger pages")
-        positions = torch.empty((batch.rows,), dtype=torch.int32, device=pages.device)
-        slots = torch.empty((batch.rows,), dtype=torch.int64, device=pages.device)
+        key = (pages.blocks, pages.block_size, pages.device)
+        like = batch._checked.get(key)
+        if like is None:
+            if batch.lengths.device != pages.device:
+                raise ValueError(f"the batch must be on {pages.device}")
+            if pages.device.type != "cuda":
+                raise ValueError(f"the pages must be on the GPU, they are on {pages.device}")
+            if batch.max_length > batch.block_table.shape[1] * pages.block_size:
+                raise ValueError("the batch is of larger pages")
+            # one number's memory in the outputs' shape: what they are made like costs less than their sizes
+            like = batch._remember(key, tuple(torch.empty((1,), dtype=dtype, device=pages.device).expand(batch.rows)
+                                              for dtype in (torch.int32, torch.int64)))
+        positions = torch.empty_like(like[0], memory_format=torch.contiguous_format)
+        slots = torch.empty_like(like[1], memory_format=torch.contiguous_format)
         self._on_device(pages.device, self._lib.rnsmx_kv_slots, batch._ref, pages.blocks, pages.block_size, positions.data_ptr(),
                         slots.data_ptr())
         self._stats["kv_slots_calls"] += 1

@@ -56,7 +56,10 @@ class _Rotate(torch.autograd.Function):
         first, second = (gq, gk) if gq is not None else (gk, None)
         if first is None:
             return (None,) * 6
-        out = _Rotate.apply(ctx.backend, ctx.rotary, not ctx.back, positions, first, second)
+        if torch.is_grad_enabled():  # the gradient itself is differentiated
+            out = _Rotate.apply(ctx.backend, ctx.rotary, not ctx.back, positions, first, second)
+        else:
+            out = ctx.backend._rotated(ctx.rotary, positions, first, second, not ctx.back, False)
         gq, gk = out if gq is not None else (None, out[0])
         return None, None, None, None, gq, gk
 

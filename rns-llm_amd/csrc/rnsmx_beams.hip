@@ -133,31 +133,25 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
 
   if (!(a.finished && a.finished[row])) {
     const T *p = static_cast<const T *>(a.logits) + request * a.request_stride + beam * a.beam_stride;
-    const int32_t before = static_cast<int32_t>(reinterpret_cast<uintptr_t>(p) / sizeof(T) % G);  // to the load's boundary
-    const int64_t first = static_cast<int64_t>(split) * a.chunk - before;
+    // Loads of 16 bytes from wherever the row begins: which value is whose does not depend on
+    // its address, so that beams of the same logits have the same sums.
+    const int64_t first = static_cast<int64_t>(split) * a.chunk;
     const int64_t end = min(first + a.chunk, static_cast<int64_t>(a.vocabulary));
-    // what is past the row's ends is as little a candidate as minus infinity
+    // what is past the row's end is as little a candidate as minus infinity
     constexpr uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, uint16_t>::value ? 0xFF80FF80u : 0xFC00FC00u;
     u32x4 raw[N];
     const T *const base = p + first;
-    const int32_t low = first < 0 ? 1 : 0, high = static_cast<int32_t>(end - first) - G;  // where whole loads may start
+    const int32_t size = static_cast<int32_t>(end - first);
     kv_for<N>([&](auto J) {
       const int32_t e = (J * 256 + tid) * G;
       raw[J] = u32x4{none, none, none, none};
-      if (e >= low && e <= high) raw[J] = *reinterpret_cast<const u32x4 *>(base + e);
+      if (e + G <= size) __builtin_memcpy(&raw[J], base + e, 16);
     });
-    // the values before the row's first whole load and after its last, one a lane
+    // the values after the last whole load, one a lane
+    const int32_t edge_place = size / G * G + lane;
     float edge = -INFINITY;
-    int64_t edge_at = 0;
-    {
-      const int64_t head = before ? min(static_cast<int64_t>(G - before), end) : 0;  // values of the first
-      const int64_t tail = (end + before) / G * G - before;                           // where the last begin
-      edge_at = lane < 16 ? lane : tail + lane - 16;
-      const bool there = lane < 16 ? split == 0 && edge_at < head : split == a.splits - 1 && tail >= head && edge_at < end;
-      if (wave == 0 && there) edge = beam_float(p[edge_at]);
-    }
+    if (wave == 0 && edge_place < size) edge = beam_float(base[edge_place]);
     auto place_of = [&](int j, int i) { return (j * 256 + tid) * G + i; };  // in the chunk
-    const int32_t edge_place = static_cast<int32_t>(edge_at - first);
     // f(value, place in the chunk)
     auto each = [&](auto &&f) {
       kv_for<N>([&](auto J) { kv_for<G>([&](auto I) { f(beam_value<T>(raw[J], I), place_of(J, I)); }); });
@@ -220,11 +214,7 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
     int32_t n = count;
     if (held > kBeamList || n > kBeamList) {
       // Digit by digit the key of the k-th largest, and how many that are it belong to the k.
-      const int32_t size = static_cast<int32_t>(end - first);
-      auto key_at = [&](int32_t i) {
-        const int64_t e = first + i;
-        return e >= 0 && i < size ? beam_key(beam_float(p[e])) : 0u;
-      };
+      auto key_at = [&](int32_t i) { return i < size ? beam_key(beam_float(base[i])) : 0u; };
       int32_t *const bins = reinterpret_cast<int32_t *>(column);
       uint32_t kth = 0;
       int32_t wanted = k;
@@ -511,7 +501,7 @@ static size_t beam_shared(int64_t lists, int32_t k) {
 // kBeamLeast values and no larger than the registers hold.
 constexpr int64_t kBeamGroups = 1024, kBeamLeast = 4096;
 static void beam_chunks(const rnsmx_beams_t &b, int32_t &chunk, int32_t &splits) {
-  const int64_t per = b.dtype == RNSMX_FLOAT32 ? 4 : 8, values = b.vocabulary + per;  // a row may start inside a load
+  const int64_t per = b.dtype == RNSMX_FLOAT32 ? 4 : 8, values = b.vocabulary;
   const int64_t rows = std::max<int64_t>(static_cast<int64_t>(b.requests) * b.beams, 1);
   const int64_t least = (values + kBeamMost - 1) / kBeamMost, most = (values + kBeamLeast - 1) / kBeamLeast;
   const int64_t n = std::max(least, std::min({most, kBeamGroups / rows, kBeamChunks / static_cast<int64_t>(b.beams)}));

@@ -334,27 +334,32 @@ __global__ __launch_bounds__(256) void kv_settle_kernel(const PoolArgs p, const 
 }
 
 // Small tables in one launch of one workgroup, which holds what every sequence becomes in
-// registers until all that stays is held (4 sequences of 17 columns 2.9 + 2.9 us in two
-// launches; 256 of 25 columns 3.1 + 3.0).
+// registers until all that stays is held.
 constexpr int kReorderEach = 8;
 __global__ __launch_bounds__(1024) void kv_reorder_kernel(const PoolArgs p, const int32_t *parents, const KvDiv by_width) {
   const int32_t threads = blockDim.x, count = p.seqs * p.width;
-  int32_t page[kReorderEach], old[kReorderEach], length[kReorderEach];
+  // loads that wait for each other do so once for all of a thread's entries
+  int32_t from[kReorderEach], page[kReorderEach], old[kReorderEach], whose[kReorderEach], length[kReorderEach];
   kv_for<kReorderEach>([&](auto J) {
-    const int32_t e = threadIdx.x + J * threads;
-    page[J] = old[J] = length[J] = -1;
-    if (e < count) {
-      uint32_t s = e;
-      const int32_t w = kv_rem(by_width, s), from = pool_parent(p, parents, s);
-      old[J] = p.table[e];
-      page[J] = from < 0 ? -1 : p.table[static_cast<int64_t>(from) * p.width + w];
-      if (page[J] != old[J] && pool_has(p, page[J]))
-        __hip_atomic_fetch_add(p.refs + page[J], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (e < p.seqs) {
-      const int32_t from = pool_parent(p, parents, e);
-      length[J] = from < 0 ? 0 : p.lengths[from];
-    }
+    const int32_t e = min(static_cast<int32_t>(threadIdx.x) + J * threads, count - 1);
+    uint32_t s = e;
+    kv_rem(by_width, s);
+    from[J] = pool_parent(p, parents, s);
+    old[J] = p.table[e];
+    whose[J] = pool_parent(p, parents, min(e, p.seqs - 1));
+  });
+  kv_for<kReorderEach>([&](auto J) {
+    const int32_t e = min(static_cast<int32_t>(threadIdx.x) + J * threads, count - 1);
+    uint32_t s = e;
+    const int32_t w = kv_rem(by_width, s);
+    page[J] = p.table[static_cast<int64_t>(max(from[J], 0)) * p.width + w];
+    if (from[J] < 0) page[J] = -1;
+    length[J] = p.lengths[max(whose[J], 0)];
+    if (whose[J] < 0) length[J] = 0;
+  });
+  kv_for<kReorderEach>([&](auto J) {
+    if (static_cast<int32_t>(threadIdx.x) + J * threads < count && page[J] != old[J] && pool_has(p, page[J]))
+      __hip_atomic_fetch_add(p.refs + page[J], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   });
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();

@@ -62,17 +62,19 @@ __device__ __forceinline__ T rotary_round(float v) {
 }
 
 // 16 bytes at p, of whose values those from `left` on are not there.
-template <bool VEC, typename T, int N>
+template <bool VEC, bool STREAM, typename T, int N>
 __device__ __forceinline__ void rotary_get(T (&x)[N], const T *p, int32_t left) {
   if constexpr (VEC) {
-    *reinterpret_cast<u32x4 *>(x) = *reinterpret_cast<const u32x4 *>(p);
+    *reinterpret_cast<u32x4 *>(x) = kv_fetch<STREAM>(reinterpret_cast<const u32x4 *>(p));
   } else {
     kv_for<N>([&](auto I) { x[I] = I < left ? p[I] : T(0); });
   }
 }
-template <bool VEC, typename T, int N>
+template <bool VEC, bool STREAM, typename T, int N>
 __device__ __forceinline__ void rotary_put(T *p, const T (&x)[N], int32_t left) {
-  if constexpr (VEC) {
+  if constexpr (VEC && STREAM) {
+    __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(x), reinterpret_cast<u32x4 *>(p));
+  } else if constexpr (VEC) {
     *reinterpret_cast<u32x4 *>(p) = *reinterpret_cast<const u32x4 *>(x);
   } else {
     kv_for<N>([&](auto I) {
@@ -84,7 +86,7 @@ __device__ __forceinline__ void rotary_put(T *p, const T (&x)[N], int32_t left) 
 // A workgroup takes some rows and heads: the rows' angles once into shared memory,
 // then a piece a thread and step: the pairs of two loads of 16 bytes.  A thread reads what it writes before it writes
 // it, so a call may be in place.
-template <typename T, bool VEC, bool NEIGHBOURS>
+template <typename T, bool VEC, bool NEIGHBOURS, bool STREAM>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
   constexpr int N = 16 / sizeof(T);  // values of a load, pairs of a piece
   __shared__ __attribute__((aligned(16))) F32x2 angles[kRotaryTable];
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
     }
     kv_for<2>([&](auto K) {
       // whole or not at all where loads are
-      if (p.there && p.left[K] > 0) rotary_get<VEC>(p.x[K], p.from + p.at[K], p.left[K]);
+      if (p.there && p.left[K] > 0) rotary_get<VEC, STREAM>(p.x[K], p.from + p.at[K], p.left[K]);
     });
   };
   auto store = [&](Piece &p) {
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
       });
     }
     kv_for<2>([&](auto K) {
-      if (p.left[K] > 0) rotary_put<VEC>(p.to + p.at[K], p.x[K], p.left[K]);
+      if (p.left[K] > 0) rotary_put<VEC, STREAM>(p.to + p.at[K], p.x[K], p.left[K]);
     });
   };
 
@@ -249,10 +251,19 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   a.turning = (a.pairs + step - 1) / step;
   a.pieces = a.turning + (copied ? (a.dim - 2 * a.pairs + 2 * step - 1) / (2 * step) : 0);
 
-  // A workgroup's rows share the angles' cost and are as many as leave the chip
-  // kRotaryGroups workgroups; where rows are fewer than that their heads are split.
-  constexpr int64_t kRotaryGroups = 1024;
-  const int64_t most_rows = std::min<int64_t>(kRotaryTable / a.pairs, 8);
+  // Inputs and outputs that the 256 MB behind the L2s would not hold go past the caches: 16384 rows
+  // of 40 heads of 128 in 16 bits (336 MB) 60 us so, 65 through them, 12288 (252 MB) 46 and 43.
+  // Float32 goes through them: loads of neighbours take their lines by halves (part of each
+  // head, 125 MB: 56 us so, 26.7 through them).
+  constexpr int64_t kRotaryStream = 256ll << 20;
+  const bool past = rows->rows * static_cast<double>(heads) * a.dim * size * 2 >= kRotaryStream && a.dim % 64 == 0;
+
+  // A workgroup takes rows of some kRotaryPieces pieces, which share the angles' cost (16383 rows
+  // of 40 heads of 128, 320 pieces each, through the caches: 66.7 us with 2 rows, 66.9 with 4, 69.2
+  // with 8, 80 with 16), but no more than leave the chip kRotaryGroups workgroups; where rows are fewer than
+  // that their heads are split.
+  constexpr int64_t kRotaryGroups = 1024, kRotaryPieces = 640;
+  const int64_t most_rows = std::min<int64_t>(kRotaryTable / a.pairs, std::max<int64_t>(1, kRotaryPieces / (static_cast<int64_t>(heads) * a.pieces)));
   a.row_tile = static_cast<int32_t>(std::max<int64_t>(1, std::min(most_rows, a.rows / kRotaryGroups)));
   const int64_t row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
   a.head_tile = heads;
@@ -267,25 +278,27 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   a.by_pairs = kv_div(a.pairs);
   const unsigned head_tiles = (heads + a.head_tile - 1) / a.head_tile;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto t) {
+  // a launch has fewer than 2^32 threads
+  const int64_t most = (1 << 23) / head_tiles;
+  auto run = [&](auto kernel) {
+    for (int64_t tile = 0; tile < row_tiles; tile += most) {
+      a.first = tile * a.row_tile;
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(std::min(most, row_tiles - tile)), head_tiles), dim3(256), 0, st, a);
+    }
+  };
+  auto with = [&](auto t, auto vector, auto streams) {
     using T = decltype(t);
-    auto with = [&](auto vector) {
-      constexpr bool V = decltype(vector)::value;
-      // a launch has fewer than 2^32 threads
-      const int64_t most = (1 << 23) / head_tiles;
-      for (int64_t tile = 0; tile < row_tiles; tile += most) {
-        a.first = tile * a.row_tile;
-        const dim3 grid(static_cast<unsigned>(std::min(most, row_tiles - tile)), head_tiles);
-        if (rotary->interleaved)
-          hipLaunchKernelGGL((rotate_kernel<T, V, true>), grid, dim3(256), 0, st, a);
-        else
-          hipLaunchKernelGGL((rotate_kernel<T, V, false>), grid, dim3(256), 0, st, a);
-      }
-    };
-    if (vec)
-      with(std::true_type{});
+    constexpr bool V = decltype(vector)::value, S = decltype(streams)::value;
+    if (rotary->interleaved)
+      run(rotate_kernel<T, V, true, S>);
     else
-      with(std::false_type{});
+      run(rotate_kernel<T, V, false, S>);
+  };
+  auto launch = [&](auto t) {
+    if (!vec) return with(t, std::false_type{}, std::false_type{});
+    if constexpr (sizeof(t) == 2)
+      if (past) return with(t, std::true_type{}, std::true_type{});
+    with(t, std::true_type{}, std::false_type{});
   };
   if (rows->dtype == RNSMX_FLOAT32)
     launch(float{});

@@ -222,6 +222,10 @@ _FLOAT_CODES = {torch.float32: _native.FLOAT32, torch.float16: _native.FLOAT16,
                 torch.bfloat16: _native.BFLOAT16}
 
 
+# the same two ways for the number of the current device
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _stream_handle(device: torch.device) -> int:
     """The current stream of `device` as a raw handle: ATen's accessor
     (~0.1 us) when this torch build has it, else the public path (~2 us per
@@ -329,7 +333,7 @@ class HipRNSBackend(KVCacheOps, KVPoolOps, RotaryOps, BeamOps):
 
     def _on_device(self, device: torch.device, call, *args) -> None:
         """A library call on `device`'s current stream, with that device the current one."""
-        if device.index is not None and device.index != torch.cuda.current_device():
+        if device.index is not None and device.index != _current_device():
             with torch.cuda.device(device):
                 rc = call(*args, _stream_handle(device))
         else:

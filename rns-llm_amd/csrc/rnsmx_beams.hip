@@ -434,16 +434,27 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
     for (int32_t i = tid >> 2; i < n; i += 64) {  // four lanes an offer
       const Offer o{key_of[i], item_of[i], beam_of[i], 0};
       if (static_cast<uint32_t>(o.key >> 32) < shared_bound) continue;
-      int32_t rank = 0;
+      int32_t rank = 0, same = 0;
       for (int32_t j0 = tid & 3; j0 < n; j0 += 16) {
         uint64_t key[4];
         kv_for<4>([&](auto U) { key[U] = key_of[min(j0 + 4 * U, n - 1)]; });
         kv_for<4>([&](auto U) {
-          const int32_t j = j0 + 4 * U;
-          if (j < n) rank += key[U] > o.key || (key[U] == o.key && better(Offer{key[U], item_of[j], beam_of[j], 0}, o)) ? 1 : 0;
+          const int32_t there = j0 + 4 * U < n ? 1 : 0;
+          rank += key[U] > o.key ? there : 0;
+          same += key[U] == o.key ? there : 0;
         });
       }
-      kv_for<2>([&](auto I) { rank += __shfl_xor(rank, 1 << I); });
+      kv_for<2>([&](auto I) {
+        rank += __shfl_xor(rank, 1 << I);
+        same += __shfl_xor(same, 1 << I);
+      });
+      if (same > 1 && rank < k) {  // of equal ones the lower beam's first, then the better of its own
+        int32_t before = 0;
+        for (int32_t j = tid & 3; j < n; j += 4)
+          if (key_of[j] == o.key) before += better(Offer{o.key, item_of[j], beam_of[j], 0}, o) ? 1 : 0;
+        kv_for<2>([&](auto I) { before += __shfl_xor(before, 1 << I); });
+        rank += before;
+      }
       if (rank < k && (tid & 3) == 0) write(rank, o);
     }
     for (int32_t j = n + tid; j < k; j += 256) {

@@ -268,8 +268,8 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   const int64_t row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
   a.head_tile = heads;
   if (row_tiles < 256) {
-    // down to a piece a thread
-    const int64_t least = std::max<int64_t>(1, 256 / a.pieces), parts = std::max<int64_t>(1, std::min<int64_t>(512 / row_tiles, heads / least));
+    // down to 128 pieces
+    const int64_t least = std::max<int64_t>(1, 128 / a.pieces), parts = std::max<int64_t>(1, std::min<int64_t>(512 / row_tiles, heads / least));
     a.head_tile = static_cast<int32_t>((heads + parts - 1) / parts);
   }
   a.per_row = a.head_tile * a.pieces;

@@ -710,7 +710,8 @@ typedef struct rnsmx_rotary_rows {
 
 /* Turns queries and keys [rows][heads][head_dim] by positions_dev [rows], in float32,
  * rounded once.  An output is its input (the same pointer and strides) or shares no
- * memory with either; no value of an output is another's. */
+ * memory with either; no value of an output is another's (queries' and keys' may lie side by
+ * side, as columns of one product). */
 int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *rows,
                      const void *positions_dev, const void *q_dev, const void *k_dev,
                      void *q_out_dev, void *k_out_dev, void *stream);
@@ -724,6 +725,7 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
  * whose logits hold a not-a-number or plus infinity, or nothing above minus infinity,
  * has none.  A place without a candidate has score minus infinity, end_token
  * (0 where that is negative) and its own beam (its number modulo beams) as its parent.
+ * beams * (vocabulary / 16384, rounded up) is at most 1024.
  */
 #define RNSMX_BEAMS_MAX 64
 typedef struct rnsmx_beams {

@@ -70,15 +70,17 @@ constexpr int32_t kPoolPicked = 4096;  // page numbers in shared memory
 constexpr int32_t kPoolOwn = 2;        // pages of a sequence that its thread enters, a wave together the others
 constexpr int32_t kPoolMost = INT_MAX;
 
-// The free ones of sixteen pages, a bit each.
+// The free ones of sixteen pages, a bit each; what lies past the last page is none.
 __device__ __forceinline__ uint32_t pool_free(const PoolArgs &p, int32_t w) {
-  const u32x4 v = reinterpret_cast<const u32x4 *>(p.free)[w];
+  const u32x4 words = reinterpret_cast<const u32x4 *>(p.free)[w];
   uint32_t bits = 0;
-  kv_for<4>([&](auto I) {  // bytes of 0 or 1 to four bits
+  kv_for<4>([&](auto I) {  // four bytes' lowest bits side by side
     constexpr int i = I;
-    bits |= ((v[i] | v[i] >> 7 | v[i] >> 14 | v[i] >> 21) & 15u) << (4 * i);
+    const uint32_t v = words[i] & 0x01010101u;
+    bits |= ((v | v >> 7 | v >> 14 | v >> 21) & 15u) << (4 * i);
   });
-  return bits;
+  const int32_t left = p.blocks - 16 * w;
+  return left < 16 ? bits & ((1u << left) - 1u) : bits;
 }
 
 struct PoolInfo {

@@ -185,6 +185,29 @@ static int64_t rotary_extent(int64_t rows, int64_t heads, int64_t dim, int64_t r
   return ((rows - 1) * rs + (heads - 1) * hs + dim) * size;
 }
 
+// Whether `a` and `b`, rows and heads of `dim` values each at its strides, share no value:
+// apart as a whole, or blocks side by side in steps of one stride (columns of one product, whose
+// rows or, transposed, heads are that far apart).
+struct RotaryGrid {
+  const void *p;
+  int64_t rs, hs, rows, heads;
+};
+static bool rotary_apart(const RotaryGrid &a, const RotaryGrid &b, int64_t dim, int64_t size) {
+  if (!ranges_meet(a.p, rotary_extent(a.rows, a.heads, dim, a.rs, a.hs, size), b.p, rotary_extent(b.rows, b.heads, dim, b.rs, b.hs, size)))
+    return true;
+  const int64_t bytes = static_cast<const char *>(b.p) - static_cast<const char *>(a.p);
+  if (bytes % size != 0) return false;
+  // what lies within one step of the stride, from a's start on, around its end
+  auto fit = [&](int64_t stride, int64_t span_a, int64_t span_b) {
+    if (stride <= 0) return false;
+    const int64_t at = ((bytes / size) % stride + stride) % stride;
+    return at >= span_a && at + span_b <= stride;
+  };
+  if (a.rs == b.rs && fit(a.rs, (a.heads - 1) * a.hs + dim, (b.heads - 1) * b.hs + dim)) return true;
+  if (a.hs == b.hs && fit(a.hs, (a.rows - 1) * a.rs + dim, (b.rows - 1) * b.rs + dim)) return true;
+  return a.rs == b.rs && a.hs == b.hs && a.rs % std::max<int64_t>(a.hs, 1) == 0 && fit(a.hs, dim, dim);
+}
+
 }  // namespace rnsmx
 
 using namespace rnsmx;
@@ -222,6 +245,10 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   const int32_t part_heads[2] = {rows->q_heads, rows->k_heads};
   const int32_t step = static_cast<int32_t>(16 / size);  // values of a load
   bool vec = rotary->pairs % step == 0 && rows->head_dim % step == 0, copied = false;
+  if (part_heads[0] > 0 && part_heads[1] > 0 && q_out_dev && k_out_dev &&
+      !rotary_apart({q_out_dev, rows->q_out_row_stride, rows->q_out_head_stride, rows->rows, rows->q_heads},
+                    {k_out_dev, rows->k_out_row_stride, rows->k_out_head_stride, rows->rows, rows->k_heads}, rows->head_dim, size))
+    return fail(RNSMX_EINVAL, "the outputs of queries and keys share values");
   for (int i = 0; i < 2; ++i) {
     if (part_heads[i] == 0) continue;
     const RotaryPart &p = a.part[i];

@@ -46,7 +46,8 @@ class BeamOps:
         -> float32 scores, int32 tokens and int32 parents ``[requests, k]``, a parent being
         ``request * beams + beam``.  A place that no candidate is left for has score minus
         infinity, ``end_token`` (0 without one) and its own number modulo the beams as its
-        parent's.  There is no gradient: a backward pass through the scores raises."""
+        parent's.  ``k`` and ``beams`` are at most 64, ``beams * ceil(vocabulary / 16384)`` 1024.
+        There is no gradient: a backward pass through the scores raises."""
         k = operator.index(k)
         key = (logits.dtype, logits.shape, logits.stride(), logits.device, scores.dtype, scores.shape, scores.stride(), scores.device,
                k, None if finished is None else (finished.dtype, finished.shape, finished.stride(), finished.device), end_token)

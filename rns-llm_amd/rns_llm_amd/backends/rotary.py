@@ -144,7 +144,7 @@ class RotaryOps:
         strides, their first ``rotary_dim`` values turned by ``positions`` (int32 or int64
         ``[rows]``, any value), in float32, rounded once, in one launch -> new tensors
         (or one, without k).  Angles are exact to 2**-32 of a turn at any position.
-        ``inplace``: the tensors themselves are turned and returned.
+        ``inplace``: the tensors themselves, which share no value, are turned and returned.
 
         Differentiable in q and k, but for calls in place."""
         if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):

@@ -294,6 +294,13 @@ def test_rotations_the_library_refuses():
     # outputs over inputs, their own apart: q's over k, and q's over its own rows moved on
     refused(turn(qo=2 << 20), "lie over")
     refused(turn(qo=(1 << 20) + 16), "lie over")
+    # queries and keys that share values, in place: the same, some heads, rows moved on, other strides
+    at = 1 << 20
+    for k, changes in ((at, {}), (at + 16, {}), (at + 2 * 24 * 2, {}), (at + 2 * 20, {}), (at + 2 * 16, {"k_row_stride": 20})):
+        both = {"rows": 4, "k_row_stride": 24}
+        both.update(changes)
+        both.update(k_out_row_stride=both["k_row_stride"])
+        refused(turn(rows_struct(**both), q=at, qo=at, k=k, ko=k), "share values")
     assert turn(rows_struct(rows=0)) == _native.OK and turn(rows_struct(q_heads=0, k_heads=0)) == _native.OK
 
 

@@ -118,6 +118,20 @@ def test_a_pool_that_is_full(backend):
     assert (cache.k_codes == 7).all() and (backend.kv_attention(one, cache, step.batch)[:1] == 0).all()
 
 
+def test_bytes_past_the_last_page(backend):
+    """They are no pages, whatever they hold, and of a page's byte the lowest bit counts."""
+    for blocks, rows in ((37, 600), (5000, 80000)):
+        pool, book = pair(backend, blocks, 16, 2, blocks)
+        pool.free[blocks:] = 1
+        pool.free[3] = 255
+        step = backend.kv_step(pool, rows=rows)
+        backend.kv_assign(pool, step, ints([16 * blocks - 40, 56]))
+        assert step.missing.tolist() == [1] and (pool.refs == 0).all()
+        backend.kv_assign(pool, step, ints([16 * blocks - 40, 40]))
+        book.assign([16 * blocks - 40, 40], rows, rows, 16 * blocks)
+        assert torch.equal(pool.table.cpu(), book.table()) and pool.refs.tolist() == book.refs and not pool.free[:blocks].any()
+
+
 def test_bounds_of_a_step(backend):
     pool, book = pair(backend, 50, 16, 3, 6)
     step = backend.kv_step(pool, rows=20, max_query=9, max_length=40)

@@ -103,8 +103,21 @@ def test_strides(backend, dtype):
     want = backend.rotate(rotary, positions, q.clone(), k.clone())
     backend.rotate(rotary, positions, q, k, inplace=True)
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(wide[:, 144:], rest)
+    # of one tensor with the heads first, with rows of several products side by side, heads in turn
+    for make in (lambda: torch.randn((9, 7, 24), generator=gen).to(dtype).to(DEV).transpose(0, 1),
+                 lambda: torch.randn((7, 2, 9, 24), generator=gen).to(dtype).to(DEV)[:, 1],
+                 lambda: torch.randn((7, 9, 48), generator=gen).to(dtype).to(DEV)):
+        x = make()
+        pairs = [(x[:, 2:6], x[:, 6:8]), (x[:, 6:8], x[:, :5])] if x.shape[2] == 24 else [(x[..., :24], x[..., 24:]), (x[..., 24:], x[..., :24])]
+        for q, k in pairs:
+            want = backend.rotate(rotary, positions, q.clone(), k.clone())
+            backend.rotate(rotary, positions, q, k, inplace=True)
+            assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    for q, k in ((x, x), (x[:, :5, :24], x[:, 4:, :24]), (x[..., :24], x[..., 8:32])):
+        with pytest.raises(ValueError, match="share values"):
+            backend.rotate(rotary, positions, q, k, inplace=True)
     assert torch.equal(backend.rotate(rotary, torch.arange(100, 114, device=DEV)[::2], wide[:, :96].view(7, 4, 24)),
-                       backend.rotate(rotary, torch.arange(100, 114, 2, device=DEV), q))
+                       backend.rotate(rotary, torch.arange(100, 114, 2, device=DEV), wide[:, :96].view(7, 4, 24)))
 
 
 def test_values_that_are_not_finite(backend):

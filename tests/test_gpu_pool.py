@@ -120,15 +120,15 @@ def test_a_pool_that_is_full(backend):
 
 def test_bytes_past_the_last_page(backend):
     """They are no pages, whatever they hold, and of a page's byte the lowest bit counts."""
-    for blocks, rows in ((37, 608), (5000, 80016)):  # as many as the first call asks for
+    for blocks, rows in ((37, 600), (5000, 80008)):  # as many as the first call asks for
         pool, book = pair(backend, blocks, 16, 2, blocks)
         pool.free[blocks:] = 1
         pool.free[3] = 255
         step = backend.kv_step(pool, rows=rows)
-        backend.kv_assign(pool, step, ints([16 * blocks - 40, 56]))
+        backend.kv_assign(pool, step, ints([16 * blocks - 48, 56]))
         assert step.missing.tolist() == [1] and (pool.refs == 0).all()
-        backend.kv_assign(pool, step, ints([16 * blocks - 40, 40]))
-        book.assign([16 * blocks - 40, 40], rows, rows, 16 * blocks)
+        backend.kv_assign(pool, step, ints([16 * blocks - 48, 48]))
+        book.assign([16 * blocks - 48, 48], rows, rows, 16 * blocks)
         assert torch.equal(pool.table.cpu(), book.table()) and pool.refs.tolist() == book.refs and not pool.free[:blocks].any()
 
 

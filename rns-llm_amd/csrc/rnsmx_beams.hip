@@ -108,12 +108,17 @@ __device__ __forceinline__ float beam_value(const u32x4 &raw, int i) {
 // reach: the k-th largest of 64 maxima, one for each lane over the four waves; of what lies
 // below it nothing more is asked, eight values at a time.  The few that reach it are put
 // in order by counting.  Where they are many (logits that are equal, or in an order that puts
-// the largest side by side) the k-th largest itself is found by halving.  The workgroup
-// that comes last of a request's joins the chunks, in the same manner.
+// the largest side by side) the k-th largest itself is found digit by digit, from the logits
+// read again.  The workgroup that comes last of a request's joins the chunks, in the same manner.
+// 4 beams of 50272 in float16: 9.6 us, a chain of loads, bound, list and ticket (6) and the
+// join (4).  256 rows of 50272 in bfloat16 (26 MB): 15.6, to 7 of it vector work, some ten
+// instructions a value and an exponential that takes four's time.  192 rows of 128257 in float32
+// (98 MB, a fifth of them finished) with k 32: 30 to 42, memory to 17 and the last joins, whose
+// chunks' results lie apart, after it.
 template <typename T, int N>
 __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
   constexpr int G = 16 / sizeof(T);  // values of a load, of which a thread has N
-  extern __shared__ uint64_t shared[];
+  extern __shared__ __attribute__((aligned(16))) uint64_t shared[];
   uint64_t *const list = shared;
   u32x4 *const load_of = reinterpret_cast<u32x4 *>(list + kBeamList);
   int32_t *const load_at = reinterpret_cast<int32_t *>(load_of + kBeamList);

@@ -49,6 +49,7 @@ class BeamOps:
         parent's.  ``k`` and ``beams`` are at most 64, ``beams * ceil(vocabulary / 16384)`` 1024.
         There is no gradient: a backward pass through the scores raises."""
         k = operator.index(k)
+        end_token = None if end_token is None else operator.index(end_token)
         key = (logits.dtype, logits.shape, logits.stride(), logits.device, scores.dtype, scores.shape, scores.stride(), scores.device,
                k, None if finished is None else (finished.dtype, finished.shape, finished.stride(), finished.device), end_token)
         checked = self._beam_checked.get(key)
@@ -92,7 +93,7 @@ class BeamOps:
                 raise ValueError(f"finished must be bool [{requests}, {beams}] on {device}")
             if end_token is None:
                 raise ValueError("finished beams need an end_token")
-        if end_token is not None and not 0 <= operator.index(end_token) < vocabulary:
+        if end_token is not None and not 0 <= end_token < vocabulary:
             raise ValueError(f"end_token must be a token of the vocabulary, got {end_token}")
         if device.type != "cuda":
             raise ValueError(f"logits must be on the GPU, they are on {device}")
@@ -102,7 +103,7 @@ class BeamOps:
     def _beam_call(self, logits: torch.Tensor, k: int, end_token: int | None):
         requests, beams, vocabulary = logits.shape
         struct = _native.BeamsStruct(logits.stride(0), logits.stride(1), _FLOAT_CODES[logits.dtype], requests, beams, vocabulary, k,
-                                     -1 if end_token is None else operator.index(end_token))
+                                     -1 if end_token is None else end_token)
         ref = ctypes.addressof(struct)
         need = int(self._lib.rnsmx_beam_workspace_bytes(ref))
         if need < 0:

@@ -186,6 +186,8 @@ def test_selections_that_are_none(x, scores, k, options, match):
         backend().beam_select(x, scores, k, **options)
     with pytest.raises(TypeError):
         backend().beam_select(x, scores, 1.5)
+    with pytest.raises(TypeError):
+        backend().beam_select(x, scores, 1, end_token=0.5)
 
 
 # ---- the C ABI ---------------------------------------------------------------

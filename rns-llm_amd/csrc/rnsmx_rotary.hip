@@ -33,8 +33,8 @@ struct RotaryArgs {
 constexpr int kRotaryTable = 1024;  // angles of a workgroup
 
 // Cosine and sine of a position's angle.  position * step mod 2^64 is the fraction
-// of a turn, exact but for the step's own last place (2^-65 turns a position): no
-// position is too far.  Its upper half is cut into quarters, so that what
+// of a turn, exact but for the step's own last place (2^-65 turns a position, below the
+// 2^-32 that is kept up to position 2^32).  Its upper half is cut into quarters, so that what
 // is converted to float32 is below an eighth of a turn and keeps its bits.
 __device__ __forceinline__ F32x2 rotary_angle(int64_t position, uint64_t step) {
   const uint32_t turn = static_cast<uint32_t>((static_cast<uint64_t>(position) * step) >> 32);

@@ -143,10 +143,12 @@ class RotaryOps:
         """``q`` ``[rows, heads, head_dim]`` and ``k`` (as many rows, heads of its own) of any
         strides, their first ``rotary_dim`` values turned by ``positions`` (int32 or int64
         ``[rows]``, any value), in float32, rounded once, in one launch -> new tensors
-        (or one, without k).  Angles are exact to 2**-32 of a turn at any position.
+        (or one, without k).  Angles are exact to 2**-32 of a turn up to position 2**32, beyond
+        it to 2**-65 of a turn a position.
         ``inplace``: the tensors themselves, which share no value, are turned and returned.
 
-        Differentiable in q and k, but for calls in place."""
+        Differentiable in q and k, but for calls in place.  As with any backward pass, one is
+        captured into a graph only when no eager pass's graph of the same leaves is alive."""
         if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
             if inplace:
                 raise ValueError("a call in place has no gradient: detach q and k, or call it under torch.no_grad()")

@@ -219,3 +219,33 @@ def test_streams_and_graphs(backend):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
     assert positions.tolist() == [8, 3, 903, 80]
+
+
+def test_captured_gradients(backend):
+    """Forward and backward in one graph; every replay's gradients are those of the moment's positions."""
+    gen = torch.Generator().manual_seed(8)
+    rotary = backend.create_rotary(device=DEV, rotary_dim=32)
+    q, k, gq, gk = (torch.randn((5, h, 40), generator=gen).to(DEV) for h in (6, 2, 6, 2))
+    positions = torch.tensor([3, 0, 700, 2 ** 20, 12], dtype=torch.int64, device=DEV)
+
+    def gradients():
+        leaves = [x.detach().requires_grad_() for x in (q, k)]
+        return torch.autograd.grad(backend.rotate(rotary, positions, *leaves), leaves, (gq, gk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gradients()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            positions.add_(1)
+            held = gradients()
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+        want = gradients()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+        cos, sin = do.rotary_angles(rotary.frequencies, positions.cpu())
+        for got, g in zip(held, (gq, gk)):
+            check(got, g, cos, -sin, 16, False)

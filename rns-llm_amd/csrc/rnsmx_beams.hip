@@ -73,6 +73,27 @@ __device__ __forceinline__ uint32_t beam_bound(uint32_t v, int32_t k) {
   return bound;
 }
 
+// The same of four numbers a lane.
+__device__ __forceinline__ uint32_t beam_bound(const uint32_t (&v)[4], int32_t k) {
+  uint32_t bound = 0;
+  for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
+    int32_t n = 0;
+    kv_for<4>([&](auto W) { n += __popcll(__ballot(v[W] >= (bound | bit))); });
+    if (n >= k) bound |= bit;
+    if (n == k) break;
+  }
+  return bound;
+}
+
+// A continuation that a request's beams offer.  key: of its score, 0: none.  tie: what
+// goes first of equal ones, the beam from below, the logit's key, the token from below.
+struct __attribute__((aligned(16))) BeamOffer {
+  uint64_t key, tie;
+};
+__device__ __forceinline__ bool beam_better(const BeamOffer &p, const BeamOffer &q) {
+  return p.key > q.key || (p.key == q.key && p.tie > q.tie);
+}
+
 // How many of n numbers in shared memory are larger than one, each of four neighbouring
 // lanes asking a quarter of them.
 __device__ __forceinline__ int32_t beam_larger(const uint64_t *of, int32_t n, uint64_t one) {
@@ -111,10 +132,10 @@ __device__ __forceinline__ float beam_value(const u32x4 &raw, int i) {
 // the largest side by side) the k-th largest itself is found digit by digit, from the logits
 // read again.  The workgroup that comes last of a request's joins the chunks, in the same manner.
 // 4 beams of 50272 in float16: 9.6 us, a chain of loads, bound, list and ticket (6) and the
-// join (4).  256 rows of 50272 in bfloat16 (26 MB): 15.6, to 7 of it vector work, some ten
+// join (4).  256 rows of 50272 in bfloat16 (26 MB): 15.1, to 10 of it without joins, some ten
 // instructions a value and an exponential that takes four's time.  192 rows of 128257 in float32
-// (98 MB, a fifth of them finished) with k 32: 30 to 42, memory to 17 and the last joins, whose
-// chunks' results lie apart, after it.
+// (98 MB, a fifth of them finished) with k 32: 27, memory to 19 and the last joins, 8 each of
+// which 2 are trips to memory, after it.
 template <typename T, int N>
 __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
   constexpr int G = 16 / sizeof(T);  // values of a load, of which a thread has N
@@ -298,10 +319,11 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
   // few results are all held in shared memory, of many each chunk's best
   const bool whole = lists * (k + 2) <= kBeamHeld;
   const int32_t each_held = whole ? k + 2 : 1;
-  uint64_t *const held = shared, *const key_of = held + lists * each_held, *const item_of = key_of + kBeamList;
-  double *const sums = reinterpret_cast<double *>(item_of + kBeamList);
+  BeamOffer *const offers = reinterpret_cast<BeamOffer *>(shared);
+  uint64_t *const held = reinterpret_cast<uint64_t *>(offers + kBeamList);
+  double *const sums = reinterpret_cast<double *>(held + lists * each_held);
   float *const tops = reinterpret_cast<float *>(sums + lists);
-  int32_t *const beam_of = reinterpret_cast<int32_t *>(tops + lists), *const chosen = beam_of + kBeamList;
+  int32_t *const chosen = reinterpret_cast<int32_t *>(tops + lists);
   if (whole) {
     for (int32_t i = tid; i < lists * (k + 2); i += 256)
       held[i] = __hip_atomic_load(from + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -345,121 +367,112 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
   }
   __syncthreads();
 
-  struct Offer {
-    uint64_t key;   // of the score, 0: none
-    uint64_t item;  // key of the logit and the token, as the chunks have them
-    int32_t beam, chunk;
-  };
-  auto better = [](const Offer &p, const Offer &q) {
-    if (p.key != q.key) return p.key > q.key;
-    if (p.beam != q.beam) return p.beam < q.beam;
-    return p.item > q.item;
-  };
   auto offer = [&](int32_t i, uint64_t item) {  // an item of chunk i
     const int32_t b = static_cast<int32_t>(kv_quot(a.by_splits, i));
-    Offer o{0, item, b, i};
-    if (item == 0) return o;
+    if (item == 0) return BeamOffer{0, 0};
     const double v = over[b] ? score[b] : score[b] + (static_cast<double>(beam_logit(static_cast<uint32_t>(item >> 32))) - total[b]);
-    o.key = fabs(v) < INFINITY ? beam_score_key(v) : 0;
-    return o;
+    // a token has 24 bits (kBeamChunks of kBeamMost)
+    return BeamOffer{fabs(v) < INFINITY ? beam_score_key(v) : 0,
+                     static_cast<uint64_t>(RNSMX_BEAMS_MAX - 1 - b) << 56 | item >> 32 << 24 | (item & 0xFFFFFFu)};
   };
-  auto write = [&](int32_t j, const Offer &o) {
+  auto write = [&](int32_t j, const BeamOffer &o) {
     a.out_scores[out + j] = static_cast<float>(beam_score(o.key));
-    a.out_tokens[out + j] = static_cast<int32_t>(~static_cast<uint32_t>(o.item));
-    a.out_parents[out + j] = static_cast<int32_t>(row0) + o.beam;
+    a.out_tokens[out + j] = static_cast<int32_t>(~o.tie & 0xFFFFFFu);
+    a.out_parents[out + j] = static_cast<int32_t>(row0) + RNSMX_BEAMS_MAX - 1 - static_cast<int32_t>(o.tie >> 56);
   };
 
-  // The chunks' best give the bound where they are as many as are wanted; only chunks whose
-  // best reaches it are looked at further.
-  auto settle = [&](uint32_t most) {
+  // A bound from the largest that each thread has, or each lane over the four waves, which
+  // is lower but found sooner.
+  auto settle = [&](uint32_t most, auto lanes) {
+    __syncthreads();
     column[wave][lane] = most;
     __syncthreads();
-    if (wave == 0) {
-      const uint32_t bound =
-          beam_bound(max(max(column[0][lane], column[1][lane]), max(column[2][lane], column[3][lane])), k);
-      if (lane == 0) shared_bound = max(bound, 1u);
-    }
-    __syncthreads();
+    const uint32_t all[4] = {column[0][lane], column[1][lane], column[2][lane], column[3][lane]};
+    if constexpr (decltype(lanes)::value) return max(beam_bound(max(max(all[0], all[1]), max(all[2], all[3])), k), 1u);
+    return max(beam_bound(all, k), 1u);
   };
+  auto best_of = [&](int32_t i) { return static_cast<uint32_t>(offer(i, held[i * each_held]).key >> 32); };
   uint32_t most_here = 0;
-  for (int32_t i = tid; i < lists; i += 256)
-    most_here = max(most_here, static_cast<uint32_t>(offer(i, held[i * each_held]).key >> 32));
+  for (int32_t i = tid; i < lists; i += 256) most_here = max(most_here, best_of(i));
   if (tid == 0) loads = 0;
-  settle(most_here);
+  uint32_t least = settle(most_here, std::true_type{});
   for (int32_t i = tid; i < lists; i += 256)
-    if (static_cast<uint32_t>(offer(i, held[i * each_held]).key >> 32) >= shared_bound) chosen[atomicAdd(&loads, 1)] = i;
+    if (best_of(i) >= least) chosen[atomicAdd(&loads, 1)] = i;
   __syncthreads();
-  // f(offer) for every result of the chunks chosen, four loads at a time
-  const int32_t offers = loads * k;
-  auto offered = [&](auto &&f) {
-    for (int32_t i0 = tid; i0 < offers; i0 += 4 * 256) {
-      uint64_t item[4];
-      int32_t chunk[4];
-      kv_for<4>([&](auto U) {
-        uint32_t q = min(i0 + 256 * U, offers - 1);
-        const int32_t n = kv_rem(a.by_k, q);
-        chunk[U] = chosen[q];
-        item[U] = n > 0 && over[kv_quot(a.by_splits, chunk[U])] ? 0 : item_at(chunk[U], n);
-      });
-      kv_for<4>([&](auto U) {
-        if (i0 + 256 * U < offers) f(offer(chunk[U], item[U]));
-      });
-    }
-  };
-  auto collect = [&]() {
-    const uint32_t least = shared_bound;
-    offered([&](const Offer &o) {
-      if (static_cast<uint32_t>(o.key >> 32) >= least) {
-        const int32_t at = atomicAdd(&count, 1);
-        if (at < kBeamList) {
-          key_of[at] = o.key;
-          item_of[at] = o.item;
-          beam_of[at] = o.beam;
+  // Only chunks whose best reaches the bound are looked at further, by eight lanes each and
+  // eight results at a time: they are in order, so the rest of a chunk whose eighth does not
+  // reach it need not be read.  Where there are many, the first that are read
+  // give a higher bound (33 to 54 chunks with k 32: 32 to 41 results left of 46 to 1027, 27.2 us;
+  // 30.2 with all of the chunks' results read and put in order).
+  const int32_t chunks = loads, in_eight = tid & 7;
+  bool measure = false, again = false;
+  for (;;) {
+    for (int32_t c0 = 0; c0 < chunks; c0 += 128) {
+      bool more[4] = {true, true, true, true};
+      for (int32_t n0 = 0; n0 < k; n0 += 8) {
+        const int32_t n = n0 + in_eight;
+        uint64_t item[4];
+        int32_t chunk[4];
+        kv_for<4>([&](auto U) {
+          item[U] = chunk[U] = 0;
+          if (c0 + 32 * U < chunks) {
+            chunk[U] = chosen[min(c0 + 32 * U + (tid >> 3), chunks - 1)];
+            item[U] = item_at(chunk[U], min(n, k - 1));
+          }
+        });
+        BeamOffer o[4];
+        kv_for<4>([&](auto U) {
+          o[U] = BeamOffer{0, 0};
+          if (c0 + 32 * U < chunks) {
+            const bool there = more[U] && c0 + 32 * U + (tid >> 3) < chunks && n < k &&
+                               (n == 0 || !over[kv_quot(a.by_splits, chunk[U])]);
+            o[U] = offer(chunk[U], there ? item[U] : 0);
+          }
+        });
+        if (c0 + n0 == 0 || measure) {
+          uint32_t most = 0;
+          kv_for<4>([&](auto U) { most = max(most, static_cast<uint32_t>(o[U].key >> 32)); });
+          most_here = c0 + n0 == 0 ? most : max(most_here, most);
         }
+        if (!measure) {
+          if (c0 + n0 == 0 && chunks * min(k, 8) > 128) least = max(least, settle(most_here, std::false_type{}));
+          kv_for<4>([&](auto U) {
+            if (static_cast<uint32_t>(o[U].key >> 32) >= least) {
+              const int32_t at = atomicAdd(&count, 1);
+              if (at < kBeamList) offers[at] = o[U];
+            }
+          });
+        }
+        bool any = false;
+        kv_for<4>([&](auto U) {
+          more[U] = __shfl(static_cast<int>(static_cast<uint32_t>(o[U].key >> 32) >= least), lane | 7) != 0;
+          any = any || more[U];
+        });
+        if (!__any(any)) break;
       }
-    });
+    }
+    if (measure) {
+      measure = false;
+      least = max(least, settle(most_here, std::false_type{}));
+      if (tid == 0) count = 0;
+      __syncthreads();
+      continue;
+    }
     __syncthreads();
-  };
-  collect();
-  if (count > kBeamList) {  // few chunks more than are wanted give a low bound: all of theirs a higher one
-    most_here = 0;
-    offered([&](const Offer &o) { most_here = max(most_here, static_cast<uint32_t>(o.key >> 32)); });
-    __syncthreads();
-    if (tid == 0) count = 0;
-    settle(most_here);
-    collect();
+    if (count <= kBeamList || again) break;
+    measure = again = true;  // all that reach it give a higher one
   }
   const int32_t n = count;
   if (n <= kBeamList) {
-    if (n > 64) {  // what the best of a lane's each reach, k of them, is as high as needs be
-      most_here = 0;
-      for (int32_t i = tid; i < n; i += 256) most_here = max(most_here, static_cast<uint32_t>(key_of[i] >> 32));
-      settle(most_here);
-    }
     for (int32_t i = tid >> 2; i < n; i += 64) {  // four lanes an offer
-      const Offer o{key_of[i], item_of[i], beam_of[i], 0};
-      if (static_cast<uint32_t>(o.key >> 32) < shared_bound) continue;
-      int32_t rank = 0, same = 0;
+      const BeamOffer o = offers[i];
+      int32_t rank = 0;
       for (int32_t j0 = tid & 3; j0 < n; j0 += 16) {
-        uint64_t key[4];
-        kv_for<4>([&](auto U) { key[U] = key_of[min(j0 + 4 * U, n - 1)]; });
-        kv_for<4>([&](auto U) {
-          const int32_t there = j0 + 4 * U < n ? 1 : 0;
-          rank += key[U] > o.key ? there : 0;
-          same += key[U] == o.key ? there : 0;
-        });
+        BeamOffer other[4];
+        kv_for<4>([&](auto U) { other[U] = offers[min(j0 + 4 * U, n - 1)]; });
+        kv_for<4>([&](auto U) { rank += j0 + 4 * U < n && beam_better(other[U], o) ? 1 : 0; });
       }
-      kv_for<2>([&](auto I) {
-        rank += __shfl_xor(rank, 1 << I);
-        same += __shfl_xor(same, 1 << I);
-      });
-      if (same > 1 && rank < k) {  // of equal ones the lower beam's first, then the better of its own
-        int32_t before = 0;
-        for (int32_t j = tid & 3; j < n; j += 4)
-          if (key_of[j] == o.key) before += better(Offer{o.key, item_of[j], beam_of[j], 0}, o) ? 1 : 0;
-        kv_for<2>([&](auto I) { before += __shfl_xor(before, 1 << I); });
-        rank += before;
-      }
+      kv_for<2>([&](auto I) { rank += __shfl_xor(rank, 1 << I); });
       if (rank < k && (tid & 3) == 0) write(rank, o);
     }
     for (int32_t j = n + tid; j < k; j += 256) {
@@ -475,33 +488,37 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
   __syncthreads();
   for (int32_t i = tid; i < lists; i += 256) taken[i] = 0;
   __syncthreads();
-  auto next = [&]() {
-    Offer most{0, 0, INT_MAX, 0};
+  auto next = [&](int32_t &from_chunk) {
+    BeamOffer most{0, 0};
     for (int32_t i = tid; i < lists; i += 256)
       if (taken[i] < (over[kv_quot(a.by_splits, i)] ? 1 : k)) {
-        const Offer o = offer(i, item_at(i, taken[i]));
-        if (o.key != 0 && better(o, most)) most = o;
+        const BeamOffer o = offer(i, item_at(i, taken[i]));
+        if (o.key != 0 && beam_better(o, most)) {
+          most = o;
+          from_chunk = i;
+        }
       }
     return most;
   };
-  Offer mine = next();
-  __shared__ Offer wave_best[4];
+  int32_t from_chunk = 0;
+  BeamOffer mine = next(from_chunk);
+  __shared__ BeamOffer wave_best[4];
   for (int32_t j = 0; j < k; ++j) {
-    Offer most = mine;
+    BeamOffer most = mine;
     kv_for<6>([&](auto I) {
       auto other = [&](uint64_t v) { return static_cast<uint64_t>(__shfl_xor(static_cast<long long>(v), 1 << I)); };
-      const Offer o{other(most.key), other(most.item), __shfl_xor(most.beam, 1 << I), __shfl_xor(most.chunk, 1 << I)};
-      if (better(o, most)) most = o;
+      const BeamOffer o{other(most.key), other(most.tie)};
+      if (beam_better(o, most)) most = o;
     });
     if (lane == 0) wave_best[wave] = most;
     __syncthreads();
     kv_for<4>([&](auto W) {
-      if (better(wave_best[W], most)) most = wave_best[W];
+      if (beam_better(wave_best[W], most)) most = wave_best[W];
     });
     if (tid == 0) write(j, most);
-    if (most.chunk == mine.chunk && mine.key != 0) {
-      ++taken[mine.chunk];
-      mine = next();
+    if (mine.key != 0 && most.key == mine.key && most.tie == mine.tie) {
+      ++taken[from_chunk];
+      mine = next(from_chunk);
     }
     __syncthreads();
   }
@@ -510,7 +527,7 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
 // Bytes of a workgroup's shared memory: what its own values need, or the join of `lists` chunks.
 static size_t beam_shared(int64_t lists, int32_t k) {
   const int64_t held = lists * (k + 2) <= kBeamHeld ? lists * (k + 2) : lists;
-  return std::max<size_t>(kBeamList * (8 + 16 + 4), held * 8 + lists * (8 + 4 + 4) + kBeamList * (8 + 8 + 4));
+  return std::max<size_t>(kBeamList * (8 + 16 + 4), kBeamList * 16 + held * 8 + lists * (8 + 4 + 4));
 }
 
 // Chunks of a beam: as many as give the chip kBeamGroups workgroups, but no smaller than

@@ -226,3 +226,32 @@ def test_the_same_results_each_time(backend):
         again = backend.beam_select(x, s, 8)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, again))
+
+
+@pytest.mark.parametrize("requests,beams,k,size", [
+    (2, 5, 64, 3 * 4096 - 40), (3, 16, 32, 9 * 4096), (1, 33, 64, 4 * 4096 + 9), (1, 64, 64, 5 * 4096), (1, 64, 50, 262144 - 3), (1, 8, 9, 17 * 4096),
+])
+def test_joins(backend, requests, beams, k, size):
+    """Many chunks of a request: the best spread over them, of one beam, side by side in one chunk,
+    and as many as are wanted in each chunk."""
+    logits, scores = made(requests, beams, size, torch.bfloat16, seed=11)
+    check(backend, logits, scores, k)
+    check(backend, logits, scores - torch.arange(beams) * 7.0, k)
+    logits[:, :, size // 2:size // 2 + 70] += 14
+    check(backend, logits, scores, k)
+    logits[:, 1:, size // 2:size // 2 + 70] -= 14
+    check(backend, logits, scores, k)
+    finished = torch.rand((requests, beams), generator=torch.Generator().manual_seed(2)) < 0.4
+    check(backend, logits, scores, k, finished, 3)
+
+
+@pytest.mark.parametrize("values", [1, 2, 40])
+def test_joins_of_equal_logits(backend, values):
+    """More chunks than are looked at side by side, whose best are the same."""
+    gen = torch.Generator().manual_seed(12)
+    logits = torch.randint(0, values, (1, 5 * 4096), generator=gen).half().expand(64, -1)[None].contiguous()
+    for k in (3, 8, 64):
+        got = backend.beam_select(logits.to(DEV), torch.full((1, 64), -0.5, device=DEV), k)
+        want = do.beam_select(logits, torch.full((1, 64), -0.5), k)
+        for a, b in zip(got[1:], want[1:]):
+            assert torch.equal(a.cpu(), b)

@@ -377,11 +377,12 @@ __global__ __launch_bounds__(1024) void kv_reorder_kernel(const PoolArgs p, cons
 
 constexpr int32_t kSlotStarts = 4096;  // row starts held in shared memory
 
-// A wave for GROUPS groups of 64 rows.  A group whose rows are all of one sequence, which
-// those of prompts mostly are, asks once for it; else each row finds its own by halving among
-// the row starts, which a workgroup reads once where they fit (1.2 million rows of 515 sequences
-// 10.3 us, 64 rows of 67 2.9; the next 64 row starts asked one after the other, in registers, 9.0
-// and 7.1).
+// A wave for GROUPS groups of 64 rows.  The sequences of a group's first and last row are found
+// by 64 steps at a time among the row starts, which a workgroup reads once where they fit; a
+// group of one sequence, which those of prompts mostly are, asks no more, else each row
+// finds its own by halving between the two.  1.2 million rows of 515 sequences 9.1 us, of them 6 the
+// chain of loads and 3 the stores' way to memory, 64 rows of 67 2.7; every first row by halving
+// among all 10.0 and 2.8, the next 64 row starts asked one after the other, in registers, 9.0 and 7.1.
 template <int GROUPS>
 __global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int32_t *positions, int64_t *slots) {
   __shared__ int32_t held[kSlotStarts];
@@ -399,9 +400,19 @@ __global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int3
   const int32_t *const starts = few ? held : b.starts;
   const int32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wave_row = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * (64 * GROUPS);
-  // the last sequence that starts at the row or before it, from `low` on, which does
-  auto find = [&](int32_t low, int64_t row) {
-    int32_t high = b.seqs;
+  // the last sequence that starts at the row or before it, from `low` on, which does, and
+  // before `high`: of a wave's one row, and of a row a lane
+  auto find_one = [&](int32_t low, int32_t high, int64_t row) {
+    while (high - low > 1) {
+      // up to 2^31 + 62
+      const uint32_t step = ((high - low - 1) >> 6) + 1, end = high, at = low + step * (lane + 1);
+      const uint32_t n = __popcll(__ballot(at < end && starts[min(at, end)] <= row));
+      high = static_cast<int32_t>(min(end, low + step * (n + 1)));
+      low += static_cast<int32_t>(step * n);
+    }
+    return __builtin_amdgcn_readfirstlane(low);
+  };
+  auto find = [&](int32_t low, int32_t high, int64_t row) {
     while (high - low > 1) {
       const int32_t mid = (low + high) >> 1;
       if (starts[mid] <= row)
@@ -415,13 +426,14 @@ __global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int3
   // sequences of all groups first, then their lengths, then their pages: loads that wait for
   // each other do so once
   int32_t seq[GROUPS], length[GROUPS], page[GROUPS], place[GROUPS], position[GROUPS];
-  int32_t known = b.starts ? __builtin_amdgcn_readfirstlane(find(-1, wave_row)) : 0;
+  int32_t known = b.starts ? find_one(-1, b.seqs, wave_row) : 0;
   kv_for<GROUPS>([&](auto I) {
     const int64_t row0 = wave_row + 64 * I, row = row0 + lane;
     seq[I] = b.starts ? known : static_cast<int32_t>(min(row, static_cast<int64_t>(b.seqs)));
     if (b.starts && !(known >= 0 && known + 1 < b.seqs && starts[known + 1] > row0 + 63)) {
-      seq[I] = find(known, row);
-      known = __builtin_amdgcn_readlane(seq[I], 63);
+      const int32_t last = find_one(known, b.seqs, row0 + 63);
+      seq[I] = find(known, last + 1, row);
+      known = last;
     }
     const bool any = seq[I] >= 0 && seq[I] < b.seqs && row < b.rows;
     if (!any) seq[I] = -1;

@@ -193,6 +193,21 @@ def test_slots_of_many_rows(backend):
     check_slots(backend, pages, batch, table[:, 2:width + 2], lengths, starts)
 
 
+@pytest.mark.parametrize("seqs", [1, 2, 63, 64, 65, 127, 4095, 4096, 4097, 70000])
+@pytest.mark.parametrize("many", [False, True])
+def test_slots_of_many_sequences(backend, seqs, many):
+    """Numbers of sequences around those that one search's steps and shared memory hold, most of them idle or not."""
+    rng = random.Random(seqs + many)
+    table = torch.randint(0, 500, (seqs, 4), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    lengths = [rng.randint(0, 64) for _ in range(seqs)]
+    starts = [0]
+    for _ in range(seqs):
+        starts.append(starts[-1] + (rng.choice((0, 1, 1, 2, 40)) if many else int(rng.random() < 0.02) * 70))
+    pages = backend.create_kv_pool(device=DEV, blocks=500, block_size=16, sequences=1, width=1)
+    batch = backend.kv_batch(pages, table.to(DEV), ints(lengths), query_starts=ints(starts), rows=starts[-1] + 1, max_query=90)
+    check_slots(backend, pages, batch, table, lengths, starts)
+
+
 # ---- copies ------------------------------------------------------------------
 @pytest.mark.parametrize("dim", [40, 96, 128, 160, 192, 256])
 @pytest.mark.parametrize("page", [16, 32, 64, 128])

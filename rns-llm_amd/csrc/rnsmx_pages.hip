@@ -38,32 +38,68 @@ __device__ __forceinline__ void pool_drop(const PoolArgs &p, int32_t page) {
     p.free[page] = 1;
 }
 
-// Sums of N values a thread over the threads before it, and over all.
+// The sum of a value over the lanes up to each: within rows of 16, then across them.
+__device__ __forceinline__ int64_t pool_lanes(int64_t v) {
+  auto step = [&](auto ctrl, auto rows) {
+    constexpr int c = ctrl, r = rows;
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), c, r, 0xF, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), c, r, 0xF, false);
+    v += static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr:1
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
+  return v;
+}
+__device__ __forceinline__ int64_t pool_lane(int64_t v, int32_t lane) {
+  const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+  const uint32_t high = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+  return static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+}
+
+// Sums of N values a thread over the threads before it, and over all.  The waves' sums are summed by
+// a wave's lanes (every thread reading them one after the other took 1.3 us of 16 waves' call).
 template <int N>
 __device__ __forceinline__ void pool_scan(int64_t (&before)[N], int64_t (&all)[N], int64_t (*wave)[N]) {
-  const int32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int32_t lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   int64_t sum[N];
-  kv_for<N>([&](auto K) { sum[K] = before[K]; });
-  kv_for<6>([&](auto I) {
-    constexpr int step = 1 << I;
-    kv_for<N>([&](auto K) {
-      const int64_t other = __shfl_up(static_cast<long long>(sum[K]), step);
-      if (lane >= step) sum[K] += other;
-    });
-  });
+  kv_for<N>([&](auto K) { sum[K] = pool_lanes(before[K]); });
   __syncthreads();
   if (lane == 63) kv_for<N>([&](auto K) { wave[w][K] = sum[K]; });
   __syncthreads();
   kv_for<N>([&](auto K) {
-    int64_t past = 0, total = 0;
-    for (int32_t i = 0; i < waves; ++i) {
-      const int64_t v = wave[i][K];
-      past += i < w ? v : 0;
-      total += v;
-    }
-    before[K] = past + sum[K] - before[K];
-    all[K] = total;
+    const int64_t past = pool_lanes(lane < waves ? wave[lane][K] : 0);
+    before[K] = sum[K] - before[K] + (w > 0 ? pool_lane(past, max(w - 1, 0)) : 0);
+    all[K] = pool_lane(past, waves - 1);
   });
+}
+
+// The last sequence that starts at a number or before it, from `low` on, which does, and before
+// `high`: of a wave's one number, by 64 steps at a time, and of a number a lane.
+__device__ __forceinline__ int32_t find_wave(const int32_t *starts, int32_t low, int32_t high, int64_t number) {
+  const int32_t lane = threadIdx.x & 63;
+  while (high - low > 1) {
+    // up to 2^31 + 62
+    const uint32_t step = ((high - low - 1) >> 6) + 1, end = high, at = low + step * (lane + 1);
+    const uint32_t n = __popcll(__ballot(at < end && starts[min(at, end)] <= number));
+    high = static_cast<int32_t>(min(end, low + step * (n + 1)));
+    low += static_cast<int32_t>(step * n);
+  }
+  return __builtin_amdgcn_readfirstlane(low);
+}
+__device__ __forceinline__ int32_t find_lane(const int32_t *starts, int32_t low, int32_t high, int64_t number) {
+  while (high - low > 1) {
+    const int32_t mid = (low + high) >> 1;
+    if (starts[mid] <= number)
+      low = mid;
+    else
+      high = mid;
+  }
+  return low;
 }
 
 constexpr int32_t kPoolPicked = 4096;  // page numbers in shared memory
@@ -71,8 +107,7 @@ constexpr int32_t kPoolOwn = 2;        // pages of a sequence that its thread en
 constexpr int32_t kPoolMost = INT_MAX;
 
 // The free ones of sixteen pages, a bit each; what lies past the last page is none.
-__device__ __forceinline__ uint32_t pool_free(const PoolArgs &p, int32_t w) {
-  const u32x4 words = reinterpret_cast<const u32x4 *>(p.free)[w];
+__device__ __forceinline__ uint32_t pool_free(const PoolArgs &p, int32_t w, const u32x4 &words) {
   uint32_t bits = 0;
   kv_for<4>([&](auto I) {  // four bytes' lowest bits side by side
     constexpr int i = I;
@@ -81,6 +116,9 @@ __device__ __forceinline__ uint32_t pool_free(const PoolArgs &p, int32_t w) {
   });
   const int32_t left = p.blocks - 16 * w;
   return left < 16 ? bits & ((1u << left) - 1u) : bits;
+}
+__device__ __forceinline__ uint32_t pool_free(const PoolArgs &p, int32_t w) {
+  return pool_free(p, w, reinterpret_cast<const u32x4 *>(p.free)[w]);
 }
 
 struct PoolInfo {
@@ -116,7 +154,8 @@ __device__ __forceinline__ void pool_want(const AssignArgs &a, PoolInfo &i) {
 // memory into the tables; else, where they may be more than it holds, through memory, and
 // kv_enter_kernel enters them.
 // Bound by its chain: lengths, tails' entries and counts, a sum over the workgroup,
-// page numbers into the tables.
+// page numbers into the tables.  One token each of 67 sequences 4.8 us, of 256 beams that all
+// copy a page 5.9, 18800 pages of 515 sequences 7.0 and kv_enter_kernel's 4.3.
 template <bool LOCAL>
 __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
   __shared__ int32_t held[LOCAL ? kPoolPicked : 1];
@@ -130,12 +169,18 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
   // this thread's words of the free pages
   const int32_t each = (p.words + threads - 1) / threads;
   const int32_t word0 = min(tid * each, p.words), word1 = min(word0 + each, p.words);
+  // the first two, mostly all, are kept
+  u32x4 raw[2] = {};
+  kv_for<2>([&](auto J) {
+    if (word0 + J < word1) raw[J] = reinterpret_cast<const u32x4 *>(p.free)[word0 + J];
+  });
   if (tid == 0) any = past = 0;
   __syncthreads();
   PoolInfo mine{};
+  int32_t tail = -1;
   for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
     mine = pool_held(a, s0 + tid);
-    mine.source = pool_tail(p, mine);
+    mine.source = tail = pool_tail(p, mine);
     if (mine.n > 0 && mine.n > room - mine.old) past = 1;
     if (mine.source >= 0) {
       any = 1;
@@ -144,7 +189,10 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
     }
   }
   int64_t wanted = 0, rows = 0, free_before = 0, free_all = 0;
-  for (int32_t w = word0; w < word1; ++w) free_before += __popc(pool_free(p, w));
+  uint32_t own[2];
+  kv_for<2>([&](auto J) { own[J] = word0 + J < word1 ? pool_free(p, word0 + J, raw[J]) : 0; });
+  auto free_of = [&](int32_t w) { return w == word0 ? own[0] : w == word0 + 1 ? own[1] : pool_free(p, w); };
+  for (int32_t w = word0; w < word1; ++w) free_before += __popc(free_of(w));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   const bool shared = any != 0;
@@ -190,8 +238,7 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
   __syncthreads();  // marks and counts are read by all before they change
   if (shared)
     for (int32_t s0 = 0; s0 < p.seqs; s0 += threads) {
-      const PoolInfo i = pool_held(a, s0 + tid);
-      const int32_t t = pool_tail(p, i);
+      const int32_t t = once ? tail : pool_tail(p, pool_held(a, s0 + tid));
       if (t >= 0) {
         p.going[t] = 0;
         p.first[t] = INT_MAX;
@@ -203,7 +250,7 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
   if constexpr (LOCAL) {
     int64_t rank = free_before;
     for (int32_t w = word0; w < word1 && rank < count; ++w)
-      for (uint32_t bits = pool_free(p, w); bits != 0 && rank < count; bits &= bits - 1) {
+      for (uint32_t bits = free_of(w); bits != 0 && rank < count; bits &= bits - 1) {
         const int32_t number = 16 * w + __ffs(bits) - 1;
         held[rank++] = number;
         p.refs[number] = 1;
@@ -214,7 +261,7 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
     int64_t rank = free_before;
     for (int32_t w = word0; w < word1; ++w) {
       p.before[w] = static_cast<int32_t>(rank);
-      rank += __popc(pool_free(p, w));
+      rank += __popc(free_of(w));
     }
     if (tid == 0) p.spare[p.seqs] = count;
   }
@@ -258,7 +305,7 @@ __global__ __launch_bounds__(1024) void kv_assign_kernel(const AssignArgs a) {
 }
 
 // A thread a page: the free ones of the lowest ranks are taken, each by the sequence in whose
-// part of the ranks it lies.
+// part of the ranks it lies (searched for a wave's first and last page first: no faster).
 __global__ __launch_bounds__(256) void kv_enter_kernel(const AssignArgs a) {
   const PoolArgs &p = a.p;
   const int64_t b = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -267,16 +314,7 @@ __global__ __launch_bounds__(256) void kv_enter_kernel(const AssignArgs a) {
   const uint32_t bits = pool_free(p, w);
   const int32_t bit = static_cast<int32_t>(b & 15), rank = p.before[w] + __popc(bits & ((1u << bit) - 1u));
   if (!(bits >> bit & 1u) || rank >= count) return;
-  const int32_t page = static_cast<int32_t>(b);
-  // the last sequence whose part begins at the rank or before it
-  int32_t low = 0, high = p.seqs;
-  while (high - low > 1) {
-    const int32_t mid = (low + high) >> 1;
-    if (p.spare[mid] <= rank)
-      low = mid;
-    else
-      high = mid;
-  }
+  const int32_t page = static_cast<int32_t>(b), low = find_lane(p.spare, 0, p.seqs, rank);
   const int32_t first = p.spare[low], need = p.spare[low + 1] - first;
   p.refs[page] = 1;
   p.free[page] = 0;
@@ -400,39 +438,17 @@ __global__ __launch_bounds__(256) void kv_slots_kernel(const KvBatchArgs b, int3
   const int32_t *const starts = few ? held : b.starts;
   const int32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wave_row = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * (64 * GROUPS);
-  // the last sequence that starts at the row or before it, from `low` on, which does, and
-  // before `high`: of a wave's one row, and of a row a lane
-  auto find_one = [&](int32_t low, int32_t high, int64_t row) {
-    while (high - low > 1) {
-      // up to 2^31 + 62
-      const uint32_t step = ((high - low - 1) >> 6) + 1, end = high, at = low + step * (lane + 1);
-      const uint32_t n = __popcll(__ballot(at < end && starts[min(at, end)] <= row));
-      high = static_cast<int32_t>(min(end, low + step * (n + 1)));
-      low += static_cast<int32_t>(step * n);
-    }
-    return __builtin_amdgcn_readfirstlane(low);
-  };
-  auto find = [&](int32_t low, int32_t high, int64_t row) {
-    while (high - low > 1) {
-      const int32_t mid = (low + high) >> 1;
-      if (starts[mid] <= row)
-        low = mid;
-      else
-        high = mid;
-    }
-    return low;
-  };
   if (wave_row >= b.rows) return;
   // sequences of all groups first, then their lengths, then their pages: loads that wait for
   // each other do so once
   int32_t seq[GROUPS], length[GROUPS], page[GROUPS], place[GROUPS], position[GROUPS];
-  int32_t known = b.starts ? find_one(-1, b.seqs, wave_row) : 0;
+  int32_t known = b.starts ? find_wave(starts, -1, b.seqs, wave_row) : 0;
   kv_for<GROUPS>([&](auto I) {
     const int64_t row0 = wave_row + 64 * I, row = row0 + lane;
     seq[I] = b.starts ? known : static_cast<int32_t>(min(row, static_cast<int64_t>(b.seqs)));
     if (b.starts && !(known >= 0 && known + 1 < b.seqs && starts[known + 1] > row0 + 63)) {
-      const int32_t last = find_one(known, b.seqs, row0 + 63);
-      seq[I] = find(known, last + 1, row);
+      const int32_t last = find_wave(starts, known, b.seqs, row0 + 63);
+      seq[I] = find_lane(starts, known, last + 1, row);
       known = last;
     }
     const bool any = seq[I] >= 0 && seq[I] < b.seqs && row < b.rows;

@@ -25,6 +25,14 @@ struct BeamArgs {
 
 constexpr int kBeamMost = 256 * 64;  // values of a workgroup at most
 constexpr int kBeamList = 512;    // of a workgroup's or request's values those that reach its bound
+// Continuations up to which the maxima of 64 lanes give a chunk's bound: some 44 of its values reach
+// it with 32, but 270 with 64, past which those of 256 threads do, 74 with 64 (12 x 16 beams of 128257
+// in float32, k 64: 338 us with lanes, 37 with threads; k 32: 30.3 and 31.2).
+constexpr int kBeamLanes = 32;
+// Of a request's offers as many are put in order as they are, which takes the square of their
+// number, and more get a higher bound first, 1 us (56 x 16 beams of 8328, k 16, 256 offers: 31.4 us
+// without it, 17.3 with it; 14 of these requests, of whose offers few reach the first bound: 11.7 and 12.9).
+constexpr int kBeamFew = 96;
 constexpr int kBeamChunks = 1024; // of a request at most
 constexpr int kBeamHeld = 1024;   // results of a request that shared memory holds all
 
@@ -126,8 +134,8 @@ __device__ __forceinline__ float beam_value(const u32x4 &raw, int i) {
 // One workgroup for a chunk of one beam's logits, which are read once, all loads in
 // flight, and stay in registers as they are stored.  They give the largest, the sum of
 // exponentials against it and the chunk's k best.  A bound that at least k of them
-// reach: the k-th largest of 64 maxima, one for each lane over the four waves; of what lies
-// below it nothing more is asked, eight values at a time.  The few that reach it are put
+// reach: the k-th largest of 64 maxima, one for each lane over the four waves, or of the
+// threads' 256; of what lies below it nothing more is asked, eight values at a time.  The few that reach it are put
 // in order by counting.  Where they are many (logits that are equal, or in an order that puts
 // the largest side by side) the k-th largest itself is found digit by digit, from the logits
 // read again.  The workgroup that comes last of a request's joins the chunks, in the same manner.
@@ -201,10 +209,11 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
     };
     keep_raw();
     __syncthreads();
-    const uint32_t mine = max(max(column[0][lane], column[1][lane]), max(column[2][lane], column[3][lane]));
+    const uint32_t four[4] = {column[0][lane], column[1][lane], column[2][lane], column[3][lane]};
+    const uint32_t mine = max(max(four[0], four[1]), max(four[2], four[3]));
     const float largest = beam_logit(beam_wave_max(mine)), reference = largest == -INFINITY ? 0.0f : largest;
     if (wave == 0) {
-      const uint32_t bound = beam_bound(mine, k);
+      const uint32_t bound = k > kBeamLanes ? beam_bound(four, k) : beam_bound(mine, k);
       if (lane == 0) shared_bound = bound;
     }
     float part[2] = {0.0f, 0.0f};
@@ -435,7 +444,7 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
           most_here = c0 + n0 == 0 ? most : max(most_here, most);
         }
         if (!measure) {
-          if (c0 + n0 == 0 && chunks * min(k, 8) > 128) least = max(least, settle(most_here, std::false_type{}));
+          if (c0 + n0 == 0 && chunks * min(k, 8) > kBeamFew) least = max(least, settle(most_here, std::false_type{}));
           kv_for<4>([&](auto U) {
             if (static_cast<uint32_t>(o[U].key >> 32) >= least) {
               const int32_t at = atomicAdd(&count, 1);
@@ -459,8 +468,23 @@ __global__ __launch_bounds__(256, 4) void beam_kernel(const BeamArgs a) {
       continue;
     }
     __syncthreads();
-    if (count <= kBeamList || again) break;
-    measure = again = true;  // all that reach it give a higher one
+    const int32_t n = count;
+    if (n > kBeamList && !again) {  // all that reach it give a higher one
+      measure = again = true;
+      continue;
+    }
+    if (n > kBeamFew && n <= kBeamList) {  // so do those in the list
+      BeamOffer o[2];
+      kv_for<2>([&](auto U) { o[U] = tid + 256 * U < n ? offers[tid + 256 * U] : BeamOffer{0, 0}; });
+      least = max(least, settle(static_cast<uint32_t>(max(o[0].key, o[1].key) >> 32), std::false_type{}));
+      if (tid == 0) count = 0;
+      __syncthreads();
+      kv_for<2>([&](auto U) {
+        if (static_cast<uint32_t>(o[U].key >> 32) >= least) offers[atomicAdd(&count, 1)] = o[U];
+      });
+      __syncthreads();
+    }
+    break;
   }
   const int32_t n = count;
   if (n <= kBeamList) {

@@ -255,3 +255,13 @@ def test_joins_of_equal_logits(backend, values):
         want = do.beam_select(logits, torch.full((1, 64), -0.5), k)
         for a, b in zip(got[1:], want[1:]):
             assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("requests,beams,k,size", [(3, 16, 16, 1100), (2, 16, 33, 2000), (2, 13, 64, 1000), (2, 2, 64, 4096 * 6), (1, 7, 48, 700)])
+def test_joins_of_few_chunks(backend, requests, beams, k, size):
+    """As many results as lists hold, and more, of chunks that are all looked at; k about where bounds change."""
+    for dtype in (torch.float32, torch.float16):
+        logits, scores = made(requests, beams, size, dtype, seed=13)
+        for n in (k, k - 1):
+            check(backend, logits, scores, n)
+        check(backend, logits, scores * 8, k)

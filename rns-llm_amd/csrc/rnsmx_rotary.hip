@@ -61,13 +61,31 @@ __device__ __forceinline__ T rotary_round(float v) {
     return static_cast<T>(v);
 }
 
-// 16 bytes at p, of whose values those from `left` on are not there.
+// f(where, how many) for the first `left` of N values: all of them, or fours, a two and a one.
+template <int N, typename F>
+__device__ __forceinline__ void rotary_parts(int32_t left, F &&f) {
+  using std::integral_constant;
+  if (left >= N) return f(integral_constant<int, 0>{}, integral_constant<int, N>{});
+  kv_for<N / 4>([&](auto Q) {
+    constexpr int q = 4 * Q;
+    if (left >= q + 4) {
+      f(integral_constant<int, q>{}, integral_constant<int, 4>{});
+    } else if (left >= q + 2) {
+      f(integral_constant<int, q>{}, integral_constant<int, 2>{});
+      if (left == q + 3) f(integral_constant<int, q + 2>{}, integral_constant<int, 1>{});
+    } else if (left == q + 1) {
+      f(integral_constant<int, q>{}, integral_constant<int, 1>{});
+    }
+  });
+}
+// 16 bytes at p, of whose values those from `left` on are not there.  Whole ones are one load or
+// store from wherever they begin (6909 rows of 64 heads of 65 in 16 bits: 36 us, 69 by values).
 template <bool VEC, bool STREAM, typename T, int N>
 __device__ __forceinline__ void rotary_get(T (&x)[N], const T *p, int32_t left) {
   if constexpr (VEC) {
     *reinterpret_cast<u32x4 *>(x) = kv_fetch<STREAM>(reinterpret_cast<const u32x4 *>(p));
   } else {
-    kv_for<N>([&](auto I) { x[I] = I < left ? p[I] : T(0); });
+    rotary_parts<N>(left, [&](auto at, auto n) { __builtin_memcpy(x + at, p + at, n * sizeof(T)); });
   }
 }
 template <bool VEC, bool STREAM, typename T, int N>
@@ -77,9 +95,7 @@ __device__ __forceinline__ void rotary_put(T *p, const T (&x)[N], int32_t left) 
   } else if constexpr (VEC) {
     *reinterpret_cast<u32x4 *>(p) = *reinterpret_cast<const u32x4 *>(x);
   } else {
-    kv_for<N>([&](auto I) {
-      if (I < left) p[I] = x[I];
-    });
+    rotary_parts<N>(left, [&](auto at, auto n) { __builtin_memcpy(p + at, x + at, n * sizeof(T)); });
   }
 }
 
@@ -97,10 +113,10 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
   const int32_t half = a.pairs;
 
   struct Piece {
-    alignas(16) T x[2][N];
+    alignas(16) T x[2][N] = {};
     const T *from;
     T *to;
-    int32_t at[2], left[2], row, first;  // columns and how many of them are there
+    int32_t at[2], left[2], row;  // columns and how many of them are there
     bool there, turned;
   };
   auto load = [&](Piece &p, int32_t i) {
@@ -118,14 +134,16 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
     p.from = static_cast<const T *>(second ? v.src : u.src) + (row * (second ? v.src_rs : u.src_rs) + h * (second ? v.src_hs : u.src_hs));
     p.to = static_cast<T *>(second ? v.dst : u.dst) + (row * (second ? v.dst_rs : u.dst_rs) + h * (second ? v.dst_hs : u.dst_hs));
     p.turned = piece < a.turning;
-    p.first = N * piece;
+    // A load of neighbours or of what is copied lies beside that of the next thread, and a
+    // piece's second as far behind it as there are pieces (side by side they take their lines by
+    // halves: 12000 rows of 64 heads of 128 neighbours in 16 bits 168 us, 66 so).
     if (p.turned && !NEIGHBOURS) {
       p.at[0] = N * piece;
       p.at[1] = half + N * piece;
       p.left[0] = p.left[1] = half - N * piece;
     } else {
-      p.at[0] = p.turned ? 2 * N * piece : 2 * half + 2 * N * (piece - a.turning);
-      p.at[1] = p.at[0] + N;
+      p.at[0] = p.turned ? N * piece : 2 * half + N * (piece - a.turning);
+      p.at[1] = p.at[0] + N * (p.turned ? a.turning : a.pieces - a.turning);
       const int32_t end = p.turned ? 2 * half : a.dim;
       p.left[0] = end - p.at[0];
       p.left[1] = end - p.at[1];
@@ -138,13 +156,14 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
   auto store = [&](Piece &p) {
     if (!p.there) return;
     if (p.turned) {
-      const F32x2 *t = angles + p.row * half + p.first;
+      const F32x2 *const t = angles + p.row * half;
       kv_for<N>([&](auto I) {
         constexpr int i = I;
-        // neighbours: pair i lies in values 2 i, 2 i + 1 of the piece
+        // neighbours: pair i lies in values 2 i, 2 i + 1 of the two loads
         constexpr int ka = NEIGHBOURS ? (2 * i) / N : 0, ia = NEIGHBOURS ? (2 * i) % N : i;
         constexpr int kb = NEIGHBOURS ? (2 * i + 1) / N : 1, ib = NEIGHBOURS ? (2 * i + 1) % N : i;
-        const F32x2 cs = VEC || p.first + i < half ? t[i] : F32x2{1.0f, 0.0f};
+        const int32_t pair = NEIGHBOURS ? p.at[ka] / 2 + ia / 2 : p.at[0] + i;
+        const F32x2 cs = VEC || pair < half ? t[pair] : F32x2{1.0f, 0.0f};
         const float u = rotary_load(p.x[ka][ia]), v = rotary_load(p.x[kb][ib]);
         p.x[ka][ia] = rotary_round<T>(fmaf(u, cs.x, -(v * cs.y)));
         p.x[kb][ib] = rotary_round<T>(fmaf(v, cs.x, u * cs.y));
@@ -280,8 +299,7 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
 
   // Inputs and outputs that the 256 MB behind the L2s would not hold go past the caches: 16384 rows
   // of 40 heads of 128 in 16 bits (336 MB) 60 us so, 65 through them, 12288 (252 MB) 46 and 43.
-  // Float32 goes through them: loads of neighbours take their lines by halves (part of each
-  // head, 125 MB: 56 us so, 26.7 through them).
+  // The same in float32: 6909 rows of 64 heads of 128 (453 MB) 80 us so, 87 through them.
   constexpr int64_t kRotaryStream = 256ll << 20;
   const bool past = rows->rows * static_cast<double>(heads) * a.dim * size * 2 >= kRotaryStream && a.dim % 64 == 0;
 
@@ -323,8 +341,7 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   };
   auto launch = [&](auto t) {
     if (!vec) return with(t, std::false_type{}, std::false_type{});
-    if constexpr (sizeof(t) == 2)
-      if (past) return with(t, std::true_type{}, std::true_type{});
+    if (past) return with(t, std::true_type{}, std::true_type{});
     with(t, std::true_type{}, std::false_type{});
   };
   if (rows->dtype == RNSMX_FLOAT32)

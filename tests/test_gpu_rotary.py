@@ -249,3 +249,48 @@ def test_captured_gradients(backend):
         cos, sin = do.rotary_angles(rotary.frequencies, positions.cpu())
         for got, g in zip(held, (gq, gk)):
             check(got, g, cos, -sin, 16, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("part", [128, 96, 16])
+def test_past_the_caches(backend, part, layout, dtype):
+    """More than the caches hold: the same bits as in small calls, one of which is checked."""
+    rows, heads, dim = 264000 // (4 if dtype == torch.float32 else 2) // 8, 33, 128
+    gen = torch.Generator(device=DEV).manual_seed(part)
+    q = torch.randn((rows, heads - 1, dim), generator=gen, device=DEV, dtype=torch.float32).to(dtype)
+    k = torch.randn((rows, 1, dim), generator=gen, device=DEV, dtype=torch.float32).to(dtype)
+    assert 2 * (q.numel() + k.numel()) * q.element_size() > 256 << 20
+    positions = torch.randint(0, 9000, (rows,), generator=gen, device=DEV, dtype=torch.int32)
+    rotary = backend.create_rotary(device=DEV, rotary_dim=part, layout=layout)
+    got = backend.rotate(rotary, positions, q, k)
+    for a in range(0, rows, 2000):
+        want = backend.rotate(rotary, positions[a:a + 2000], q[a:a + 2000], k[a:a + 2000])
+        assert all(torch.equal(x[a:a + 2000], y) for x, y in zip(got, want))
+    n = rows - 9
+    angles = do.rotary_angles(rotary.frequencies, positions[n:].cpu())
+    check(got[0][n:], q[n:], *angles, part // 2, layout == "interleaved")
+    again = [x.clone() for x in (q, k)]
+    backend.rotate(rotary, positions, *again, inplace=True)
+    assert all(torch.equal(x, y) for x, y in zip(again, got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_every_size(backend, layout, dtype):
+    """Every head dimension and part of it up to 42, wherever rows begin, apart and in place; what is not turned
+    is copied, what lies between the rows stays."""
+    gen = torch.Generator().manual_seed(17)
+    for dim in range(2, 43):
+        part = 2 * (1 + (dim * 7) % (dim // 2))
+        wide = torch.randn((5, 3 * dim + 3), generator=gen).to(dtype).to(DEV)
+        positions = torch.tensor([0, 3, 9, 1000, 77], dtype=torch.int64, device=DEV)
+        rotary = backend.create_rotary(device=DEV, rotary_dim=part, layout=layout)
+        angles = do.rotary_angles(rotary.frequencies, positions.cpu())
+        x = wide[:, 1:1 + 3 * dim].view(5, 3, dim)
+        got = backend.rotate(rotary, positions, x)
+        check(got, x, *angles, part // 2, layout == "interleaved")
+        held = wide.clone()
+        backend.rotate(rotary, positions, x, inplace=True)
+        assert torch.equal(x, got)
+        assert torch.equal(wide[:, :1], held[:, :1]) and torch.equal(wide[:, 1 + 3 * dim:], held[:, 1 + 3 * dim:])

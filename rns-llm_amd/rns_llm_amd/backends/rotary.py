@@ -145,7 +145,8 @@ class RotaryOps:
         ``[rows]``, any value), in float32, rounded once, in one launch -> new tensors
         (or one, without k).  Angles are exact to 2**-32 of a turn up to position 2**32, beyond
         it to 2**-65 of a turn a position.
-        ``inplace``: the tensors themselves, which share no value, are turned and returned.
+        ``inplace``: the tensors themselves, which share no value, are turned and returned, a change
+        that autograd sees like that of any operation in place.
 
         Differentiable in q and k, but for calls in place.  As with any backward pass, one is
         captured into a graph only when no eager pass's graph of the same leaves is alive."""
@@ -155,6 +156,8 @@ class RotaryOps:
             out = _Rotate.apply(self, rotary, False, positions, q, k)
         else:
             out = self._rotated(rotary, positions, q, k, False, bool(inplace))
+            if inplace:  # torch has not seen the write, and an operation may have kept what was there
+                torch.autograd.graph.increment_version((q,) if k is None else (q, k))
         return out if k is not None else out[0]
 
     def _rotated(self, rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, back: bool, inplace: bool):

@@ -69,9 +69,8 @@ class RNSCachedAttention(nn.Module):
         if self.rotary is not None:
             if positions is None:
                 positions = self.backend.kv_slots(cache, batch)[0]
-            # the product's own columns, unless a gradient needs them as they are
-            inplace = not (torch.is_grad_enabled() and q.requires_grad)
-            q, k = self.backend.rotate(self.rotary, positions, q, k, inplace=inplace)
+            # not in place: the product's columns are also a forward hook's on the projection
+            q, k = self.backend.rotate(self.rotary, positions, q, k)
         self.backend.kv_append(cache, batch, k, v)
         out = self.backend.kv_attention(q, cache, batch, scale=self.scale, window=window, mask=mask)
         return self.out_proj(out.view(rows, self.num_heads * self.head_dim))

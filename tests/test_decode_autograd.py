@@ -1,9 +1,10 @@
 """What the decoding loop's calls tell autograd, with a stand-in for the library on tensors in host memory."""
 import pytest
 import torch
+from torch import nn
 
 from oracle import decode_oracle as do
-from rns_llm_amd import HipRNSBackend, _native
+from rns_llm_amd import HipRNSBackend, RNSCachedAttention, _native
 
 CPU = torch.device("cpu")
 
@@ -26,6 +27,16 @@ class HostBackend(HipRNSBackend):
                 x.detach().numpy()[...] = y.numpy()
             outs.append(x if inplace else y)
         return tuple(outs)
+
+    def kv_slots(self, pages, batch):
+        return torch.arange(batch.rows, dtype=torch.int32), None
+
+    def kv_append(self, cache, batch, k, v):
+        pass
+
+    def kv_attention(self, q, cache, batch, **options):
+        return q.clone()
+
 
 
 def turning(backend, dim=8):
@@ -63,3 +74,32 @@ def test_calls_in_place_are_seen_by_autograd():
     assert q._version == version
     with torch.inference_mode():  # tensors without a version
         b.rotate(rotary, positions, made(2, 3, 8), inplace=True)
+
+
+class Projection(nn.Module):
+    split_sizes = (16, 8, 8)
+
+    def forward(self, hidden):
+        return hidden.split(self.split_sizes, dim=-1)
+
+
+class Batch:
+    rows = 5
+
+
+@pytest.mark.parametrize("gradients", [True, False])
+def test_the_layer_leaves_its_projection_alone(gradients):
+    """What a hook keeps of the projection stays as it was, and can be trained on."""
+    b = HostBackend()
+    layer = RNSCachedAttention(Projection(), nn.Identity(), backend=b, num_heads=2, num_kv_heads=1, rotary=turning(b))
+    kept = []
+    layer.projection.register_forward_hook(lambda module, inputs, outputs: kept.extend(outputs))
+    hidden = made(5, 32, seed=1)
+    before = hidden.clone()
+    head = torch.ones(16, requires_grad=True)
+    with torch.set_grad_enabled(gradients):
+        out = layer(hidden, None, Batch())
+    assert not torch.equal(out, before[:, :16]) and torch.equal(hidden, before)
+    assert torch.equal(torch.cat(kept, dim=1), before)
+    (head * kept[0]).sum().backward()
+    assert torch.equal(head.grad, before[:, :16].sum(0))

@@ -1,6 +1,9 @@
 """What the decoding loop's calls tell autograd, on the GPU."""
 import pytest
 import torch
+from torch import nn
+
+from rns_llm_amd import RNSCachedAttention
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +31,26 @@ def test_calls_in_place_are_seen_by_autograd(backend):
         backend.rotate(rotary, positions, kept[:, 8:32].view(2, 3, 8), inplace=True)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         kept.sum().backward()
+
+
+@pytest.mark.parametrize("gradients", [True, False])
+def test_the_layer_leaves_its_projection_alone(backend, gradients):
+    """What a hook keeps of the fused product stays as it was, and can be trained on."""
+    torch.manual_seed(5)
+    linears = [nn.Linear(m, n).to(DEV) for m, n in ((64, 128), (64, 64), (64, 64), (128, 64))]
+    layer = RNSCachedAttention.from_linears(*linears, backend=backend, num_heads=2, num_kv_heads=1,
+                                            rotary=backend.create_rotary(device=DEV, rotary_dim=64))
+    kept = []
+    layer.projection.combined.register_forward_hook(lambda module, inputs, output: kept.append(output))
+    cache = layer.create_cache(blocks=2, block_size=16)
+    batch = backend.kv_batch(cache, torch.tensor([[0, 1]], dtype=torch.int32, device=DEV), [5], query_lengths=[5])
+    hidden = made(5, 64, seed=2)
+    with torch.no_grad():
+        want = layer.projection(hidden)[0].clone()
+    kept.clear()
+    with torch.set_grad_enabled(gradients):
+        layer(hidden, cache, batch)
+    head = torch.ones(128, device=DEV, requires_grad=True)
+    assert torch.equal(kept[0][:, :128], want)
+    (head * kept[0][:, :128].detach()).sum().backward()
+    assert torch.equal(head.grad, want.sum(0))

@@ -16,6 +16,7 @@ from dataclasses import dataclass, field
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -93,6 +94,12 @@ class KVBatch:
             self._checked.clear()
         self._checked[key] = value
         return value
+
+
+def _has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether forward-mode differentiation goes through one of the tensors, which their requires_grad does not say."""
+    return (getattr(forward_ad, "_current_level", 0) >= 0  # outside of it a question of no cost
+            and any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors))
 
 
 class _WithoutGradient(torch.autograd.Function):

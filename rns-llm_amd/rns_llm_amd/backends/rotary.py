@@ -15,7 +15,7 @@ from typing import Sequence
 import torch
 
 from .. import _native
-from .kv_cache import _FLOAT_CODES
+from .kv_cache import _FLOAT_CODES, _has_tangent
 
 _POSITION_CODES = {torch.int32: _native.INT32, torch.int64: _native.INT64}
 _MAX_CHECKED = 64
@@ -41,12 +41,13 @@ class Rotary:
 
 
 class _Rotate(torch.autograd.Function):
-    """The gradient turns back by the same angles, with the same magnitude."""
+    """The gradient turns back by the same angles, with the same magnitude; a tangent turns with its value."""
 
     @staticmethod
     def forward(ctx, backend, rotary, back, positions, q, k):
         ctx.backend, ctx.rotary, ctx.back = backend, rotary, back
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.set_materialize_grads(False)
         return backend._rotated(rotary, positions, q, k, back, False)
 
@@ -56,12 +57,14 @@ class _Rotate(torch.autograd.Function):
         first, second = (gq, gk) if gq is not None else (gk, None)
         if first is None:
             return (None,) * 6
-        if torch.is_grad_enabled():  # the gradient itself is differentiated
-            out = _Rotate.apply(ctx.backend, ctx.rotary, not ctx.back, positions, first, second)
-        else:
-            out = ctx.backend._rotated(ctx.rotary, positions, first, second, not ctx.back, False)
+        out = ctx.backend._turned(ctx.rotary, positions, first, second, not ctx.back)  # itself differentiated, it may be
         gq, gk = out if gq is not None else (None, out[0])
         return None, None, None, None, gq, gk
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        positions, = ctx.saved_tensors
+        return ctx.backend._turned(ctx.rotary, positions, tangents[4], None, ctx.back)
 
 
 def _disjoint(x: torch.Tensor) -> bool:
@@ -148,17 +151,25 @@ class RotaryOps:
         ``inplace``: the tensors themselves, which share no value, are turned and returned, a change
         that autograd sees like that of any operation in place.
 
-        Differentiable in q and k, but for calls in place.  As with any backward pass, one is
+        Differentiable in q and k, backward and in forward mode, but for calls in place.  As with any backward pass, one is
         captured into a graph only when no eager pass's graph of the same leaves is alive."""
-        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
-            if inplace:
-                raise ValueError("a call in place has no gradient: detach q and k, or call it under torch.no_grad()")
-            out = _Rotate.apply(self, rotary, False, positions, q, k)
+        if not inplace:
+            out = self._turned(rotary, positions, q, k, False)
+        elif _has_tangent(q, k) or torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+            raise ValueError("a call in place has no gradient: detach q and k, or call it under torch.no_grad()")
         else:
-            out = self._rotated(rotary, positions, q, k, False, bool(inplace))
-            if inplace:  # torch has not seen the write, and an operation may have kept what was there
-                torch.autograd.graph.increment_version((q,) if k is None else (q, k))
+            out = self._rotated(rotary, positions, q, k, False, True)
+            # torch has not seen the write, and an operation may have kept what was there
+            torch.autograd.graph.increment_version((q,) if k is None else (q, k))
         return out if k is not None else out[0]
+
+    def _turned(self, rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, back: bool):
+        """New tensors, with what autograd asks for."""
+        if _has_tangent(q, k):  # each by itself, so that one without a tangent gets none
+            return tuple(None if x is None else _Rotate.apply(self, rotary, back, positions, x, None)[0] for x in (q, k))
+        if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+            return _Rotate.apply(self, rotary, back, positions, q, k)
+        return self._rotated(rotary, positions, q, k, back, False)
 
     def _rotated(self, rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None, back: bool, inplace: bool):
         key = (q.dtype, q.shape, q.stride(), q.device, None if k is None else (k.dtype, k.shape, k.stride(), k.device),

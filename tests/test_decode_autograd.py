@@ -2,6 +2,7 @@
 import pytest
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from oracle import decode_oracle as do
 from rns_llm_amd import HipRNSBackend, RNSCachedAttention, _native
@@ -22,7 +23,8 @@ class HostBackend(HipRNSBackend):
             if x is None:
                 outs.append(None)
                 continue
-            y = do.rotate(x.detach(), cos, -sin if back else sin, rotary.interleaved, rotary.magnitude).to(x.dtype)
+            plain = torch.from_numpy(x.detach().numpy().copy())  # a tangent stays behind
+            y = do.rotate(plain, cos, -sin if back else sin, rotary.interleaved, rotary.magnitude).to(x.dtype)
             if inplace:
                 x.detach().numpy()[...] = y.numpy()
             outs.append(x if inplace else y)
@@ -103,3 +105,51 @@ def test_the_layer_leaves_its_projection_alone(gradients):
     assert torch.equal(torch.cat(kept, dim=1), before)
     (head * kept[0]).sum().backward()
     assert torch.equal(head.grad, before[:, :16].sum(0))
+
+
+@pytest.mark.parametrize("gradients", [True, False])
+def test_tangents_turn_with_their_values(gradients):
+    """Forward mode: of queries, of keys, of both; the rotation is linear."""
+    b = HostBackend()
+    rotary, positions = turning(b, 6), torch.tensor([3, 700])
+    q, k, tq, tk = (made(2, h, 8, seed=i) for i, h in enumerate((3, 1, 3, 1)))
+    want = b.rotate(rotary, positions, q, k)
+    turned = b.rotate(rotary, positions, tq, tk)
+    with forward_ad.dual_level(), torch.set_grad_enabled(gradients):
+        dq, dk = forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk)
+        for args, tangents in (((dq, dk), turned), ((dq, k), (turned[0], None)), ((q, dk), (None, turned[1])), ((q, k), (None, None))):
+            got = [forward_ad.unpack_dual(x) for x in b.rotate(rotary, positions, *args)]
+            for x, y, t in zip(got, want, tangents):
+                assert torch.equal(x.primal, y) and (x.tangent is None if t is None else torch.equal(x.tangent, t))
+        assert torch.equal(forward_ad.unpack_dual(b.rotate(rotary, positions, dk)).tangent, turned[1])
+        for args in ((dq, k), (q, dk), (dq, None)):
+            with pytest.raises(ValueError, match="no gradient"):
+                b.rotate(rotary, positions, *args, inplace=True)
+        assert torch.equal(b.rotate(rotary, positions, q.clone(), inplace=True), want[0])
+
+
+def test_tangents_and_gradients_together():
+    """Forward over reverse: of the sum of y^3, y = R x, the Hessian's product with a direction."""
+    b = HostBackend()
+    rotary, positions = turning(b), torch.tensor([3, 70])
+    x, t = made(2, 3, 8, seed=1), made(2, 3, 8, seed=2)
+
+    def loss(y):
+        return (y ** 3).sum()
+
+    with forward_ad.dual_level():
+        leaf = x.clone().requires_grad_()
+        gradient, = torch.autograd.grad(loss(b.rotate(rotary, positions, forward_ad.make_dual(leaf, t))), leaf)
+        got = forward_ad.unpack_dual(gradient).tangent
+    # R' (6 y R t)
+    y, turned = b.rotate(rotary, positions, x), b.rotate(rotary, positions, t)
+    g = 6 * y * turned
+    want = b._rotated(rotary, positions, g, None, True, False)[0]
+    # some four roundings of 2^-24 before both values of a pair are turned, one after
+    assert ((got - want).abs() <= 2.0 ** -22 * 2 * g.abs().amax(dim=2, keepdim=True)).all()
+    # a tangent that itself has a gradient
+    with forward_ad.dual_level():
+        direction = t.clone().requires_grad_()
+        out = forward_ad.unpack_dual(b.rotate(rotary, positions, forward_ad.make_dual(x, direction))).tangent
+        got, = torch.autograd.grad(out, direction, y)
+    assert ((got - x).abs() <= 2.0 ** -22 * 2 * x.abs().amax(dim=2, keepdim=True)).all()  # R' R x

@@ -2,6 +2,7 @@
 import pytest
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from rns_llm_amd import RNSCachedAttention
 
@@ -54,3 +55,32 @@ def test_the_layer_leaves_its_projection_alone(backend, gradients):
     assert torch.equal(kept[0][:, :128], want)
     (head * kept[0][:, :128].detach()).sum().backward()
     assert torch.equal(head.grad, want.sum(0))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_tangents_turn_with_their_values(backend, layout):
+    """Forward mode: the rotation is linear, so a tangent is turned like a value, bit for bit, and a column of
+    differences agrees; in reverse over it too."""
+    rotary = backend.create_rotary(device=DEV, rotary_dim=24, layout=layout, magnitude=1.5)
+    positions = torch.tensor([3, 700, 2 ** 20], device=DEV)
+    q, k, tq, tk = (made(3, h, 40, seed=i) for i, h in enumerate((5, 2, 5, 2)))
+    want, turned = (backend.rotate(rotary, positions, *x) for x in ((q, k), (tq, tk)))
+    with forward_ad.dual_level():
+        dq, dk = forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk)
+        for args, tangents in (((dq, dk), turned), ((dq, k), (turned[0], None)), ((q, dk), (None, turned[1]))):
+            for x, y, t in zip(backend.rotate(rotary, positions, *args), want, tangents):
+                x = forward_ad.unpack_dual(x)
+                assert torch.equal(x.primal, y) and (x.tangent is None if t is None else torch.equal(x.tangent, t))
+        for args in ((dq, k), (q, dk)):
+            with pytest.raises(ValueError, match="no gradient"):
+                backend.rotate(rotary, positions, *args, inplace=True)
+        leaf = q.clone().requires_grad_()
+        y = backend.rotate(rotary, positions, forward_ad.make_dual(leaf, tq))
+        gradient, = torch.autograd.grad((y ** 3).sum(), leaf)
+        got = forward_ad.unpack_dual(gradient).tangent
+    # the same values but for some four roundings of 2^-24 (powers, products, a rotation's sum), turned back: a
+    # value of a pair by 2^-22 of both of its pair, each no larger than the row's largest
+    x = q.clone().requires_grad_()
+    g = 6 * want[0] * turned[0]
+    product, = torch.autograd.grad(backend.rotate(rotary, positions, x), x, g)
+    assert ((got - product).abs() <= 2.0 ** -22 * 2 * 1.5 * g.abs().amax(dim=2, keepdim=True)).all()

@@ -12,12 +12,13 @@ import operator
 import torch
 
 from .. import _native
-from .kv_cache import _FLOAT_CODES
+from .kv_cache import _FLOAT_CODES, _has_tangent
 
 _MAX_CHECKED = 64
 
+
 class _WithoutGradient(torch.autograd.Function):
-    """Scores as they are; a backward pass that reaches them says that it ends there."""
+    """Scores as they are; a backward pass that reaches them, or a tangent, is told that it ends there."""
 
     @staticmethod
     def forward(ctx, out, *inputs):
@@ -26,6 +27,10 @@ class _WithoutGradient(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *gradients):
         raise RuntimeError("beam_select has no gradient: detach its logits and scores, or call it under torch.no_grad()")
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        raise RuntimeError("beam_select has no gradient, nor a tangent: detach its logits and scores")
 
 
 class BeamOps:
@@ -47,7 +52,7 @@ class BeamOps:
         ``request * beams + beam``.  A place that no candidate is left for has score minus
         infinity, ``end_token`` (0 without one) and its own number modulo the beams as its
         parent's.  ``k`` and ``beams`` are at most 64, ``beams * ceil(vocabulary / 16384)`` 1024.
-        There is no gradient: a backward pass through the scores raises."""
+        There is no gradient: a backward pass through the scores raises, a call with a tangent too."""
         k = operator.index(k)
         end_token = None if end_token is None else operator.index(end_token)
         key = (logits.dtype, logits.shape, logits.stride(), logits.device, scores.dtype, scores.shape, scores.stride(), scores.device,
@@ -71,7 +76,7 @@ class BeamOps:
                         None if finished is None else finished.data_ptr(), space.data_ptr(), space.numel(), out.data_ptr(),
                         tokens.data_ptr(), parents.data_ptr())
         self._stats["beam_select_calls"] += 1
-        if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+        if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad) or _has_tangent(logits, scores):
             out = _WithoutGradient.apply(out, logits, scores)
         return out, tokens, parents
 

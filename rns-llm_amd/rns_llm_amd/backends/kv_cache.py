@@ -103,7 +103,7 @@ def _has_tangent(*tensors: torch.Tensor | None) -> bool:
 
 
 class _WithoutGradient(torch.autograd.Function):
-    """An output as it is; a backward pass that reaches it says that it ends there."""
+    """An output as it is; a backward pass that reaches it, or a tangent, is told that it ends there."""
 
     @staticmethod
     def forward(ctx, out, *inputs):
@@ -112,6 +112,10 @@ class _WithoutGradient(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *gradients):
         raise RuntimeError("kv_attention has no gradient: detach its queries and mask, or call it under torch.no_grad()")
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        raise RuntimeError("kv_attention has no gradient, nor a tangent: detach its queries and mask")
 
 
 def _device_ints(values: torch.Tensor, name: str, ndim: int, device: torch.device) -> torch.Tensor:
@@ -302,7 +306,8 @@ class KVCacheOps:
         graph capture one of the graph's, cleared by each replay).
 
         There is no gradient: where queries or mask require one, a backward pass
-        through the result raises (a given ``out`` holds numbers alone)."""
+        through the result raises, and where they carry a tangent, the call (a given
+        ``out`` holds numbers alone)."""
         if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()):
             raise ValueError("out must be contiguous and like q")
         scale = None if scale is None else float(scale)
@@ -320,7 +325,8 @@ class KVCacheOps:
             need = int(self._lib.rnsmx_kv_attention_workspace_bytes(cache._ref, batch._ref, ctypes.addressof(query)))
             checked = batch._remember(key, (query, ctypes.addressof(query), need))
         _, ref, need = checked
-        wanted = out is None and (q.requires_grad or mask is not None and mask.requires_grad) and torch.is_grad_enabled()
+        wanted = out is None and ((q.requires_grad or mask is not None and mask.requires_grad) and torch.is_grad_enabled()
+                                  or _has_tangent(q, mask))
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         stream = self._stream_of(cache.device)

@@ -1,11 +1,13 @@
 """What the decoding loop's calls tell autograd, with a stand-in for the library on tensors in host memory."""
+from collections import Counter
+
 import pytest
 import torch
 from torch import nn
 from torch.autograd import forward_ad
 
 from oracle import decode_oracle as do
-from rns_llm_amd import HipRNSBackend, RNSCachedAttention, _native
+from rns_llm_amd import HipRNSBackend, KVCache, RNSCachedAttention, _native
 
 CPU = torch.device("cpu")
 
@@ -153,3 +155,52 @@ def test_tangents_and_gradients_together():
         out = forward_ad.unpack_dual(b.rotate(rotary, positions, forward_ad.make_dual(x, direction))).tangent
         got, = torch.autograd.grad(out, direction, y)
     assert ((got - x).abs() <= 2.0 ** -22 * 2 * x.abs().amax(dim=2, keepdim=True)).all()  # R' R x
+
+
+class NoLibrary:
+    """Calls that succeed and do nothing, sizes that are small."""
+
+    def __getattr__(self, name):
+        return lambda *args: 0 if name.startswith("rnsmx_kv_attention") else 64
+
+
+class CallsBackend(HostBackend):
+    """Selection and attention as far as the call, whose outputs nothing is written to."""
+
+    def __init__(self):
+        self._lib, self._beam_checked, self._stats = NoLibrary(), {}, Counter()
+
+    kv_attention = HipRNSBackend.kv_attention
+
+    @staticmethod
+    def _plain_beams(logits, scores, k, finished, end_token):
+        return logits, scores, finished
+
+    def _kv_scratch_for(self, need, device, stream):
+        return torch.zeros(need, dtype=torch.uint8)
+
+    def _on_device(self, device, call, *args):
+        pass
+
+    _stream_of = staticmethod(lambda device: 0)
+    _check_gpu = staticmethod(lambda cache: None)
+
+
+def test_calls_without_a_gradient_refuse_tangents():
+    """Their results would read as if they did not depend on what carries one."""
+    b = CallsBackend()
+    cache = KVCache(None, None, made(1, 1, 2), 1, 16, 1, 8, CPU, _shape=(1, 16, 8, CPU))
+    batch = b.kv_batch(cache, torch.zeros((2, 1), dtype=torch.int32), [3, 4])
+    q, mask, logits, scores = made(2, 3, 8), made(2, 3, 16), made(2, 3, 5), made(2, 3)
+    assert b.kv_attention(q, cache, batch, mask=mask).shape == q.shape and b.beam_select(logits, scores, 2)[0].shape == (2, 2)
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for gradients in (True, False):
+            with torch.set_grad_enabled(gradients):
+                for call in (lambda: b.kv_attention(dual(q), cache, batch), lambda: b.kv_attention(q, cache, batch, mask=dual(mask)),
+                             lambda: b.beam_select(dual(logits), scores, 2), lambda: b.beam_select(logits, dual(scores), 2)):
+                    with pytest.raises(RuntimeError, match="nor a tangent"):
+                        call()
+        # numbers alone
+        assert b.kv_attention(dual(q), cache, batch, out=torch.empty_like(q)).shape == q.shape
+        assert b.beam_select(logits, scores, 2)[0].shape == (2, 2)

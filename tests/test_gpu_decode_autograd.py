@@ -84,3 +84,17 @@ def test_tangents_turn_with_their_values(backend, layout):
     g = 6 * want[0] * turned[0]
     product, = torch.autograd.grad(backend.rotate(rotary, positions, x), x, g)
     assert ((got - product).abs() <= 2.0 ** -22 * 2 * 1.5 * g.abs().amax(dim=2, keepdim=True)).all()
+
+
+def test_calls_without_a_gradient_refuse_tangents(backend):
+    """Their results would read as if they did not depend on what carries one; detached it carries none."""
+    cache = backend.create_kv_cache(device=DEV, blocks=1, block_size=16, kv_heads=1, head_dim=64)
+    batch = backend.kv_batch(cache, torch.zeros((2, 1), dtype=torch.int32, device=DEV), [3, 4])
+    q, logits, scores = made(2, 3, 64), made(2, 3, 50), made(2, 3)
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for call in (lambda x: backend.kv_attention(x, cache, batch), lambda x: backend.beam_select(x[..., :50], scores, 2)[0],
+                     lambda x: backend.beam_select(logits, x[..., 0], 2)[0]):
+            with pytest.raises(RuntimeError, match="nor a tangent"):
+                call(dual(q))
+            assert torch.equal(call(dual(q).detach()), call(q))

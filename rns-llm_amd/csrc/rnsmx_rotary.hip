@@ -278,11 +278,15 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
     vec = vec && rotary_vec(size, p.src, p.src_rs, p.src_hs) && rotary_vec(size, p.dst, p.dst_rs, p.dst_hs);
     // Outputs meet an input's memory only where they are it; columns of one
     // product interleave without sharing a value, which ranges cannot tell.
-    for (int j = 0; j < 2; ++j)
-      if (part_heads[j] > 0 && !in_place &&
-          ranges_meet(p.dst, rotary_extent(rows->rows, part_heads[i], rows->head_dim, p.dst_rs, p.dst_hs, size), a.part[j].src,
-                      rotary_extent(rows->rows, part_heads[j], rows->head_dim, a.part[j].src_rs, a.part[j].src_hs, size)))
+    for (int j = 0; j < 2; ++j) {
+      if (part_heads[j] == 0 || (in_place && j == i)) continue;
+      const RotaryPart &other = a.part[j];
+      if (in_place ? !rotary_apart({p.dst, p.dst_rs, p.dst_hs, rows->rows, part_heads[i]},
+                                   {other.src, other.src_rs, other.src_hs, rows->rows, part_heads[j]}, rows->head_dim, size)
+                   : ranges_meet(p.dst, rotary_extent(rows->rows, part_heads[i], rows->head_dim, p.dst_rs, p.dst_hs, size), other.src,
+                                 rotary_extent(rows->rows, part_heads[j], rows->head_dim, other.src_rs, other.src_hs, size)))
         return fail(RNSMX_EINVAL, "outputs lie over queries or keys without being them");
+    }
   }
   a.steps = rotary->steps_dev;
   a.positions = positions_dev;

@@ -710,8 +710,9 @@ typedef struct rnsmx_rotary_rows {
 
 /* Turns queries and keys [rows][heads][head_dim] by positions_dev [rows], in float32,
  * rounded once.  An output is its input (the same pointer and strides) or shares no
- * memory with either; no value of an output is another's (queries' and keys' may lie side by
- * side, as columns of one product). */
+ * memory with either; no value of an output is another's, or an input's that is not it (queries
+ * and keys may lie side by side, as columns of one product, or, at one row stride, head by head
+ * among each other). */
 int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *rows,
                      const void *positions_dev, const void *q_dev, const void *k_dev,
                      void *q_out_dev, void *k_out_dev, void *stream);

@@ -1,6 +1,7 @@
 // Rotary positions: queries and keys turned by their positions' angles.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <type_traits>
 
 #include "rnsmx_kv_attn.hpp"
@@ -204,9 +205,10 @@ static int64_t rotary_extent(int64_t rows, int64_t heads, int64_t dim, int64_t r
   return ((rows - 1) * rs + (heads - 1) * hs + dim) * size;
 }
 
-// Whether `a` and `b`, rows and heads of `dim` values each at its strides, share no value:
-// apart as a whole, or blocks side by side in steps of one stride (columns of one product, whose
-// rows or, transposed, heads are that far apart).
+// Whether `a` and `b`, rows and heads of `dim` values each at its strides and as many rows, share no
+// value: apart as a whole, blocks side by side in steps of one stride (columns of one product, whose
+// rows or, transposed, heads are that far apart), or, rows being one stride apart, no two heads
+// the same.  Rows at other strides that lie among each other are taken to share.
 struct RotaryGrid {
   const void *p;
   int64_t rs, hs, rows, heads;
@@ -222,9 +224,23 @@ static bool rotary_apart(const RotaryGrid &a, const RotaryGrid &b, int64_t dim, 
     const int64_t at = ((bytes / size) % stride + stride) % stride;
     return at >= span_a && at + span_b <= stride;
   };
-  if (a.rs == b.rs && fit(a.rs, (a.heads - 1) * a.hs + dim, (b.heads - 1) * b.hs + dim)) return true;
+  const int64_t rs = a.rows == 1 ? 0 : a.rs;
   if (a.hs == b.hs && fit(a.hs, (a.rows - 1) * a.rs + dim, (b.rows - 1) * b.rs + dim)) return true;
-  return a.rs == b.rs && a.hs == b.hs && a.rs % std::max<int64_t>(a.hs, 1) == 0 && fit(a.hs, dim, dim);
+  if ((a.rows > 1 && a.rs != b.rs) || (a.rows > 1 && rs < dim)) return false;
+  if (fit(rs, (a.heads - 1) * a.hs + dim, (b.heads - 1) * b.hs + dim)) return true;
+  // a head of b begins `at` past one of a, and `rows` strides more in other rows
+  auto meet = [&](int64_t at) {
+    if (rs == 0) return std::abs(at) < dim;
+    const int64_t over = (at % rs + rs) % rs, down = (at - over) / rs;  // at - down * rs = over, the row before: over - rs
+    return (over < dim && std::abs(down) < a.rows) || (rs - over < dim && std::abs(down + 1) < a.rows);
+  };
+  for (int64_t h = 0; h < b.heads; ++h) {
+    if (meet(bytes / size + h * b.hs)) return false;
+    // at one stride of heads only how far they are apart counts
+    for (int64_t g = 1; g < (a.hs == b.hs && h > 0 ? 0 : a.heads); ++g)
+      if (meet(bytes / size + h * b.hs - g * a.hs)) return false;
+  }
+  return true;
 }
 
 }  // namespace rnsmx
@@ -267,7 +283,7 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   if (part_heads[0] > 0 && part_heads[1] > 0 && q_out_dev && k_out_dev &&
       !rotary_apart({q_out_dev, rows->q_out_row_stride, rows->q_out_head_stride, rows->rows, rows->q_heads},
                     {k_out_dev, rows->k_out_row_stride, rows->k_out_head_stride, rows->rows, rows->k_heads}, rows->head_dim, size))
-    return fail(RNSMX_EINVAL, "the outputs of queries and keys share values");
+    return fail(RNSMX_EINVAL, "the outputs of queries and keys share values, or lie among each other's rows at another row stride");
   for (int i = 0; i < 2; ++i) {
     if (part_heads[i] == 0) continue;
     const RotaryPart &p = a.part[i];

@@ -148,8 +148,9 @@ class RotaryOps:
         ``[rows]``, any value), in float32, rounded once, in one launch -> new tensors
         (or one, without k).  Angles are exact to 2**-32 of a turn up to position 2**32, beyond
         it to 2**-65 of a turn a position.
-        ``inplace``: the tensors themselves, which share no value, are turned and returned, a change
-        that autograd sees like that of any operation in place.
+        ``inplace``: the tensors themselves, which share no value (and lie among each other at one
+        row stride alone), are turned and returned, a change that autograd sees like that of any
+        operation in place.
 
         Differentiable in q and k, backward and in forward mode, but for calls in place.  As with any backward pass, one is
         captured into a graph only when no eager pass's graph of the same leaves is alive."""

@@ -197,12 +197,17 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
 }
 
 static bool rotary_vec(int64_t size, const void *p, int64_t rs, int64_t hs) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && rs * size % 16 == 0 && hs * size % 16 == 0;
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && rs % 16 * size % 16 == 0 && hs % 16 * size % 16 == 0;
 }
 
 // Bytes from the first to past the last of a tensor's rows.
 static int64_t rotary_extent(int64_t rows, int64_t heads, int64_t dim, int64_t rs, int64_t hs, int64_t size) {
   return ((rows - 1) * rs + (heads - 1) * hs + dim) * size;
+}
+
+// No address space has 2^57 bytes, and below that no extent wraps.
+static bool rotary_addressed(int64_t rows, int64_t heads, int64_t dim, int64_t rs, int64_t hs, int64_t size) {
+  return (static_cast<double>(rows - 1) * rs + static_cast<double>(heads - 1) * hs + dim) * size < 0x1p57;
 }
 
 // Whether `a` and `b`, rows and heads of `dim` values each at its strides and as many rows, share no
@@ -279,6 +284,10 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   a.part[1] = {k_dev, k_out_dev, rows->k_row_stride, rows->k_head_stride, rows->k_out_row_stride, rows->k_out_head_stride};
   const int32_t part_heads[2] = {rows->q_heads, rows->k_heads};
   const int32_t step = static_cast<int32_t>(16 / size);  // values of a load
+  for (int i = 0; i < 2; ++i)
+    if (part_heads[i] > 0 && !(rotary_addressed(rows->rows, part_heads[i], rows->head_dim, a.part[i].src_rs, a.part[i].src_hs, size) &&
+                               rotary_addressed(rows->rows, part_heads[i], rows->head_dim, a.part[i].dst_rs, a.part[i].dst_hs, size)))
+      return fail(RNSMX_EINVAL, "strides past the address space");
   bool vec = rotary->pairs % step == 0 && rows->head_dim % step == 0, copied = false;
   if (part_heads[0] > 0 && part_heads[1] > 0 && q_out_dev && k_out_dev &&
       !rotary_apart({q_out_dev, rows->q_out_row_stride, rows->q_out_head_stride, rows->rows, rows->q_heads},

@@ -27,3 +27,13 @@ def test_one_in_place_the_other_read_from_its_memory(moved, strides):
         args = {mine: AT, mine + "_out": AT, other: AT + moved, other + "_out": ELSEWHERE}
         rc, message = turn(args["q"], args["k"], args["q_out"], args["k_out"], **changes)
         assert rc == _native.EINVAL and "lie over queries or keys" in message
+
+
+@pytest.mark.parametrize("changes", [
+    {"q_row_stride": 2 ** 61, "q_out_row_stride": 2 ** 61, "rows": 9}, {"k_row_stride": 2 ** 62, "k_out_row_stride": 2 ** 62},
+    {"q_head_stride": 2 ** 62, "q_out_head_stride": 2 ** 62}, {"k_out_head_stride": 2 ** 63 - 1},
+])
+def test_strides_past_the_address_space(changes):
+    """Extents that pass 64 bits would not tell what lies over what."""
+    rc, message = turn(AT, AT + (1 << 40), AT, AT + (1 << 40), **changes)
+    assert rc == _native.EINVAL and "address space" in message

@@ -324,8 +324,8 @@ __global__ __launch_bounds__(256) void kv_enter_kernel(const AssignArgs a) {
 }
 
 // A workgroup for a sequence: the pages past `to` tokens are let go.
-__global__ __launch_bounds__(256) void kv_trim_kernel(const PoolArgs p, const int32_t *to) {
-  const int32_t s = blockIdx.x;
+__global__ __launch_bounds__(256) void kv_trim_kernel(const PoolArgs p, const int32_t *to, uint32_t first) {
+  const int32_t s = first + blockIdx.x;
   const int32_t old = min(max(p.lengths[s], 0), p.width << p.log_page), n = min(old, max(to[s], 0));
   if (n == old) return;
   int32_t *row = p.table + static_cast<int64_t>(s) * p.width;
@@ -347,8 +347,8 @@ __device__ __forceinline__ int32_t pool_parent(const PoolArgs &p, const int32_t 
 // Two launches, a workgroup for a sequence each: what every sequence becomes is laid
 // aside and held once more; then it takes its place and what was there is let go, after all
 // that stays is held.
-__global__ __launch_bounds__(256) void kv_gather_kernel(const PoolArgs p, const int32_t *parents) {
-  const int32_t s = blockIdx.x, from = pool_parent(p, parents, s);
+__global__ __launch_bounds__(256) void kv_gather_kernel(const PoolArgs p, const int32_t *parents, uint32_t first) {
+  const int32_t s = first + blockIdx.x, from = pool_parent(p, parents, s);
   if (from == s) return;
   const int32_t *row = p.table + static_cast<int64_t>(s) * p.width, *source = p.table + static_cast<int64_t>(max(from, 0)) * p.width;
   int32_t *to = p.spare + static_cast<int64_t>(s) * p.width;
@@ -359,8 +359,8 @@ __global__ __launch_bounds__(256) void kv_gather_kernel(const PoolArgs p, const 
   }
   if (threadIdx.x == 0) p.spare_lengths[s] = from < 0 ? 0 : p.lengths[from];
 }
-__global__ __launch_bounds__(256) void kv_settle_kernel(const PoolArgs p, const int32_t *parents) {
-  const int32_t s = blockIdx.x, from = pool_parent(p, parents, s);
+__global__ __launch_bounds__(256) void kv_settle_kernel(const PoolArgs p, const int32_t *parents, uint32_t first) {
+  const int32_t s = first + blockIdx.x, from = pool_parent(p, parents, s);
   if (from == s) return;
   int32_t *row = p.table + static_cast<int64_t>(s) * p.width;
   const int32_t *source = p.spare + static_cast<int64_t>(s) * p.width;
@@ -562,8 +562,15 @@ static int32_t pool_args(const rnsmx_kv_pool_t *pool, PoolArgs &a) {
   return RNSMX_OK;
 }
 
-// Threads for a sequence's row of the table.
-static unsigned row_threads(const PoolArgs &a) { return a.width <= 64 ? 64 : 256; }
+// A workgroup for each sequence's row of the table, of the threads that it needs; several launches
+// from 2^26 (rows past 64 pages: 2^24) sequences on.
+template <typename K>
+static void launch_rows(K kernel, const PoolArgs &a, const int32_t *numbers, void *stream) {
+  const unsigned threads = a.width <= 64 ? 64 : 256;
+  kv_launches(a.seqs, threads, [&](uint32_t first, uint32_t groups) {
+    hipLaunchKernelGGL(kernel, dim3(groups), dim3(threads), 0, static_cast<hipStream_t>(stream), a, numbers, first);
+  });
+}
 
 }  // namespace rnsmx
 
@@ -613,7 +620,7 @@ int32_t rnsmx_kv_trim(const rnsmx_kv_pool_t *pool, const int32_t *lengths_dev, v
   PoolArgs a{};
   if (int32_t rc = pool_args(pool, a)) return rc;
   if (!on(lengths_dev, 4)) return fail(RNSMX_EINVAL, "lengths null or not on a 4-byte boundary");
-  hipLaunchKernelGGL(kv_trim_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, static_cast<hipStream_t>(stream), a, lengths_dev);
+  launch_rows(kv_trim_kernel, a, lengths_dev, stream);
   return pages_check("kv_trim");
 }
 
@@ -622,15 +629,14 @@ int32_t rnsmx_kv_reorder(const rnsmx_kv_pool_t *pool, const int32_t *parents_dev
   PoolArgs a{};
   if (int32_t rc = pool_args(pool, a)) return rc;
   if (!on(parents_dev, 4)) return fail(RNSMX_EINVAL, "parents null or not on a 4-byte boundary");
-  hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t entries = static_cast<int64_t>(a.seqs) * a.width;
   if (entries <= kReorderEach * 1024) {
     const unsigned threads = static_cast<unsigned>(std::min<int64_t>(1024, (entries + 63) / 64 * 64));
-    hipLaunchKernelGGL(kv_reorder_kernel, dim3(1), dim3(threads), 0, st, a, parents_dev, kv_div(a.width));
+    hipLaunchKernelGGL(kv_reorder_kernel, dim3(1), dim3(threads), 0, static_cast<hipStream_t>(stream), a, parents_dev, kv_div(a.width));
     return pages_check("kv_reorder");
   }
-  hipLaunchKernelGGL(kv_gather_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, st, a, parents_dev);
-  hipLaunchKernelGGL(kv_settle_kernel, dim3(a.seqs), dim3(row_threads(a)), 0, st, a, parents_dev);
+  launch_rows(kv_gather_kernel, a, parents_dev, stream);
+  launch_rows(kv_settle_kernel, a, parents_dev, stream);
   return pages_check("kv_reorder");
 }
 

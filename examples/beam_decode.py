@@ -87,6 +87,7 @@ def search(model: Decoder, backend, prompts, beams: int, steps: int, page: int, 
     new[firsts.long()] = torch.tensor(lengths, dtype=torch.int32, device=device)
     prompt = backend.kv_step(pool, rows=sum(lengths), max_query=max(lengths))
     backend.kv_assign(pool, prompt, new)
+    lacking = prompt.missing != 0  # any step of the search, asked at its end
     positions, slots = backend.kv_slots(pool, prompt.batch)
     ids = torch.cat(list(prompts)).int()
     history[slots] = ids
@@ -100,6 +101,7 @@ def search(model: Decoder, backend, prompts, beams: int, steps: int, page: int, 
 
     def advance() -> None:
         backend.kv_assign(pool, step, (~finished).int().view(-1))
+        lacking.logical_or_(step.missing)
         for cache in caches:
             backend.kv_copy(cache, step)
         pages = history.view(-1, page)
@@ -114,7 +116,7 @@ def search(model: Decoder, backend, prompts, beams: int, steps: int, page: int, 
         finished.copy_(finished.view(-1)[best[2].long()] | (best[1] == end_token))
         backend.kv_reorder(pool, best[2].view(-1))
 
-    state = (pool.table, pool.lengths, pool.refs, pool.free, scores, ids, finished)
+    state = (pool.table, pool.lengths, pool.refs, pool.free, scores, ids, finished, lacking)
     replay = None
     for i in range(1, steps):
         if replay is None:
@@ -144,8 +146,8 @@ def search(model: Decoder, backend, prompts, beams: int, steps: int, page: int, 
     text = F.pad(text, (0, 1), value=end_token).scatter(1, pool.lengths.long().view(-1, 1), ids.view(-1, 1))
     first = torch.tensor(lengths, device=device).repeat_interleave(beams).view(-1, 1)
     got = text.gather(1, (first + torch.arange(steps, device=device)).clamp(max=text.shape[1] - 1))
-    if int(step.missing):
-        raise RuntimeError(f"the last step lacked pages: {int(step.missing)}")
+    if bool(lacking):
+        raise RuntimeError("a step of the search lacked pages")
     return got.view(requests, beams, steps), scores
 
 

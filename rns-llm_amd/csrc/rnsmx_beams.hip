@@ -1,6 +1,5 @@
 // Beam search's selection: the best continuations of each request's beams.
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -20,7 +19,7 @@ struct BeamArgs {
   int32_t first, apart;  // first: a launch's first request
   int32_t beams, vocabulary, k, end_token;
   int32_t chunk, splits;  // values of a workgroup, and workgroups of a beam
-  KvDiv by_splits, by_beams, by_k;
+  KvDiv by_splits, by_beams;
 };
 
 constexpr int kBeamMost = 256 * 64;  // values of a workgroup at most
@@ -637,7 +636,6 @@ int32_t rnsmx_beam_select(const rnsmx_beams_t *beams, const void *logits_dev, co
   a.end_token = beams->end_token;
   a.by_splits = kv_div(a.splits);
   a.by_beams = kv_div(a.beams);
-  a.by_k = kv_div(a.k);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t lists = static_cast<int64_t>(a.beams) * a.splits;
   // a ticket a request, and fewer than 2^32 threads

@@ -720,8 +720,12 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
 /*
  * Beam search's selection: for each request the k best continuations of its beams,
  *   score(b, v) = scores[b] + (x[v] - log sum_u exp x[u]),  x the logits of beam b,
- * compared in 64 bits; of equal ones the lower beam's go first, within a beam the
- * larger logit, then the lower token.  A finished beam goes on as it is, once, with
+ * compared in 64 bits as they come out; of equal ones the lower beam's go first, within
+ * a beam the larger logit, then the lower token.  The exponentials are float32, some dozens
+ * of which are added in float32, so a log-sum is off by up to (3 ln(vocabulary + 1) + 35) 2^-24:
+ * the order is exact within a beam and among beams of the same logits in one call, while other beams'
+ * continuations whose scores are nearer than twice that (8.4e-6 with 128257 tokens) come in
+ * either order, which may differ with the number of requests.  A finished beam goes on as it is, once, with
  * end_token; its logits are not read.  What is not finite is no candidate, and a beam
  * whose logits hold a not-a-number or plus infinity, or nothing above minus infinity,
  * has none.  A place without a candidate has score minus infinity, end_token

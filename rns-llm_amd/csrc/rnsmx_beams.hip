@@ -132,7 +132,9 @@ __device__ __forceinline__ float beam_value(const u32x4 &raw, int i) {
 
 // One workgroup for a chunk of one beam's logits, which are read once, all loads in
 // flight, and stay in registers as they are stored.  They give the largest, the sum of
-// exponentials against it and the chunk's k best.  A bound that at least k of them
+// exponentials against it and the chunk's k best.  Exponentials are float32, up to 33 of which are
+// added in float32: scores have no more bits when they come out, and what it leaves open is the
+// order of different beams' continuations nearer than some 1e-5.  A bound that at least k of them
 // reach: the k-th largest of 64 maxima, one for each lane over the four waves, or of the
 // threads' 256; of what lies below it nothing more is asked, eight values at a time.  The few that reach it are put
 // in order by counting.  Where they are many (logits that are equal, or in an order that puts

@@ -38,13 +38,17 @@ class BeamOps:
 
     def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, k: int, *, finished: torch.Tensor | None = None,
                     end_token: int | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """The ``k`` best continuations of each request's beams, best first, in one launch.
+        """The ``k`` best continuations of each request's beams, best first, in one launch for
+        up to 16384 requests.
 
         ``logits`` ``[requests, beams, vocabulary]`` (rows of any strides), ``scores``
         float32 ``[requests, beams]``, each beam's so far.  A continuation's score is its beam's
-        plus the token's log-probability (``log_softmax`` over the vocabulary), compared in
-        64 bits; of equal ones the lower beam's goes first, within a beam the larger logit,
-        then the lower token.  A beam that is ``finished`` (bool ``[requests, beams]``) goes on
+        plus the token's log-probability (``log_softmax`` over the vocabulary); of equal ones
+        the lower beam's goes first, within a beam the larger logit, then the lower token.
+        Exponentials are float32, log-sums and scores 64 bits: a log-sum is off by up to
+        ``(3 ln(vocabulary + 1) + 35) 2**-24``.  The order is exact within a beam and among beams
+        of the same logits; other beams' continuations nearer than twice that may come in
+        either order (and in another where a call has more requests).  A beam that is ``finished`` (bool ``[requests, beams]``) goes on
         as it is, once, with ``end_token``; its logits are not read.  A logit or score of
         minus infinity is no candidate; a beam whose logits hold a NaN or plus infinity has none.
 

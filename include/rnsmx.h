@@ -686,7 +686,7 @@ int32_t rnsmx_kv_copy(const rnsmx_kv_cache_t *cache, const int32_t *copies_dev, 
  * (i, i + pairs) or, interleaved, (2 i, 2 i + 1).  A pair (u, v) at position p becomes
  *   magnitude (u cos t - v sin t), magnitude (v cos t + u sin t),
  *   t = 2 pi p steps_dev[i] / 2^64,
- * the fraction of a turn being exact in 64 bits; the values past them stay.
+ * the fraction of a turn being taken in 64 bits and cut to 2^-32; the values past them stay.
  */
 #define RNSMX_ROTARY_MAX_DIM 1024
 #define RNSMX_ROTARY_MAX_HEADS 4096

@@ -27,7 +27,8 @@ class KVPool:
     ``table``: int32 ``[sequences, width]``, each sequence's pages, -1 past them;
     ``lengths``: int32 ``[sequences]``; ``refs``: int32 ``[blocks]``, how many sequences
     hold a page; ``free``: uint8, 1 for a page that nobody holds.  Calls on a pool
-    change it in their order, so they belong on one stream (or behind its events)."""
+    change it in their order, so they belong on one stream (or behind its events).  Autograd
+    is not told of these changes, nor of a step's: what it is to keep is cloned first."""
 
     table: torch.Tensor
     lengths: torch.Tensor
@@ -122,7 +123,8 @@ class KVPoolOps:
     def kv_assign(self, pool: KVPool, step: KVStep, new: torch.Tensor | None = None) -> None:
         """Gives the sequences pages for ``new`` tokens each (int32 ``[sequences]``, cut
         to 0 and ``max_query``; None: one each), adds them to ``pool.lengths`` and
-        fills ``step``, in one launch.
+        fills ``step``, in one launch, or two where the step's rows could need more than 4096
+        pages (so a step of few tokens has its own ``kv_step``).
 
         Pages are the lowest that nobody holds, in the order of the sequences.  A
         partly filled page that others hold too is replaced by a page of the sequence's

@@ -196,8 +196,9 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotaryArgs a) {
   }
 }
 
-static bool rotary_vec(int64_t size, const void *p, int64_t rs, int64_t hs) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && rs % 16 * size % 16 == 0 && hs % 16 * size % 16 == 0;
+// Whether every row and head begins at a multiple of `bytes`.
+static bool rotary_on(int64_t bytes, int64_t size, const void *p, int64_t rs, int64_t hs) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && rs % bytes * size % bytes == 0 && hs % bytes * size % bytes == 0;
 }
 
 // Bytes from the first to past the last of a tensor's rows.
@@ -288,7 +289,7 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
     if (part_heads[i] > 0 && !(rotary_addressed(rows->rows, part_heads[i], rows->head_dim, a.part[i].src_rs, a.part[i].src_hs, size) &&
                                rotary_addressed(rows->rows, part_heads[i], rows->head_dim, a.part[i].dst_rs, a.part[i].dst_hs, size)))
       return fail(RNSMX_EINVAL, "strides past the address space");
-  bool vec = rotary->pairs % step == 0 && rows->head_dim % step == 0, copied = false;
+  bool vec = rotary->pairs % step == 0 && rows->head_dim % step == 0, copied = false, lines = true;
   if (part_heads[0] > 0 && part_heads[1] > 0 && q_out_dev && k_out_dev &&
       !rotary_apart({q_out_dev, rows->q_out_row_stride, rows->q_out_head_stride, rows->rows, rows->q_heads},
                     {k_out_dev, rows->k_out_row_stride, rows->k_out_head_stride, rows->rows, rows->k_heads}, rows->head_dim, size))
@@ -300,7 +301,8 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
       return fail(RNSMX_EINVAL, "queries, keys or outputs null or not aligned to their type");
     const bool in_place = p.src == p.dst && p.src_rs == p.dst_rs && p.src_hs == p.dst_hs;
     copied = copied || !in_place;
-    vec = vec && rotary_vec(size, p.src, p.src_rs, p.src_hs) && rotary_vec(size, p.dst, p.dst_rs, p.dst_hs);
+    vec = vec && rotary_on(16, size, p.src, p.src_rs, p.src_hs) && rotary_on(16, size, p.dst, p.dst_rs, p.dst_hs);
+    lines = lines && rotary_on(128, size, p.src, p.src_rs, p.src_hs) && rotary_on(128, size, p.dst, p.dst_rs, p.dst_hs);
     // Outputs meet an input's memory only where they are it; columns of one
     // product interleave without sharing a value, which ranges cannot tell.
     for (int j = 0; j < 2; ++j) {
@@ -329,8 +331,16 @@ int32_t rnsmx_rotate(const rnsmx_rotary_t *rotary, const rnsmx_rotary_rows_t *ro
   // Inputs and outputs that the 256 MB behind the L2s would not hold go past the caches: 16384 rows
   // of 40 heads of 128 in 16 bits (336 MB) 60 us so, 65 through them, 12288 (252 MB) 46 and 43.
   // The same in float32: 6909 rows of 64 heads of 128 (453 MB) 80 us so, 87 through them.
+  // But only where neighbouring threads' loads, a head's pairs or half of what is copied, take whole
+  // lines of 128 bytes, or few in parts: a line taken by halves travels twice.  340 MB of 40 heads, us so
+  // and through the caches: heads of 64 in 16 bits (64 bytes) 82 and 71, 64 of 128 turned 82 and 69, heads
+  // of 80 and 96 130 and 72, 160 (160 bytes) 89 and 70, 192 68 and 68 (900 MB: 175 and 166), 320 (320 bytes) 68
+  // and 70; in float32 heads of 64 (128 bytes) 60 and 66, 80 90 and 67, 160 65 and 68, 32 of 128 69 and
+  // 67.  Heads of 128 in 16 bits that begin 16 bytes off a line 67 and 65, in float32 61 and 64.
   constexpr int64_t kRotaryStream = 256ll << 20;
-  const bool past = rows->rows * static_cast<double>(heads) * a.dim * size * 2 >= kRotaryStream && a.dim % 64 == 0;
+  auto whole = [&](int64_t bytes) { return bytes >= 256 || (bytes % 128 == 0 && lines); };
+  const bool past = rows->rows * static_cast<double>(heads) * a.dim * size * 2 >= kRotaryStream && whole(a.pairs * size) &&
+                    (a.pieces == a.turning || whole(16 * (a.pieces - a.turning)));
 
   // A workgroup takes rows of some kRotaryPieces pieces, which share the angles' cost (16383 rows
   // of 40 heads of 128, 320 pieces each, through the caches: 66.7 us with 2 rows, 66.9 with 4, 69.2

@@ -99,8 +99,8 @@ class RotaryOps:
             raise ValueError(f"rotary_dim must be even, 2 to {_native.ROTARY_MAX_DIM}")
         if layout not in ("half", "interleaved"):
             raise ValueError("layout must be 'half' or 'interleaved'")
-        if not math.isfinite(magnitude):
-            raise ValueError("magnitude must be finite")
+        if not math.isfinite(ctypes.c_float(magnitude).value):  # as the library takes it
+            raise ValueError("magnitude must be finite in float32")
         if frequencies is not None:
             if scaling is not None:
                 raise ValueError("frequencies are given, nothing is left to scale")
@@ -108,8 +108,13 @@ class RotaryOps:
             if len(values) != rotary_dim // 2 or not all(map(math.isfinite, values)):
                 raise ValueError(f"frequencies must be {rotary_dim // 2} finite numbers")
         else:
-            values = self._frequencies(rotary_dim, float(base), scaling, float(factor), original_length, float(low_turns),
-                                       float(high_turns))
+            try:
+                values = self._frequencies(rotary_dim, float(base), scaling, float(factor), original_length, float(low_turns),
+                                           float(high_turns))
+            except (OverflowError, ZeroDivisionError):
+                values = [math.inf]
+            if not all(map(math.isfinite, values)):
+                raise ValueError(f"base {base} and factor {factor} give frequencies that are not finite")
         turns = [round(Fraction(f) * 2 ** 64 / (2 * _PI)) % 2 ** 64 for f in values]
         steps = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
         struct = _native.RotaryStruct(steps.data_ptr(), rotary_dim // 2, layout == "interleaved", float(magnitude))

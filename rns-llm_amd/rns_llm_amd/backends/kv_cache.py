@@ -327,7 +327,8 @@ class KVCacheOps:
         _, ref, need = checked
         wanted = out is None and ((q.requires_grad or mask is not None and mask.requires_grad) and torch.is_grad_enabled()
                                   or _has_tangent(q, mask))
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         stream = self._stream_of(cache.device)
         space, size = None, 0
@@ -344,6 +345,8 @@ class KVCacheOps:
                                           stream)
         if rc:
             _native.check(rc)
+        if given:  # torch has not seen the write, and an operation may have kept what was there
+            torch.autograd.graph.increment_version(out)
         self._stats["kv_attention_calls"] += 1
         return _WithoutGradient.apply(out, q, mask) if wanted else out
 

@@ -204,3 +204,16 @@ def test_calls_without_a_gradient_refuse_tangents():
         # numbers alone
         assert b.kv_attention(dual(q), cache, batch, out=torch.empty_like(q)).shape == q.shape
         assert b.beam_select(logits, scores, 2)[0].shape == (2, 2)
+
+
+def test_a_given_output_is_seen_by_autograd():
+    """What an operation keeps of an attention's result, and the next call writes over: the backward pass raises."""
+    b = CallsBackend()
+    cache = KVCache(None, None, made(1, 1, 2), 1, 16, 1, 8, CPU, _shape=(1, 16, 8, CPU))
+    batch = b.kv_batch(cache, torch.zeros((2, 1), dtype=torch.int32), [3, 4])
+    q, out = made(2, 3, 8), made(2, 3, 8)
+    w = torch.ones_like(out).requires_grad_()
+    kept = (w * b.kv_attention(q, cache, batch, out=out)).sum()
+    b.kv_attention(q, cache, batch, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
